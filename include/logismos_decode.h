@@ -608,6 +608,137 @@ logismos_status_t logismos_launch_embed_lookup_bf16(const void* table_bf16, cons
                                                     long long vocab, logismos_stream_t stream);
 
 /* ------------------------------------------------------------------------
+ * Operators over packed rows: the attention half of a block whose rows a caller keeps himself
+ * ------------------------------------------------------------------------
+ * A batch is `total_tokens` rows, the tokens of sequence s in rows [cu_seqlens[s], cu_seqlens[s+1])
+ * (int32 `[num_seqs + 1]`, non-decreasing, starting at or behind 0; empty sequences are allowed).  Rows
+ * behind the last sequence are neither read nor written.  A stride is the distance of two rows in elements, so that q, k
+ * and v may be columns of one fused projection.  At most 2^24 rows and sequences together.  A call needs
+ * nothing but its arguments, allocates nothing and can be captured into a graph; it runs on the device that is current. */
+
+/* Rotary positions of q and k heads (`rope_apply`, crates/kernels/src/rope/cpu.rs:56-127, and
+ * `rope_halves_in_place`, crates/kernels/src/cpu_f32/mod.rs, for rows at any positions): of the first rotary_dim
+ * elements of every head the pairs (i, i + rotary_dim / 2), or with interleaved != 0 the pairs (2i, 2i + 1),
+ * become
+ *   (x_i cos t - x_j sin t, x_i sin t + x_j cos t) * amplitude,   t = positions[row] * inv_freq[i],
+ * and the others are copied.  fp16, bf16 or fp32 in and out; the angle is reduced in 64 bits, the rest is
+ * fp32, rounded once.
+ *
+ *   q_in, q_out   `[tokens]` rows of `[num_q_heads][head_dim]`, q_in_stride and q_out_stride apart
+ *   k_in, k_out   the same with num_kv_heads; num_kv_heads == 0: none (pointers and strides are not looked at)
+ *   positions     int32 `[tokens]`, any value
+ *   inv_freq      double `[rotary_dim / 2]` in device memory, radians per position, e.g. from
+ *                 `logismos_rope_frequencies`
+ *
+ * In place: the same address and stride as output and input.  Otherwise no output may overlap an input.  Addresses are
+ * aligned to an element; where addresses, strides and widths are multiples of 16 bytes it is fastest.
+ * rotary_dim even, at most head_dim; head_dim at most 1024; (num_q_heads + num_kv_heads) * head_dim at most 65536. */
+logismos_status_t logismos_check_rope_packed_shape(int tokens, int num_q_heads, int num_kv_heads, int head_dim,
+                                                   int rotary_dim, int q_in_stride, int k_in_stride,
+                                                   int q_out_stride, int k_out_stride, char* msg, size_t msg_cap);
+logismos_status_t logismos_launch_rope_packed_fp16(const void* q_in, const void* k_in, void* q_out, void* k_out,
+                                                   const int32_t* positions, const double* inv_freq, int tokens,
+                                                   int num_q_heads, int num_kv_heads, int head_dim,
+                                                   int rotary_dim, int q_in_stride, int k_in_stride,
+                                                   int q_out_stride, int k_out_stride, float amplitude,
+                                                   int interleaved, logismos_stream_t stream);
+logismos_status_t logismos_launch_rope_packed_bf16(const void* q_in, const void* k_in, void* q_out, void* k_out,
+                                                   const int32_t* positions, const double* inv_freq, int tokens,
+                                                   int num_q_heads, int num_kv_heads, int head_dim,
+                                                   int rotary_dim, int q_in_stride, int k_in_stride,
+                                                   int q_out_stride, int k_out_stride, float amplitude,
+                                                   int interleaved, logismos_stream_t stream);
+logismos_status_t logismos_launch_rope_packed_f32(const void* q_in, const void* k_in, void* q_out, void* k_out,
+                                                  const int32_t* positions, const double* inv_freq, int tokens,
+                                                  int num_q_heads, int num_kv_heads, int head_dim,
+                                                  int rotary_dim, int q_in_stride, int k_in_stride,
+                                                  int q_out_stride, int k_out_stride, float amplitude,
+                                                  int interleaved, logismos_stream_t stream);
+
+/* Frequencies of rotary positions, on the host: inv_freq[i] = base^(-2i / rotary_dim), i < rotary_dim / 2
+ * (`build_rope_table_f32`, crates/kernels/src/cpu_f32/mod.rs:599-619), scaled for contexts `factor`
+ * (>= 1) times as long as those a model was trained on:
+ *   NONE    as they are (factor is not looked at)
+ *   LINEAR  divided by factor (positions interpolated)
+ *   BASE    base * factor^(rotary_dim / (rotary_dim - 2)): the highest frequency stays, the lowest is divided by
+ *           factor (rotary_dim > 2)
+ *   PARTS   a pair that turns more than turns_fast times over original_positions stays, one that turns less
+ *           than turns_slow times is divided by factor, between the two a mixture, linear in the turns; amplitude
+ *           0.1 ln(factor) + 1 (YaRN, Peng et al. 2023; turns_fast 32, turns_slow 1 there)
+ * amplitude: what the launch multiplies cos and sin by (1 but for PARTS).  No device access. */
+#define LOGISMOS_ROPE_SCALE_NONE 0
+#define LOGISMOS_ROPE_SCALE_LINEAR 1
+#define LOGISMOS_ROPE_SCALE_BASE 2
+#define LOGISMOS_ROPE_SCALE_PARTS 3
+logismos_status_t logismos_rope_frequencies(double* inv_freq, float* amplitude, int rotary_dim, double base,
+                                            int scaling, double factor, int original_positions,
+                                            double turns_fast, double turns_slow);
+
+/* out[t][h][:] = softmax_j( (q[t][h] . k[j][h/g]) * scale ) . v[j][h/g] over the tokens j of t's own sequence, up
+ * to t itself where causal != 0 (`QwenAttention::forward` without a cache, crates/transformers/src/attention.rs:225-296,
+ * over rows without padding; bidirectional in the encoders).
+ *
+ *   q, out  rows of `[num_q_heads][head_dim]`, k and v of `[num_kv_heads][head_dim]`, fp16 or bf16;
+ *           16-byte aligned, strides multiples of 8
+ *
+ * fp32 scores, softmax and sums; the probabilities are rounded to the rows' type for the second product.  Elements of
+ * keys that a token does not see do not reach its result, whatever they hold; a token whose keys all score
+ * -inf gives zeros.  scale finite and > 0 (else hipErrorInvalidValue); head_dim a multiple of 32 up to 256; num_q_heads a
+ * multiple of num_kv_heads; k and v strides up to 2^22; (total_tokens + num_seqs) * num_q_heads up to
+ * 2^28.  out does not overlap q, k or v. */
+logismos_status_t logismos_check_attn_packed_shape(int num_seqs, int total_tokens, int num_q_heads,
+                                                   int num_kv_heads, int head_dim, int q_stride, int k_stride,
+                                                   int v_stride, int out_stride, char* msg, size_t msg_cap);
+logismos_status_t logismos_launch_attn_packed_fp16(const void* q, const void* k, const void* v,
+                                                   const int32_t* cu_seqlens, void* out, int num_seqs,
+                                                   int total_tokens, int num_q_heads, int num_kv_heads,
+                                                   int head_dim, int q_stride, int k_stride, int v_stride,
+                                                   int out_stride, float scale, int causal,
+                                                   logismos_stream_t stream);
+logismos_status_t logismos_launch_attn_packed_bf16(const void* q, const void* k, const void* v,
+                                                   const int32_t* cu_seqlens, void* out, int num_seqs,
+                                                   int total_tokens, int num_q_heads, int num_kv_heads,
+                                                   int head_dim, int q_stride, int k_stride, int v_stride,
+                                                   int out_stride, float scale, int causal,
+                                                   logismos_stream_t stream);
+
+/* Low-rank adapters of many requests beside a shared `linear_t` (crates/kernels/src/cpu_f32/mod.rs:271-345):
+ *   out[t][:] = base[t][:] + scales[a] * (x[t] . A_a^T) . B_a^T,   a = adapter_of_seq[s], s the sequence of row t.
+ *
+ *   x               fp16 or bf16 rows of k
+ *   a, b            `[num_adapters][max_rank][k]` and `[num_adapters][n][max_rank]` of x's type; of adapter a the first
+ *                   ranks[a] rows of A and columns of B count, what lies behind them is not looked at
+ *   ranks, scales   int32 and fp32 `[num_adapters]`; a rank of 0 or less: the adapter adds nothing; more than
+ *                   max_rank: max_rank
+ *   adapter_of_seq  int32 `[num_seqs]`; a value outside [0, num_adapters): no adapter, the base alone
+ *   base, out       rows of n of x's type, or fp32 with out_is_f32 != 0 (the products of the shared projection); the
+ *                   same address and stride: in place (rows without an adapter are not touched then), otherwise they
+ *                   may not overlap.  out does not overlap x
+ *   workspace       `logismos_adapter_add_workspace_bytes(total_tokens, max_rank)` bytes, contents don't matter;
+ *                   not shared by calls that can overlap in time
+ *
+ * fp32 sums; x . A^T is not rounded below what the result's type holds; one rounding at the end.  max_rank a multiple of 8
+ * up to 256, n, k and strides multiples of 8; x, a, b, base, out, workspace 16-byte aligned. */
+logismos_status_t logismos_check_adapter_add_shape(int num_seqs, int total_tokens, int num_adapters,
+                                                   int max_rank, int n, int k, int x_stride, int base_stride,
+                                                   int out_stride, char* msg, size_t msg_cap);
+size_t logismos_adapter_add_workspace_bytes(int total_tokens, int max_rank);
+logismos_status_t logismos_launch_adapter_add_fp16(const void* x, const void* a, const void* b,
+                                                   const int32_t* ranks, const float* scales,
+                                                   const int32_t* adapter_of_seq, const int32_t* cu_seqlens,
+                                                   const void* base, void* out, int out_is_f32, void* workspace,
+                                                   int num_seqs, int total_tokens, int num_adapters,
+                                                   int max_rank, int n, int k, int x_stride, int base_stride,
+                                                   int out_stride, logismos_stream_t stream);
+logismos_status_t logismos_launch_adapter_add_bf16(const void* x, const void* a, const void* b,
+                                                   const int32_t* ranks, const float* scales,
+                                                   const int32_t* adapter_of_seq, const int32_t* cu_seqlens,
+                                                   const void* base, void* out, int out_is_f32, void* workspace,
+                                                   int num_seqs, int total_tokens, int num_adapters,
+                                                   int max_rank, int n, int k, int x_stride, int base_stride,
+                                                   int out_stride, logismos_stream_t stream);
+
+/* ------------------------------------------------------------------------
  * The launchers the reference already has (built there for gfx1100), for gfx950
  * ------------------------------------------------------------------------
  * Same symbols, argument lists and meaning as the reference's own, so its private

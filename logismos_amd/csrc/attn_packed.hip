@@ -1,0 +1,290 @@
+// Attention of whole packed sequences: q, k and v are rows of the same tokens, sequences one behind the
+// other (cu_seqlens), causal or over the whole sequence, G = num_q_heads / num_kv_heads query heads per KV head.
+//
+// A column is a (token, head of the group) pair of one KV head, in that order over the sequence.  A wave owns 32 columns,
+// their queries in registers; a workgroup's waves share the key tiles in LDS.  Per tile of 32 keys:
+//
+//   S^T[32 keys x 32 columns] = K . Q^T         v_mfma_f32_32x32x16
+//   online softmax of a column, which lives in two lanes (fp32)
+//   O^T[D x 32 columns] += V^T . P              v_mfma_f32_32x32x16
+//
+// The result layout of S^T is the operand layout of P when the keys of a step of 16 are taken in the order
+// 4h + i, 8 + 4h + i (h: half of the wave, i < 4); V comes out of its row-major tile in that order through the
+// transposing LDS read.  P goes in rounded to the rows' type: every term is off by at most half a step of that type
+// relative to itself, as every output is by its own rounding.
+#include "device_utils.hpp"
+#include "launch_common.hpp"
+#include "packed_rows.hpp"
+
+#include <math.h>
+
+namespace lg {
+
+struct AttnPackedParams {
+    const unsigned short* q;
+    const unsigned short* k;
+    const unsigned short* v;
+    const int32_t* cu;
+    unsigned short* out;
+    int num_seqs, total, hkv, g;
+    int64_t q_stride, k_stride, v_stride, out_stride;
+    float scale_log2e;
+    int causal;
+};
+
+constexpr int kApKeys = 32;
+
+template <typename T, int D, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void attn_packed_kernel(const AttnPackedParams p) {
+    constexpr int kCols = 32 * WAVES, kPieces = D / 8, kStride = D + 8;
+    __shared__ __attribute__((aligned(16))) unsigned short ks[kApKeys * kStride], vs[kApKeys * kStride];
+    __shared__ unsigned odd_waves[WAVES];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int h = lane >> 5, col = lane & 31;
+    const int kvh = (int)(blockIdx.x % (unsigned)p.hkv);
+    const PackedTile t = packed_tile(p.cu, p.num_seqs, p.total, p.g, kCols, (int)(blockIdx.x / (unsigned)p.hkv));
+    const int cols = t.rows * p.g;
+    const int groups = (cols + kCols - 1) / kCols;
+    const int group = groups - 1 - t.tile;  // (the last columns see the most keys: they start first)
+    if (t.rows <= 0 || group < 0) return;
+    const int c0 = group * kCols + wave * 32;
+    const int gc = c0 + col;
+    const bool live = gc < cols;
+    const int tok = (live ? gc : cols - 1) / p.g, head = kvh * p.g + (live ? gc : cols - 1) % p.g;
+    const int vis = p.causal ? tok + 1 : t.rows;  // keys of this lane's column
+    const int last = (group + 1) * kCols < cols ? (group + 1) * kCols - 1 : cols - 1;
+    const int visible = p.causal ? last / p.g + 1 : t.rows;  // ... of the workgroup's last
+    const int first_vis = p.causal ? (c0 < cols ? c0 : cols - 1) / p.g + 1 : t.rows;  // ... of the wave's first
+    const int last_vis = p.causal ? (c0 + 31 < cols ? c0 + 31 : cols - 1) / p.g + 1 : t.rows;
+
+    uint4_t qb[D / 16];
+    {
+        const unsigned short* q = p.q + (int64_t)(t.row0 + tok) * p.q_stride + (int64_t)head * D + 8 * h;
+#pragma unroll
+        for (int j = 0; j < D / 16; ++j) qb[j] = *reinterpret_cast<const uint4_t*>(q + 16 * j);
+    }
+    const unsigned short* kp = p.k + (int64_t)t.row0 * p.k_stride + (int64_t)kvh * D;
+    const unsigned short* vp = p.v + (int64_t)t.row0 * p.v_stride + (int64_t)kvh * D;
+    const int s16 = lane & 15;
+    const int v_lane = (4 * h + (s16 >> 2)) * kStride + 16 * ((lane >> 4) & 1) + 4 * (s16 & 3);
+    auto v_operand = [&](int kb, int dt) LG_INLINE {
+        typedef short short4_t __attribute__((ext_vector_type(4)));
+        typedef __attribute__((address_space(3))) short4_t lds_short4_t;
+        const unsigned short* a = vs + v_lane + 16 * kb * kStride + 32 * dt;
+        const uint2_t lo = __builtin_bit_cast(uint2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4_t*)a));
+        const uint2_t hi = __builtin_bit_cast(
+            uint2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4_t*)(a + 8 * kStride)));
+        return uint4_t{lo[0], lo[1], hi[0], hi[1]};
+    };
+
+    float m, l;
+    float16_t o[D / 32];
+    // CAREFUL: a key that a column does not see has the probability 0 there, and 0 times an infinity or NaN of its
+    // V row is a NaN.  The first walk takes no notice; if its results are not all finite, a second one takes
+    // a pass of its own for every number of keys that a column of the wave sees in a tile.
+    auto walk = [&](auto careful_c) LG_INLINE {
+        constexpr bool CAREFUL = decltype(careful_c)::value != 0;
+        m = -INFINITY;
+        l = 0.0f;
+#pragma unroll
+        for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[dt][e] = 0.0f;
+        for (int key0 = 0; key0 < visible; key0 += kApKeys) {
+            __syncthreads();
+            for (int i = tid; i < kApKeys * kPieces; i += 64 * WAVES) {
+                const int key = i / kPieces, piece = i - key * kPieces;
+                // (past the last visible key that key again: its probability is 0 for everybody who sees less)
+                const int64_t row = key0 + key < visible ? key0 + key : visible - 1;
+                *reinterpret_cast<uint4_t*>(ks + key * kStride + 8 * piece) =
+                    *reinterpret_cast<const uint4_t*>(kp + row * p.k_stride + 8 * piece);
+                *reinterpret_cast<uint4_t*>(vs + key * kStride + 8 * piece) =
+                    *reinterpret_cast<const uint4_t*>(vp + row * p.v_stride + 8 * piece);
+            }
+            __syncthreads();
+            float16_t sc;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) sc[e] = 0.0f;
+#pragma unroll
+            for (int j = 0; j < D / 16; ++j)
+                sc = T::mfma32(*reinterpret_cast<const uint4_t*>(ks + col * kStride + 16 * j + 8 * h), qb[j], sc);
+            float tm = -INFINITY;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                sc[e] = key0 + 8 * (e >> 2) + 4 * h + (e & 3) < vis ? sc[e] : -INFINITY;
+                tm = fmaxf(tm, sc[e]);
+            }
+            tm = fmaxf(tm, lane_xor_f32<32>(tm)) * p.scale_log2e;
+            const float m_new = fmaxf(m, tm);
+            const float ref = m_new == -INFINITY ? 0.0f : m_new;
+            const float alpha = fast_exp2(m - ref);
+            m = m_new;
+            l *= alpha;
+#pragma unroll
+            for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[dt][e] *= alpha;
+            uint4_t pb[2];
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) {
+                const float p0 = fast_exp2(fmaf(sc[e], p.scale_log2e, -ref));
+                const float p1 = fast_exp2(fmaf(sc[e + 1], p.scale_log2e, -ref));
+                l += p0 + p1;
+                pb[e >> 3][(e & 7) >> 1] = T::pack2(p0, p1);
+            }
+            if (!CAREFUL || key0 + kApKeys <= first_vis) {
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                    for (int dt = 0; dt < D / 32; ++dt) o[dt] = T::mfma32(v_operand(kb, dt), pb[kb], o[dt]);
+            } else {
+                for (int seen = first_vis; seen <= last_vis; ++seen) {
+                    const int keys = seen - key0 - 4 * h;
+#pragma unroll
+                    for (int dt = 0; dt < D / 32; ++dt) {
+                        float16_t acc = o[dt];
+#pragma unroll
+                        for (int kb = 0; kb < 2; ++kb) {
+                            uint4_t v = v_operand(kb, dt);
+#pragma unroll
+                            for (int w = 0; w < 4; ++w) {
+                                const int at = 16 * kb + 2 * w + (w > 1 ? 4 : 0);  // (and 4 h: its first key)
+                                v[w] &= keys >= at + 2 ? ~0u : keys == at + 1 ? 0xffffu : 0u;
+                            }
+                            acc = T::mfma32(v, pb[kb], acc);
+                        }
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) o[dt][e] = vis == seen ? acc[e] : o[dt][e];
+                    }
+                }
+            }
+        }
+        l += lane_xor_f32<32>(l);
+    };
+    walk(ic<0>{});
+    {
+        float odd = 0.0f;  // NaN if a result is not finite
+#pragma unroll
+        for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) odd = fmaf(o[dt][e], 0.0f, odd);
+        const bool any = __builtin_amdgcn_ballot_w64(odd != odd) != 0;
+        if (lane == 0) odd_waves[wave] = any;
+        __syncthreads();
+        unsigned all = 0;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) all |= odd_waves[w];
+        if (__builtin_amdgcn_readfirstlane(all) != 0) walk(ic<1>{});
+    }
+    if (!live) return;
+    const float inv = l > 0.0f ? 1.0f / l : l == l ? 0.0f : l;  // (only keys that score -inf: zeros)
+    unsigned short* out = p.out + (int64_t)(t.row0 + tok) * p.out_stride + (int64_t)head * D + 4 * h;
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+            *reinterpret_cast<uint2_t*>(out + 32 * dt + 8 * b) =
+                uint2_t{T::pack2(o[dt][4 * b] * inv, o[dt][4 * b + 1] * inv),
+                        T::pack2(o[dt][4 * b + 2] * inv, o[dt][4 * b + 3] * inv)};
+}
+
+template <typename T, int D>
+static hipError_t attn_packed_launch(const AttnPackedParams& p, hipStream_t stream) {
+    constexpr int kWaves = 4;
+    const int64_t tiles = packed_tiles(p.total, p.num_seqs, p.g, 32 * kWaves);
+    attn_packed_kernel<T, D, kWaves><<<(unsigned)(tiles * p.hkv), 64 * kWaves, 0, stream>>>(p);
+    return hipGetLastError();
+}
+
+template <typename T>
+static hipError_t attn_packed_by_width(const AttnPackedParams& p, int d, hipStream_t stream) {
+    switch (d) {
+        case 32: return attn_packed_launch<T, 32>(p, stream);
+        case 64: return attn_packed_launch<T, 64>(p, stream);
+        case 96: return attn_packed_launch<T, 96>(p, stream);
+        case 128: return attn_packed_launch<T, 128>(p, stream);
+        case 160: return attn_packed_launch<T, 160>(p, stream);
+        case 192: return attn_packed_launch<T, 192>(p, stream);
+        case 224: return attn_packed_launch<T, 224>(p, stream);
+        default: return attn_packed_launch<T, 256>(p, stream);
+    }
+}
+
+static logismos_status_t attn_packed(bool bf16, const void* q, const void* k, const void* v, const int32_t* cu,
+                                     void* out, int num_seqs, int total, int hq, int hkv, int d, int q_stride,
+                                     int k_stride, int v_stride, int out_stride, float scale, int causal,
+                                     logismos_stream_t stream) {
+    const logismos_status_t bad = static_cast<logismos_status_t>(hipErrorInvalidValue);
+    if (logismos_check_attn_packed_shape(num_seqs, total, hq, hkv, d, q_stride, k_stride, v_stride, out_stride,
+                                         nullptr, 0) != 0)
+        return bad;
+    if (!q || !k || !v || !cu || !out || !(scale > 0.0f) || !isfinite(scale)) return bad;
+    if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) |
+         reinterpret_cast<uintptr_t>(out)) % 16 != 0 ||
+        reinterpret_cast<uintptr_t>(cu) % 4 != 0)
+        return bad;
+    AttnPackedParams p = {};
+    p.q = static_cast<const unsigned short*>(q);
+    p.k = static_cast<const unsigned short*>(k);
+    p.v = static_cast<const unsigned short*>(v);
+    p.cu = cu;
+    p.out = static_cast<unsigned short*>(out);
+    p.num_seqs = num_seqs;
+    p.total = total;
+    p.hkv = hkv;
+    p.g = hq / hkv;
+    p.q_stride = q_stride;
+    p.k_stride = k_stride;
+    p.v_stride = v_stride;
+    p.out_stride = out_stride;
+    p.scale_log2e = scale * 1.4426950408889634f;
+    p.causal = causal != 0;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    return static_cast<logismos_status_t>(bf16 ? attn_packed_by_width<PackedBf16>(p, d, st)
+                                               : attn_packed_by_width<PackedF16>(p, d, st));
+}
+
+}  // namespace lg
+
+extern "C" {
+
+logismos_status_t logismos_check_attn_packed_shape(int num_seqs, int total_tokens, int num_q_heads, int num_kv_heads,
+                                                   int head_dim, int q_stride, int k_stride, int v_stride,
+                                                   int out_stride, char* msg, size_t cap) {
+    using lg::reject;
+    if (num_seqs <= 0 || total_tokens <= 0) return reject(msg, cap, "num_seqs and total_tokens must be positive (%d, %d)", num_seqs, total_tokens);
+    if (num_q_heads <= 0 || num_kv_heads <= 0)
+        return reject(msg, cap, "num_q_heads and num_kv_heads must be positive (%d, %d)", num_q_heads, num_kv_heads);
+    if (num_q_heads % num_kv_heads != 0)
+        return reject(msg, cap, "num_q_heads %d is not a multiple of num_kv_heads %d", num_q_heads, num_kv_heads);
+    if (head_dim <= 0 || head_dim % 32 != 0 || head_dim > 256)
+        return reject(msg, cap, "head_dim must be a multiple of 32 up to 256 (%d)", head_dim);
+    if ((int64_t)total_tokens + num_seqs > lg::kPackedMaxRows)
+        return reject(msg, cap, "total_tokens + num_seqs exceeds %d", lg::kPackedMaxRows);
+    if (((int64_t)total_tokens + num_seqs) * num_q_heads > (1 << 28))
+        return reject(msg, cap, "(total_tokens + num_seqs) * num_q_heads exceeds %d", 1 << 28);
+    const int64_t qw = (int64_t)num_q_heads * head_dim, kw = (int64_t)num_kv_heads * head_dim;
+    if (q_stride < qw || out_stride < qw || k_stride < kw || v_stride < kw)
+        return reject(msg, cap, "a stride is smaller than its row (%d and %d of %lld, %d and %d of %lld)", q_stride,
+                      out_stride, (long long)qw, k_stride, v_stride, (long long)kw);
+    if ((q_stride | k_stride | v_stride | out_stride) % 8 != 0)
+        return reject(msg, cap, "strides must be multiples of 8 (%d, %d, %d, %d)", q_stride, k_stride, v_stride,
+                      out_stride);
+    if (k_stride > (1 << 22) || v_stride > (1 << 22))
+        return reject(msg, cap, "k and v strides must be at most %d (%d, %d)", 1 << 22, k_stride, v_stride);
+    return 0;
+}
+
+#define LOGISMOS_ATTN_PACKED(name, bf16)                                                                              \
+    logismos_status_t logismos_launch_attn_packed_##name(                                                             \
+        const void* q, const void* k, const void* v, const int32_t* cu_seqlens, void* out, int num_seqs,              \
+        int total_tokens, int num_q_heads, int num_kv_heads, int head_dim, int q_stride, int k_stride, int v_stride,  \
+        int out_stride, float scale, int causal, logismos_stream_t stream) {                                          \
+        return lg::attn_packed(bf16, q, k, v, cu_seqlens, out, num_seqs, total_tokens, num_q_heads, num_kv_heads,     \
+                               head_dim, q_stride, k_stride, v_stride, out_stride, scale, causal, stream);            \
+    }
+LOGISMOS_ATTN_PACKED(fp16, false)
+LOGISMOS_ATTN_PACKED(bf16, true)
+#undef LOGISMOS_ATTN_PACKED
+
+}  // extern "C"

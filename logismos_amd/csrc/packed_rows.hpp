@@ -1,0 +1,91 @@
+// What the operators over packed rows share (attention, rotary positions, adapters): the 16-bit
+// element types with their matrix instructions, and the way from a workgroup to the rows it takes.
+#pragma once
+
+#include "device_utils.hpp"
+
+namespace lg {
+
+typedef __bf16 bf16x4_t __attribute__((ext_vector_type(4)));
+
+// Element types: vectors of eight (a matrix operand), two values packed into a word (rounded to
+// nearest even, one v_cvt_pk each), the matrix instructions with their fp32 sums.
+struct PackedF16 {
+    typedef _Float16 elem;
+    typedef half8_t vec8;
+    static __device__ __forceinline__ unsigned pack2(float a, float b) {
+        return __builtin_bit_cast(unsigned, half2_t{(_Float16)a, (_Float16)b});
+    }
+    static __device__ __forceinline__ float16_t mfma32(uint4_t a, uint4_t b, float16_t c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, a),
+                                                      __builtin_bit_cast(half8_t, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ float4_t mfma16(uint4_t a, uint4_t b, float4_t c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, a),
+                                                      __builtin_bit_cast(half8_t, b), c, 0, 0, 0);
+    }
+};
+struct PackedBf16 {
+    typedef __bf16 elem;
+    typedef bf16x8_t vec8;
+    static __device__ __forceinline__ unsigned pack2(float a, float b) {
+        return __builtin_bit_cast(unsigned, bf16x2_t{(__bf16)a, (__bf16)b});
+    }
+    static __device__ __forceinline__ float16_t mfma32(uint4_t a, uint4_t b, float16_t c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a),
+                                                       __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ float4_t mfma16(uint4_t a, uint4_t b, float4_t c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a),
+                                                       __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+    }
+};
+
+constexpr int kPackedMaxRows = 1 << 24;  // rows and sequences of a launch
+
+// Packed sequences in tiles of `tile` units (a row is `per_row` units).  Only the device knows the
+// lengths, so a launch has packed_tiles() workgroups, the most that can be needed, and sequence s
+// owns those from floor(cu[s] * per_row / tile) + s on: ceil(b - a) <= floor(b) - floor(a) + 1, so the
+// ranges never overlap, and at most one workgroup per sequence finds nothing to do.
+inline int64_t packed_tiles(int64_t rows, int num_seqs, int64_t per_row, int64_t tile) {
+    return rows * per_row / tile + num_seqs;
+}
+
+struct PackedTile {
+    int seq;
+    int row0;  // first row of the sequence
+    int rows;  // its rows (0: nothing to do)
+    int tile;  // which of its tiles
+};
+
+// The sequence of workgroup `b` and its tile: 64 candidates per round, by the whole wave.  Whatever
+// the lengths hold, rows lie in [0, total).
+__device__ __forceinline__ PackedTile packed_tile(const int32_t* __restrict__ cu, int num_seqs,
+                                                  int total, int per_row, int tile, int b) {
+    const int lane = threadIdx.x & 63;
+    auto start = [&](int s) LG_INLINE {
+        return (int)((unsigned)cu[s] * (unsigned)per_row / (unsigned)tile) + s;
+    };
+    int lo = 0, n = num_seqs;
+    while (n > 1) {
+        const int step = (n + 63) / 64;
+        const int at = lane * step;
+        const bool in = at < n && start(lo + (at < n ? at : 0)) <= b;
+        const int count = __builtin_popcountll(__builtin_amdgcn_ballot_w64(in));
+        const int skip = (count > 0 ? count - 1 : 0) * step;
+        lo += skip;
+        n = n - skip < step ? n - skip : step;
+    }
+    lo = __builtin_amdgcn_readfirstlane(lo);
+    PackedTile t;
+    t.seq = lo;
+    const int r0 = __builtin_amdgcn_readfirstlane(cu[lo]);
+    const int r1 = __builtin_amdgcn_readfirstlane(cu[lo + 1]);
+    t.row0 = r0;
+    t.rows = r0 >= 0 && r0 < total ? (r1 < total ? r1 : total) - r0 : 0;
+    t.tile = b - __builtin_amdgcn_readfirstlane(start(lo));
+    if (t.tile < 0) t.rows = 0;
+    return t;
+}
+
+}  // namespace lg

@@ -9,6 +9,8 @@ from __future__ import annotations
 import ctypes as C
 import os
 
+import numpy as np
+
 from . import hip
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -39,7 +41,7 @@ class LaunchError(RuntimeError):
         super().__init__(f"kernel {kernel}: launch failed: {self.kind} (code {self.code})")
 
 
-_vp, _i, _f, _sz = C.c_void_p, C.c_int, C.c_float, C.c_size_t
+_vp, _i, _f, _d, _sz = C.c_void_p, C.c_int, C.c_float, C.c_double, C.c_size_t
 
 _SIGNATURES = {
     "logismos_decode_abi_version": (C.c_int, []),
@@ -95,6 +97,19 @@ _SIGNATURES = {
     "logismos_launch_silu_mul_bf16": (C.c_uint32, [_vp, _vp, _i, _i, _vp]),
     "logismos_launch_cast_f16_bf16": (C.c_uint32, [_vp, _vp, _sz, _vp]),
     "logismos_launch_greedy_f32": (C.c_uint32, [_vp, _vp, _i, _i, _vp]),
+    "logismos_check_rope_packed_shape": (C.c_uint32, [_i] * 9 + [C.c_char_p, _sz]),
+    "logismos_launch_rope_packed_fp16": (C.c_uint32, [_vp] * 6 + [_i] * 9 + [_f, _i, _vp]),
+    "logismos_launch_rope_packed_bf16": (C.c_uint32, [_vp] * 6 + [_i] * 9 + [_f, _i, _vp]),
+    "logismos_launch_rope_packed_f32": (C.c_uint32, [_vp] * 6 + [_i] * 9 + [_f, _i, _vp]),
+    "logismos_rope_frequencies":
+        (C.c_uint32, [_vp, C.POINTER(_f), _i, _d, _i, _d, _i, _d, _d]),
+    "logismos_check_attn_packed_shape": (C.c_uint32, [_i] * 9 + [C.c_char_p, _sz]),
+    "logismos_launch_attn_packed_fp16": (C.c_uint32, [_vp] * 5 + [_i] * 9 + [_f, _i, _vp]),
+    "logismos_launch_attn_packed_bf16": (C.c_uint32, [_vp] * 5 + [_i] * 9 + [_f, _i, _vp]),
+    "logismos_check_adapter_add_shape": (C.c_uint32, [_i] * 9 + [C.c_char_p, _sz]),
+    "logismos_adapter_add_workspace_bytes": (_sz, [_i, _i]),
+    "logismos_launch_adapter_add_fp16": (C.c_uint32, [_vp] * 9 + [_i, _vp] + [_i] * 9 + [_vp]),
+    "logismos_launch_adapter_add_bf16": (C.c_uint32, [_vp] * 9 + [_i, _vp] + [_i] * 9 + [_vp]),
     "logismos_launch_rms_norm_fp16": (C.c_uint32, [_vp, _vp, _vp, _i, _i, _f, _vp]),
     "logismos_launch_softmax_fp16": (C.c_uint32, [_vp, _vp, _i, _i, _vp]),
     "logismos_launch_mask_additive_f32": (C.c_uint32, [_vp, _vp, _sz, _sz, _sz, _vp]),
@@ -546,6 +561,86 @@ def launch_cast_f16_bf16(src, dst, count: int, stream=None) -> None:
 def launch_greedy_f32(logits, out, rows: int, n: int, stream=None) -> None:
     _status("greedy_f32", library().logismos_launch_greedy_f32(
         _ptr(logits), _ptr(out), rows, n, _raw(stream)))
+
+
+# ---- operators over packed rows
+
+_ROPE_SCALES = {"none": 0, "linear": 1, "base": 2, "parts": 3}
+
+
+def rope_frequencies(rotary_dim: int, base: float, scaling: str = "none", factor: float = 1.0,
+                     original_positions: int = 0, turns_fast: float = 32.0,
+                     turns_slow: float = 1.0) -> tuple[np.ndarray, float]:
+    """Radians per position of every pair (float64 [rotary_dim / 2], for the device) and the amplitude."""
+    if scaling not in _ROPE_SCALES:
+        raise ValueError(f"scaling must be one of {', '.join(_ROPE_SCALES)}, not {scaling!r}")
+    out = np.empty(max(rotary_dim, 0) // 2, np.float64)
+    amplitude = _f(0.0)
+    if library().logismos_rope_frequencies(
+            out.ctypes.data_as(_vp), C.byref(amplitude), rotary_dim, float(base),
+            _ROPE_SCALES[scaling], float(factor), original_positions, float(turns_fast),
+            float(turns_slow)) != 0:
+        raise UnsupportedShape("rope_frequencies", "rotary_dim, base or the scaling's numbers are "
+                               "out of range")
+    return out, amplitude.value
+
+
+def launch_rope_packed(q_in, k_in, q_out, k_out, positions, inv_freq, tokens: int,
+                       num_q_heads: int, num_kv_heads: int, head_dim: int, rotary_dim: int,
+                       interleaved: bool = False, amplitude: float = 1.0, q_in_stride=None,
+                       k_in_stride=None, q_out_stride=None, k_out_stride=None,
+                       dtype: str = "fp16", stream=None) -> None:
+    """Rotary positions of packed rows; `dtype` fp16, bf16 or f32; strides in elements, None:
+    rows one behind the other.  k_in and k_out may be None with num_kv_heads == 0."""
+    if dtype not in ("fp16", "bf16", "f32"):
+        raise ValueError(f"dtype must be fp16, bf16 or f32, not {dtype!r}")
+    name = f"rope_packed_{dtype}"
+    qw, kw = num_q_heads * head_dim, num_kv_heads * head_dim
+    strides = [w if s is None else s for s, w in ((q_in_stride, qw), (k_in_stride, kw),
+                                                  (q_out_stride, qw), (k_out_stride, kw))]
+    _guard(name, library().logismos_check_rope_packed_shape, tokens, num_q_heads, num_kv_heads,
+           head_dim, rotary_dim, *strides)
+    _status(name, getattr(library(), f"logismos_launch_{name}")(
+        _ptr(q_in), _ptr(k_in), _ptr(q_out), _ptr(k_out), _ptr(positions), _ptr(inv_freq), tokens,
+        num_q_heads, num_kv_heads, head_dim, rotary_dim, *strides, float(amplitude),
+        1 if interleaved else 0, _raw(stream)))
+
+
+def launch_attn_packed(q, k, v, cu_seqlens, out, num_seqs: int, total_tokens: int,
+                       num_q_heads: int, num_kv_heads: int, head_dim: int, scale: float,
+                       causal: bool = True, q_stride=None, k_stride=None, v_stride=None,
+                       out_stride=None, bf16: bool = False, stream=None) -> None:
+    """Attention of whole packed sequences; strides in elements, None: rows one behind the other."""
+    name = "attn_packed_bf16" if bf16 else "attn_packed_fp16"
+    qw, kw = num_q_heads * head_dim, num_kv_heads * head_dim
+    strides = [w if s is None else s for s, w in ((q_stride, qw), (k_stride, kw), (v_stride, kw),
+                                                  (out_stride, qw))]
+    _guard(name, library().logismos_check_attn_packed_shape, num_seqs, total_tokens, num_q_heads,
+           num_kv_heads, head_dim, *strides)
+    _status(name, getattr(library(), f"logismos_launch_{name}")(
+        _ptr(q), _ptr(k), _ptr(v), _ptr(cu_seqlens), _ptr(out), num_seqs, total_tokens,
+        num_q_heads, num_kv_heads, head_dim, *strides, float(scale), 1 if causal else 0,
+        _raw(stream)))
+
+
+def adapter_add_workspace_bytes(total_tokens: int, max_rank: int) -> int:
+    return library().logismos_adapter_add_workspace_bytes(total_tokens, max_rank)
+
+
+def launch_adapter_add(x, a, b, ranks, scales, adapter_of_seq, cu_seqlens, base, out, workspace,
+                       num_seqs: int, total_tokens: int, num_adapters: int, max_rank: int, n: int,
+                       k: int, x_stride=None, base_stride=None, out_stride=None,
+                       bf16: bool = False, f32_out: bool = False, stream=None) -> None:
+    """`out = base + scale * (x A^T) B^T` with each sequence's adapter; strides in elements, None:
+    rows one behind the other; base and out may be the same."""
+    name = "adapter_add_bf16" if bf16 else "adapter_add_fp16"
+    strides = [w if s is None else s for s, w in ((x_stride, k), (base_stride, n), (out_stride, n))]
+    _guard(name, library().logismos_check_adapter_add_shape, num_seqs, total_tokens, num_adapters,
+           max_rank, n, k, *strides)
+    _status(name, getattr(library(), f"logismos_launch_{name}")(
+        _ptr(x), _ptr(a), _ptr(b), _ptr(ranks), _ptr(scales), _ptr(adapter_of_seq),
+        _ptr(cu_seqlens), _ptr(base), _ptr(out), 1 if f32_out else 0, _ptr(workspace), num_seqs,
+        total_tokens, num_adapters, max_rank, n, k, *strides, _raw(stream)))
 
 
 # ---- the reference's existing launchers (same names as its Rust wrappers,

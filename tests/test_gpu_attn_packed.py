@@ -1,0 +1,246 @@
+"""Attention of whole packed sequences against the 64-bit form, element by element within the bound
+that the documented roundings add up to."""
+import numpy as np
+import pytest
+
+from logismos_amd import hip, kernels
+from tests import packed_reference as R
+
+pytestmark = pytest.mark.gpu
+
+GUARD = 3  # rows behind the last sequence
+
+
+def _case(seed, lens, hq, hkv, d, dtype, fused=False, size=1.0):
+    rng = np.random.default_rng(seed)
+    T = int(sum(lens)) + GUARD
+    width = (hq + 2 * hkv) * d
+    rows = R.to_bits(rng.standard_normal((T, width), np.float32) * np.float32(size), dtype)
+    return dict(rows=rows, lens=list(lens), hq=hq, hkv=hkv, d=d, dtype=dtype, fused=fused, T=T)
+
+
+def _parts(c):
+    a, b = c["hq"] * c["d"], c["hkv"] * c["d"]
+    r = c["rows"]
+    return r[:, :a], r[:, a:a + b], r[:, a + b:]
+
+
+class Run:
+    def __init__(self, c, causal, scale=None, stream=None, out_pad=0):
+        self.c, self.causal, self.stream = c, causal, stream
+        self.scale = scale or 1.0 / np.sqrt(c["d"])
+        q, k, v = _parts(c)
+        self.qw, self.out_stride = q.shape[1], q.shape[1] + out_pad
+        if c["fused"]:
+            self.rows = hip.DeviceBuffer.from_numpy(c["rows"])
+            at = [self.rows.offset(2 * x) for x in (0, q.shape[1], q.shape[1] + k.shape[1])]
+            self.strides = [c["rows"].shape[1]] * 3
+        else:
+            self.rows = [hip.DeviceBuffer.from_numpy(x) for x in (q, k, v)]
+            at, self.strides = self.rows, [q.shape[1], k.shape[1], v.shape[1]]
+        self.at = at
+        self.cu = hip.DeviceBuffer.from_numpy(np.concatenate([[0], np.cumsum(c["lens"])]).astype(np.int32))
+        self.out = hip.DeviceBuffer(c["T"] * self.out_stride * 2)
+        self.out.fill(0xFF)
+
+    def launch(self):
+        c = self.c
+        kernels.launch_attn_packed(*self.at, self.cu, self.out, len(c["lens"]), c["T"], c["hq"],
+                                   c["hkv"], c["d"], self.scale, self.causal, *self.strides,
+                                   self.out_stride, bf16=c["dtype"] == "bf16", stream=self.stream)
+
+    def bits(self):
+        (self.stream.synchronize() if self.stream else hip.synchronize())
+        return self.out.to_numpy(np.uint16, (self.c["T"], self.out_stride))
+
+    def result(self):
+        """The rows of the sequences in 64 bits; what lies behind and beside them is as it was."""
+        got = self.bits()
+        n = sum(self.c["lens"])
+        assert (got[n:] == 0xFFFF).all() and (got[:, self.qw:] == 0xFFFF).all()
+        got = got[:n, :self.qw]
+        got = got.view(np.float16) if self.c["dtype"] == "fp16" else got
+        return R.from_bits(np.ascontiguousarray(got), self.c["dtype"])
+
+
+def _want(c, causal, scale=None):
+    n = sum(c["lens"])
+    q, k, v = (R.from_bits(np.ascontiguousarray(x[:n]), c["dtype"]).reshape(n, -1, c["d"])
+               for x in _parts(c))
+    o, bound = R.attention(q, k, v, c["lens"], scale or 1.0 / np.sqrt(c["d"]), causal, c["dtype"])
+    return o.reshape(n, -1), bound.reshape(n, -1)
+
+
+def _check(c, causal, scale=None, **kw):
+    r = Run(c, causal, scale, **kw)
+    r.launch()
+    R.assert_within(r.result(), *_want(c, causal, scale),
+                    what=f"{c['lens']} {c['hq']}/{c['hkv']} x {c['d']} {c['dtype']} causal={causal}")
+    return r
+
+
+LENGTHS = [[1], [2, 1, 1], [1, 0, 5, 33], [31, 32, 33, 64, 65], [0, 0, 7, 0], [127, 128, 129],
+           [300, 1, 17]]
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("lens", LENGTHS, ids=str)
+@pytest.mark.parametrize("hq,hkv,d", [(4, 4, 64), (14, 2, 64), (12, 2, 128), (8, 1, 128)])
+def test_lengths(lens, hq, hkv, d, causal, dtype):
+    _check(_case(1, lens, hq, hkv, d, dtype), causal)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("d", [32, 64, 96, 128, 160, 192, 224, 256])
+def test_widths(d, causal, dtype):
+    _check(_case(2, [70, 3, 200, 40], 6, 2, d, dtype), causal)
+
+
+@pytest.mark.parametrize("hq,hkv", [(1, 1), (3, 1), (5, 5), (9, 3), (32, 1), (40, 1), (7, 7), (48, 16)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_groups(hq, hkv, d):
+    _check(_case(3, [1, 50, 97], hq, hkv, d, "fp16"), True)
+    _check(_case(4, [1, 50, 97], hq, hkv, d, "bf16"), False)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("hq,hkv,d", [(14, 2, 64), (12, 2, 128), (4, 2, 96), (4, 2, 256)])
+def test_columns_of_fused_rows(hq, hkv, d, dtype):
+    c = _case(5, [129, 1, 64, 31], hq, hkv, d, dtype, fused=True)
+    _check(c, True, out_pad=8)
+    _check(c, False)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_many_key_tiles(d, causal, dtype):
+    _check(_case(6, [1500, 777], 2, 1, d, dtype), causal)
+
+
+@pytest.mark.parametrize("hq,hkv,d,lens", [(16, 2, 128, [900, 1100, 650]), (16, 4, 64, [2100, 333]),
+                                           (8, 1, 128, [2600]), (16, 16, 64, [600] * 3)])
+def test_many_workgroups(hq, hkv, d, lens):
+    _check(_case(16, lens, hq, hkv, d, "bf16", fused=True), True)
+
+
+def test_many_short_sequences():
+    rng = np.random.default_rng(7)
+    _check(_case(7, rng.integers(0, 5, 700), 4, 2, 64, "bf16"), True)
+    _check(_case(8, rng.integers(0, 40, 130), 4, 2, 128, "fp16"), False)
+
+
+@pytest.mark.parametrize("d", [64, 128, 192])
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_large_scores(d, dtype):
+    """Scores up to some hundreds: the running maximum rises by much, often and late."""
+    c = _case(9, [260, 90], 4, 2, d, dtype, size=4.0)
+    _check(c, True)
+    # rising and falling along the keys
+    q, k, _ = _parts(c)
+    order = np.linspace(0.05, 3.0, c["T"])[:, None]
+    k[:] = R.to_bits(R.from_bits(np.ascontiguousarray(k), dtype) * order, dtype)
+    _check(c, False)
+    k[:] = k[::-1].copy()
+    _check(c, True)
+
+
+@pytest.mark.parametrize("scale", [1e-4, 1.0])
+def test_scales(scale):
+    _check(_case(10, [100, 60], 4, 2, 128, "fp16"), True, scale)
+    _check(_case(10, [100, 60], 4, 2, 64, "bf16"), False, scale)
+
+
+def _nan(dtype):
+    return np.float16(np.nan) if dtype == "fp16" else np.uint16(0x7FC0)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("d", [64, 96, 128, 256])
+@pytest.mark.parametrize("n,bad", [(70, 33), (70, 69), (40, 1), (300, 200), (300, 129)])
+def test_what_later_keys_hold_does_not_reach_a_token(d, n, bad, dtype):
+    """NaN in the K and V rows of token `bad` and in everything of the sequence behind: tokens in
+    front of it keep their results, those that see it are NaN."""
+    c = _case(11, [n, 50], 6, 2, d, dtype)
+    want, bound = _want(c, True)
+    q, k, v = _parts(c)
+    q, k, v = q.copy(), k.copy(), v.copy()
+    k[bad], v[bad] = _nan(dtype), _nan(dtype)
+    k[n:n + 50], v[n:n + 50], q[n:n + 50] = _nan(dtype), _nan(dtype), _nan(dtype)
+    c["rows"] = np.concatenate([q, k, v], 1)
+    r = Run(c, True)
+    r.launch()
+    got = r.result()
+    R.assert_within(got[:bad], want[:bad], bound[:bad])
+    assert np.isnan(got[bad:]).all()
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("d", [64, 128])
+def test_infinite_values_of_later_keys(d, dtype):
+    c = _case(12, [90], 4, 4, d, dtype)
+    want, bound = _want(c, True)
+    _, _, v = _parts(c)
+    v[45] = np.float16(np.inf) if dtype == "fp16" else np.uint16(0x7F80)
+    r = Run(c, True)
+    r.launch()
+    got = r.result()
+    R.assert_within(got[:45], want[:45], bound[:45])
+    assert np.isposinf(got[45:]).all()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_keys_that_all_score_minus_infinity_give_zeros(d):
+    c = _case(13, [40, 3], 2, 2, d, "bf16")
+    q, k, _ = _parts(c)
+    q[:] = np.uint16(0x3F80)  # 1
+    k[:5] = np.uint16(0xFF80)  # -inf
+    r = Run(c, True)
+    r.launch()
+    got = r.result()
+    assert (got[:5] == 0).all() and np.isfinite(got).all()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_lengths_past_the_rows_are_cut(d):
+    """cu_seqlens that names more rows than there are: those that are there count."""
+    c = _case(14, [20, 30], 4, 2, d, "fp16")
+    r = Run(c, True)
+    cu = np.array([0, 20, 5000], np.int32)
+    r.cu.copy_from_host(cu)
+    r.launch()
+    c2 = dict(c, lens=[20, 30 + GUARD])
+    got = R.from_bits(r.bits().view(np.float16), "fp16")
+    R.assert_within(got, *_want(c2, True))
+
+
+def test_a_captured_call_replays():
+    stream = hip.Stream()
+    c = _case(15, [129, 40, 1], 4, 2, 128, "bf16")
+    r = Run(c, True, stream=stream)
+    r.launch()
+    want = r.bits().copy()
+    r.out.fill(0xFF)
+    hip.synchronize()
+    graph = hip.Graph(stream)
+    with graph:
+        r.launch()
+    for _ in range(3):
+        r.out.fill(0xFF)
+        hip.synchronize()
+        graph.launch()
+        assert np.array_equal(r.bits(), want)
+        r.launch()
+        assert np.array_equal(r.bits(), want)
+
+
+def test_two_streams_at_once():
+    runs = [Run(_case(20 + i, [200 + i, 77], 8, 2, 64, "fp16"), True, stream=hip.Stream())
+            for i in range(2)]
+    for _ in range(4):
+        for r in runs:
+            r.launch()
+    for r in runs:
+        R.assert_within(r.result(), *_want(r.c, True))
