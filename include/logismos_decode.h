@@ -613,7 +613,7 @@ logismos_status_t logismos_launch_embed_lookup_bf16(const void* table_bf16, cons
  * A batch is `total_tokens` rows, the tokens of sequence s in rows [cu_seqlens[s], cu_seqlens[s+1])
  * (int32 `[num_seqs + 1]`, non-decreasing, starting at or behind 0; empty sequences are allowed).  Rows
  * behind the last sequence are neither read nor written.  A stride is the distance of two rows in elements, so that q, k
- * and v may be columns of one fused projection.  At most 2^24 rows and sequences together.  A call needs
+ * and v may be columns of one fused projection.  At most 2^23 rows and sequences together.  A call needs
  * nothing but its arguments, allocates nothing and can be captured into a graph; it runs on the device that is current. */
 
 /* Rotary positions of q and k heads (`rope_apply`, crates/kernels/src/rope/cpu.rs:56-127, and
@@ -684,8 +684,8 @@ logismos_status_t logismos_rope_frequencies(double* inv_freq, float* amplitude, 
  * fp32 scores, softmax and sums; the probabilities are rounded to the rows' type for the second product.  Elements of
  * keys that a token does not see do not reach its result, whatever they hold; a token whose keys all score
  * -inf gives zeros.  scale finite and > 0 (else hipErrorInvalidValue); head_dim a multiple of 32 up to 256; num_q_heads a
- * multiple of num_kv_heads; k and v strides up to 2^22; (total_tokens + num_seqs) * num_q_heads up to
- * 2^28.  out does not overlap q, k or v. */
+ * multiple of num_kv_heads; k and v strides up to 2^22; total_tokens * num_q_heads / 128 +
+ * num_seqs * num_kv_heads up to 2^22.  out does not overlap q, k or v. */
 logismos_status_t logismos_check_attn_packed_shape(int num_seqs, int total_tokens, int num_q_heads,
                                                    int num_kv_heads, int head_dim, int q_stride, int k_stride,
                                                    int v_stride, int out_stride, char* msg, size_t msg_cap);

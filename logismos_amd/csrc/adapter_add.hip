@@ -24,7 +24,6 @@
 
 namespace lg {
 
-constexpr int kAdapterRows = 16;      // rows of a tile
 constexpr int kAdapterMaxRank = 256;
 constexpr int kAdapterMaxParts = 8;   // K parts of v
 
@@ -42,209 +41,321 @@ struct AdapterParams {
     int num_seqs, total, adapters, max_rank, n, k;
     int64_t x_stride, base_stride, out_stride;
     int parts, part_steps;  // K parts, steps of 32 columns of a part
+    int n_slice, slices;    // outputs of a workgroup, a multiple of 256; how many of them
 };
 
-// The rank that counts for sequence s; 0: no adapter.
-__device__ __forceinline__ int adapter_rank(const AdapterParams& p, int s, int* adapter) {
-    const int a = __builtin_amdgcn_readfirstlane(p.adapter_of_seq[s]);
-    *adapter = a;
-    if (a < 0 || a >= p.adapters) return 0;
-    const int r = __builtin_amdgcn_readfirstlane(p.ranks[a]);
+__device__ __forceinline__ int adapter_rank(const AdapterParams& p, int adapter) {
+    if (adapter < 0 || adapter >= p.adapters) return 0;
+    const int r = __builtin_amdgcn_readfirstlane(p.ranks[adapter]);
     return r < 0 ? 0 : r < p.max_rank ? r : p.max_rank;
 }
 
-// v[part][t][r] = sum over the part's columns of x[t][c] * A[r][c].  grid (tiles, K parts, 16 ranks each);
-// the four waves share the part's steps and add up in LDS.
-template <typename T>
+// v[part][t][r] = sum over the part's columns of x[t][c] * A[r][c].  grid (tiles of 16 MT rows by K parts, 16 RT ranks
+// each); the four waves share the part's steps of 32 columns and add up in LDS.
+template <typename T, int MT, int RT>
 __global__ __launch_bounds__(256) void adapter_down_kernel(const AdapterParams p) {
-    __shared__ float sums[4][256];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    constexpr int kDeep = MT > 1 ? 4 : 8;  // steps asked for together, side by side: whole cache lines
+    __shared__ float sums[4][MT * RT * 256];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c = lane & 15, q = lane >> 4;
-    const PackedTile t = packed_tile(p.cu, p.num_seqs, p.total, 1, kAdapterRows, blockIdx.x);
-    const int r0 = t.tile * kAdapterRows;
-    if (r0 >= t.rows) return;
-    int adapter;
-    const int rank = adapter_rank(p, t.seq, &adapter);
-    const int rank0 = blockIdx.z * 16;
-    if (rank0 >= rank) return;
-    const int row = r0 + c < t.rows ? r0 + c : t.rows - 1;
-    const unsigned short* x = p.x + (int64_t)(t.row0 + row) * p.x_stride;
-    const int ar = rank0 + c < rank ? rank0 + c : rank - 1;
-    const unsigned short* a = p.a + ((int64_t)adapter * p.max_rank + ar) * p.k;
-    const int first = blockIdx.y * p.part_steps;
-    const int all = (p.k + 31) / 32;
-    const int last = first + p.part_steps < all ? first + p.part_steps : all;
-    float4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int s = first + wave; s < last; s += 4) {
-        const int at = 32 * s + 8 * q;
-        uint4_t xv = {0, 0, 0, 0}, av = {0, 0, 0, 0};
-        if (at < p.k) {  // (k is a multiple of 8)
-            xv = *reinterpret_cast<const uint4_t*>(x + at);
-            av = *reinterpret_cast<const uint4_t*>(a + at);
-        }
-        acc = T::mfma16(av, xv, acc);
+    const int part = (int)(blockIdx.x % (unsigned)p.parts);
+    const PackedTile t = packed_tile<true>(p.cu, p.num_seqs, p.total, 1, 16 * MT, (int)(blockIdx.x / (unsigned)p.parts),
+                                           p.adapter_of_seq);
+    const int r0 = t.tile * 16 * MT;
+    if (r0 >= t.rows || t.of < 0 || t.of >= p.adapters) return;
+    const int rank0 = blockIdx.y * 16 * RT;
+    // (ranks of the first tile are not waited for: what lies behind the rank is left out when v is read)
+    if ((RT > 1 || rank0 > 0) && rank0 >= adapter_rank(p, t.of)) return;
+    const unsigned short* x[MT];
+    const unsigned short* a[RT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+        const int row = r0 + 16 * m + c < t.rows ? r0 + 16 * m + c : t.rows - 1;
+        x[m] = p.x + (int64_t)(t.row0 + row) * p.x_stride;
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) sums[wave][lane * 4 + i] = acc[i];
+    for (int i = 0; i < RT; ++i) {
+        const int r = rank0 + 16 * i + c < p.max_rank ? rank0 + 16 * i + c : p.max_rank - 1;
+        a[i] = p.a + ((int64_t)t.of * p.max_rank + r) * p.k;
+    }
+    const int all = (p.k + 31) / 32;
+    const int first = part * p.part_steps + wave * kDeep;
+    const int last = min((part + 1) * p.part_steps, all);
+    float4_t acc[MT][RT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int i = 0; i < RT; ++i) acc[m][i] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int s0 = first; s0 < last; s0 += 4 * kDeep) {
+        uint4_t xv[kDeep][MT], av[kDeep][RT];
+#pragma unroll
+        for (int d = 0; d < kDeep; ++d) {
+            const int at = 32 * (s0 + d) + 8 * q;
+            const bool in = s0 + d < last && at < p.k;  // (k is a multiple of 8)
+#pragma unroll
+            for (int m = 0; m < MT; ++m) xv[d][m] = in ? *reinterpret_cast<const uint4_t*>(x[m] + at) : uint4_t{0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < RT; ++i) av[d][i] = in ? *reinterpret_cast<const uint4_t*>(a[i] + at) : uint4_t{0, 0, 0, 0};
+        }
+#pragma unroll
+        for (int d = 0; d < kDeep; ++d)
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int i = 0; i < RT; ++i) acc[m][i] = T::mfma16(av[d][i], xv[d][m], acc[m][i]);
+    }
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+            *reinterpret_cast<float4_t*>(&sums[wave][((m * RT + i) * 64 + lane) * 4]) = acc[m][i];
     __syncthreads();
-    // thread (row, rank): the value of lane (rank / 4, row), element rank % 4
-    const int vr = threadIdx.x >> 4, rk = threadIdx.x & 15;
-    if (r0 + vr < t.rows && rank0 + rk < p.max_rank) {
-        const int i = ((rk >> 2) * 16 + vr) * 4 + (rk & 3);
-        const float sum = (sums[0][i] + sums[1][i]) + (sums[2][i] + sums[3][i]);
-        p.v[((int64_t)blockIdx.y * p.total + t.row0 + r0 + vr) * p.max_rank + rank0 + rk] = sum;
+    // four ranks of a row per thread and turn: what lane (q, c) holds of tile (m, i)
+    for (int e = threadIdx.x; e < MT * RT * 64; e += 256) {
+        const int tile = e >> 6, m = tile / RT, i = tile - m * RT;
+        const int row = r0 + 16 * m + (e & 15), rank = rank0 + 16 * i + 4 * ((e >> 4) & 3);
+        float4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) v += *reinterpret_cast<const float4_t*>(&sums[w][e * 4]);
+        if (row < t.rows && rank < p.max_rank)
+            *reinterpret_cast<float4_t*>(p.v + ((int64_t)part * p.total + t.row0 + row) * p.max_rank + rank) = v;
     }
 }
 
-// out = base + s (v . B^T): grid (tiles, 256 outputs each), a wave 64 of them.
-template <typename T, bool F32, int TERMS>
+// out = base + s (v . B^T).  grid: slices of the outputs (fastest: a slice of B then stays in the L2 of the XCDs that
+// take it, for all rows of its adapter) by tiles of 16 MT rows; ranks in RS steps of 32.  The workgroup splits v
+// into terms once, in the order of the matrix operand, into LDS; a wave keeps them in registers for all its outputs, 64
+// at a time, the four waves side by side.
+template <typename T, bool F32, int TERMS, int MT, int RS>
 __global__ __launch_bounds__(256) void adapter_up_kernel(const AdapterParams p) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    constexpr int kRows = 16 * MT, kChunks = 4 * RS;  // chunks of eight ranks
+    __shared__ uint4_t operand[MT * RS * TERMS * 64];
+    __shared__ float growth[kRows];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c = lane & 15, q = lane >> 4;
-    const PackedTile t = packed_tile(p.cu, p.num_seqs, p.total, 1, kAdapterRows, blockIdx.x);
-    const int r0 = t.tile * kAdapterRows;
+    const int slice = (int)(blockIdx.x % (unsigned)p.slices);
+    const PackedTile t = packed_tile<true>(p.cu, p.num_seqs, p.total, 1, kRows, (int)(blockIdx.x / (unsigned)p.slices),
+                                           p.adapter_of_seq);
+    const int r0 = t.tile * kRows;
     if (r0 >= t.rows) return;
-    int adapter;
-    const int rank = adapter_rank(p, t.seq, &adapter);
-    const int n0 = blockIdx.y * 256 + wave * 64;
-    if (n0 >= p.n) return;
+    const int rank = adapter_rank(p, t.of);
     if (rank == 0 && p.base == p.out) return;
-    const bool live = r0 + c < t.rows;
-    const int64_t row = t.row0 + (live ? r0 + c : t.rows - 1);
-    // lane (c, q) holds row c's outputs n0 + 16 q .. + 15: element i of tile j is output 16 q + 4 j + i
-    const int nl = n0 + 16 * q;
-    float y[16];
+    const int left = t.rows - r0 < kRows ? t.rows - r0 : kRows;  // rows of this tile
+    const int64_t row0 = t.row0 + r0;
+    const int n_last = (slice + 1) * p.n_slice < p.n ? (slice + 1) * p.n_slice : p.n;
+    int n0 = slice * p.n_slice + 64 * wave;
+    // A wave's 64 outputs are four tiles of 16, ordered so that a lane (c, q) holds 16 bytes side by side of row c and
+    // the four q of a row 64: fp32, element i of tile j is output 16 j + 4 q + i; 16 bits, 32 (j / 2) + 8 q + 4 (j % 2) + i.
+    // What comes from memory is asked for one step ahead, the first step's in front of v.
+    constexpr int kBase = F32 ? 4 : 2;
+    uint4_t base[MT][kBase], bn[RS][4];
+    const unsigned short* const b = p.b + (int64_t)(rank > 0 ? t.of : 0) * p.n * p.max_rank + 8 * q;
+    auto load = [&](int at_n) LG_INLINE {
 #pragma unroll
-    for (int e = 0; e < 16; e += 8) {
-        if (nl + e < p.n) {  // (n is a multiple of 8)
-            if constexpr (F32) {
-                const float4_t* src = reinterpret_cast<const float4_t*>(static_cast<const float*>(p.base) + row * p.base_stride + nl + e);
-                const float4_t u0 = src[0], u1 = src[1];
+        for (int m = 0; m < MT; ++m)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    y[e + i] = u0[i];
-                    y[e + 4 + i] = u1[i];
-                }
-            } else {
-                const auto u = __builtin_bit_cast(typename T::vec8, *reinterpret_cast<const uint4_t*>(
-                    static_cast<const unsigned short*>(p.base) + row * p.base_stride + nl + e));
-#pragma unroll
-                for (int i = 0; i < 8; ++i) y[e + i] = (float)u[i];
+            for (int e = 0; e < kBase; ++e) {
+                const int n = at_n + (F32 ? 16 * e + 4 * q : 32 * e + 8 * q);
+                const int64_t at = (row0 + 16 * m + c) * p.base_stride + n;
+                const bool in = 16 * m + c < left && n < p.n;  // (n is a multiple of 8)
+                base[m][e] = !in ? uint4_t{0, 0, 0, 0}
+                             : F32 ? *reinterpret_cast<const uint4_t*>(static_cast<const float*>(p.base) + at)
+                                   : *reinterpret_cast<const uint4_t*>(static_cast<const unsigned short*>(p.base) + at);
             }
-        }
-    }
-    if (rank > 0) {
-        const float* v = p.v + row * p.max_rank;
-        const int64_t part = (int64_t)p.total * p.max_rank;
-        auto value = [&](int r) LG_INLINE {  // (of 8 from r on, those behind the rank are 0)
-            struct { float e[8]; } o;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) o.e[i] = 0.0f;
-            if (r < rank) {
+        for (int s = 0; s < RS; ++s)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int nr = at_n + (F32 ? 16 * j + c : 32 * (j >> 1) + 8 * (c >> 2) + 4 * (j & 1) + (c & 3));
+                bn[s][j] = nr < p.n && 32 * s + 8 * q < rank
+                               ? *reinterpret_cast<const uint4_t*>(b + (int64_t)nr * p.max_rank + 32 * s)
+                               : uint4_t{0, 0, 0, 0};
+            }
+    };
+    if (n0 < n_last) load(n0);
+    if (rank > 0) {
+        // thread (row, chunk), the chunks of a row side by side
+        for (int i = threadIdx.x; i < kRows * kChunks; i += 256) {
+            const int row = i / kChunks, chunk = i % kChunks, r = 8 * chunk;
+            float u[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) u[e] = 0.0f;
+            if (row < left && r < rank) {
+                const float* v = p.v + (row0 + row) * p.max_rank + r;
+                const int64_t part = (int64_t)p.total * p.max_rank;
                 for (int s = 0; s < p.parts; ++s) {
-                    const float4_t* src = reinterpret_cast<const float4_t*>(v + s * part + r);
+                    const float4_t* src = reinterpret_cast<const float4_t*>(v + s * part);
                     const float4_t u0 = src[0], u1 = src[1];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        o.e[i] += u0[i];
-                        o.e[4 + i] += u1[i];
+                    for (int e = 0; e < 4; ++e) {
+                        u[e] += u0[e];
+                        u[4 + e] += u1[e];
                     }
                 }
             }
+            float top = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) o.e[i] = r + i < rank ? o.e[i] : 0.0f;
-            return o;
-        };
-        float top = 0.0f;
-        for (int s = 0; s < rank; s += 32) {
-            const auto u = value(s + 8 * q);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(u.e[i]));
-        }
-        top = fmaxf(top, lane_xor_f32<16>(top));
-        top = fmaxf(top, lane_xor_f32<32>(top));
-        // 2^-e of the largest value's exponent e, as far as fp32 has it
-        const int ex = (int)(__float_as_uint(top) >> 23);
-        const int down = ex < 1 ? 1 : ex > 253 ? 253 : ex;
-        const float shrink = __uint_as_float((unsigned)(254 - down) << 23);
-        const float grow = __uint_as_float((unsigned)down << 23);
-        float4_t acc[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[j] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
-        for (int s = 0; s < rank; s += 32) {
-            const int r = s + 8 * q;
-            const auto u = value(r);
-            uint4_t term[TERMS];
-#pragma unroll
-            for (int i = 0; i < 8; i += 2) {
-                float a0 = u.e[i] * shrink, a1 = u.e[i + 1] * shrink;
-#pragma unroll
-                for (int k = 0; k < TERMS; ++k) {
-                    const unsigned w = T::pack2(a0, a1);
-                    term[k][i >> 1] = w;
-                    typedef typename T::elem elem;
-                    a0 -= (float)__builtin_bit_cast(elem, (unsigned short)(w & 0xffffu));
-                    a1 -= (float)__builtin_bit_cast(elem, (unsigned short)(w >> 16));
-                    a0 = a0 == a0 ? a0 : 0.0f;  // (an infinity is in its first term, with nothing left)
-                    a1 = a1 == a1 ? a1 : 0.0f;
-                }
+            for (int e = 0; e < 8; ++e) {
+                u[e] = r + e < rank ? u[e] : 0.0f;
+                top = fmaxf(top, fabsf(u[e]));
             }
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                // row c of tile j
-                const int nr = n0 + 16 * (c >> 2) + 4 * j + (c & 3);
-                uint4_t bv = {0, 0, 0, 0};
-                if (nr < p.n && r < rank) {
-                    bv = *reinterpret_cast<const uint4_t*>(p.b + ((int64_t)adapter * p.n + nr) * p.max_rank + r);
+            for (int m = 1; m < kChunks; m *= 2) top = fmaxf(top, shfl_xor_f32(top, m));
+            // 2^-e of the largest value's exponent e, as far as fp32 has it
+            const int ex = (int)(__float_as_uint(top) >> 23);
+            const int down = ex < 1 ? 1 : ex > 253 ? 253 : ex;
+            const float shrink = __uint_as_float((unsigned)(254 - down) << 23);
+            if (chunk == 0) growth[row] = __uint_as_float((unsigned)down << 23);
+            typedef typename T::elem elem;
 #pragma unroll
-                    for (int w = 0; w < 4; ++w)
-                        bv[w] &= rank >= r + 2 * w + 2 ? ~0u : rank == r + 2 * w + 1 ? 0xffffu : 0u;
+            for (int e = 0; e < 8; ++e) u[e] *= shrink;
+#pragma unroll
+            for (int k = 0; k < TERMS; ++k) {
+                uint4_t w;
+#pragma unroll
+                for (int e = 0; e < 8; e += 2) {
+                    w[e >> 1] = T::pack2(u[e], u[e + 1]);
+                    u[e] -= (float)__builtin_bit_cast(elem, (unsigned short)(w[e >> 1] & 0xffffu));
+                    u[e + 1] -= (float)__builtin_bit_cast(elem, (unsigned short)(w[e >> 1] >> 16));
+                    u[e] = u[e] == u[e] ? u[e] : 0.0f;  // (an infinity is in its first term, with nothing left)
+                    u[e + 1] = u[e + 1] == u[e + 1] ? u[e + 1] : 0.0f;
                 }
-#pragma unroll
-                for (int k = 0; k < TERMS; ++k) acc[j] = T::mfma16(bv, term[k], acc[j]);
+                operand[(((row >> 4) * RS + (chunk >> 2)) * TERMS + k) * 64 + (chunk & 3) * 16 + (row & 15)] = w;
             }
         }
-        const float scale = p.scales[adapter];
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) y[4 * j + i] = fmaf(acc[j][i] * grow, scale, y[4 * j + i]);
+        __syncthreads();
     }
-    if (!live) return;
+    uint4_t term[MT][RS][TERMS];
+    float grow[MT], scale = 0.0f;
+    if (rank > 0) {
+        scale = p.scales[t.of];
 #pragma unroll
-    for (int e = 0; e < 16; e += 8) {
-        if (nl + e < p.n) {
-            if constexpr (F32) {
-                float4_t* dst = reinterpret_cast<float4_t*>(static_cast<float*>(p.out) + row * p.out_stride + nl + e);
-                dst[0] = float4_t{y[e], y[e + 1], y[e + 2], y[e + 3]};
-                dst[1] = float4_t{y[e + 4], y[e + 5], y[e + 6], y[e + 7]};
-            } else {
-                uint4_t o;
+        for (int m = 0; m < MT; ++m) {
+            grow[m] = growth[16 * m + c];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) o[i] = T::pack2(y[e + 2 * i], y[e + 2 * i + 1]);
-                *reinterpret_cast<uint4_t*>(static_cast<unsigned short*>(p.out) + row * p.out_stride + nl + e) = o;
+            for (int s = 0; s < RS; ++s)
+#pragma unroll
+                for (int k = 0; k < TERMS; ++k) term[m][s][k] = operand[((m * RS + s) * TERMS + k) * 64 + lane];
+        }
+    }
+    while (n0 < n_last) {
+        const int at_n = n0;
+        uint4_t cb[MT][kBase], bv[RS][4];
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int e = 0; e < kBase; ++e) cb[m][e] = base[m][e];
+#pragma unroll
+        for (int s = 0; s < RS; ++s)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) bv[s][j] = bn[s][j];
+        n0 += 256;
+        if (n0 < n_last) load(n0);
+        float4_t acc[MT][4];
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[m][j] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int s = 0; s < RS; ++s) {
+            if (rank <= 32 * s) break;
+            if (rank < 32 * s + 32 && rank % 8 != 0) {  // a chunk that the rank ends in
+                const int r = 32 * s + 8 * q;
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    const unsigned keep = rank >= r + 2 * w + 2 ? ~0u : rank == r + 2 * w + 1 ? 0xffffu : 0u;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) bv[s][j][w] &= keep;
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < TERMS; ++k)
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) acc[m][j] = T::mfma16(bv[s][j], term[m][s][k], acc[m][j]);
+        }
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            if (16 * m + c >= left) continue;
+#pragma unroll
+            for (int e = 0; e < kBase; ++e) {
+                const int n = at_n + (F32 ? 16 * e + 4 * q : 32 * e + 8 * q);
+                if (n >= p.n) continue;
+                const int64_t at = (row0 + 16 * m + c) * p.out_stride + n;
+                uint4_t o = cb[m][e];
+                if constexpr (F32) {
+                    float4_t y = __builtin_bit_cast(float4_t, o);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) y[i] = fmaf(acc[m][e][i] * grow[m], scale, y[i]);
+                    if (rank > 0) o = __builtin_bit_cast(uint4_t, y);
+                    *reinterpret_cast<uint4_t*>(static_cast<float*>(p.out) + at) = o;
+                } else {
+                    const auto u = __builtin_bit_cast(typename T::vec8, o);
+                    float y[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        y[i] = fmaf(acc[m][2 * e + (i >> 2)][i & 3] * grow[m], scale, (float)u[i]);
+                    if (rank > 0) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) o[i] = T::pack2(y[2 * i], y[2 * i + 1]);
+                    }
+                    *reinterpret_cast<uint4_t*>(static_cast<unsigned short*>(p.out) + at) = o;
+                }
             }
         }
     }
 }
 
-// K parts of the first product
-static int adapter_parts(int k) {
-    const int steps = (k + 31) / 32;
-    int parts = steps / 16;
-    return parts < 1 ? 1 : parts > kAdapterMaxParts ? kAdapterMaxParts : parts;
+template <typename T, int MT, int RT>
+static hipError_t adapter_down(AdapterParams p, hipStream_t stream) {
+    const int64_t tiles = packed_tiles(p.total, p.num_seqs, 1, 16 * MT);
+    const unsigned z = (unsigned)(p.max_rank + 16 * RT - 1) / (16 * RT);
+    adapter_down_kernel<T, MT, RT><<<dim3((unsigned)(tiles * p.parts), z), 256, 0, stream>>>(p);
+    return hipGetLastError();
+}
+
+template <typename T, bool F32, int MT, int RS>
+static hipError_t adapter_up(AdapterParams p, hipStream_t stream) {
+    constexpr int kTerms = F32 && std::is_same<T, PackedBf16>::value ? 3 : 2;
+    const int64_t tiles = packed_tiles(p.total, p.num_seqs, 1, 16 * MT);
+    // a workgroup takes 256 outputs, and more as long as there are workgroups for eight rounds of the chip
+    const int64_t steps = (p.n + 255) / 256;
+    int64_t per = 1;
+    while (2 * per <= steps && tiles * ((steps + 2 * per - 1) / (2 * per)) >= 8 * device_cu_count()) per *= 2;
+    p.n_slice = (int)per * 256;
+    p.slices = (int)((steps + per - 1) / per);
+    adapter_up_kernel<T, F32, kTerms, MT, RS><<<(unsigned)(tiles * p.slices), 256, 0, stream>>>(p);
+    return hipGetLastError();
+}
+
+template <typename T, bool F32>
+static hipError_t adapter_up_by_rank(const AdapterParams& p, bool long_seqs, hipStream_t stream) {
+    constexpr int kLong = F32 ? 2 : 4;  // (what fits the registers twice: this step's and the next one's)
+    if (p.max_rank <= 32) return long_seqs ? adapter_up<T, F32, kLong, 1>(p, stream) : adapter_up<T, F32, 1, 1>(p, stream);
+    if (p.max_rank <= 64) return long_seqs ? adapter_up<T, F32, kLong, 2>(p, stream) : adapter_up<T, F32, 1, 2>(p, stream);
+    if (p.max_rank <= 128) return long_seqs ? adapter_up<T, F32, 2, 4>(p, stream) : adapter_up<T, F32, 1, 4>(p, stream);
+    return adapter_up<T, F32, 1, 8>(p, stream);
 }
 
 template <typename T>
 static hipError_t adapter_launch(AdapterParams p, bool f32, hipStream_t stream) {
-    const unsigned tiles = (unsigned)packed_tiles(p.total, p.num_seqs, 1, kAdapterRows);
-    adapter_down_kernel<T><<<dim3(tiles, p.parts, (p.max_rank + 15) / 16), 256, 0, stream>>>(p);
-    const hipError_t rc = hipGetLastError();
+    const bool long_seqs = p.total >= 32 * (int64_t)p.num_seqs;
+    const int steps = (p.k + 31) / 32, mt = long_seqs ? 4 : 1;
+    const int rt = !long_seqs || p.max_rank <= 16 ? 1 : p.max_rank <= 32 ? 2 : 4;
+    // K parts: two workgroups per compute unit, and steps for four waves
+    const int64_t groups = packed_tiles(p.total, p.num_seqs, 1, 16 * mt) * ((p.max_rank + 16 * rt - 1) / (16 * rt));
+    int parts = 1;
+    while (parts < kAdapterMaxParts && groups * parts < 2 * device_cu_count() && steps >= 16 * parts) parts *= 2;
+    p.parts = parts;
+    p.part_steps = (steps + parts - 1) / parts;
+    hipError_t rc;
+    if (!long_seqs) rc = adapter_down<T, 1, 1>(p, stream);
+    else if (rt == 1) rc = adapter_down<T, 4, 1>(p, stream);
+    else if (rt == 2) rc = adapter_down<T, 4, 2>(p, stream);
+    else rc = adapter_down<T, 4, 4>(p, stream);
     if (rc != hipSuccess) return rc;
-    const dim3 grid(tiles, (p.n + 255) / 256);
-    if (!f32) adapter_up_kernel<T, false, 2><<<grid, 256, 0, stream>>>(p);
-    else adapter_up_kernel<T, true, std::is_same<T, PackedF16>::value ? 2 : 3><<<grid, 256, 0, stream>>>(p);
-    return hipGetLastError();
+    return f32 ? adapter_up_by_rank<T, true>(p, long_seqs, stream) : adapter_up_by_rank<T, false>(p, long_seqs, stream);
 }
 
 static logismos_status_t adapter_add(bool bf16, const void* x, const void* a, const void* b, const int32_t* ranks,
@@ -285,8 +396,6 @@ static logismos_status_t adapter_add(bool bf16, const void* x, const void* a, co
     p.x_stride = x_stride;
     p.base_stride = base_stride;
     p.out_stride = out_stride;
-    p.parts = adapter_parts(k);
-    p.part_steps = ((k + 31) / 32 + p.parts - 1) / p.parts;
     hipStream_t st = static_cast<hipStream_t>(stream);
     return static_cast<logismos_status_t>(bf16 ? adapter_launch<PackedBf16>(p, f32 != 0, st)
                                                : adapter_launch<PackedF16>(p, f32 != 0, st));

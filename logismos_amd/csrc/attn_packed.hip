@@ -261,8 +261,8 @@ logismos_status_t logismos_check_attn_packed_shape(int num_seqs, int total_token
         return reject(msg, cap, "head_dim must be a multiple of 32 up to 256 (%d)", head_dim);
     if ((int64_t)total_tokens + num_seqs > lg::kPackedMaxRows)
         return reject(msg, cap, "total_tokens + num_seqs exceeds %d", lg::kPackedMaxRows);
-    if (((int64_t)total_tokens + num_seqs) * num_q_heads > (1 << 28))
-        return reject(msg, cap, "(total_tokens + num_seqs) * num_q_heads exceeds %d", 1 << 28);
+    if ((int64_t)total_tokens * num_q_heads / 128 + (int64_t)num_seqs * num_kv_heads > (1 << 22))
+        return reject(msg, cap, "total_tokens * num_q_heads / 128 + num_seqs * num_kv_heads exceeds %d", 1 << 22);
     const int64_t qw = (int64_t)num_q_heads * head_dim, kw = (int64_t)num_kv_heads * head_dim;
     if (q_stride < qw || out_stride < qw || k_stride < kw || v_stride < kw)
         return reject(msg, cap, "a stride is smaller than its row (%d and %d of %lld, %d and %d of %lld)", q_stride,

@@ -41,7 +41,7 @@ struct PackedBf16 {
     }
 };
 
-constexpr int kPackedMaxRows = 1 << 24;  // rows and sequences of a launch
+constexpr int kPackedMaxRows = 1 << 23;  // rows and sequences of a launch
 
 // Packed sequences in tiles of `tile` units (a row is `per_row` units).  Only the device knows the
 // lengths, so a launch has packed_tiles() workgroups, the most that can be needed, and sequence s
@@ -54,37 +54,47 @@ inline int64_t packed_tiles(int64_t rows, int num_seqs, int64_t per_row, int64_t
 struct PackedTile {
     int seq;
     int row0;  // first row of the sequence
-    int rows;  // its rows (0: nothing to do)
+    int rows;  // its rows (0 or less: nothing to do)
     int tile;  // which of its tiles
+    int of;    // of_seq[seq], where given
 };
 
-// The sequence of workgroup `b` and its tile: 64 candidates per round, by the whole wave.  Whatever
-// the lengths hold, rows lie in [0, total).
-__device__ __forceinline__ PackedTile packed_tile(const int32_t* __restrict__ cu, int num_seqs,
-                                                  int total, int per_row, int tile, int b) {
+// The sequence of workgroup `b` and its tile: candidates by the whole wave, 64 per round, and in the last round every lane
+// holds what there is to know about one of them (nothing is loaded twice: few rows are all latency).
+// Whatever the lengths hold, rows lie in [0, total).
+template <bool OF = false>
+__device__ __forceinline__ PackedTile packed_tile(const int32_t* __restrict__ cu, int num_seqs, int total,
+                                                  int per_row, int tile, int b,
+                                                  const int32_t* __restrict__ of_seq = nullptr) {
     const int lane = threadIdx.x & 63;
-    auto start = [&](int s) LG_INLINE {
-        return (int)((unsigned)cu[s] * (unsigned)per_row / (unsigned)tile) + s;
+    auto start = [&](int at, int s) LG_INLINE {
+        return (int)((unsigned)at * (unsigned)per_row / (unsigned)tile) + s;
     };
     int lo = 0, n = num_seqs;
-    while (n > 1) {
+    while (n > 63) {
         const int step = (n + 63) / 64;
-        const int at = lane * step;
-        const bool in = at < n && start(lo + (at < n ? at : 0)) <= b;
+        const int at = lane * step < n ? lane * step : 0;
+        const bool in = lane * step < n && start(cu[lo + at], lo + at) <= b;
         const int count = __builtin_popcountll(__builtin_amdgcn_ballot_w64(in));
         const int skip = (count > 0 ? count - 1 : 0) * step;
         lo += skip;
         n = n - skip < step ? n - skip : step;
     }
-    lo = __builtin_amdgcn_readfirstlane(lo);
+    const int mine = lo + (lane < n ? lane : n);
+    const int edge = cu[mine];
+    int of = 0;
+    if constexpr (OF) of = of_seq[mine < num_seqs ? mine : num_seqs - 1];
+    const bool in = lane < n && start(edge, mine) <= b;
+    int last = __builtin_popcountll(__builtin_amdgcn_ballot_w64(in));
+    last = __builtin_amdgcn_readfirstlane(last > 0 ? last - 1 : 0);
+    const int r0 = __builtin_amdgcn_readlane(edge, last), r1 = __builtin_amdgcn_readlane(edge, last + 1);
     PackedTile t;
-    t.seq = lo;
-    const int r0 = __builtin_amdgcn_readfirstlane(cu[lo]);
-    const int r1 = __builtin_amdgcn_readfirstlane(cu[lo + 1]);
+    t.seq = lo + last;
     t.row0 = r0;
     t.rows = r0 >= 0 && r0 < total ? (r1 < total ? r1 : total) - r0 : 0;
-    t.tile = b - __builtin_amdgcn_readfirstlane(start(lo));
+    t.tile = b - start(r0, t.seq);
     if (t.tile < 0) t.rows = 0;
+    t.of = OF ? __builtin_amdgcn_readlane(of, last) : 0;
     return t;
 }
 

@@ -28,7 +28,8 @@ ATTN = dict(num_seqs=2, total=10, hq=8, hkv=2, d=64, qs=512, ks=128, vs=128, os=
     (dict(hq=7), "not a multiple of num_kv_heads"), (dict(d=80), "multiple of 32 up to 256"),
     (dict(d=288, qs=8 * 288, os=8 * 288, ks=576, vs=576), "multiple of 32 up to 256"),
     (dict(total=1 << 24), "exceeds"), (dict(total=1 << 23, num_seqs=(1 << 23) + 1), "exceeds"),
-    (dict(total=1 << 23, hq=64, hkv=2, qs=4096, os=4096), "exceeds"),
+    (dict(total=1 << 22, hq=256, hkv=2, qs=16384, os=16384), "exceeds"),
+    (dict(total=1 << 22, num_seqs=1 << 22, hkv=8, ks=512, vs=512), "exceeds"),
     (dict(qs=504), "smaller than its row"), (dict(os=504), "smaller than its row"),
     (dict(ks=120), "smaller than its row"), (dict(vs=120), "smaller than its row"),
     (dict(qs=516), "multiples of 8"), (dict(vs=130), "multiples of 8"),
