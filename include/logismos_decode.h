@@ -718,7 +718,7 @@ logismos_status_t logismos_launch_attn_packed_bf16(const void* q, const void* k,
  *                   not shared by calls that can overlap in time
  *
  * fp32 sums; x . A^T is not rounded below what the result's type holds; one rounding at the end.  max_rank a multiple of 8
- * up to 256, n, k and strides multiples of 8; x, a, b, base, out, workspace 16-byte aligned. */
+ * up to 256, n, k and strides multiples of 8, n, k and the strides of base and out at most 2^22; x, a, b, base, out, workspace 16-byte aligned. */
 logismos_status_t logismos_check_adapter_add_shape(int num_seqs, int total_tokens, int num_adapters,
                                                    int max_rank, int n, int k, int x_stride, int base_stride,
                                                    int out_stride, char* msg, size_t msg_cap);

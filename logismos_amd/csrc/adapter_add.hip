@@ -86,24 +86,38 @@ __global__ __launch_bounds__(256) void adapter_down_kernel(const AdapterParams p
     for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int i = 0; i < RT; ++i) acc[m][i] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
-    for (int s0 = first; s0 < last; s0 += 4 * kDeep) {
+    // (whole: all steps are the wave's and inside the rows.  The others load the last columns instead of what is not there,
+    // and take zeros: k is a multiple of 8)
+    auto round = [&](auto whole_c, int s0) LG_INLINE {
+        constexpr bool WHOLE = decltype(whole_c)::value != 0;
         uint4_t xv[kDeep][MT], av[kDeep][RT];
 #pragma unroll
         for (int d = 0; d < kDeep; ++d) {
-            const int at = 32 * (s0 + d) + 8 * q;
-            const bool in = s0 + d < last && at < p.k;  // (k is a multiple of 8)
+            const int want = 32 * (s0 + d) + 8 * q;
+            const int at = WHOLE || want < p.k ? want : p.k - 8;
 #pragma unroll
-            for (int m = 0; m < MT; ++m) xv[d][m] = in ? *reinterpret_cast<const uint4_t*>(x[m] + at) : uint4_t{0, 0, 0, 0};
+            for (int m = 0; m < MT; ++m) xv[d][m] = *reinterpret_cast<const uint4_t*>(x[m] + at);
 #pragma unroll
-            for (int i = 0; i < RT; ++i) av[d][i] = in ? *reinterpret_cast<const uint4_t*>(a[i] + at) : uint4_t{0, 0, 0, 0};
+            for (int i = 0; i < RT; ++i) av[d][i] = *reinterpret_cast<const uint4_t*>(a[i] + at);
         }
 #pragma unroll
-        for (int d = 0; d < kDeep; ++d)
+        for (int d = 0; d < kDeep; ++d) {
+            if constexpr (!WHOLE) {
+                const bool in = s0 + d < last && 32 * (s0 + d) + 8 * q < p.k;
+#pragma unroll
+                for (int m = 0; m < MT; ++m) xv[d][m] = in ? xv[d][m] : uint4_t{0, 0, 0, 0};
+#pragma unroll
+                for (int i = 0; i < RT; ++i) av[d][i] = in ? av[d][i] : uint4_t{0, 0, 0, 0};
+            }
 #pragma unroll
             for (int m = 0; m < MT; ++m)
 #pragma unroll
                 for (int i = 0; i < RT; ++i) acc[m][i] = T::mfma16(av[d][i], xv[d][m], acc[m][i]);
-    }
+        }
+    };
+    int s0 = first;
+    for (; s0 + kDeep <= last && 32 * (s0 + kDeep) <= p.k; s0 += 4 * kDeep) round(ic<1>{}, s0);
+    if (s0 < last) round(ic<0>{}, s0);
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -124,10 +138,10 @@ __global__ __launch_bounds__(256) void adapter_down_kernel(const AdapterParams p
 
 // out = base + s (v . B^T).  grid: slices of the outputs (fastest: a slice of B then stays in the L2 of the XCDs that
 // take it, for all rows of its adapter) by tiles of 16 MT rows; ranks in RS steps of 32.  The workgroup splits v
-// into terms once, in the order of the matrix operand, into LDS; a wave keeps them in registers for all its outputs, 64
-// at a time, the four waves side by side.
+// into terms once, in the order of the matrix operand, into LDS; a wave takes 64 outputs at a time, the four
+// waves side by side.
 template <typename T, bool F32, int TERMS, int MT, int RS>
-__global__ __launch_bounds__(256) void adapter_up_kernel(const AdapterParams p) {
+__global__ __launch_bounds__(256, RS == 8 ? 1 : 2) void adapter_up_kernel(const AdapterParams p) {
     constexpr int kRows = 16 * MT, kChunks = 4 * RS;  // chunks of eight ranks
     __shared__ uint4_t operand[MT * RS * TERMS * 64];
     __shared__ float growth[kRows];
@@ -146,34 +160,42 @@ __global__ __launch_bounds__(256) void adapter_up_kernel(const AdapterParams p) 
     int n0 = slice * p.n_slice + 64 * wave;
     // A wave's 64 outputs are four tiles of 16, ordered so that a lane (c, q) holds 16 bytes side by side of row c and
     // the four q of a row 64: fp32, element i of tile j is output 16 j + 4 q + i; 16 bits, 32 (j / 2) + 8 q + 4 (j % 2) + i.
-    // What comes from memory is asked for one step ahead, the first step's in front of v.
-    constexpr int kBase = F32 ? 4 : 2;
-    uint4_t base[MT][kBase], bn[RS][4];
-    const unsigned short* const b = p.b + (int64_t)(rank > 0 ? t.of : 0) * p.n * p.max_rank + 8 * q;
-    auto load = [&](int at_n) LG_INLINE {
+    // What comes from memory is asked for ahead: the base by a step, B as soon as the step's products are done, the first step's
+    // in front of v.
+    constexpr int kBase = F32 ? 4 : 2, kSize = F32 ? 4 : 2;
+    // (rows behind the tile's last, outputs behind the last and ranks behind the rank: others in their place, which count
+    // for nothing -- a load under a condition of its own is a branch around it.  Offsets from the tile's first row and the
+    // adapter's B have 32 bits.)
+    uint4_t even[MT][kBase], odd[MT][kBase], bv[RS][4];
+    const char* const base = static_cast<const char*>(p.base) + row0 * p.base_stride * kSize;
+    char* const out = static_cast<char*>(p.out) + row0 * p.out_stride * kSize;
+    const char* const b = reinterpret_cast<const char*>(p.b + (int64_t)(rank > 0 ? t.of : 0) * p.n * p.max_rank);
+    auto load_base = [&](uint4_t(&w)[MT][kBase], int at_n) LG_INLINE {
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
+        for (int m = 0; m < MT; ++m) {
+            const unsigned row = (unsigned)min(16 * m + c, left - 1) * (unsigned)p.base_stride;
 #pragma unroll
             for (int e = 0; e < kBase; ++e) {
-                const int n = at_n + (F32 ? 16 * e + 4 * q : 32 * e + 8 * q);
-                const int64_t at = (row0 + 16 * m + c) * p.base_stride + n;
-                const bool in = 16 * m + c < left && n < p.n;  // (n is a multiple of 8)
-                base[m][e] = !in ? uint4_t{0, 0, 0, 0}
-                             : F32 ? *reinterpret_cast<const uint4_t*>(static_cast<const float*>(p.base) + at)
-                                   : *reinterpret_cast<const uint4_t*>(static_cast<const unsigned short*>(p.base) + at);
+                const unsigned n = (unsigned)min(at_n + (F32 ? 16 * e + 4 * q : 32 * e + 8 * q), p.n - 16 / kSize);
+                w[m][e] = *reinterpret_cast<const uint4_t*>(base + (row + n) * (unsigned)kSize);
             }
-#pragma unroll
-        for (int s = 0; s < RS; ++s)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int nr = at_n + (F32 ? 16 * j + c : 32 * (j >> 1) + 8 * (c >> 2) + 4 * (j & 1) + (c & 3));
-                bn[s][j] = nr < p.n && 32 * s + 8 * q < rank
-                               ? *reinterpret_cast<const uint4_t*>(b + (int64_t)nr * p.max_rank + 32 * s)
-                               : uint4_t{0, 0, 0, 0};
-            }
+        }
     };
-    if (n0 < n_last) load(n0);
+    auto load_b = [&](int at_n) LG_INLINE {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int want = at_n + (F32 ? 16 * j + c : 32 * (j >> 1) + 8 * (c >> 2) + 4 * (j & 1) + (c & 3));
+            const unsigned row = (unsigned)min(want, p.n - 1) * (unsigned)p.max_rank;
+#pragma unroll
+            for (int s = 0; s < RS; ++s)
+                bv[s][j] = *reinterpret_cast<const uint4_t*>(b + (row + (32 * s + 8 * q < rank ? 32 * s + 8 * q : 0)) * 2u);
+        }
+    };
     if (rank > 0) {
+        if (n0 < n_last) {
+            load_base(even, n0);
+            load_b(n0);
+        }
         // thread (row, chunk), the chunks of a row side by side
         for (int i = threadIdx.x; i < kRows * kChunks; i += 256) {
             const int row = i / kChunks, chunk = i % kChunks, r = 8 * chunk;
@@ -225,84 +247,104 @@ __global__ __launch_bounds__(256) void adapter_up_kernel(const AdapterParams p) 
         }
         __syncthreads();
     }
-    uint4_t term[MT][RS][TERMS];
-    float grow[MT], scale = 0.0f;
-    if (rank > 0) {
-        scale = p.scales[t.of];
-#pragma unroll
-        for (int m = 0; m < MT; ++m) {
-            grow[m] = growth[16 * m + c];
+    float grow[MT], scale;
+    uint4_t keep[RS];  // (the columns of B that count)
+    // One step over the base `w`; WHOLE: of whole tiles, and the next one's B is asked for.
+    auto compute = [&](auto adds_c, auto whole_c, uint4_t(&w)[MT][kBase], int at_n, int next_n) LG_INLINE {
+        constexpr bool ADDS = decltype(adds_c)::value != 0, WHOLE = decltype(whole_c)::value != 0;
+        float4_t acc[MT][4];
+        if (ADDS) {
+            asm volatile("" ::: "memory");  // (the terms are read again: kept over the steps they would not fit)
 #pragma unroll
             for (int s = 0; s < RS; ++s)
 #pragma unroll
-                for (int k = 0; k < TERMS; ++k) term[m][s][k] = operand[((m * RS + s) * TERMS + k) * 64 + lane];
-        }
-    }
-    while (n0 < n_last) {
-        const int at_n = n0;
-        uint4_t cb[MT][kBase], bv[RS][4];
+                for (int j = 0; j < 4; ++j) bv[s][j] &= keep[s];
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
+            for (int m = 0; m < MT; ++m) {
 #pragma unroll
-            for (int e = 0; e < kBase; ++e) cb[m][e] = base[m][e];
+                for (int j = 0; j < 4; ++j) acc[m][j] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int s = 0; s < RS; ++s)
+                for (int s = 0; s < RS; ++s)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) bv[s][j] = bn[s][j];
-        n0 += 256;
-        if (n0 < n_last) load(n0);
-        float4_t acc[MT][4];
+                    for (int k = 0; k < TERMS; ++k) {
+                        const uint4_t v = operand[((m * RS + s) * TERMS + k) * 64 + lane];
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) acc[m][j] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int s = 0; s < RS; ++s) {
-            if (rank <= 32 * s) break;
-            if (rank < 32 * s + 32 && rank % 8 != 0) {  // a chunk that the rank ends in
-                const int r = 32 * s + 8 * q;
-#pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    const unsigned keep = rank >= r + 2 * w + 2 ? ~0u : rank == r + 2 * w + 1 ? 0xffffu : 0u;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) bv[s][j][w] &= keep;
-                }
+                        for (int j = 0; j < 4; ++j) acc[m][j] = T::mfma16(bv[s][j], v, acc[m][j]);
+                    }
             }
-#pragma unroll
-            for (int k = 0; k < TERMS; ++k)
-#pragma unroll
-                for (int m = 0; m < MT; ++m)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) acc[m][j] = T::mfma16(bv[s][j], term[m][s][k], acc[m][j]);
+            if (WHOLE) {
+                __builtin_amdgcn_sched_barrier(0);  // (into the registers that the products just read)
+                load_b(next_n);
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
-            if (16 * m + c >= left) continue;
+            if (!WHOLE && 16 * m + c >= left) continue;
+            const unsigned row = (unsigned)(16 * m + c) * (unsigned)p.out_stride;
 #pragma unroll
             for (int e = 0; e < kBase; ++e) {
                 const int n = at_n + (F32 ? 16 * e + 4 * q : 32 * e + 8 * q);
-                if (n >= p.n) continue;
-                const int64_t at = (row0 + 16 * m + c) * p.out_stride + n;
-                uint4_t o = cb[m][e];
-                if constexpr (F32) {
+                if (!WHOLE && n >= p.n) continue;
+                uint4_t o = w[m][e];
+                if constexpr (!ADDS) {
+                } else if constexpr (F32) {
                     float4_t y = __builtin_bit_cast(float4_t, o);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) y[i] = fmaf(acc[m][e][i] * grow[m], scale, y[i]);
-                    if (rank > 0) o = __builtin_bit_cast(uint4_t, y);
-                    *reinterpret_cast<uint4_t*>(static_cast<float*>(p.out) + at) = o;
+                    o = __builtin_bit_cast(uint4_t, y);
                 } else {
                     const auto u = __builtin_bit_cast(typename T::vec8, o);
                     float y[8];
 #pragma unroll
                     for (int i = 0; i < 8; ++i)
                         y[i] = fmaf(acc[m][2 * e + (i >> 2)][i & 3] * grow[m], scale, (float)u[i]);
-                    if (rank > 0) {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) o[i] = T::pack2(y[2 * i], y[2 * i + 1]);
-                    }
-                    *reinterpret_cast<uint4_t*>(static_cast<unsigned short*>(p.out) + at) = o;
+                    for (int i = 0; i < 4; ++i) o[i] = T::pack2(y[2 * i], y[2 * i + 1]);
                 }
+                *reinterpret_cast<uint4_t*>(out + (row + (unsigned)n) * (unsigned)kSize) = o;
             }
+        }
+    };
+    if (rank > 0) {
+        scale = p.scales[t.of];
+#pragma unroll
+        for (int m = 0; m < MT; ++m) grow[m] = growth[16 * m + c];
+#pragma unroll
+        for (int s = 0; s < RS; ++s)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int r = 32 * s + 8 * q + 2 * i;
+                keep[s][i] = rank >= r + 2 ? ~0u : rank == r + 1 ? 0xffffu : 0u;
+            }
+        if (left == kRows && n_last % 64 == 0) {
+            // Straight-line code, two steps a turn: a condition around a load or a store would make every wait one for
+            // everything in flight.  (The last step asks for itself again.)
+            const int end = n0 < n_last ? n0 + (n_last - 1 - n0) / 256 * 256 : 0;
+            while (n0 < n_last) {
+                int next = min(n0 + 256, end);
+                load_base(odd, next);
+                compute(ic<1>{}, ic<1>{}, even, n0, next);
+                n0 += 256;
+                if (n0 >= n_last) break;
+                next = min(n0 + 256, end);
+                load_base(even, next);
+                compute(ic<1>{}, ic<1>{}, odd, n0, next);
+                n0 += 256;
+            }
+        } else {
+            while (n0 < n_last) {
+                compute(ic<1>{}, ic<0>{}, even, n0, 0);
+                n0 += 256;
+                if (n0 >= n_last) break;
+                load_base(even, n0);
+                load_b(n0);
+            }
+        }
+    } else {
+        for (; n0 < n_last; n0 += 256) {
+            load_base(even, n0);
+            compute(ic<0>{}, ic<0>{}, even, n0, 0);
         }
     }
 }
@@ -334,7 +376,7 @@ static hipError_t adapter_up_by_rank(const AdapterParams& p, bool long_seqs, hip
     constexpr int kLong = F32 ? 2 : 4;  // (what fits the registers twice: this step's and the next one's)
     if (p.max_rank <= 32) return long_seqs ? adapter_up<T, F32, kLong, 1>(p, stream) : adapter_up<T, F32, 1, 1>(p, stream);
     if (p.max_rank <= 64) return long_seqs ? adapter_up<T, F32, kLong, 2>(p, stream) : adapter_up<T, F32, 1, 2>(p, stream);
-    if (p.max_rank <= 128) return long_seqs ? adapter_up<T, F32, 2, 4>(p, stream) : adapter_up<T, F32, 1, 4>(p, stream);
+    if (p.max_rank <= 128) return !F32 && long_seqs ? adapter_up<T, F32, F32 ? 1 : 2, 4>(p, stream) : adapter_up<T, F32, 1, 4>(p, stream);
     return adapter_up<T, F32, 1, 8>(p, stream);
 }
 
@@ -420,7 +462,9 @@ logismos_status_t logismos_check_adapter_add_shape(int num_seqs, int total_token
                       out_stride, n);
     if (x_stride % 8 != 0 || base_stride % 8 != 0 || out_stride % 8 != 0)
         return reject(msg, cap, "strides must be multiples of 8 (%d, %d, %d)", x_stride, base_stride, out_stride);
-    if (n > 65535 * 256) return reject(msg, cap, "n must be at most %d (%d)", 65535 * 256, n);
+    if (n > (1 << 22) || k > (1 << 22)) return reject(msg, cap, "n and k must be at most %d (%d, %d)", 1 << 22, n, k);
+    if (base_stride > (1 << 22) || out_stride > (1 << 22))
+        return reject(msg, cap, "base and out strides must be at most %d (%d, %d)", 1 << 22, base_stride, out_stride);
     if ((int64_t)total_tokens + num_seqs > lg::kPackedMaxRows)
         return reject(msg, cap, "total_tokens + num_seqs exceeds %d", lg::kPackedMaxRows);
     return 0;

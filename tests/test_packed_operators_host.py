@@ -167,7 +167,9 @@ ADAPTER = dict(num_seqs=2, total=10, adapters=3, max_rank=16, n=64, k=128, xs=12
     (dict(xs=120), "smaller than its row"), (dict(bs=56), "smaller than its row"),
     (dict(os=56), "smaller than its row"), (dict(xs=132), "strides must be multiples of 8"),
     (dict(os=68), "strides must be multiples of 8"), (dict(total=1 << 24), "exceeds"),
-    (dict(n=1 << 25, bs=1 << 25, os=1 << 25), "n must be at most"),
+    (dict(n=1 << 23, bs=1 << 23, os=1 << 23), "n and k must be at most"),
+    (dict(k=1 << 23, xs=1 << 23), "n and k must be at most"),
+    (dict(bs=(1 << 22) + 8), "base and out strides"), (dict(os=(1 << 22) + 8), "base and out strides"),
 ])
 def test_adapter_add_shapes(change, frag):
     code, msg = _msg("logismos_check_adapter_add_shape", *{**ADAPTER, **change}.values())
