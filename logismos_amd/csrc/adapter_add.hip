@@ -20,6 +20,7 @@
 
 #include <math.h>
 
+#include <algorithm>
 #include <type_traits>
 
 namespace lg {
@@ -53,7 +54,7 @@ __device__ __forceinline__ int adapter_rank(const AdapterParams& p, int adapter)
 // v[part][t][r] = sum over the part's columns of x[t][c] * A[r][c].  grid (tiles of 16 MT rows by K parts, 16 RT ranks
 // each); the four waves share the part's steps of 32 columns and add up in LDS.
 template <typename T, int MT, int RT>
-__global__ __launch_bounds__(256) void adapter_down_kernel(const AdapterParams p) {
+__global__ __launch_bounds__(256, 2) void adapter_down_kernel(const AdapterParams p) {
     constexpr int kDeep = MT > 1 ? 4 : 8;  // steps asked for together, side by side: whole cache lines
     __shared__ float sums[4][MT * RT * 256];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -100,6 +101,7 @@ __global__ __launch_bounds__(256) void adapter_down_kernel(const AdapterParams p
 #pragma unroll
             for (int i = 0; i < RT; ++i) av[d][i] = *reinterpret_cast<const uint4_t*>(a[i] + at);
         }
+        __builtin_amdgcn_sched_barrier(0);  // (all of them, then the products)
 #pragma unroll
         for (int d = 0; d < kDeep; ++d) {
             if constexpr (!WHOLE) {
@@ -192,33 +194,48 @@ __global__ __launch_bounds__(256, RS == 8 ? 1 : 2) void adapter_up_kernel(const 
         }
     };
     if (rank > 0) {
-        if (n0 < n_last) {
-            load_base(even, n0);
-            load_b(n0);
-        }
-        // thread (row, chunk), the chunks of a row side by side
-        for (int i = threadIdx.x; i < kRows * kChunks; i += 256) {
+        // thread (row, chunk), the chunks of a row side by side.  (The parts of v are asked for first, four at a time: what is
+        // waited for first must not stand behind the base and B.)
+        const int64_t part = (int64_t)p.total * p.max_rank;
+        bool first = true;
+        for (int i = threadIdx.x; first || i < kRows * kChunks; i += 256) {
             const int row = i / kChunks, chunk = i % kChunks, r = 8 * chunk;
+            const bool mine = i < kRows * kChunks;
+            const float* v = p.v + (row0 + (row < left ? row : left - 1)) * p.max_rank + (r < rank ? r : 0);
             float u[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) u[e] = 0.0f;
-            if (row < left && r < rank) {
-                const float* v = p.v + (row0 + row) * p.max_rank + r;
-                const int64_t part = (int64_t)p.total * p.max_rank;
-                for (int s = 0; s < p.parts; ++s) {
-                    const float4_t* src = reinterpret_cast<const float4_t*>(v + s * part);
-                    const float4_t u0 = src[0], u1 = src[1];
+            float4_t w[4][2];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        u[e] += u0[e];
-                        u[4 + e] += u1[e];
-                    }
+            for (int s = 0; s < 4; ++s)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                    w[s][e] = *reinterpret_cast<const float4_t*>(v + min(s, p.parts - 1) * part + 4 * e);
+            if (first && n0 < n_last) {
+                load_base(even, n0);
+                load_b(n0);
+            }
+            first = false;
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+                if (s < p.parts) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) u[e] += w[s][e >> 2][e & 3];
+                }
+            for (int s = 4; s < p.parts; ++s) {
+                const float4_t* src = reinterpret_cast<const float4_t*>(v + s * part);
+                const float4_t u0 = src[0], u1 = src[1];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    u[e] += u0[e];
+                    u[4 + e] += u1[e];
                 }
             }
+            if (!mine) continue;
             float top = 0.0f;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                u[e] = r + e < rank ? u[e] : 0.0f;
+                u[e] = row < left && r + e < rank ? u[e] : 0.0f;
                 top = fmaxf(top, fabsf(u[e]));
             }
 #pragma unroll
@@ -361,10 +378,9 @@ template <typename T, bool F32, int MT, int RS>
 static hipError_t adapter_up(AdapterParams p, hipStream_t stream) {
     constexpr int kTerms = F32 && std::is_same<T, PackedBf16>::value ? 3 : 2;
     const int64_t tiles = packed_tiles(p.total, p.num_seqs, 1, 16 * MT);
-    // a workgroup takes 256 outputs, and more as long as there are workgroups for eight rounds of the chip
+    // a workgroup takes 256 outputs, and more as long as there are eight workgroups per compute unit
     const int64_t steps = (p.n + 255) / 256;
-    int64_t per = 1;
-    while (2 * per <= steps && tiles * ((steps + 2 * per - 1) / (2 * per)) >= 8 * device_cu_count()) per *= 2;
+    const int64_t per = std::max<int64_t>(1, std::min(steps, tiles * steps / (8 * device_cu_count())));
     p.n_slice = (int)per * 256;
     p.slices = (int)((steps + per - 1) / per);
     adapter_up_kernel<T, F32, kTerms, MT, RS><<<(unsigned)(tiles * p.slices), 256, 0, stream>>>(p);
@@ -387,7 +403,7 @@ static hipError_t adapter_launch(AdapterParams p, bool f32, hipStream_t stream) 
     const int rt = !long_seqs || p.max_rank <= 16 ? 1 : p.max_rank <= 32 ? 2 : 4;
     // K parts: two workgroups per compute unit, and steps for four waves
     const int64_t groups = packed_tiles(p.total, p.num_seqs, 1, 16 * mt) * ((p.max_rank + 16 * rt - 1) / (16 * rt));
-    int parts = 1;
+    int parts = 1;  // (at most four for the loads of one round)
     while (parts < kAdapterMaxParts && groups * parts < 2 * device_cu_count() && steps >= 16 * parts) parts *= 2;
     p.parts = parts;
     p.part_steps = (steps + parts - 1) / parts;
