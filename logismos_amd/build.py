@@ -52,6 +52,7 @@ EXTRA_FLAGS = {
     "ref_ops.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "paged_attn_chunk64.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "qgemm_q4g32.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "attn_packed.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 
 # Kernels that ask for operands in one assembly statement and wait for them in a later one, so that

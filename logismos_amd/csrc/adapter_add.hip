@@ -7,7 +7,7 @@
 // same rows through B and adds the base.  Products on the matrix cores, the ranks as rows of the first product's
 // result and the rows of x as its columns, the outputs as rows of the second's.
 //
-// v has to be an operand of the second product, so it is split into 16-bit terms: per row scaled by a power
+// s v has to be an operand of the second product, so it is split into 16-bit terms: per row scaled by a power
 // of two that brings its largest value into [1, 2) (exact, and undone in the fp32 result; fp16 could not hold the values
 // as they are), then the rounded value and what the rounding left.  fp16: two terms, 22 bits; bf16: two terms,
 // 16 bits, for outputs of 8, three, 24 bits, for fp32 outputs.
@@ -138,9 +138,9 @@ __global__ __launch_bounds__(256, 2) void adapter_down_kernel(const AdapterParam
     }
 }
 
-// out = base + s (v . B^T).  grid: slices of the outputs (fastest: a slice of B then stays in the L2 of the XCDs that
-// take it, for all rows of its adapter) by tiles of 16 MT rows; ranks in RS steps of 32.  The workgroup splits v
-// into terms once, in the order of the matrix operand, into LDS; a wave takes 64 outputs at a time, the four
+// out = base + (s v) . B^T.  grid: slices of the outputs (fastest: a slice of B then stays in the L2 of the XCDs that
+// take it, for all rows of its adapter) by tiles of 16 MT rows; ranks in RS steps of 32.  The workgroup splits
+// s v into terms once, in the order of the matrix operand, into LDS; a wave takes 64 outputs at a time, the four
 // waves side by side.
 template <typename T, bool F32, int TERMS, int MT, int RS>
 __global__ __launch_bounds__(256, RS == 8 ? 1 : 2) void adapter_up_kernel(const AdapterParams p) {
@@ -197,6 +197,7 @@ __global__ __launch_bounds__(256, RS == 8 ? 1 : 2) void adapter_up_kernel(const 
         // thread (row, chunk), the chunks of a row side by side.  (The parts of v are asked for first, four at a time: what is
         // waited for first must not stand behind the base and B.)
         const int64_t part = (int64_t)p.total * p.max_rank;
+        const float scale = p.scales[t.of];
         bool first = true;
         for (int i = threadIdx.x; first || i < kRows * kChunks; i += 256) {
             const int row = i / kChunks, chunk = i % kChunks, r = 8 * chunk;
@@ -235,7 +236,7 @@ __global__ __launch_bounds__(256, RS == 8 ? 1 : 2) void adapter_up_kernel(const 
             float top = 0.0f;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                u[e] = row < left && r + e < rank ? u[e] : 0.0f;
+                u[e] = row < left && r + e < rank ? u[e] * scale : 0.0f;
                 top = fmaxf(top, fabsf(u[e]));
             }
 #pragma unroll
@@ -264,7 +265,7 @@ __global__ __launch_bounds__(256, RS == 8 ? 1 : 2) void adapter_up_kernel(const 
         }
         __syncthreads();
     }
-    float grow[MT], scale;
+    float grow[MT];
     uint4_t keep[RS];  // (the columns of B that count)
     // One step over the base `w`; WHOLE: of whole tiles, and the next one's B is asked for.
     auto compute = [&](auto adds_c, auto whole_c, uint4_t(&w)[MT][kBase], int at_n, int next_n) LG_INLINE {
@@ -308,14 +309,14 @@ __global__ __launch_bounds__(256, RS == 8 ? 1 : 2) void adapter_up_kernel(const 
                 } else if constexpr (F32) {
                     float4_t y = __builtin_bit_cast(float4_t, o);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) y[i] = fmaf(acc[m][e][i] * grow[m], scale, y[i]);
+                    for (int i = 0; i < 4; ++i) y[i] = fmaf(acc[m][e][i], grow[m], y[i]);
                     o = __builtin_bit_cast(uint4_t, y);
                 } else {
                     const auto u = __builtin_bit_cast(typename T::vec8, o);
                     float y[8];
 #pragma unroll
                     for (int i = 0; i < 8; ++i)
-                        y[i] = fmaf(acc[m][2 * e + (i >> 2)][i & 3] * grow[m], scale, (float)u[i]);
+                        y[i] = fmaf(acc[m][2 * e + (i >> 2)][i & 3], grow[m], (float)u[i]);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) o[i] = T::pack2(y[2 * i], y[2 * i + 1]);
                 }
@@ -324,7 +325,6 @@ __global__ __launch_bounds__(256, RS == 8 ? 1 : 2) void adapter_up_kernel(const 
         }
     };
     if (rank > 0) {
-        scale = p.scales[t.of];
 #pragma unroll
         for (int m = 0; m < MT; ++m) grow[m] = growth[16 * m + c];
 #pragma unroll

@@ -34,6 +34,58 @@ struct AttnPackedParams {
 
 constexpr int kApKeys = 32;
 
+// Probabilities of the 16 keys that a lane holds of its column (keys first + 8 (e / 4) + e % 4), the running maximum and sum;
+// returns what the sums so far are to be multiplied by.
+template <typename T>
+__device__ __forceinline__ float attn_packed_softmax(float16_t sc, int first, int vis, float scale_log2e, float& m,
+                                                     float& l, uint4_t (&pb)[2]) {
+    float tm = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+        sc[e] = first + 8 * (e >> 2) + (e & 3) < vis ? sc[e] : -INFINITY;
+        tm = fmaxf(tm, sc[e]);
+    }
+    tm = fmaxf(tm, lane_xor_f32<32>(tm)) * scale_log2e;
+    const float m_new = fmaxf(m, tm);
+    const float ref = m_new == -INFINITY ? 0.0f : m_new;
+    const float alpha = fast_exp2(m - ref);
+    m = m_new;
+    l *= alpha;
+#pragma unroll
+    for (int e = 0; e < 16; e += 2) {
+        const float p0 = fast_exp2(fmaf(sc[e], scale_log2e, -ref));
+        const float p1 = fast_exp2(fmaf(sc[e + 1], scale_log2e, -ref));
+        l += p0 + p1;
+        pb[e >> 3][(e & 7) >> 1] = T::pack2(p0, p1);
+    }
+    return alpha;
+}
+
+// Of a V operand of 16 keys (lane: keys 4 h .. + 3 and 8 + 4 h .. + 3 of them) the first ones, the others zero: `keys` counts
+// from key 4 h of the tile of 32.
+__device__ __forceinline__ uint4_t attn_packed_first_keys(uint4_t v, int kb, int keys) {
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        const int at = 16 * kb + 2 * w + (w > 1 ? 4 : 0);
+        v[w] &= keys >= at + 2 ? ~0u : keys == at + 1 ? 0xffffu : 0u;
+    }
+    return v;
+}
+
+template <typename T, int D>
+__device__ __forceinline__ void attn_packed_write(const AttnPackedParams& p, int row, int head, int h,
+                                                  const float16_t (&o)[D / 32], float l) {
+    const float inv = l > 0.0f ? 1.0f / l : l == l ? 0.0f : l;  // (only keys that score -inf: zeros)
+    unsigned short* out = p.out + (int64_t)row * p.out_stride + (int64_t)head * D + 4 * h;
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+            *reinterpret_cast<uint2_t*>(out + 32 * dt + 8 * b) =
+                uint2_t{T::pack2(o[dt][4 * b] * inv, o[dt][4 * b + 1] * inv),
+                        T::pack2(o[dt][4 * b + 2] * inv, o[dt][4 * b + 3] * inv)};
+}
+
 template <typename T, int D, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void attn_packed_kernel(const AttnPackedParams p) {
     constexpr int kCols = 32 * WAVES, kPieces = D / 8, kStride = D + 8;
@@ -108,30 +160,12 @@ __global__ __launch_bounds__(64 * WAVES) void attn_packed_kernel(const AttnPacke
 #pragma unroll
             for (int j = 0; j < D / 16; ++j)
                 sc = T::mfma32(*reinterpret_cast<const uint4_t*>(ks + col * kStride + 16 * j + 8 * h), qb[j], sc);
-            float tm = -INFINITY;
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                sc[e] = key0 + 8 * (e >> 2) + 4 * h + (e & 3) < vis ? sc[e] : -INFINITY;
-                tm = fmaxf(tm, sc[e]);
-            }
-            tm = fmaxf(tm, lane_xor_f32<32>(tm)) * p.scale_log2e;
-            const float m_new = fmaxf(m, tm);
-            const float ref = m_new == -INFINITY ? 0.0f : m_new;
-            const float alpha = fast_exp2(m - ref);
-            m = m_new;
-            l *= alpha;
+            uint4_t pb[2];
+            const float alpha = attn_packed_softmax<T>(sc, key0 + 4 * h, vis, p.scale_log2e, m, l, pb);
 #pragma unroll
             for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) o[dt][e] *= alpha;
-            uint4_t pb[2];
-#pragma unroll
-            for (int e = 0; e < 16; e += 2) {
-                const float p0 = fast_exp2(fmaf(sc[e], p.scale_log2e, -ref));
-                const float p1 = fast_exp2(fmaf(sc[e + 1], p.scale_log2e, -ref));
-                l += p0 + p1;
-                pb[e >> 3][(e & 7) >> 1] = T::pack2(p0, p1);
-            }
             if (!CAREFUL || key0 + kApKeys <= first_vis) {
 #pragma unroll
                 for (int kb = 0; kb < 2; ++kb)
@@ -139,20 +173,12 @@ __global__ __launch_bounds__(64 * WAVES) void attn_packed_kernel(const AttnPacke
                     for (int dt = 0; dt < D / 32; ++dt) o[dt] = T::mfma32(v_operand(kb, dt), pb[kb], o[dt]);
             } else {
                 for (int seen = first_vis; seen <= last_vis; ++seen) {
-                    const int keys = seen - key0 - 4 * h;
 #pragma unroll
                     for (int dt = 0; dt < D / 32; ++dt) {
                         float16_t acc = o[dt];
 #pragma unroll
-                        for (int kb = 0; kb < 2; ++kb) {
-                            uint4_t v = v_operand(kb, dt);
-#pragma unroll
-                            for (int w = 0; w < 4; ++w) {
-                                const int at = 16 * kb + 2 * w + (w > 1 ? 4 : 0);  // (and 4 h: its first key)
-                                v[w] &= keys >= at + 2 ? ~0u : keys == at + 1 ? 0xffffu : 0u;
-                            }
-                            acc = T::mfma32(v, pb[kb], acc);
-                        }
+                        for (int kb = 0; kb < 2; ++kb)
+                            acc = T::mfma32(attn_packed_first_keys(v_operand(kb, dt), kb, seen - key0 - 4 * h), pb[kb], acc);
 #pragma unroll
                         for (int e = 0; e < 16; ++e) o[dt][e] = vis == seen ? acc[e] : o[dt][e];
                     }
@@ -177,15 +203,288 @@ __global__ __launch_bounds__(64 * WAVES) void attn_packed_kernel(const AttnPacke
         if (__builtin_amdgcn_readfirstlane(all) != 0) walk(ic<1>{});
     }
     if (!live) return;
-    const float inv = l > 0.0f ? 1.0f / l : l == l ? 0.0f : l;  // (only keys that score -inf: zeros)
-    unsigned short* out = p.out + (int64_t)(t.row0 + tok) * p.out_stride + (int64_t)head * D + 4 * h;
+    attn_packed_write<T, D>(p, t.row0 + tok, head, h, o, l);
+}
+
+// The same for heads of 64 and 128 and long sequences: eight waves, two per SIMD, over 256 columns, and the stages of a
+// tile of 32 keys -- S(t) = K . Q^T and O(t) = V^T . P on the matrix cores, F(t), the softmax, on the vector units --
+// run one behind the other in a wave: step t issues S(t + 1) and O(t - 1) around F(t), so that the products of a step
+// do not depend on its vector work and the two can be interleaved instruction by instruction.  K is stored into LDS two
+// tiles ahead of its use and V one step, by waves 0-3 and 4-7; the rings are two deep.  Rows of K lie 2 D + 16 bytes
+// apart and those of V 2 D + 64: the operand reads of 16 (32) lanes then touch every bank once.
+//
+// The reference that the exponentials are taken relative to follows the maximum lazily: it is raised when a tile
+// exceeds it by more than 2^8 (a probability is then at most 2^8 and the sums at most 2^8 times as large, far
+// inside the range of all types), so that rescaling the sums is rare.
+constexpr int kPipeWaves = 8, kPipeCols = 32 * kPipeWaves;
+constexpr float kPipeLazy = 8.0f;
+
+template <typename T, int D>
+__global__ __launch_bounds__(64 * kPipeWaves) void attn_packed_pipe_kernel(const AttnPackedParams p) {
+    constexpr int kSteps = D / 16, kTiles = D / 32;  // operands of K (and of V) per key tile; output tiles
+    constexpr int kKRow = D + 8, kVRow = D + 32;     // elements
+    constexpr int kKTile = kApKeys * kKRow, kVTile = kApKeys * kVRow;
+    constexpr int kPer = kApKeys * D / 8 / 256;      // 16-byte pieces that a thread moves per tile
+    __shared__ __attribute__((aligned(16))) unsigned short lds[2 * kKTile + 2 * kVTile];
+    __shared__ unsigned odd_waves[kPipeWaves];
+    unsigned short* const ks = lds;
+    unsigned short* const vs = lds + 2 * kKTile;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int h = lane >> 5, col = lane & 31;
+    const int kvh = (int)(blockIdx.x % (unsigned)p.hkv);
+    const PackedTile t = packed_tile(p.cu, p.num_seqs, p.total, p.g, kPipeCols, (int)(blockIdx.x / (unsigned)p.hkv));
+    const int cols = t.rows * p.g;
+    const int groups = (cols + kPipeCols - 1) / kPipeCols;
+    const int group = groups - 1 - t.tile;  // (the last columns see the most keys: they start first)
+    if (t.rows <= 0 || group < 0) return;
+    const int c0 = group * kPipeCols + wave * 32;
+    const int gc = c0 + col;
+    const bool live = gc < cols;
+    const int tok = (live ? gc : cols - 1) / p.g, head = kvh * p.g + (live ? gc : cols - 1) % p.g;
+    const int vis = p.causal ? tok + 1 : t.rows;  // keys of this lane's column
+    const int last = (group + 1) * kPipeCols < cols ? (group + 1) * kPipeCols - 1 : cols - 1;
+    const int visible = p.causal ? last / p.g + 1 : t.rows;  // ... of the workgroup's last
+    const int all_see = p.causal ? group * kPipeCols / p.g + 1 : t.rows;  // ... of the workgroup's first
+    const int first_vis = p.causal ? (c0 < cols ? c0 : cols - 1) / p.g + 1 : t.rows;  // ... of the wave's first
+    const int last_vis = p.causal ? (c0 + 31 < cols ? c0 + 31 : cols - 1) / p.g + 1 : t.rows;
+
+    uint4_t qb[kSteps];
+    {
+        const unsigned short* q = p.q + (int64_t)(t.row0 + tok) * p.q_stride + (int64_t)head * D + 8 * h;
 #pragma unroll
-    for (int dt = 0; dt < D / 32; ++dt)
+        for (int j = 0; j < kSteps; ++j) qb[j] = *reinterpret_cast<const uint4_t*>(q + 16 * j);
+    }
+
+    // ---- movement: waves 0-3 carry K, waves 4-7 V, a thread kPer pieces of 16 bytes of a tile
+    const bool moves_v = wave >= 4;
+    const int64_t stride = moves_v ? p.v_stride : p.k_stride;
+    const unsigned short* const src = (moves_v ? p.v : p.k) + (int64_t)t.row0 * stride + (int64_t)kvh * D;
+    const unsigned piece = (unsigned)(tid & 255) % (D / 8), key_of = (unsigned)(tid & 255) / (D / 8);
+    constexpr int kRowsPer = 256 / (D / 8);  // keys between a thread's pieces
+    struct Regs {
+        uint4_t x[kPer];
+    };
+    auto gload = [&](int tile, Regs& r) LG_INLINE {
+        // (past the last visible key that key again: its probability is 0 for everybody who sees less)
+        const int key0 = min(tile * kApKeys, visible - 1);
+        const unsigned short* at = src + (int64_t)key0 * stride;
 #pragma unroll
-        for (int b = 0; b < 4; ++b)
-            *reinterpret_cast<uint2_t*>(out + 32 * dt + 8 * b) =
-                uint2_t{T::pack2(o[dt][4 * b] * inv, o[dt][4 * b + 1] * inv),
-                        T::pack2(o[dt][4 * b + 2] * inv, o[dt][4 * b + 3] * inv)};
+        for (int u = 0; u < kPer; ++u) {
+            const unsigned k = (unsigned)min((int)key_of + kRowsPer * u, visible - 1 - key0);
+            r.x[u] = *reinterpret_cast<const uint4_t*>(at + (k * (unsigned)stride + 8u * piece));
+        }
+    };
+    auto lstore = [&](int buf, const Regs& r) LG_INLINE {
+        unsigned short* at = moves_v ? vs + buf * kVTile + key_of * kVRow : ks + buf * kKTile + key_of * kKRow;
+        const int step = kRowsPer * (moves_v ? kVRow : kKRow);
+#pragma unroll
+        for (int u = 0; u < kPer; ++u) *reinterpret_cast<uint4_t*>(at + u * step + 8 * piece) = r.x[u];
+    };
+    const int s16 = lane & 15;
+    const int v_lane = (4 * h + (s16 >> 2)) * kVRow + 16 * ((lane >> 4) & 1) + 4 * (s16 & 3);
+    auto v_operand = [&](int buf, int kb, int dt) LG_INLINE {
+        typedef short short4_t __attribute__((ext_vector_type(4)));
+        typedef __attribute__((address_space(3))) short4_t lds_short4_t;
+        const unsigned short* a = vs + buf * kVTile + v_lane + 16 * kb * kVRow + 32 * dt;
+        const uint2_t lo = __builtin_bit_cast(uint2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4_t*)a));
+        const uint2_t hi = __builtin_bit_cast(
+            uint2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4_t*)(a + 8 * kVRow)));
+        return uint4_t{lo[0], lo[1], hi[0], hi[1]};
+    };
+    auto k_operand = [&](int buf, int j) LG_INLINE {
+        return *reinterpret_cast<const uint4_t*>(ks + buf * kKTile + col * kKRow + 16 * j + 8 * h);
+    };
+
+    float m = -INFINITY, l = 0.0f;
+    float16_t o[kTiles];
+#pragma unroll
+    for (int dt = 0; dt < kTiles; ++dt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[dt][e] = 0.0f;
+    uint4_t p_prev[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+    float16_t s_cur;
+
+    // Tile `tile` with S(tile) in s_cur, K(tile + 1) in K buffer 1 - H and V(tile - 1) in V buffer 1 - H; leaves
+    // S(tile + 1) and P(tile).  MASKED: a column of the workgroup ends in the tile or in front of it.
+    auto step = [&](auto masked_c, auto h_c, int tile) LG_INLINE {
+        constexpr bool MASKED = decltype(masked_c)::value != 0;
+        constexpr int H = decltype(h_c)::value;
+        uint4_t ka[kSteps], va[kSteps];
+#pragma unroll
+        for (int j = 0; j < kSteps; ++j) {
+            ka[j] = k_operand(1 - H, j);
+            va[j] = v_operand(1 - H, j / kTiles, j % kTiles);
+        }
+        const int key0 = tile * kApKeys;
+        float sc[16];
+        float tm = -INFINITY;
+        if (!MASKED || key0 + kApKeys <= first_vis) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                sc[e] = s_cur[e];
+                tm = fmaxf(tm, sc[e]);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                sc[e] = key0 + 8 * (e >> 2) + 4 * h + (e & 3) < vis ? s_cur[e] : -INFINITY;
+                tm = fmaxf(tm, sc[e]);
+            }
+        }
+        tm = fmaxf(tm, lane_xor_f32<32>(tm)) * p.scale_log2e;
+        const bool raise = tm > m + kPipeLazy;
+        const float alpha = raise ? fast_exp2(m - tm) : 1.0f;
+        m = raise ? tm : m;
+        const float ref = m == -INFINITY ? 0.0f : -m;
+        float16_t s_nxt;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s_nxt[e] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < kSteps; ++j) {
+            s_nxt = T::mfma32(ka[j], qb[j], s_nxt);
+            o[j % kTiles] = T::mfma32(va[j], p_prev[j / kTiles], o[j % kTiles]);
+        }
+        float sum = 0.0f;
+        uint4_t pb[2];
+#pragma unroll
+        for (int e = 0; e < 16; e += 2) {
+            const float p0 = fast_exp2(fmaf(sc[e], p.scale_log2e, ref));
+            const float p1 = fast_exp2(fmaf(sc[e + 1], p.scale_log2e, ref));
+            sum += p0;
+            sum += p1;
+            pb[e >> 3][(e & 7) >> 1] = T::pack2(p0, p1);
+        }
+        l = fmaf(l, alpha, sum);
+        if constexpr (!MASKED) {
+            // half of the operand reads, then the products, each followed by a read (into registers freed before) and
+            // its share of the vector work
+            constexpr int kReads = 3 * kSteps, kFirst = 12 * kSteps / 8;
+            __builtin_amdgcn_sched_group_barrier(0x100, kFirst, 0);
+#pragma unroll
+            for (int g = 0; g < 2 * kSteps; ++g) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                if (g < kReads - kFirst) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x002, 80 / (2 * kSteps), 0);
+            }
+        }
+        // (F belongs to this step: its results are used by the next one only, and would sink there)
+        asm volatile("" : "+v"(pb[0]), "+v"(pb[1]), "+v"(l));
+        if (__builtin_expect(__builtin_amdgcn_ballot_w64(raise) != 0, 0)) {  // O(tile - 1) was relative to the old one
+#pragma unroll
+            for (int dt = 0; dt < kTiles; ++dt)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[dt][e] *= alpha;
+        }
+        s_cur = s_nxt;
+        p_prev[0] = pb[0];
+        p_prev[1] = pb[1];
+    };
+
+    const int tiles = (visible + kApKeys - 1) / kApKeys;
+    Regs ra, rb;
+    {
+        // V buffer 1 plays V(-1) in the first step, whose P is 0: finite values
+        for (int i = tid; i < kVTile / 2; i += 64 * kPipeWaves) reinterpret_cast<unsigned*>(vs + kVTile)[i] = 0u;
+        gload(0, ra);
+        if (!moves_v) {
+            gload(1, rb);
+            lstore(0, ra);
+            lstore(1, rb);
+            gload(2, ra);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s_cur[e] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < kSteps; ++j) s_cur = T::mfma32(k_operand(0, j), qb[j], s_cur);
+        __syncthreads();  // (the first step ends with a store into the buffer just read)
+        const int ahead = moves_v ? 1 : 3;  // K(tile + 3), V(tile + 1)
+        auto two_steps = [&](auto masked_c, int tile) LG_INLINE {
+            gload(tile + ahead, rb);
+            __builtin_amdgcn_sched_barrier(0);
+            step(masked_c, ic<0>{}, tile);
+            __builtin_amdgcn_sched_barrier(0);
+            lstore(0, ra);  // K(tile + 2), V(tile)
+            __syncthreads();
+            gload(tile + 1 + ahead, ra);
+            __builtin_amdgcn_sched_barrier(0);
+            step(masked_c, ic<1>{}, tile + 1);
+            __builtin_amdgcn_sched_barrier(0);
+            lstore(1, rb);  // K(tile + 3), V(tile + 1)
+            __syncthreads();
+        };
+        // (a tile past the last repeats loads and is masked for everybody)
+        const int plain = min(tiles, all_see / kApKeys) & ~1;
+        int tile = 0;
+        for (; tile < plain; tile += 2) two_steps(ic<0>{}, tile);
+        for (; tile < tiles; tile += 2) two_steps(ic<1>{}, tile);
+#pragma unroll
+        for (int j = 0; j < kSteps; ++j)
+            o[j % kTiles] = T::mfma32(v_operand(1, j / kTiles, j % kTiles), p_prev[j / kTiles], o[j % kTiles]);
+    }
+    // A key that a column does not see has the probability 0 there, and 0 times an infinity or NaN of its V row is a NaN.
+    // If the results are not all finite, the keys are gone through again, plainly, and in the tiles in which columns of the wave end
+    // with a pass of its own for every number of keys that one of them sees.
+    {
+        float odd = 0.0f;  // NaN if a result is not finite
+#pragma unroll
+        for (int dt = 0; dt < kTiles; ++dt)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) odd = fmaf(o[dt][e], 0.0f, odd);
+        const bool any = __builtin_amdgcn_ballot_w64(odd != odd) != 0;
+        if (lane == 0) odd_waves[wave] = any;
+        __syncthreads();
+        unsigned all = 0;
+#pragma unroll
+        for (int w = 0; w < kPipeWaves; ++w) all |= odd_waves[w];
+        if (__builtin_expect(__builtin_amdgcn_readfirstlane(all) != 0, 0)) {
+            m = -INFINITY;
+            l = 0.0f;
+#pragma unroll
+            for (int dt = 0; dt < kTiles; ++dt)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[dt][e] = 0.0f;
+            for (int tile = 0; tile < tiles; ++tile) {
+                const int key0 = tile * kApKeys;
+                __syncthreads();
+                gload(tile, ra);
+                lstore(0, ra);
+                __syncthreads();
+                float16_t sc;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) sc[e] = 0.0f;
+#pragma unroll
+                for (int j = 0; j < kSteps; ++j) sc = T::mfma32(k_operand(0, j), qb[j], sc);
+                uint4_t pb[2];
+                const float alpha = attn_packed_softmax<T>(sc, key0 + 4 * h, vis, p.scale_log2e, m, l, pb);
+#pragma unroll
+                for (int dt = 0; dt < kTiles; ++dt)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) o[dt][e] *= alpha;
+                if (key0 + kApKeys <= first_vis) {
+#pragma unroll
+                    for (int j = 0; j < kSteps; ++j)
+                        o[j % kTiles] = T::mfma32(v_operand(0, j / kTiles, j % kTiles), pb[j / kTiles], o[j % kTiles]);
+                } else {
+                    for (int seen = first_vis; seen <= last_vis; ++seen) {
+#pragma unroll
+                        for (int dt = 0; dt < kTiles; ++dt) {
+                            float16_t acc = o[dt];
+#pragma unroll
+                            for (int kb = 0; kb < 2; ++kb)
+                                acc = T::mfma32(attn_packed_first_keys(v_operand(0, kb, dt), kb, seen - key0 - 4 * h),
+                                                pb[kb], acc);
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) o[dt][e] = vis == seen ? acc[e] : o[dt][e];
+                        }
+                    }
+                }
+            }
+        }
+    }
+    l += lane_xor_f32<32>(l);
+    if (!live) return;
+    attn_packed_write<T, D>(p, t.row0 + tok, head, h, o, l);
 }
 
 template <typename T, int D>
@@ -196,13 +495,20 @@ static hipError_t attn_packed_launch(const AttnPackedParams& p, hipStream_t stre
     return hipGetLastError();
 }
 
+template <typename T, int D>
+static hipError_t attn_packed_pipe_launch(const AttnPackedParams& p, hipStream_t stream) {
+    const int64_t tiles = packed_tiles(p.total, p.num_seqs, p.g, kPipeCols);
+    attn_packed_pipe_kernel<T, D><<<(unsigned)(tiles * p.hkv), 64 * kPipeWaves, 0, stream>>>(p);
+    return hipGetLastError();
+}
+
 template <typename T>
 static hipError_t attn_packed_by_width(const AttnPackedParams& p, int d, hipStream_t stream) {
     switch (d) {
         case 32: return attn_packed_launch<T, 32>(p, stream);
-        case 64: return attn_packed_launch<T, 64>(p, stream);
+        case 64: return attn_packed_pipe_launch<T, 64>(p, stream);
         case 96: return attn_packed_launch<T, 96>(p, stream);
-        case 128: return attn_packed_launch<T, 128>(p, stream);
+        case 128: return attn_packed_pipe_launch<T, 128>(p, stream);
         case 160: return attn_packed_launch<T, 160>(p, stream);
         case 192: return attn_packed_launch<T, 192>(p, stream);
         case 224: return attn_packed_launch<T, 224>(p, stream);

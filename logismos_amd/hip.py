@@ -148,6 +148,8 @@ class DevicePtrView:
     def ptr(self) -> C.c_void_p:
         return self._p
 
+    _as_parameter_ = ptr  # (what a foreign function that takes a pointer is given)
+
     def to_numpy(self, dtype, shape=None) -> np.ndarray:
         out = np.empty(self.nbytes // np.dtype(dtype).itemsize if shape is None else shape, dtype)
         assert out.nbytes <= self.nbytes
@@ -168,6 +170,8 @@ class DeviceBuffer:
     @property
     def ptr(self) -> C.c_void_p:
         return self._p
+
+    _as_parameter_ = ptr
 
     def offset(self, nbytes: int) -> C.c_void_p:
         return C.c_void_p(self._p.value + int(nbytes))

@@ -585,6 +585,24 @@ def rope_frequencies(rotary_dim: int, base: float, scaling: str = "none", factor
     return out, amplitude.value
 
 
+_launchers = {}
+
+
+def _launcher(name: str):
+    fn = _launchers.get(name)
+    if fn is None:
+        fn = _launchers[name] = getattr(library(), "logismos_launch_" + name)
+    return fn
+
+
+def _refused(name: str, code: int, check, *dims) -> None:
+    """What a launcher's status means.  The launchers over packed rows guard their shapes themselves,
+    so that a call of a few microseconds is one foreign call; a refused one is asked for the reason."""
+    if code == 1:
+        _guard(name, check, *dims)
+    _status(name, code)
+
+
 def launch_rope_packed(q_in, k_in, q_out, k_out, positions, inv_freq, tokens: int,
                        num_q_heads: int, num_kv_heads: int, head_dim: int, rotary_dim: int,
                        interleaved: bool = False, amplitude: float = 1.0, q_in_stride=None,
@@ -594,16 +612,16 @@ def launch_rope_packed(q_in, k_in, q_out, k_out, positions, inv_freq, tokens: in
     rows one behind the other.  k_in and k_out may be None with num_kv_heads == 0."""
     if dtype not in ("fp16", "bf16", "f32"):
         raise ValueError(f"dtype must be fp16, bf16 or f32, not {dtype!r}")
-    name = f"rope_packed_{dtype}"
+    name = "rope_packed_" + dtype
     qw, kw = num_q_heads * head_dim, num_kv_heads * head_dim
-    strides = [w if s is None else s for s, w in ((q_in_stride, qw), (k_in_stride, kw),
-                                                  (q_out_stride, qw), (k_out_stride, kw))]
-    _guard(name, library().logismos_check_rope_packed_shape, tokens, num_q_heads, num_kv_heads,
-           head_dim, rotary_dim, *strides)
-    _status(name, getattr(library(), f"logismos_launch_{name}")(
-        _ptr(q_in), _ptr(k_in), _ptr(q_out), _ptr(k_out), _ptr(positions), _ptr(inv_freq), tokens,
-        num_q_heads, num_kv_heads, head_dim, rotary_dim, *strides, float(amplitude),
-        1 if interleaved else 0, _raw(stream)))
+    dims = (tokens, num_q_heads, num_kv_heads, head_dim, rotary_dim,
+            qw if q_in_stride is None else q_in_stride, kw if k_in_stride is None else k_in_stride,
+            qw if q_out_stride is None else q_out_stride,
+            kw if k_out_stride is None else k_out_stride)
+    code = _launcher(name)(q_in, k_in, q_out, k_out, positions, inv_freq, *dims, amplitude,
+                           1 if interleaved else 0, _raw(stream))
+    if code != 0:
+        _refused(name, code, library().logismos_check_rope_packed_shape, *dims)
 
 
 def launch_attn_packed(q, k, v, cu_seqlens, out, num_seqs: int, total_tokens: int,
@@ -613,14 +631,12 @@ def launch_attn_packed(q, k, v, cu_seqlens, out, num_seqs: int, total_tokens: in
     """Attention of whole packed sequences; strides in elements, None: rows one behind the other."""
     name = "attn_packed_bf16" if bf16 else "attn_packed_fp16"
     qw, kw = num_q_heads * head_dim, num_kv_heads * head_dim
-    strides = [w if s is None else s for s, w in ((q_stride, qw), (k_stride, kw), (v_stride, kw),
-                                                  (out_stride, qw))]
-    _guard(name, library().logismos_check_attn_packed_shape, num_seqs, total_tokens, num_q_heads,
-           num_kv_heads, head_dim, *strides)
-    _status(name, getattr(library(), f"logismos_launch_{name}")(
-        _ptr(q), _ptr(k), _ptr(v), _ptr(cu_seqlens), _ptr(out), num_seqs, total_tokens,
-        num_q_heads, num_kv_heads, head_dim, *strides, float(scale), 1 if causal else 0,
-        _raw(stream)))
+    dims = (num_seqs, total_tokens, num_q_heads, num_kv_heads, head_dim,
+            qw if q_stride is None else q_stride, kw if k_stride is None else k_stride,
+            kw if v_stride is None else v_stride, qw if out_stride is None else out_stride)
+    code = _launcher(name)(q, k, v, cu_seqlens, out, *dims, scale, 1 if causal else 0, _raw(stream))
+    if code != 0:
+        _refused(name, code, library().logismos_check_attn_packed_shape, *dims)
 
 
 def adapter_add_workspace_bytes(total_tokens: int, max_rank: int) -> int:
@@ -634,13 +650,12 @@ def launch_adapter_add(x, a, b, ranks, scales, adapter_of_seq, cu_seqlens, base,
     """`out = base + scale * (x A^T) B^T` with each sequence's adapter; strides in elements, None:
     rows one behind the other; base and out may be the same."""
     name = "adapter_add_bf16" if bf16 else "adapter_add_fp16"
-    strides = [w if s is None else s for s, w in ((x_stride, k), (base_stride, n), (out_stride, n))]
-    _guard(name, library().logismos_check_adapter_add_shape, num_seqs, total_tokens, num_adapters,
-           max_rank, n, k, *strides)
-    _status(name, getattr(library(), f"logismos_launch_{name}")(
-        _ptr(x), _ptr(a), _ptr(b), _ptr(ranks), _ptr(scales), _ptr(adapter_of_seq),
-        _ptr(cu_seqlens), _ptr(base), _ptr(out), 1 if f32_out else 0, _ptr(workspace), num_seqs,
-        total_tokens, num_adapters, max_rank, n, k, *strides, _raw(stream)))
+    dims = (num_seqs, total_tokens, num_adapters, max_rank, n, k, k if x_stride is None else x_stride,
+            n if base_stride is None else base_stride, n if out_stride is None else out_stride)
+    code = _launcher(name)(x, a, b, ranks, scales, adapter_of_seq, cu_seqlens, base, out,
+                           1 if f32_out else 0, workspace, *dims, _raw(stream))
+    if code != 0:
+        _refused(name, code, library().logismos_check_adapter_add_shape, *dims)
 
 
 # ---- the reference's existing launchers (same names as its Rust wrappers,
