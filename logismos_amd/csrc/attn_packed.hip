@@ -18,6 +18,12 @@
 
 #include <math.h>
 
+#ifndef AP_W
+#define AP_W 8
+#endif
+#ifndef AP_LB
+#define AP_LB 1
+#endif
 namespace lg {
 
 struct AttnPackedParams {
@@ -72,24 +78,45 @@ __device__ __forceinline__ uint4_t attn_packed_first_keys(uint4_t v, int kb, int
     return v;
 }
 
+// Normalises a wave's 32 columns and writes them, 16 at a time through its part of LDS (`stage`, 16 rows of D + 8): straight
+// from the registers a store would put 16 bytes into each of 32 rows, from there it writes whole head rows.  `to` is where this
+// lane's column goes, in elements from `out`, less than 2^31; cols the number of columns that are there.
 template <typename T, int D>
-__device__ __forceinline__ void attn_packed_write(const AttnPackedParams& p, int row, int head, int h,
+__device__ __forceinline__ void attn_packed_write(unsigned short* out, unsigned to, int cols, unsigned short* stage,
                                                   const float16_t (&o)[D / 32], float l) {
+    constexpr int kRow = D + 8, kLanes = D / 8;
+    const int lane = threadIdx.x & 63, h = lane >> 5, col = lane & 31;
     const float inv = l > 0.0f ? 1.0f / l : l == l ? 0.0f : l;  // (only keys that score -inf: zeros)
-    unsigned short* out = p.out + (int64_t)row * p.out_stride + (int64_t)head * D + 4 * h;
 #pragma unroll
-    for (int dt = 0; dt < D / 32; ++dt)
+    for (int half = 0; half < 2; ++half) {
+        if (16 * half >= cols) break;
+        if ((col >> 4) == half) {
 #pragma unroll
-        for (int b = 0; b < 4; ++b)
-            *reinterpret_cast<uint2_t*>(out + 32 * dt + 8 * b) =
-                uint2_t{T::pack2(o[dt][4 * b] * inv, o[dt][4 * b + 1] * inv),
-                        T::pack2(o[dt][4 * b + 2] * inv, o[dt][4 * b + 3] * inv)};
+            for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+                for (int b = 0; b < 4; ++b)
+                    *reinterpret_cast<uint2_t*>(stage + (col & 15) * kRow + 32 * dt + 8 * b + 4 * h) =
+                        uint2_t{T::pack2(o[dt][4 * b] * inv, o[dt][4 * b + 1] * inv),
+                                T::pack2(o[dt][4 * b + 2] * inv, o[dt][4 * b + 3] * inv)};
+        }
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int i = lane; i < 16 * kLanes; i += 64) {
+            const int c = i / kLanes, piece = i % kLanes;
+            const unsigned at = __shfl(to, 16 * half + c);
+            const uint4_t v = *reinterpret_cast<const uint4_t*>(stage + c * kRow + 8 * piece);
+            if (16 * half + c < cols) *reinterpret_cast<uint4_t*>(out + (at + 8u * piece)) = v;
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
 }
 
 template <typename T, int D, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void attn_packed_kernel(const AttnPackedParams p) {
     constexpr int kCols = 32 * WAVES, kPieces = D / 8, kStride = D + 8;
-    __shared__ __attribute__((aligned(16))) unsigned short ks[kApKeys * kStride], vs[kApKeys * kStride];
+    __shared__ __attribute__((aligned(16))) unsigned short lds[2 * kApKeys * kStride];
+    static_assert(WAVES * 16 <= 2 * kApKeys, "the columns on their way out fit");
+    unsigned short *const ks = lds, *const vs = lds + kApKeys * kStride;
     __shared__ unsigned odd_waves[WAVES];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int h = lane >> 5, col = lane & 31;
@@ -200,10 +227,16 @@ __global__ __launch_bounds__(64 * WAVES) void attn_packed_kernel(const AttnPacke
         unsigned all = 0;
 #pragma unroll
         for (int w = 0; w < WAVES; ++w) all |= odd_waves[w];
-        if (__builtin_amdgcn_readfirstlane(all) != 0) walk(ic<1>{});
+        if (__builtin_amdgcn_readfirstlane(all) != 0) {
+            walk(ic<1>{});
+            __syncthreads();
+        }
     }
-    if (!live) return;
-    attn_packed_write<T, D>(p, t.row0 + tok, head, h, o, l);
+    if (c0 >= cols) return;
+    const int tok0 = c0 / p.g;  // of the wave's first column
+    attn_packed_write<T, D>(p.out + (int64_t)(t.row0 + tok0) * p.out_stride,
+                            (unsigned)(tok - tok0) * (unsigned)p.out_stride + (unsigned)(head * D), cols - c0,
+                            lds + wave * 16 * kStride, o, l);
 }
 
 // The same for heads of 64 and 128 and long sequences: eight waves, two per SIMD, over 256 columns, and the stages of a
@@ -216,35 +249,35 @@ __global__ __launch_bounds__(64 * WAVES) void attn_packed_kernel(const AttnPacke
 // The reference that the exponentials are taken relative to follows the maximum lazily: it is raised when a tile
 // exceeds it by more than 2^8 (a probability is then at most 2^8 and the sums at most 2^8 times as large, far
 // inside the range of all types), so that rescaling the sums is rare.
-constexpr int kPipeWaves = 8, kPipeCols = 32 * kPipeWaves;
 constexpr float kPipeLazy = 8.0f;
 
-template <typename T, int D>
-__global__ __launch_bounds__(64 * kPipeWaves) void attn_packed_pipe_kernel(const AttnPackedParams p) {
+template <typename T, int D, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, AP_LB) void attn_packed_pipe_kernel(const AttnPackedParams p) {
+    constexpr int kCols = 32 * WAVES, kMovers = 32 * WAVES;  // threads that move K, and V
     constexpr int kSteps = D / 16, kTiles = D / 32;  // operands of K (and of V) per key tile; output tiles
     constexpr int kKRow = D + 8, kVRow = D + 32;     // elements
     constexpr int kKTile = kApKeys * kKRow, kVTile = kApKeys * kVRow;
-    constexpr int kPer = kApKeys * D / 8 / 256;      // 16-byte pieces that a thread moves per tile
+    constexpr int kPer = kApKeys * D / 8 / kMovers;      // 16-byte pieces that a thread moves per tile
     __shared__ __attribute__((aligned(16))) unsigned short lds[2 * kKTile + 2 * kVTile];
-    __shared__ unsigned odd_waves[kPipeWaves];
+    __shared__ unsigned odd_waves[WAVES];
     unsigned short* const ks = lds;
     unsigned short* const vs = lds + 2 * kKTile;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int h = lane >> 5, col = lane & 31;
     const int kvh = (int)(blockIdx.x % (unsigned)p.hkv);
-    const PackedTile t = packed_tile(p.cu, p.num_seqs, p.total, p.g, kPipeCols, (int)(blockIdx.x / (unsigned)p.hkv));
+    const PackedTile t = packed_tile(p.cu, p.num_seqs, p.total, p.g, kCols, (int)(blockIdx.x / (unsigned)p.hkv));
     const int cols = t.rows * p.g;
-    const int groups = (cols + kPipeCols - 1) / kPipeCols;
+    const int groups = (cols + kCols - 1) / kCols;
     const int group = groups - 1 - t.tile;  // (the last columns see the most keys: they start first)
     if (t.rows <= 0 || group < 0) return;
-    const int c0 = group * kPipeCols + wave * 32;
+    const int c0 = group * kCols + wave * 32;
     const int gc = c0 + col;
     const bool live = gc < cols;
     const int tok = (live ? gc : cols - 1) / p.g, head = kvh * p.g + (live ? gc : cols - 1) % p.g;
     const int vis = p.causal ? tok + 1 : t.rows;  // keys of this lane's column
-    const int last = (group + 1) * kPipeCols < cols ? (group + 1) * kPipeCols - 1 : cols - 1;
+    const int last = (group + 1) * kCols < cols ? (group + 1) * kCols - 1 : cols - 1;
     const int visible = p.causal ? last / p.g + 1 : t.rows;  // ... of the workgroup's last
-    const int all_see = p.causal ? group * kPipeCols / p.g + 1 : t.rows;  // ... of the workgroup's first
+    const int all_see = p.causal ? group * kCols / p.g + 1 : t.rows;  // ... of the workgroup's first
     const int first_vis = p.causal ? (c0 < cols ? c0 : cols - 1) / p.g + 1 : t.rows;  // ... of the wave's first
     const int last_vis = p.causal ? (c0 + 31 < cols ? c0 + 31 : cols - 1) / p.g + 1 : t.rows;
 
@@ -256,11 +289,11 @@ __global__ __launch_bounds__(64 * kPipeWaves) void attn_packed_pipe_kernel(const
     }
 
     // ---- movement: waves 0-3 carry K, waves 4-7 V, a thread kPer pieces of 16 bytes of a tile
-    const bool moves_v = wave >= 4;
+    const bool moves_v = wave >= WAVES / 2;
     const int64_t stride = moves_v ? p.v_stride : p.k_stride;
     const unsigned short* const src = (moves_v ? p.v : p.k) + (int64_t)t.row0 * stride + (int64_t)kvh * D;
-    const unsigned piece = (unsigned)(tid & 255) % (D / 8), key_of = (unsigned)(tid & 255) / (D / 8);
-    constexpr int kRowsPer = 256 / (D / 8);  // keys between a thread's pieces
+    const unsigned piece = (unsigned)(tid % kMovers) % (D / 8), key_of = (unsigned)(tid % kMovers) / (D / 8);
+    constexpr int kRowsPer = kMovers / (D / 8);  // keys between a thread's pieces
     struct Regs {
         uint4_t x[kPer];
     };
@@ -384,7 +417,7 @@ __global__ __launch_bounds__(64 * kPipeWaves) void attn_packed_pipe_kernel(const
     Regs ra, rb;
     {
         // V buffer 1 plays V(-1) in the first step, whose P is 0: finite values
-        for (int i = tid; i < kVTile / 2; i += 64 * kPipeWaves) reinterpret_cast<unsigned*>(vs + kVTile)[i] = 0u;
+        for (int i = tid; i < kVTile / 2; i += 64 * WAVES) reinterpret_cast<unsigned*>(vs + kVTile)[i] = 0u;
         gload(0, ra);
         if (!moves_v) {
             gload(1, rb);
@@ -399,44 +432,48 @@ __global__ __launch_bounds__(64 * kPipeWaves) void attn_packed_pipe_kernel(const
         for (int j = 0; j < kSteps; ++j) s_cur = T::mfma32(k_operand(0, j), qb[j], s_cur);
         __syncthreads();  // (the first step ends with a store into the buffer just read)
         const int ahead = moves_v ? 1 : 3;  // K(tile + 3), V(tile + 1)
-        auto two_steps = [&](auto masked_c, int tile) LG_INLINE {
-            gload(tile + ahead, rb);
+        // step `tile`, H its parity: what the step after the next needs is asked for in front of it and goes to LDS behind it
+        auto one = [&](auto masked_c, auto h_c, int tile, Regs& now, Regs& next) LG_INLINE {
+            gload(tile + ahead, next);
             __builtin_amdgcn_sched_barrier(0);
-            step(masked_c, ic<0>{}, tile);
+            step(masked_c, h_c, tile);
             __builtin_amdgcn_sched_barrier(0);
-            lstore(0, ra);  // K(tile + 2), V(tile)
-            __syncthreads();
-            gload(tile + 1 + ahead, ra);
-            __builtin_amdgcn_sched_barrier(0);
-            step(masked_c, ic<1>{}, tile + 1);
-            __builtin_amdgcn_sched_barrier(0);
-            lstore(1, rb);  // K(tile + 3), V(tile + 1)
+            lstore(decltype(h_c)::value, now);  // K(tile + 2), V(tile)
             __syncthreads();
         };
-        // (a tile past the last repeats loads and is masked for everybody)
         const int plain = min(tiles, all_see / kApKeys) & ~1;
         int tile = 0;
-        for (; tile < plain; tile += 2) two_steps(ic<0>{}, tile);
-        for (; tile < tiles; tile += 2) two_steps(ic<1>{}, tile);
+        for (; tile < plain; tile += 2) {
+            one(ic<0>{}, ic<0>{}, tile, ra, rb);
+            one(ic<0>{}, ic<1>{}, tile + 1, rb, ra);
+        }
+        while (tile < tiles) {
+            one(ic<1>{}, ic<0>{}, tile, ra, rb);
+            if (++tile >= tiles) break;
+            one(ic<1>{}, ic<1>{}, tile, rb, ra);
+            ++tile;
+        }
+        const int buf = (tiles - 1) & 1;
 #pragma unroll
         for (int j = 0; j < kSteps; ++j)
-            o[j % kTiles] = T::mfma32(v_operand(1, j / kTiles, j % kTiles), p_prev[j / kTiles], o[j % kTiles]);
+            o[j % kTiles] = T::mfma32(v_operand(buf, j / kTiles, j % kTiles), p_prev[j / kTiles], o[j % kTiles]);
     }
     // A key that a column does not see has the probability 0 there, and 0 times an infinity or NaN of its V row is a NaN.
     // If the results are not all finite, the keys are gone through again, plainly, and in the tiles in which columns of the wave end
     // with a pass of its own for every number of keys that one of them sees.
     {
-        float odd = 0.0f;  // NaN if a result is not finite
+        float odds[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // NaN if a result is not finite
 #pragma unroll
         for (int dt = 0; dt < kTiles; ++dt)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) odd = fmaf(o[dt][e], 0.0f, odd);
+            for (int e = 0; e < 16; ++e) odds[e & 3] = fmaf(o[dt][e], 0.0f, odds[e & 3]);
+        const float odd = (odds[0] + odds[1]) + (odds[2] + odds[3]);
         const bool any = __builtin_amdgcn_ballot_w64(odd != odd) != 0;
         if (lane == 0) odd_waves[wave] = any;
         __syncthreads();
         unsigned all = 0;
 #pragma unroll
-        for (int w = 0; w < kPipeWaves; ++w) all |= odd_waves[w];
+        for (int w = 0; w < WAVES; ++w) all |= odd_waves[w];
         if (__builtin_expect(__builtin_amdgcn_readfirstlane(all) != 0, 0)) {
             m = -INFINITY;
             l = 0.0f;
@@ -480,11 +517,16 @@ __global__ __launch_bounds__(64 * kPipeWaves) void attn_packed_pipe_kernel(const
                     }
                 }
             }
+            __syncthreads();
         }
     }
     l += lane_xor_f32<32>(l);
-    if (!live) return;
-    attn_packed_write<T, D>(p, t.row0 + tok, head, h, o, l);
+    if (c0 >= cols) return;
+    static_assert(WAVES * 16 * kKRow <= 2 * kKTile + 2 * kVTile, "the columns on their way out fit");
+    const int tok0 = c0 / p.g;  // of the wave's first column
+    attn_packed_write<T, D>(p.out + (int64_t)(t.row0 + tok0) * p.out_stride,
+                            (unsigned)(tok - tok0) * (unsigned)p.out_stride + (unsigned)(head * D), cols - c0,
+                            lds + wave * 16 * kKRow, o, l);
 }
 
 template <typename T, int D>
@@ -495,10 +537,10 @@ static hipError_t attn_packed_launch(const AttnPackedParams& p, hipStream_t stre
     return hipGetLastError();
 }
 
-template <typename T, int D>
+template <typename T, int D, int WAVES>
 static hipError_t attn_packed_pipe_launch(const AttnPackedParams& p, hipStream_t stream) {
-    const int64_t tiles = packed_tiles(p.total, p.num_seqs, p.g, kPipeCols);
-    attn_packed_pipe_kernel<T, D><<<(unsigned)(tiles * p.hkv), 64 * kPipeWaves, 0, stream>>>(p);
+    const int64_t tiles = packed_tiles(p.total, p.num_seqs, p.g, 32 * WAVES);
+    attn_packed_pipe_kernel<T, D, WAVES><<<(unsigned)(tiles * p.hkv), 64 * WAVES, 0, stream>>>(p);
     return hipGetLastError();
 }
 
@@ -506,9 +548,9 @@ template <typename T>
 static hipError_t attn_packed_by_width(const AttnPackedParams& p, int d, hipStream_t stream) {
     switch (d) {
         case 32: return attn_packed_launch<T, 32>(p, stream);
-        case 64: return attn_packed_pipe_launch<T, 64>(p, stream);
+        case 64: return attn_packed_pipe_launch<T, 64, AP_W>(p, stream);
         case 96: return attn_packed_launch<T, 96>(p, stream);
-        case 128: return attn_packed_pipe_launch<T, 128>(p, stream);
+        case 128: return attn_packed_pipe_launch<T, 128, AP_W>(p, stream);
         case 160: return attn_packed_launch<T, 160>(p, stream);
         case 192: return attn_packed_launch<T, 192>(p, stream);
         case 224: return attn_packed_launch<T, 224>(p, stream);
@@ -576,8 +618,9 @@ logismos_status_t logismos_check_attn_packed_shape(int num_seqs, int total_token
     if ((q_stride | k_stride | v_stride | out_stride) % 8 != 0)
         return reject(msg, cap, "strides must be multiples of 8 (%d, %d, %d, %d)", q_stride, k_stride, v_stride,
                       out_stride);
-    if (k_stride > (1 << 22) || v_stride > (1 << 22))
-        return reject(msg, cap, "k and v strides must be at most %d (%d, %d)", 1 << 22, k_stride, v_stride);
+    if (k_stride > (1 << 22) || v_stride > (1 << 22) || out_stride > (1 << 22))
+        return reject(msg, cap, "k, v and out strides must be at most %d (%d, %d, %d)", 1 << 22, k_stride, v_stride,
+                      out_stride);
     return 0;
 }
 

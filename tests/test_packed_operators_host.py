@@ -33,7 +33,7 @@ ATTN = dict(num_seqs=2, total=10, hq=8, hkv=2, d=64, qs=512, ks=128, vs=128, os=
     (dict(qs=504), "smaller than its row"), (dict(os=504), "smaller than its row"),
     (dict(ks=120), "smaller than its row"), (dict(vs=120), "smaller than its row"),
     (dict(qs=516), "multiples of 8"), (dict(vs=130), "multiples of 8"),
-    (dict(ks=(1 << 22) + 8), "at most"),
+    (dict(ks=(1 << 22) + 8), "at most"), (dict(os=(1 << 22) + 8), "at most"),
 ])
 def test_attn_packed_shapes(change, frag):
     code, msg = _msg("logismos_check_attn_packed_shape", *{**ATTN, **change}.values())
