@@ -12,18 +12,27 @@
 // 4h + i, 8 + 4h + i (h: half of the wave, i < 4); V comes out of its row-major tile in that order through the
 // transposing LDS read.  P goes in rounded to the rows' type: every term is off by at most half a step of that type
 // relative to itself, as every output is by its own rounding.
+//
+// Schedule: the stages of a tile -- S(t) and O(t) on the matrix cores, F(t), the softmax, on the vector units -- run
+// one behind the other in a wave: step t issues S(t + 1) and O(t - 1) around F(t), so that the products of a step
+// do not depend on its vector work and the two can be interleaved instruction by instruction.  K is stored into LDS two
+// tiles ahead of its use and V one step, each by half of the waves; the rings are two deep.  Rows of K lie 2 D + 16 bytes
+// apart and those of V an odd multiple of 64: the operand reads of 16 (32) lanes then touch every bank once.
+//
+// The reference that the exponentials are taken relative to follows the maximum lazily: it is raised when a tile
+// exceeds it by more than 2^8 (a probability is then at most 2^8 and the sums at most 2^8 times as large, far
+// inside the range of all types), so that rescaling the sums is rare.
+//
+// Bound by the matrix cores at heads of 128 and long sequences (one prompt of 16384 tokens, 32 / 8 heads: 2007 us, 1096 TFLOP/s,
+// a large matrix product of the library 1130); by the vector units at heads of 64 (per step 84 vector
+// instructions, 17 of them exponentials of four times the time, to 8 products: 4 prompts of 8192, 14 / 2 heads, 826 TFLOP/s).
 #include "device_utils.hpp"
 #include "launch_common.hpp"
 #include "packed_rows.hpp"
+#include "q4_common.hpp"
 
 #include <math.h>
 
-#ifndef AP_W
-#define AP_W 8
-#endif
-#ifndef AP_LB
-#define AP_LB 1
-#endif
 namespace lg {
 
 struct AttnPackedParams {
@@ -36,6 +45,7 @@ struct AttnPackedParams {
     int64_t q_stride, k_stride, v_stride, out_stride;
     float scale_log2e;
     int causal;
+    int ordered;  // longest sequences first
 };
 
 constexpr int kApKeys = 32;
@@ -111,151 +121,13 @@ __device__ __forceinline__ void attn_packed_write(unsigned short* out, unsigned 
     }
 }
 
+constexpr float kApLazy = 8.0f;
+
 template <typename T, int D, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void attn_packed_kernel(const AttnPackedParams p) {
-    constexpr int kCols = 32 * WAVES, kPieces = D / 8, kStride = D + 8;
-    __shared__ __attribute__((aligned(16))) unsigned short lds[2 * kApKeys * kStride];
-    static_assert(WAVES * 16 <= 2 * kApKeys, "the columns on their way out fit");
-    unsigned short *const ks = lds, *const vs = lds + kApKeys * kStride;
-    __shared__ unsigned odd_waves[WAVES];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int h = lane >> 5, col = lane & 31;
-    const int kvh = (int)(blockIdx.x % (unsigned)p.hkv);
-    const PackedTile t = packed_tile(p.cu, p.num_seqs, p.total, p.g, kCols, (int)(blockIdx.x / (unsigned)p.hkv));
-    const int cols = t.rows * p.g;
-    const int groups = (cols + kCols - 1) / kCols;
-    const int group = groups - 1 - t.tile;  // (the last columns see the most keys: they start first)
-    if (t.rows <= 0 || group < 0) return;
-    const int c0 = group * kCols + wave * 32;
-    const int gc = c0 + col;
-    const bool live = gc < cols;
-    const int tok = (live ? gc : cols - 1) / p.g, head = kvh * p.g + (live ? gc : cols - 1) % p.g;
-    const int vis = p.causal ? tok + 1 : t.rows;  // keys of this lane's column
-    const int last = (group + 1) * kCols < cols ? (group + 1) * kCols - 1 : cols - 1;
-    const int visible = p.causal ? last / p.g + 1 : t.rows;  // ... of the workgroup's last
-    const int first_vis = p.causal ? (c0 < cols ? c0 : cols - 1) / p.g + 1 : t.rows;  // ... of the wave's first
-    const int last_vis = p.causal ? (c0 + 31 < cols ? c0 + 31 : cols - 1) / p.g + 1 : t.rows;
-
-    uint4_t qb[D / 16];
-    {
-        const unsigned short* q = p.q + (int64_t)(t.row0 + tok) * p.q_stride + (int64_t)head * D + 8 * h;
-#pragma unroll
-        for (int j = 0; j < D / 16; ++j) qb[j] = *reinterpret_cast<const uint4_t*>(q + 16 * j);
-    }
-    const unsigned short* kp = p.k + (int64_t)t.row0 * p.k_stride + (int64_t)kvh * D;
-    const unsigned short* vp = p.v + (int64_t)t.row0 * p.v_stride + (int64_t)kvh * D;
-    const int s16 = lane & 15;
-    const int v_lane = (4 * h + (s16 >> 2)) * kStride + 16 * ((lane >> 4) & 1) + 4 * (s16 & 3);
-    auto v_operand = [&](int kb, int dt) LG_INLINE {
-        typedef short short4_t __attribute__((ext_vector_type(4)));
-        typedef __attribute__((address_space(3))) short4_t lds_short4_t;
-        const unsigned short* a = vs + v_lane + 16 * kb * kStride + 32 * dt;
-        const uint2_t lo = __builtin_bit_cast(uint2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4_t*)a));
-        const uint2_t hi = __builtin_bit_cast(
-            uint2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4_t*)(a + 8 * kStride)));
-        return uint4_t{lo[0], lo[1], hi[0], hi[1]};
-    };
-
-    float m, l;
-    float16_t o[D / 32];
-    // CAREFUL: a key that a column does not see has the probability 0 there, and 0 times an infinity or NaN of its
-    // V row is a NaN.  The first walk takes no notice; if its results are not all finite, a second one takes
-    // a pass of its own for every number of keys that a column of the wave sees in a tile.
-    auto walk = [&](auto careful_c) LG_INLINE {
-        constexpr bool CAREFUL = decltype(careful_c)::value != 0;
-        m = -INFINITY;
-        l = 0.0f;
-#pragma unroll
-        for (int dt = 0; dt < D / 32; ++dt)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) o[dt][e] = 0.0f;
-        for (int key0 = 0; key0 < visible; key0 += kApKeys) {
-            __syncthreads();
-            for (int i = tid; i < kApKeys * kPieces; i += 64 * WAVES) {
-                const int key = i / kPieces, piece = i - key * kPieces;
-                // (past the last visible key that key again: its probability is 0 for everybody who sees less)
-                const int64_t row = key0 + key < visible ? key0 + key : visible - 1;
-                *reinterpret_cast<uint4_t*>(ks + key * kStride + 8 * piece) =
-                    *reinterpret_cast<const uint4_t*>(kp + row * p.k_stride + 8 * piece);
-                *reinterpret_cast<uint4_t*>(vs + key * kStride + 8 * piece) =
-                    *reinterpret_cast<const uint4_t*>(vp + row * p.v_stride + 8 * piece);
-            }
-            __syncthreads();
-            float16_t sc;
-#pragma unroll
-            for (int e = 0; e < 16; ++e) sc[e] = 0.0f;
-#pragma unroll
-            for (int j = 0; j < D / 16; ++j)
-                sc = T::mfma32(*reinterpret_cast<const uint4_t*>(ks + col * kStride + 16 * j + 8 * h), qb[j], sc);
-            uint4_t pb[2];
-            const float alpha = attn_packed_softmax<T>(sc, key0 + 4 * h, vis, p.scale_log2e, m, l, pb);
-#pragma unroll
-            for (int dt = 0; dt < D / 32; ++dt)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) o[dt][e] *= alpha;
-            if (!CAREFUL || key0 + kApKeys <= first_vis) {
-#pragma unroll
-                for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                    for (int dt = 0; dt < D / 32; ++dt) o[dt] = T::mfma32(v_operand(kb, dt), pb[kb], o[dt]);
-            } else {
-                for (int seen = first_vis; seen <= last_vis; ++seen) {
-#pragma unroll
-                    for (int dt = 0; dt < D / 32; ++dt) {
-                        float16_t acc = o[dt];
-#pragma unroll
-                        for (int kb = 0; kb < 2; ++kb)
-                            acc = T::mfma32(attn_packed_first_keys(v_operand(kb, dt), kb, seen - key0 - 4 * h), pb[kb], acc);
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) o[dt][e] = vis == seen ? acc[e] : o[dt][e];
-                    }
-                }
-            }
-        }
-        l += lane_xor_f32<32>(l);
-    };
-    walk(ic<0>{});
-    {
-        float odd = 0.0f;  // NaN if a result is not finite
-#pragma unroll
-        for (int dt = 0; dt < D / 32; ++dt)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) odd = fmaf(o[dt][e], 0.0f, odd);
-        const bool any = __builtin_amdgcn_ballot_w64(odd != odd) != 0;
-        if (lane == 0) odd_waves[wave] = any;
-        __syncthreads();
-        unsigned all = 0;
-#pragma unroll
-        for (int w = 0; w < WAVES; ++w) all |= odd_waves[w];
-        if (__builtin_amdgcn_readfirstlane(all) != 0) {
-            walk(ic<1>{});
-            __syncthreads();
-        }
-    }
-    if (c0 >= cols) return;
-    const int tok0 = c0 / p.g;  // of the wave's first column
-    attn_packed_write<T, D>(p.out + (int64_t)(t.row0 + tok0) * p.out_stride,
-                            (unsigned)(tok - tok0) * (unsigned)p.out_stride + (unsigned)(head * D), cols - c0,
-                            lds + wave * 16 * kStride, o, l);
-}
-
-// The same for heads of 64 and 128 and long sequences: eight waves, two per SIMD, over 256 columns, and the stages of a
-// tile of 32 keys -- S(t) = K . Q^T and O(t) = V^T . P on the matrix cores, F(t), the softmax, on the vector units --
-// run one behind the other in a wave: step t issues S(t + 1) and O(t - 1) around F(t), so that the products of a step
-// do not depend on its vector work and the two can be interleaved instruction by instruction.  K is stored into LDS two
-// tiles ahead of its use and V one step, by waves 0-3 and 4-7; the rings are two deep.  Rows of K lie 2 D + 16 bytes
-// apart and those of V 2 D + 64: the operand reads of 16 (32) lanes then touch every bank once.
-//
-// The reference that the exponentials are taken relative to follows the maximum lazily: it is raised when a tile
-// exceeds it by more than 2^8 (a probability is then at most 2^8 and the sums at most 2^8 times as large, far
-// inside the range of all types), so that rescaling the sums is rare.
-constexpr float kPipeLazy = 8.0f;
-
-template <typename T, int D, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, AP_LB) void attn_packed_pipe_kernel(const AttnPackedParams p) {
     constexpr int kCols = 32 * WAVES, kMovers = 32 * WAVES;  // threads that move K, and V
     constexpr int kSteps = D / 16, kTiles = D / 32;  // operands of K (and of V) per key tile; output tiles
-    constexpr int kKRow = D + 8, kVRow = D + 32;     // elements
+    constexpr int kKRow = D + 8, kVRow = D / 32 % 2 ? D : D + 32;  // elements
     constexpr int kKTile = kApKeys * kKRow, kVTile = kApKeys * kVRow;
     constexpr int kPer = kApKeys * D / 8 / kMovers;      // 16-byte pieces that a thread moves per tile
     __shared__ __attribute__((aligned(16))) unsigned short lds[2 * kKTile + 2 * kVTile];
@@ -265,7 +137,9 @@ __global__ __launch_bounds__(64 * WAVES, AP_LB) void attn_packed_pipe_kernel(con
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int h = lane >> 5, col = lane & 31;
     const int kvh = (int)(blockIdx.x % (unsigned)p.hkv);
-    const PackedTile t = packed_tile(p.cu, p.num_seqs, p.total, p.g, kCols, (int)(blockIdx.x / (unsigned)p.hkv));
+    const int at = (int)(blockIdx.x / (unsigned)p.hkv);
+    const PackedTile t = p.ordered != 0 ? packed_tile_ordered(p.cu, p.num_seqs, p.total, p.g, kCols, at)
+                                                      : packed_tile(p.cu, p.num_seqs, p.total, p.g, kCols, at);
     const int cols = t.rows * p.g;
     const int groups = (cols + kCols - 1) / kCols;
     const int group = groups - 1 - t.tile;  // (the last columns see the most keys: they start first)
@@ -292,26 +166,26 @@ __global__ __launch_bounds__(64 * WAVES, AP_LB) void attn_packed_pipe_kernel(con
     const bool moves_v = wave >= WAVES / 2;
     const int64_t stride = moves_v ? p.v_stride : p.k_stride;
     const unsigned short* const src = (moves_v ? p.v : p.k) + (int64_t)t.row0 * stride + (int64_t)kvh * D;
-    const unsigned piece = (unsigned)(tid % kMovers) % (D / 8), key_of = (unsigned)(tid % kMovers) / (D / 8);
-    constexpr int kRowsPer = kMovers / (D / 8);  // keys between a thread's pieces
     struct Regs {
         uint4_t x[kPer];
     };
+    auto key_of = [&](int u) LG_INLINE { return (tid % kMovers + kMovers * u) / (D / 8); };
+    auto piece_of = [&](int u) LG_INLINE { return (tid % kMovers + kMovers * u) % (D / 8); };
     auto gload = [&](int tile, Regs& r) LG_INLINE {
         // (past the last visible key that key again: its probability is 0 for everybody who sees less)
         const int key0 = min(tile * kApKeys, visible - 1);
         const unsigned short* at = src + (int64_t)key0 * stride;
 #pragma unroll
         for (int u = 0; u < kPer; ++u) {
-            const unsigned k = (unsigned)min((int)key_of + kRowsPer * u, visible - 1 - key0);
-            r.x[u] = *reinterpret_cast<const uint4_t*>(at + (k * (unsigned)stride + 8u * piece));
+            const unsigned k = (unsigned)min(key_of(u), visible - 1 - key0);
+            r.x[u] = *reinterpret_cast<const uint4_t*>(at + (k * (unsigned)stride + 8u * (unsigned)piece_of(u)));
         }
     };
     auto lstore = [&](int buf, const Regs& r) LG_INLINE {
-        unsigned short* at = moves_v ? vs + buf * kVTile + key_of * kVRow : ks + buf * kKTile + key_of * kKRow;
-        const int step = kRowsPer * (moves_v ? kVRow : kKRow);
+        unsigned short* at = moves_v ? vs + buf * kVTile : ks + buf * kKTile;
+        const int row = moves_v ? kVRow : kKRow;
 #pragma unroll
-        for (int u = 0; u < kPer; ++u) *reinterpret_cast<uint4_t*>(at + u * step + 8 * piece) = r.x[u];
+        for (int u = 0; u < kPer; ++u) *reinterpret_cast<uint4_t*>(at + key_of(u) * row + 8 * piece_of(u)) = r.x[u];
     };
     const int s16 = lane & 15;
     const int v_lane = (4 * h + (s16 >> 2)) * kVRow + 16 * ((lane >> 4) & 1) + 4 * (s16 & 3);
@@ -365,7 +239,7 @@ __global__ __launch_bounds__(64 * WAVES, AP_LB) void attn_packed_pipe_kernel(con
             }
         }
         tm = fmaxf(tm, lane_xor_f32<32>(tm)) * p.scale_log2e;
-        const bool raise = tm > m + kPipeLazy;
+        const bool raise = tm > m + kApLazy;
         const float alpha = raise ? fast_exp2(m - tm) : 1.0f;
         m = raise ? tm : m;
         const float ref = m == -INFINITY ? 0.0f : -m;
@@ -529,32 +403,30 @@ __global__ __launch_bounds__(64 * WAVES, AP_LB) void attn_packed_pipe_kernel(con
                             lds + wave * 16 * kKRow, o, l);
 }
 
-template <typename T, int D>
-static hipError_t attn_packed_launch(const AttnPackedParams& p, hipStream_t stream) {
-    constexpr int kWaves = 4;
-    const int64_t tiles = packed_tiles(p.total, p.num_seqs, p.g, 32 * kWaves);
-    attn_packed_kernel<T, D, kWaves><<<(unsigned)(tiles * p.hkv), 64 * kWaves, 0, stream>>>(p);
-    return hipGetLastError();
-}
-
 template <typename T, int D, int WAVES>
-static hipError_t attn_packed_pipe_launch(const AttnPackedParams& p, hipStream_t stream) {
+static hipError_t attn_packed_launch(const AttnPackedParams& p, hipStream_t stream) {
     const int64_t tiles = packed_tiles(p.total, p.num_seqs, p.g, 32 * WAVES);
-    attn_packed_pipe_kernel<T, D, WAVES><<<(unsigned)(tiles * p.hkv), 64 * WAVES, 0, stream>>>(p);
+    attn_packed_kernel<T, D, WAVES><<<(unsigned)(tiles * p.hkv), 64 * WAVES, 0, stream>>>(p);
     return hipGetLastError();
 }
 
 template <typename T>
 static hipError_t attn_packed_by_width(const AttnPackedParams& p, int d, hipStream_t stream) {
+    // 256 columns to a workgroup (eight waves, K and V moved half as often) where the sequences are long and there are
+    // many of them; otherwise 128, of which a compute unit holds two or three that fill each other's waits.  us, 8 / 4 waves, 128
+    // wide: one of 16384, 32 / 8 heads, 2007 / 2107; 4 x 4096, 12 / 2, 397 / 416; one of 8192, 12 / 2, 236 / 229; one of 4096,
+    // 32 / 8, 156 / 154; 16 of 512, 32 / 8, 76 / 71.  64 wide: 4 x 8192, 14 / 2, 586 / 582; one of 2048 41 / 31.
+    const bool wide = d == 128 && p.total >= 4096 * (int64_t)p.num_seqs &&
+                      packed_tiles(p.total, p.num_seqs, p.g, 256) * p.hkv >= 3 * device_cu_count();
     switch (d) {
-        case 32: return attn_packed_launch<T, 32>(p, stream);
-        case 64: return attn_packed_pipe_launch<T, 64, AP_W>(p, stream);
-        case 96: return attn_packed_launch<T, 96>(p, stream);
-        case 128: return attn_packed_pipe_launch<T, 128, AP_W>(p, stream);
-        case 160: return attn_packed_launch<T, 160>(p, stream);
-        case 192: return attn_packed_launch<T, 192>(p, stream);
-        case 224: return attn_packed_launch<T, 224>(p, stream);
-        default: return attn_packed_launch<T, 256>(p, stream);
+        case 32: return attn_packed_launch<T, 32, 4>(p, stream);
+        case 64: return attn_packed_launch<T, 64, 4>(p, stream);
+        case 96: return attn_packed_launch<T, 96, 4>(p, stream);
+        case 128: return wide ? attn_packed_launch<T, 128, 8>(p, stream) : attn_packed_launch<T, 128, 4>(p, stream);
+        case 160: return attn_packed_launch<T, 160, 4>(p, stream);
+        case 192: return attn_packed_launch<T, 192, 4>(p, stream);
+        case 224: return attn_packed_launch<T, 224, 4>(p, stream);
+        default: return attn_packed_launch<T, 256, 4>(p, stream);
     }
 }
 
@@ -587,6 +459,9 @@ static logismos_status_t attn_packed(bool bf16, const void* q, const void* k, co
     p.out_stride = out_stride;
     p.scale_log2e = scale * 1.4426950408889634f;
     p.causal = causal != 0;
+    // (putting them in order takes every workgroup about 1 us: 8 prompts of 100 to 4096 tokens 93 -> 85 us, 8 of 1000 43 -> 40,
+    // but 16 of 512 76 -> 79)
+    p.ordered = num_seqs > 1 && num_seqs <= kPackedOrdered && total > 512 * (int64_t)num_seqs;
     hipStream_t st = static_cast<hipStream_t>(stream);
     return static_cast<logismos_status_t>(bf16 ? attn_packed_by_width<PackedBf16>(p, d, st)
                                                : attn_packed_by_width<PackedF16>(p, d, st));

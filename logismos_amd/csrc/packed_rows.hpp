@@ -98,4 +98,43 @@ __device__ __forceinline__ PackedTile packed_tile(const int32_t* __restrict__ cu
     return t;
 }
 
+// The same in the order of the sequences' lengths, longest first, for up to kPackedOrdered of them (every lane
+// holds one): workgroups start in the order of their index, and long ones that start last are waited for by everybody.  The tiles
+// of a sequence stay side by side, last ones first.  Every sequence has exactly the tiles that it needs.
+constexpr int kPackedOrdered = 63;
+__device__ __forceinline__ PackedTile packed_tile_ordered(const int32_t* __restrict__ cu, int num_seqs, int total,
+                                                          int per_row, int tile, int b) {
+    const int lane = threadIdx.x & 63;
+    const int edge = cu[lane < num_seqs ? lane : num_seqs];
+    const int next = __shfl_down(edge, 1);
+    int rows = edge >= 0 && edge < total && lane < num_seqs ? (next < total ? next : total) - edge : 0;
+    rows = rows > 0 ? rows : 0;
+    const int tiles = (int)(((unsigned)rows * (unsigned)per_row + (unsigned)tile - 1) / (unsigned)tile);
+    // (one key per lane, all different: longer first, then the earlier one; lanes behind the last have no rows and no tiles)
+    const int key = rows * 64 + (63 - lane);
+    int before = 0;  // tiles of the sequences in front of this lane's
+    const int first = __builtin_amdgcn_readfirstlane(rows);
+    if (__builtin_amdgcn_ballot_w64(lane < num_seqs && rows != first) == 0) {
+        before = lane * tiles;
+    } else {
+        for (int j0 = 0; j0 < num_seqs; j0 += 8)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int other = __builtin_amdgcn_readlane(key, j0 + j);
+                const int theirs =
+                    (int)(((unsigned)(other >> 6) * (unsigned)per_row + (unsigned)tile - 1) / (unsigned)tile);
+                before += other > key ? theirs : 0;
+            }
+    }
+    const uint64_t mine = __builtin_amdgcn_ballot_w64(b >= before && b < before + tiles);
+    PackedTile t = {0, 0, 0, 0, 0};
+    if (mine == 0) return t;
+    const int s = __builtin_ctzll(mine);
+    t.seq = s;
+    t.row0 = __builtin_amdgcn_readlane(edge, s);
+    t.rows = __builtin_amdgcn_readlane(rows, s);
+    t.tile = b - __builtin_amdgcn_readlane(before, s);
+    return t;
+}
+
 }  // namespace lg
