@@ -65,8 +65,8 @@ __global__ __launch_bounds__(256, 2) void adapter_down_kernel(const AdapterParam
     const int r0 = t.tile * 16 * MT;
     if (r0 >= t.rows || t.of < 0 || t.of >= p.adapters) return;
     const int rank0 = blockIdx.y * 16 * RT;
-    // (ranks of the first tile are not waited for: what lies behind the rank is left out when v is read)
-    if ((RT > 1 || rank0 > 0) && rank0 >= adapter_rank(p, t.of)) return;
+    // (ranks of the first tiles are not waited for: what lies behind the rank is left out when v is read)
+    if (rank0 > 0 && rank0 >= adapter_rank(p, t.of)) return;
     const unsigned short* x[MT];
     const unsigned short* a[RT];
 #pragma unroll
@@ -154,16 +154,18 @@ __global__ __launch_bounds__(256, RS == 8 ? 1 : 2) void adapter_up_kernel(const 
                                            p.adapter_of_seq);
     const int r0 = t.tile * kRows;
     if (r0 >= t.rows) return;
-    const int rank = adapter_rank(p, t.of);
-    if (rank == 0 && p.base == p.out) return;
+    // What hangs on nothing but the tile is asked for in one go: rank and scale, the parts of v, the base.
+    const bool named = t.of >= 0 && t.of < p.adapters;
+    if (!named && p.base == p.out) return;
+    const int raw_rank = p.ranks[named ? t.of : 0];
+    const float scale = p.scales[named ? t.of : 0];
     const int left = t.rows - r0 < kRows ? t.rows - r0 : kRows;  // rows of this tile
     const int64_t row0 = t.row0 + r0;
     const int n_last = (slice + 1) * p.n_slice < p.n ? (slice + 1) * p.n_slice : p.n;
     int n0 = slice * p.n_slice + 64 * wave;
     // A wave's 64 outputs are four tiles of 16, ordered so that a lane (c, q) holds 16 bytes side by side of row c and
     // the four q of a row 64: fp32, element i of tile j is output 16 j + 4 q + i; 16 bits, 32 (j / 2) + 8 q + 4 (j % 2) + i.
-    // What comes from memory is asked for ahead: the base by a step, B as soon as the step's products are done, the first step's
-    // in front of v.
+    // What comes from memory is asked for ahead: the base by a step, B as soon as the step's products are done.
     constexpr int kBase = F32 ? 4 : 2, kSize = F32 ? 4 : 2;
     // (rows behind the tile's last, outputs behind the last and ranks behind the rank: others in their place, which count
     // for nothing -- a load under a condition of its own is a branch around it.  Offsets from the tile's first row and the
@@ -171,7 +173,7 @@ __global__ __launch_bounds__(256, RS == 8 ? 1 : 2) void adapter_up_kernel(const 
     uint4_t even[MT][kBase], odd[MT][kBase], bv[RS][4];
     const char* const base = static_cast<const char*>(p.base) + row0 * p.base_stride * kSize;
     char* const out = static_cast<char*>(p.out) + row0 * p.out_stride * kSize;
-    const char* const b = reinterpret_cast<const char*>(p.b + (int64_t)(rank > 0 ? t.of : 0) * p.n * p.max_rank);
+    const char* const b = reinterpret_cast<const char*>(p.b + (int64_t)(named ? t.of : 0) * p.n * p.max_rank);
     auto load_base = [&](uint4_t(&w)[MT][kBase], int at_n) LG_INLINE {
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
@@ -183,6 +185,7 @@ __global__ __launch_bounds__(256, RS == 8 ? 1 : 2) void adapter_up_kernel(const 
             }
         }
     };
+    int rank = 0;
     auto load_b = [&](int at_n) LG_INLINE {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -193,38 +196,42 @@ __global__ __launch_bounds__(256, RS == 8 ? 1 : 2) void adapter_up_kernel(const 
                 bv[s][j] = *reinterpret_cast<const uint4_t*>(b + (row + (32 * s + 8 * q < rank ? 32 * s + 8 * q : 0)) * 2u);
         }
     };
+    // Thread (row, chunk of eight ranks), the chunks of a row side by side; four parts of v at a time.
+    struct Parts {
+        float4_t w[4][2];
+    };
+    const int64_t part = (int64_t)p.total * p.max_rank;
+    auto v_at = [&](int i) LG_INLINE {
+        return p.v + (row0 + min(i / kChunks, left - 1)) * p.max_rank + min(8 * (i % kChunks), p.max_rank - 8);
+    };
+    auto load_v = [&](Parts& v, const float* at) LG_INLINE {
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                v.w[s][e] = *reinterpret_cast<const float4_t*>(at + min(s, p.parts - 1) * part + 4 * e);
+    };
+    Parts v;
+    load_v(v, v_at(threadIdx.x));
+    load_base(even, min(n0, p.n - 1));
+    if (named) rank = max(0, min(__builtin_amdgcn_readfirstlane(raw_rank), p.max_rank));
+    if (rank == 0 && p.base == p.out) return;
     if (rank > 0) {
-        // thread (row, chunk), the chunks of a row side by side.  (The parts of v are asked for first, four at a time: what is
-        // waited for first must not stand behind the base and B.)
-        const int64_t part = (int64_t)p.total * p.max_rank;
-        const float scale = p.scales[t.of];
-        bool first = true;
-        for (int i = threadIdx.x; first || i < kRows * kChunks; i += 256) {
+        load_b(n0);
+        for (int i = threadIdx.x; i < kRows * kChunks; i += 256) {
             const int row = i / kChunks, chunk = i % kChunks, r = 8 * chunk;
-            const bool mine = i < kRows * kChunks;
-            const float* v = p.v + (row0 + (row < left ? row : left - 1)) * p.max_rank + (r < rank ? r : 0);
+            if (i >= 256) load_v(v, v_at(i));
             float u[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) u[e] = 0.0f;
-            float4_t w[4][2];
-#pragma unroll
-            for (int s = 0; s < 4; ++s)
-#pragma unroll
-                for (int e = 0; e < 2; ++e)
-                    w[s][e] = *reinterpret_cast<const float4_t*>(v + min(s, p.parts - 1) * part + 4 * e);
-            if (first && n0 < n_last) {
-                load_base(even, n0);
-                load_b(n0);
-            }
-            first = false;
 #pragma unroll
             for (int s = 0; s < 4; ++s)
                 if (s < p.parts) {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) u[e] += w[s][e >> 2][e & 3];
+                    for (int e = 0; e < 8; ++e) u[e] += v.w[s][e >> 2][e & 3];
                 }
             for (int s = 4; s < p.parts; ++s) {
-                const float4_t* src = reinterpret_cast<const float4_t*>(v + s * part);
+                const float4_t* src = reinterpret_cast<const float4_t*>(v_at(i) + s * part);
                 const float4_t u0 = src[0], u1 = src[1];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
@@ -232,7 +239,6 @@ __global__ __launch_bounds__(256, RS == 8 ? 1 : 2) void adapter_up_kernel(const 
                     u[4 + e] += u1[e];
                 }
             }
-            if (!mine) continue;
             float top = 0.0f;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
@@ -359,9 +365,10 @@ __global__ __launch_bounds__(256, RS == 8 ? 1 : 2) void adapter_up_kernel(const 
             }
         }
     } else {
-        for (; n0 < n_last; n0 += 256) {
-            load_base(even, n0);
+        while (n0 < n_last) {
             compute(ic<0>{}, ic<0>{}, even, n0, 0);
+            n0 += 256;
+            if (n0 < n_last) load_base(even, n0);
         }
     }
 }
