@@ -2,17 +2,19 @@
 //
 //   out[t][:] = base[t][:] + s_a * (x[t] . A_a^T) . B_a^T,   a = the adapter of the row's sequence
 //
-// Two launches.  The first takes a tile of one sequence's rows through A: v = x . A^T in fp32 into the workspace, in K parts
-// (v is small; adding the parts up is the second launch's first step, in their order).  The second takes the
-// same rows through B and adds the base.  Products on the matrix cores, the ranks as rows of the first product's
-// result and the rows of x as its columns, the outputs as rows of the second's.
+// Two launches (one for few rows).  The first takes a tile of one sequence's rows through A: v = x . A^T in fp32 into the
+// workspace, in K parts (v is small; adding the parts up is the second launch's first step, in their order).  The second
+// takes the same rows through B and adds the base.  Products on the matrix cores.
 //
 // s v has to be an operand of the second product, so it is split into 16-bit terms: per row scaled by a power
 // of two that brings its largest value into [1, 2) (exact, and undone in the fp32 result; fp16 could not hold the values
 // as they are), then the rounded value and what the rounding left.  fp16: two terms, 22 bits; bf16: two terms,
 // 16 bits, for outputs of 8, three, 24 bits, for fp32 outputs.
 //
-// Bound by memory: x, base and out once, A and B of the adapters in use.
+// Bound by memory: x, base and out once, A and B of the adapters in use.  16 prompts of 512 x 4096, rank 64, 24576 outputs in 16
+// bits: 900 MB in 237 us, 3.8 TB/s (a large copy 5.2; the first launch 26 us, the second 211: its beginnings, and
+// vector work that the memory time does not all cover); 13 single rows and 5 chunks of 31 to 600, 8960 columns to 1536 in
+// fp32: 54 MB in 23 us; 32 single rows on 8 adapters, 4096 to 6144: 10.9 us, a chain of dependent loads.
 #include "device_utils.hpp"
 #include "launch_common.hpp"
 #include "packed_rows.hpp"
@@ -51,14 +53,31 @@ __device__ __forceinline__ int adapter_rank(const AdapterParams& p, int adapter)
     return r < 0 ? 0 : r < p.max_rank ? r : p.max_rank;
 }
 
+// A matrix operand (16 rows of 32 elements: lane (c, q) = row c, elements 8 q .. + 7) out of rows in memory.  Loaded as it
+// is used, neighbouring lanes ask for different rows, and 16 bytes from each of 64 rows take four times as long as 64 bytes from
+// each of 16 (measured in L2: 38 against 153 bytes per ns and compute unit, whatever the rows' distance).  So lane l loads
+// chunk operand_chunk() of row l / 4, and the values change lanes through 1 KB of LDS that belongs to the wave; the
+// chunks' order differs from row to row so that both ways touch every bank once.
+__device__ __forceinline__ int operand_row() { return (threadIdx.x & 63) >> 2; }
+__device__ __forceinline__ int operand_chunk() { return (threadIdx.x & 3) ^ ((threadIdx.x >> 4) & 3); }
+__device__ __forceinline__ uint4_t operand_of(uint4_t loaded, uint4_t* scratch) {
+    const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
+    scratch[lane] = loaded;
+    __builtin_amdgcn_wave_barrier();
+    const uint4_t v = scratch[4 * c + (q ^ (c >> 2))];
+    __builtin_amdgcn_wave_barrier();
+    return v;
+}
+
 // v[part][t][r] = sum over the part's columns of x[t][c] * A[r][c].  grid (tiles of 16 MT rows by K parts, 16 RT ranks
 // each); the four waves share the part's steps of 32 columns and add up in LDS.
 template <typename T, int MT, int RT>
 __global__ __launch_bounds__(256, 2) void adapter_down_kernel(const AdapterParams p) {
     constexpr int kDeep = MT > 1 ? 4 : 8;  // steps asked for together, side by side: whole cache lines
-    __shared__ float sums[4][MT * RT * 256];
+    constexpr int kSlots = MT * RT > 4 ? MT * RT : 4;  // (1 KB each, on their way to the sums the operands' scratch)
+    __shared__ __attribute__((aligned(16))) float sums[4][kSlots * 256];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int c = lane & 15, q = lane >> 4;
+    uint4_t* const scratch = reinterpret_cast<uint4_t*>(sums[wave]);
     const int part = (int)(blockIdx.x % (unsigned)p.parts);
     const PackedTile t = packed_tile<true>(p.cu, p.num_seqs, p.total, 1, 16 * MT, (int)(blockIdx.x / (unsigned)p.parts),
                                            p.adapter_of_seq);
@@ -71,13 +90,11 @@ __global__ __launch_bounds__(256, 2) void adapter_down_kernel(const AdapterParam
     const unsigned short* a[RT];
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
-        const int row = r0 + 16 * m + c < t.rows ? r0 + 16 * m + c : t.rows - 1;
-        x[m] = p.x + (int64_t)(t.row0 + row) * p.x_stride;
+        x[m] = p.x + (int64_t)(t.row0 + min(r0 + 16 * m + operand_row(), t.rows - 1)) * p.x_stride;
     }
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
-        const int r = rank0 + 16 * i + c < p.max_rank ? rank0 + 16 * i + c : p.max_rank - 1;
-        a[i] = p.a + ((int64_t)t.of * p.max_rank + r) * p.k;
+        a[i] = p.a + ((int64_t)t.of * p.max_rank + min(rank0 + 16 * i + operand_row(), p.max_rank - 1)) * p.k;
     }
     const int all = (p.k + 31) / 32;
     const int first = part * p.part_steps + wave * kDeep;
@@ -94,7 +111,7 @@ __global__ __launch_bounds__(256, 2) void adapter_down_kernel(const AdapterParam
         uint4_t xv[kDeep][MT], av[kDeep][RT];
 #pragma unroll
         for (int d = 0; d < kDeep; ++d) {
-            const int want = 32 * (s0 + d) + 8 * q;
+            const int want = 32 * (s0 + d) + 8 * operand_chunk();
             const int at = WHOLE || want < p.k ? want : p.k - 8;
 #pragma unroll
             for (int m = 0; m < MT; ++m) xv[d][m] = *reinterpret_cast<const uint4_t*>(x[m] + at);
@@ -105,7 +122,7 @@ __global__ __launch_bounds__(256, 2) void adapter_down_kernel(const AdapterParam
 #pragma unroll
         for (int d = 0; d < kDeep; ++d) {
             if constexpr (!WHOLE) {
-                const bool in = s0 + d < last && 32 * (s0 + d) + 8 * q < p.k;
+                const bool in = s0 + d < last && 32 * (s0 + d) + 8 * operand_chunk() < p.k;
 #pragma unroll
                 for (int m = 0; m < MT; ++m) xv[d][m] = in ? xv[d][m] : uint4_t{0, 0, 0, 0};
 #pragma unroll
@@ -113,8 +130,13 @@ __global__ __launch_bounds__(256, 2) void adapter_down_kernel(const AdapterParam
             }
 #pragma unroll
             for (int m = 0; m < MT; ++m)
+                xv[d][m] = operand_of(xv[d][m], scratch + (d * (MT + RT) + m) % kSlots * 64);
 #pragma unroll
-                for (int i = 0; i < RT; ++i) acc[m][i] = T::mfma16(av[d][i], xv[d][m], acc[m][i]);
+            for (int i = 0; i < RT; ++i) {
+                const uint4_t av_of = operand_of(av[d][i], scratch + (d * (MT + RT) + MT + i) % kSlots * 64);
+#pragma unroll
+                for (int m = 0; m < MT; ++m) acc[m][i] = T::mfma16(av_of, xv[d][m], acc[m][i]);
+            }
         }
     };
     int s0 = first;
@@ -138,17 +160,98 @@ __global__ __launch_bounds__(256, 2) void adapter_down_kernel(const AdapterParam
     }
 }
 
+// Eight ranks u of a row (from rank r on), the chunks of a row in neighbouring lanes: times the adapter's scale, zero behind the
+// rank and the rows, brought by a power of two to where the row's largest value lies in [1, 2), split into terms of the
+// operand's type, 64 words of four apart.  growth: what undoes the power of two.
+template <typename T, int TERMS, int CHUNKS>
+__device__ __forceinline__ void adapter_terms(float (&u)[8], bool live, int r, int rank, float scale, float* growth,
+                                              uint4_t* operand) {
+    typedef typename T::elem elem;
+    float top = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        u[e] = live && r + e < rank ? u[e] * scale : 0.0f;
+        top = fmaxf(top, fabsf(u[e]));
+    }
+#pragma unroll
+    for (int m = 1; m < CHUNKS; m *= 2) top = fmaxf(top, shfl_xor_f32(top, m));
+    const int ex = (int)(__float_as_uint(top) >> 23);  // (as far as fp32 has the power of two)
+    const int down = ex < 1 ? 1 : ex > 253 ? 253 : ex;
+    const float shrink = __uint_as_float((unsigned)(254 - down) << 23);
+    if (r == 0) *growth = __uint_as_float((unsigned)down << 23);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) u[e] *= shrink;
+#pragma unroll
+    for (int k = 0; k < TERMS; ++k) {
+        uint4_t w;
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+            w[e >> 1] = T::pack2(u[e], u[e + 1]);
+            u[e] -= (float)__builtin_bit_cast(elem, (unsigned short)(w[e >> 1] & 0xffffu));
+            u[e + 1] -= (float)__builtin_bit_cast(elem, (unsigned short)(w[e >> 1] >> 16));
+            u[e] = u[e] == u[e] ? u[e] : 0.0f;  // (an infinity is in its first term, with nothing left)
+            u[e + 1] = u[e + 1] == u[e + 1] ? u[e + 1] : 0.0f;
+        }
+        operand[64 * k] = w;
+    }
+}
+
+// Which of the eight columns of B from r on lie in front of the rank.
+__device__ __forceinline__ uint4_t adapter_keep(int r, int rank) {
+    uint4_t keep;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) keep[i] = rank >= r + 2 * i + 2 ? ~0u : rank == r + 2 * i + 1 ? 0xffffu : 0u;
+    return keep;
+}
+
+// Four outputs of a row: fp32 or two to a word.
+template <bool F32>
+struct Four {
+    typedef uint2_t bits;
+};
+template <>
+struct Four<true> {
+    typedef uint4_t bits;
+};
+// The base's and the sums that belong to them, element e of the tiles.
+template <typename T, bool F32>
+__device__ __forceinline__ typename Four<F32>::bits adapter_sum(typename Four<F32>::bits base, const float4_t (&acc)[4], int e,
+                                                                float grow) {
+    if constexpr (F32) {
+        float4_t y = __builtin_bit_cast(float4_t, base);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[j] = fmaf(acc[j][e], grow, y[j]);
+        return __builtin_bit_cast(uint4_t, y);
+    } else {
+        typedef typename T::elem elem;
+        float y[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            y[j] = fmaf(acc[j][e], grow,
+                        (float)__builtin_bit_cast(elem, (unsigned short)(j & 1 ? base[j >> 1] >> 16 : base[j >> 1] & 0xffffu)));
+        return uint2_t{T::pack2(y[0], y[1]), T::pack2(y[2], y[3])};
+    }
+}
+
 // out = base + (s v) . B^T.  grid: slices of the outputs (fastest: a slice of B then stays in the L2 of the XCDs that
-// take it, for all rows of its adapter) by tiles of 16 MT rows; ranks in RS steps of 32.  The workgroup splits
-// s v into terms once, in the order of the matrix operand, into LDS; a wave takes 64 outputs at a time, the four
-// waves side by side.
-template <typename T, bool F32, int TERMS, int MT, int RS>
-__global__ __launch_bounds__(256, RS == 8 ? 1 : 2) void adapter_up_kernel(const AdapterParams p) {
-    constexpr int kRows = 16 * MT, kChunks = 4 * RS;  // chunks of eight ranks
-    __shared__ uint4_t operand[MT * RS * TERMS * 64];
+// take it, for all rows of its adapter) by tiles of 16 MT GROUPS rows; ranks in RS steps of 32.  The workgroup splits
+// s v into terms once, in the order of the matrix operand, into LDS.  A wave takes 16 MT rows by four tiles of 16 outputs at
+// a time; GROUPS of the four waves lie one below the other (and read the same B), the others side by side.
+//
+// The rows are the rows of the product and the outputs its columns, output 4 c + j being column c of tile j: a lane then
+// holds four outputs side by side of four rows, and the 16 lanes next to it those around them.
+template <typename T, bool F32, int TERMS, int MT, int RS, int GROUPS>
+__global__ __launch_bounds__(256, 2) void adapter_up_kernel(const AdapterParams p) {
+    constexpr int kRows = 16 * MT * GROUPS, kChunks = 4 * RS;  // rows of a tile, chunks of eight ranks
+    constexpr int kTiles = 4, kSize = F32 ? 4 : 2, kAcross = 16 * kTiles * (4 / GROUPS);
+    typedef typename Four<F32>::bits four;
+    __shared__ uint4_t operand[MT * GROUPS * RS * TERMS * 64];
     __shared__ float growth[kRows];
+    __shared__ uint4_t scratches[4][kTiles][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c = lane & 15, q = lane >> 4;
+    const int group = wave % GROUPS;
+    uint4_t(&scratch)[kTiles][64] = scratches[wave];
     const int slice = (int)(blockIdx.x % (unsigned)p.slices);
     const PackedTile t = packed_tile<true>(p.cu, p.num_seqs, p.total, 1, kRows, (int)(blockIdx.x / (unsigned)p.slices),
                                            p.adapter_of_seq);
@@ -161,40 +264,35 @@ __global__ __launch_bounds__(256, RS == 8 ? 1 : 2) void adapter_up_kernel(const 
     const float scale = p.scales[named ? t.of : 0];
     const int left = t.rows - r0 < kRows ? t.rows - r0 : kRows;  // rows of this tile
     const int64_t row0 = t.row0 + r0;
+    const int my_row = 16 * MT * group + 4 * q;  // (16 m + e: the rows of this lane)
     const int n_last = (slice + 1) * p.n_slice < p.n ? (slice + 1) * p.n_slice : p.n;
-    int n0 = slice * p.n_slice + 64 * wave;
-    // A wave's 64 outputs are four tiles of 16, ordered so that a lane (c, q) holds 16 bytes side by side of row c and
-    // the four q of a row 64: fp32, element i of tile j is output 16 j + 4 q + i; 16 bits, 32 (j / 2) + 8 q + 4 (j % 2) + i.
-    // What comes from memory is asked for ahead: the base by a step, B as soon as the step's products are done.
-    constexpr int kBase = F32 ? 4 : 2, kSize = F32 ? 4 : 2;
+    int n0 = slice * p.n_slice + 16 * kTiles * (wave / GROUPS);
     // (rows behind the tile's last, outputs behind the last and ranks behind the rank: others in their place, which count
     // for nothing -- a load under a condition of its own is a branch around it.  Offsets from the tile's first row and the
     // adapter's B have 32 bits.)
-    uint4_t even[MT][kBase], odd[MT][kBase], bv[RS][4];
+    // (B 32 ranks at a time, asked for as soon as the products of those before are done: more does not fit)
+    four even[MT][4], odd[MT][4];
+    uint4_t bv[kTiles];
     const char* const base = static_cast<const char*>(p.base) + row0 * p.base_stride * kSize;
     char* const out = static_cast<char*>(p.out) + row0 * p.out_stride * kSize;
     const char* const b = reinterpret_cast<const char*>(p.b + (int64_t)(named ? t.of : 0) * p.n * p.max_rank);
-    auto load_base = [&](uint4_t(&w)[MT][kBase], int at_n) LG_INLINE {
+    auto load_base = [&](four(&w)[MT][4], int at_n) LG_INLINE {
+        const unsigned n = (unsigned)min(at_n + kTiles * c, p.n - kTiles);
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-            const unsigned row = (unsigned)min(16 * m + c, left - 1) * (unsigned)p.base_stride;
+        for (int m = 0; m < MT; ++m)
 #pragma unroll
-            for (int e = 0; e < kBase; ++e) {
-                const unsigned n = (unsigned)min(at_n + (F32 ? 16 * e + 4 * q : 32 * e + 8 * q), p.n - 16 / kSize);
-                w[m][e] = *reinterpret_cast<const uint4_t*>(base + (row + n) * (unsigned)kSize);
-            }
-        }
+            for (int e = 0; e < 4; ++e)
+                w[m][e] = *reinterpret_cast<const four*>(
+                    base + ((unsigned)min(my_row + 16 * m + e, left - 1) * (unsigned)p.base_stride + n) * (unsigned)kSize);
     };
     int rank = 0;
-    auto load_b = [&](int at_n) LG_INLINE {
+    auto load_b = [&](int at_n, int s) LG_INLINE {
+        const int r = 32 * s + 8 * operand_chunk();
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int want = at_n + (F32 ? 16 * j + c : 32 * (j >> 1) + 8 * (c >> 2) + 4 * (j & 1) + (c & 3));
-            const unsigned row = (unsigned)min(want, p.n - 1) * (unsigned)p.max_rank;
-#pragma unroll
-            for (int s = 0; s < RS; ++s)
-                bv[s][j] = *reinterpret_cast<const uint4_t*>(b + (row + (32 * s + 8 * q < rank ? 32 * s + 8 * q : 0)) * 2u);
-        }
+        for (int j = 0; j < kTiles; ++j)
+            bv[j] = *reinterpret_cast<const uint4_t*>(
+                b + ((unsigned)min(at_n + kTiles * operand_row() + j, p.n - 1) * (unsigned)p.max_rank +
+                     (unsigned)(r < rank ? r : 0)) * 2u);
     };
     // Thread (row, chunk of eight ranks), the chunks of a row side by side; four parts of v at a time.
     struct Parts {
@@ -213,11 +311,11 @@ __global__ __launch_bounds__(256, RS == 8 ? 1 : 2) void adapter_up_kernel(const 
     };
     Parts v;
     load_v(v, v_at(threadIdx.x));
-    load_base(even, min(n0, p.n - 1));
+    load_base(even, n0);
     if (named) rank = max(0, min(__builtin_amdgcn_readfirstlane(raw_rank), p.max_rank));
     if (rank == 0 && p.base == p.out) return;
     if (rank > 0) {
-        load_b(n0);
+        load_b(n0, 0);
         for (int i = threadIdx.x; i < kRows * kChunks; i += 256) {
             const int row = i / kChunks, chunk = i % kChunks, r = 8 * chunk;
             if (i >= 256) load_v(v, v_at(i));
@@ -239,137 +337,222 @@ __global__ __launch_bounds__(256, RS == 8 ? 1 : 2) void adapter_up_kernel(const 
                     u[4 + e] += u1[e];
                 }
             }
-            float top = 0.0f;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                u[e] = row < left && r + e < rank ? u[e] * scale : 0.0f;
-                top = fmaxf(top, fabsf(u[e]));
-            }
-#pragma unroll
-            for (int m = 1; m < kChunks; m *= 2) top = fmaxf(top, shfl_xor_f32(top, m));
-            // 2^-e of the largest value's exponent e, as far as fp32 has it
-            const int ex = (int)(__float_as_uint(top) >> 23);
-            const int down = ex < 1 ? 1 : ex > 253 ? 253 : ex;
-            const float shrink = __uint_as_float((unsigned)(254 - down) << 23);
-            if (chunk == 0) growth[row] = __uint_as_float((unsigned)down << 23);
-            typedef typename T::elem elem;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) u[e] *= shrink;
-#pragma unroll
-            for (int k = 0; k < TERMS; ++k) {
-                uint4_t w;
-#pragma unroll
-                for (int e = 0; e < 8; e += 2) {
-                    w[e >> 1] = T::pack2(u[e], u[e + 1]);
-                    u[e] -= (float)__builtin_bit_cast(elem, (unsigned short)(w[e >> 1] & 0xffffu));
-                    u[e + 1] -= (float)__builtin_bit_cast(elem, (unsigned short)(w[e >> 1] >> 16));
-                    u[e] = u[e] == u[e] ? u[e] : 0.0f;  // (an infinity is in its first term, with nothing left)
-                    u[e + 1] = u[e + 1] == u[e + 1] ? u[e + 1] : 0.0f;
-                }
-                operand[(((row >> 4) * RS + (chunk >> 2)) * TERMS + k) * 64 + (chunk & 3) * 16 + (row & 15)] = w;
-            }
+            adapter_terms<T, TERMS, kChunks>(
+                u, row < left, r, rank, scale, &growth[row],
+                &operand[((row >> 4) * RS + (chunk >> 2)) * TERMS * 64 + (chunk & 3) * 16 + (row & 15)]);
         }
         __syncthreads();
     }
-    float grow[MT];
-    uint4_t keep[RS];  // (the columns of B that count)
+    uint4_t keep[RS];
+    float4_t grow[MT];
     // One step over the base `w`; WHOLE: of whole tiles, and the next one's B is asked for.
-    auto compute = [&](auto adds_c, auto whole_c, uint4_t(&w)[MT][kBase], int at_n, int next_n) LG_INLINE {
+    auto compute = [&](auto adds_c, auto whole_c, four(&w)[MT][4], int at_n, int next_n) LG_INLINE {
         constexpr bool ADDS = decltype(adds_c)::value != 0, WHOLE = decltype(whole_c)::value != 0;
-        float4_t acc[MT][4];
+        float4_t acc[MT][kTiles];
         if (ADDS) {
-            asm volatile("" ::: "memory");  // (the terms are read again: kept over the steps they would not fit)
+            asm volatile("" ::: "memory");  // (the terms are read again: kept over the steps they cost a wave its place)
 #pragma unroll
-            for (int s = 0; s < RS; ++s)
+            for (int j = 0; j < kTiles; ++j)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) bv[s][j] &= keep[s];
+                for (int m = 0; m < MT; ++m) acc[m][j] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int m = 0; m < MT; ++m) {
+            for (int s = 0; s < RS; ++s) {
+                uint4_t term[MT][TERMS];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) acc[m][j] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+                for (int m = 0; m < MT; ++m)
 #pragma unroll
-                for (int s = 0; s < RS; ++s)
+                    for (int k = 0; k < TERMS; ++k)
+                        term[m][k] = operand[(((group * MT + m) * RS + s) * TERMS + k) * 64 + lane];
 #pragma unroll
-                    for (int k = 0; k < TERMS; ++k) {
-                        const uint4_t v = operand[((m * RS + s) * TERMS + k) * 64 + lane];
+                for (int j = 0; j < kTiles; ++j) {
+                    const uint4_t f = operand_of(bv[j] & keep[s], scratch[j]);
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) acc[m][j] = T::mfma16(bv[s][j], v, acc[m][j]);
-                    }
-            }
-            if (WHOLE) {
-                __builtin_amdgcn_sched_barrier(0);  // (into the registers that the products just read)
-                load_b(next_n);
-                __builtin_amdgcn_sched_barrier(0);
-            }
-        }
+                    for (int k = 0; k < TERMS; ++k)
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-            if (!WHOLE && 16 * m + c >= left) continue;
-            const unsigned row = (unsigned)(16 * m + c) * (unsigned)p.out_stride;
-#pragma unroll
-            for (int e = 0; e < kBase; ++e) {
-                const int n = at_n + (F32 ? 16 * e + 4 * q : 32 * e + 8 * q);
-                if (!WHOLE && n >= p.n) continue;
-                uint4_t o = w[m][e];
-                if constexpr (!ADDS) {
-                } else if constexpr (F32) {
-                    float4_t y = __builtin_bit_cast(float4_t, o);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) y[i] = fmaf(acc[m][e][i], grow[m], y[i]);
-                    o = __builtin_bit_cast(uint4_t, y);
-                } else {
-                    const auto u = __builtin_bit_cast(typename T::vec8, o);
-                    float y[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        y[i] = fmaf(acc[m][2 * e + (i >> 2)][i & 3], grow[m], (float)u[i]);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) o[i] = T::pack2(y[2 * i], y[2 * i + 1]);
+                        for (int m = 0; m < MT; ++m) acc[m][j] = T::mfma16(term[m][k], f, acc[m][j]);
                 }
-                *reinterpret_cast<uint4_t*>(out + (row + (unsigned)n) * (unsigned)kSize) = o;
+                if (s + 1 < RS) load_b(at_n, s + 1);
+                else if (WHOLE) load_b(next_n, 0);
+                __builtin_amdgcn_sched_barrier(0);  // (into the registers that the products just read)
             }
         }
+        const int n = at_n + kTiles * c;
+        if (!WHOLE && n >= p.n) return;
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (!WHOLE && my_row + 16 * m + e >= left) continue;
+                four o = w[m][e];
+                if constexpr (ADDS) o = adapter_sum<T, F32>(o, acc[m], e, grow[m][e]);
+                *reinterpret_cast<four*>(
+                    out + ((unsigned)(my_row + 16 * m + e) * (unsigned)p.out_stride + (unsigned)n) * (unsigned)kSize) = o;
+            }
     };
     if (rank > 0) {
 #pragma unroll
-        for (int m = 0; m < MT; ++m) grow[m] = growth[16 * m + c];
+        for (int m = 0; m < MT; ++m) {
+            grow[m] = *reinterpret_cast<const float4_t*>(&growth[my_row + 16 * m]);
+        }
 #pragma unroll
-        for (int s = 0; s < RS; ++s)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int r = 32 * s + 8 * q + 2 * i;
-                keep[s][i] = rank >= r + 2 ? ~0u : rank == r + 1 ? 0xffffu : 0u;
-            }
-        if (left == kRows && n_last % 64 == 0) {
+        for (int s = 0; s < RS; ++s) keep[s] = adapter_keep(32 * s + 8 * operand_chunk(), rank);
+        if (left >= 16 * MT * (group + 1) && n_last % (16 * kTiles) == 0) {
             // Straight-line code, two steps a turn: a condition around a load or a store would make every wait one for
             // everything in flight.  (The last step asks for itself again.)
-            const int end = n0 < n_last ? n0 + (n_last - 1 - n0) / 256 * 256 : 0;
+            const int end = n0 < n_last ? n0 + (n_last - 1 - n0) / kAcross * kAcross : 0;
             while (n0 < n_last) {
-                int next = min(n0 + 256, end);
+                int next = min(n0 + kAcross, end);
                 load_base(odd, next);
                 compute(ic<1>{}, ic<1>{}, even, n0, next);
-                n0 += 256;
+                n0 += kAcross;
                 if (n0 >= n_last) break;
-                next = min(n0 + 256, end);
+                next = min(n0 + kAcross, end);
                 load_base(even, next);
                 compute(ic<1>{}, ic<1>{}, odd, n0, next);
-                n0 += 256;
+                n0 += kAcross;
             }
         } else {
             while (n0 < n_last) {
                 compute(ic<1>{}, ic<0>{}, even, n0, 0);
-                n0 += 256;
+                n0 += kAcross;
                 if (n0 >= n_last) break;
                 load_base(even, n0);
-                load_b(n0);
+                load_b(n0, 0);
             }
         }
     } else {
         while (n0 < n_last) {
             compute(ic<0>{}, ic<0>{}, even, n0, 0);
-            n0 += 256;
+            n0 += kAcross;
             if (n0 < n_last) load_base(even, n0);
         }
+    }
+}
+
+// Few rows: both products in one launch.  Every workgroup takes its tile of 16 rows through all of A by itself (sixteen waves
+// share the steps of K) and then sixteen waves' outputs, tiles as in adapter_up_kernel: A is read once per 1024
+// outputs, from L2, which for a handful of tiles costs less than a second launch.
+template <typename T, bool F32, int TERMS, int RT>
+__global__ __launch_bounds__(1024) void adapter_small_kernel(const AdapterParams p) {
+    constexpr int kWaves = 16, kDeep = RT == 1 ? 8 : RT == 2 ? 4 : 2, RS = RT > 2 ? 2 : 1, kChunks = 4 * RS;
+    constexpr int kTiles = 4, kSize = F32 ? 4 : 2, kAcross = 16 * kTiles * kWaves, kSlots = 4;
+    typedef typename Four<F32>::bits four;
+    static_assert(RT <= kSlots, "the sums fit the slots of 1 KB");
+    __shared__ __attribute__((aligned(16))) float sums[kWaves][kSlots * 256];
+    __shared__ uint4_t operand[RS * TERMS * 64];
+    __shared__ float growth[16];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int c = lane & 15, q = lane >> 4;
+    uint4_t* const scratch = reinterpret_cast<uint4_t*>(sums[wave]);
+    const int slice = (int)(blockIdx.x % (unsigned)p.slices);
+    const PackedTile t = packed_tile<true>(p.cu, p.num_seqs, p.total, 1, 16, (int)(blockIdx.x / (unsigned)p.slices),
+                                           p.adapter_of_seq);
+    const int r0 = t.tile * 16;
+    if (r0 >= t.rows) return;
+    const bool named = t.of >= 0 && t.of < p.adapters;
+    if (!named && p.base == p.out) return;
+    const int raw_rank = p.ranks[named ? t.of : 0];
+    const float scale = p.scales[named ? t.of : 0];
+    const int left = t.rows - r0 < 16 ? t.rows - r0 : 16;
+    const int64_t row0 = t.row0 + r0;
+    const int n0 = slice * kAcross + 16 * kTiles * wave, n = n0 + kTiles * c;
+    int rank = 0;
+    // (base and B: what lies behind the rank is masked where it is used)
+    four base[4];
+    uint4_t bv[RS][kTiles];
+    const char* const base_rows = static_cast<const char*>(p.base) + (row0 * p.base_stride + min(n, p.n - kTiles)) * kSize;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        base[e] = *reinterpret_cast<const four*>(
+            base_rows + (unsigned)min(4 * q + e, left - 1) * (unsigned)p.base_stride * (unsigned)kSize);
+    const unsigned short* const b = p.b + (int64_t)(named ? t.of : 0) * p.n * p.max_rank;
+#pragma unroll
+    for (int j = 0; j < kTiles; ++j)
+#pragma unroll
+        for (int s = 0; s < RS; ++s)
+            bv[s][j] = *reinterpret_cast<const uint4_t*>(b + (int64_t)min(n0 + kTiles * operand_row() + j, p.n - 1) * p.max_rank +
+                                                         min(32 * s + 8 * operand_chunk(), p.max_rank - 8));
+    if (named) {
+        const unsigned short* const x = p.x + (row0 + min(operand_row(), left - 1)) * p.x_stride;
+        const unsigned short* a[RT];
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+            a[i] = p.a + ((int64_t)t.of * p.max_rank + min(16 * i + operand_row(), p.max_rank - 1)) * p.k;
+        const int last = (p.k + 31) / 32;
+        float4_t acc[RT];
+#pragma unroll
+        for (int i = 0; i < RT; ++i) acc[i] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+        // (columns behind the last: the last ones, taken as zeros)
+        for (int s0 = wave * kDeep; s0 < last; s0 += kWaves * kDeep) {
+            uint4_t xv[kDeep], av[kDeep][RT];
+#pragma unroll
+            for (int d = 0; d < kDeep; ++d) {
+                const int at = min(32 * (s0 + d) + 8 * operand_chunk(), p.k - 8);
+                xv[d] = *reinterpret_cast<const uint4_t*>(x + at);
+#pragma unroll
+                for (int i = 0; i < RT; ++i) av[d][i] = *reinterpret_cast<const uint4_t*>(a[i] + at);
+            }
+            __builtin_amdgcn_sched_barrier(0);  // (all of them, then the products)
+#pragma unroll
+            for (int d = 0; d < kDeep; ++d) {
+                const bool in = 32 * (s0 + d) + 8 * operand_chunk() < p.k;
+                const uint4_t xf = operand_of(in ? xv[d] : uint4_t{0, 0, 0, 0}, scratch + d * (1 + RT) % kSlots * 64);
+#pragma unroll
+                for (int i = 0; i < RT; ++i)
+                    acc[i] = T::mfma16(operand_of(in ? av[d][i] : uint4_t{0, 0, 0, 0},
+                                                  scratch + (d * (1 + RT) + 1 + i) % kSlots * 64), xf, acc[i]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < RT; ++i) *reinterpret_cast<float4_t*>(&sums[wave][(i * 64 + lane) * 4]) = acc[i];
+        rank = max(0, min(__builtin_amdgcn_readfirstlane(raw_rank), p.max_rank));
+    }
+    if (rank == 0 && p.base == p.out) return;
+    if (rank > 0) {
+        __syncthreads();
+        if (threadIdx.x < 16 * kChunks) {
+            const int row = threadIdx.x / kChunks, chunk = threadIdx.x % kChunks;
+            float u[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) u[e] = 0.0f;
+            if (8 * chunk < 16 * RT) {
+#pragma unroll
+                for (int w = 0; w < kWaves; ++w)
+#pragma unroll
+                    for (int g = 0; g < 2; ++g) {
+                        const float4_t v = *reinterpret_cast<const float4_t*>(
+                            &sums[w][((chunk >> 1) * 64 + (2 * (chunk & 1) + g) * 16 + row) * 4]);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) u[4 * g + e] += v[e];
+                    }
+            }
+            adapter_terms<T, TERMS, kChunks>(u, row < left, 8 * chunk, rank, scale, &growth[row],
+                                             &operand[(chunk >> 2) * TERMS * 64 + (chunk & 3) * 16 + row]);
+        }
+        __syncthreads();
+    }
+    float4_t acc[kTiles];
+    float4_t grow = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (rank > 0) {
+        grow = *reinterpret_cast<const float4_t*>(&growth[4 * q]);
+#pragma unroll
+        for (int j = 0; j < kTiles; ++j) {
+            acc[j] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int s = 0; s < RS; ++s) {
+                const uint4_t f = operand_of(bv[s][j] & adapter_keep(32 * s + 8 * operand_chunk(), rank), scratch + j * 64);
+#pragma unroll
+                for (int k = 0; k < TERMS; ++k) acc[j] = T::mfma16(operand[(s * TERMS + k) * 64 + lane], f, acc[j]);
+            }
+        }
+    }
+    if (n >= p.n) return;
+    char* const out_rows = static_cast<char*>(p.out) + (row0 * p.out_stride + n) * kSize;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if (4 * q + e >= left) continue;
+        const four o = rank > 0 ? adapter_sum<T, F32>(base[e], acc, e, grow[e]) : base[e];
+        *reinterpret_cast<four*>(out_rows + (unsigned)(4 * q + e) * (unsigned)p.out_stride * (unsigned)kSize) = o;
     }
 }
 
@@ -381,30 +564,47 @@ static hipError_t adapter_down(AdapterParams p, hipStream_t stream) {
     return hipGetLastError();
 }
 
-template <typename T, bool F32, int MT, int RS>
+template <typename T, bool F32, int MT, int RS, int GROUPS>
 static hipError_t adapter_up(AdapterParams p, hipStream_t stream) {
     constexpr int kTerms = F32 && std::is_same<T, PackedBf16>::value ? 3 : 2;
-    const int64_t tiles = packed_tiles(p.total, p.num_seqs, 1, 16 * MT);
-    // a workgroup takes 256 outputs, and more as long as there are eight workgroups per compute unit
-    const int64_t steps = (p.n + 255) / 256;
-    const int64_t per = std::max<int64_t>(1, std::min(steps, tiles * steps / (8 * device_cu_count())));
-    p.n_slice = (int)per * 256;
+    constexpr int kAcross = 64 * (4 / GROUPS);
+    const int64_t tiles = packed_tiles(p.total, p.num_seqs, 1, 16 * MT * GROUPS);
+    // A workgroup takes one step of outputs, and more as long as there are sixteen workgroups per compute unit: more of them spend
+    // more on their beginnings, fewer stream worse (8192 rows x 24576 outputs, rank 64: 8 per unit 228 us, 16 215, 32 227).
+    const int64_t steps = (p.n + kAcross - 1) / kAcross;
+    const int64_t per = std::max<int64_t>(1, std::min(steps, tiles * steps / (16 * device_cu_count())));
+    p.n_slice = (int)per * kAcross;
     p.slices = (int)((steps + per - 1) / per);
-    adapter_up_kernel<T, F32, kTerms, MT, RS><<<(unsigned)(tiles * p.slices), 256, 0, stream>>>(p);
+    adapter_up_kernel<T, F32, kTerms, MT, RS, GROUPS><<<(unsigned)(tiles * p.slices), 256, 0, stream>>>(p);
     return hipGetLastError();
 }
 
 template <typename T, bool F32>
 static hipError_t adapter_up_by_rank(const AdapterParams& p, bool long_seqs, hipStream_t stream) {
-    constexpr int kLong = F32 ? 2 : 4;  // (what fits the registers twice: this step's and the next one's)
-    if (p.max_rank <= 32) return long_seqs ? adapter_up<T, F32, kLong, 1>(p, stream) : adapter_up<T, F32, 1, 1>(p, stream);
-    if (p.max_rank <= 64) return long_seqs ? adapter_up<T, F32, kLong, 2>(p, stream) : adapter_up<T, F32, 1, 2>(p, stream);
-    if (p.max_rank <= 128) return !F32 && long_seqs ? adapter_up<T, F32, F32 ? 1 : 2, 4>(p, stream) : adapter_up<T, F32, 1, 4>(p, stream);
-    return adapter_up<T, F32, 1, 8>(p, stream);
+    if (p.max_rank <= 32) return long_seqs ? adapter_up<T, F32, 2, 1, 2>(p, stream) : adapter_up<T, F32, 1, 1, 1>(p, stream);
+    if (p.max_rank <= 64) return long_seqs ? adapter_up<T, F32, 2, 2, 2>(p, stream) : adapter_up<T, F32, 1, 2, 1>(p, stream);
+    if (p.max_rank <= 128) return long_seqs ? adapter_up<T, F32, 1, 4, 2>(p, stream) : adapter_up<T, F32, 1, 4, 1>(p, stream);
+    return adapter_up<T, F32, 1, 8, 1>(p, stream);
+}
+
+template <typename T, bool F32>
+static hipError_t adapter_small(AdapterParams p, hipStream_t stream) {
+    constexpr int kTerms = F32 && std::is_same<T, PackedBf16>::value ? 3 : 2;
+    p.slices = (p.n + 1023) / 1024;
+    const unsigned grid = (unsigned)(packed_tiles(p.total, p.num_seqs, 1, 16) * p.slices);
+    if (p.max_rank <= 16) adapter_small_kernel<T, F32, kTerms, 1><<<grid, 1024, 0, stream>>>(p);
+    else if (p.max_rank <= 32) adapter_small_kernel<T, F32, kTerms, 2><<<grid, 1024, 0, stream>>>(p);
+    else adapter_small_kernel<T, F32, kTerms, 4><<<grid, 1024, 0, stream>>>(p);
+    return hipGetLastError();
 }
 
 template <typename T>
 static hipError_t adapter_launch(AdapterParams p, bool f32, hipStream_t stream) {
+    // One launch where a workgroup reads little of A: in a graph it takes about as long as two (us, one row: rank 16 of 4096 to
+    // 4096 7.8 / 6.9; 32 of 896 to 896 6.0 / 6.4; 32 of 4096 9.0 / 7.3), launched one by one a call costs the host 3.4 us less.
+    if (p.max_rank <= 64 && (int64_t)p.max_rank * p.k <= 65536 &&
+        packed_tiles(p.total, p.num_seqs, 1, 16) * ((p.n + 1023) / 1024) <= device_cu_count())
+        return f32 ? adapter_small<T, true>(p, stream) : adapter_small<T, false>(p, stream);
     const bool long_seqs = p.total >= 32 * (int64_t)p.num_seqs;
     const int steps = (p.k + 31) / 32, mt = long_seqs ? 4 : 1;
     const int rt = !long_seqs || p.max_rank <= 16 ? 1 : p.max_rank <= 32 ? 2 : 4;

@@ -131,6 +131,25 @@ def test_many_rows(lens, max_rank, dtype, out):
                  dtype, out))
 
 
+@pytest.mark.parametrize("dtype,out", OUTS)
+@pytest.mark.parametrize("max_rank", [16, 32, 48, 64, 104])
+@pytest.mark.parametrize("n,k", [(1100, 256), (264, 5000)])
+def test_many_short_sequences(n, k, max_rank, dtype, out):
+    """More tiles than take both products at once."""
+    n = n // 8 * 8
+    lens = [1, 2, 0, 1] * 90 + [17]
+    _check(_case(13, lens, np.arange(len(lens)) % 5 - 1, [max_rank, 7, max_rank - 3, 12], max_rank, n, k, dtype,
+                 out))
+
+
+@pytest.mark.parametrize("dtype,out", OUTS)
+@pytest.mark.parametrize("max_rank", [8, 16, 32, 40, 64])
+@pytest.mark.parametrize("lens", [[1], [16, 1, 3, 33]], ids=str)
+def test_few_rows(lens, max_rank, dtype, out):
+    _check(_case(14, lens, np.arange(len(lens)) % 3, [max_rank, max_rank - 5, 0], max_rank, 2104, 1096, dtype, out))
+    _check(_case(15, lens, np.arange(len(lens)) % 3 - 1, [max_rank, 1], max_rank, 1024, 4096, dtype, out))
+
+
 def test_a_rank_above_the_slot_is_the_slots():
     c = _case(8, [20], [0], [16], 16, 136, 128, "fp16")
     want = Run(c)
