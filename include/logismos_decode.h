@@ -683,7 +683,7 @@ logismos_status_t logismos_rope_frequencies(double* inv_freq, float* amplitude, 
  *
  * fp32 scores, softmax and sums; the probabilities are rounded to the rows' type for the second product.  Elements of
  * keys that a token does not see do not reach its result, whatever they hold; a token whose keys all score
- * -inf gives zeros.  scale finite and > 0 (else hipErrorInvalidValue); head_dim a multiple of 32 up to 256; num_q_heads a
+ * -inf gives zeros.  scale > 0 and scale * log2(e) finite (else hipErrorInvalidValue); head_dim a multiple of 32 up to 256; num_q_heads a
  * multiple of num_kv_heads; k, v and out strides up to 2^22; total_tokens * num_q_heads / 128 +
  * num_seqs * num_kv_heads up to 2^22.  out does not overlap q, k or v. */
 logismos_status_t logismos_check_attn_packed_shape(int num_seqs, int total_tokens, int num_q_heads,

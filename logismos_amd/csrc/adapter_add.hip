@@ -246,7 +246,7 @@ __global__ __launch_bounds__(256, 2) void adapter_up_kernel(const AdapterParams 
     constexpr int kTiles = 4, kSize = F32 ? 4 : 2, kAcross = 16 * kTiles * (4 / GROUPS);
     typedef typename Four<F32>::bits four;
     __shared__ uint4_t operand[MT * GROUPS * RS * TERMS * 64];
-    __shared__ float growth[kRows];
+    __shared__ __attribute__((aligned(16))) float growth[kRows];
     __shared__ uint4_t scratches[4][kTiles][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c = lane & 15, q = lane >> 4;
@@ -440,7 +440,7 @@ __global__ __launch_bounds__(1024) void adapter_small_kernel(const AdapterParams
     static_assert(RT <= kSlots, "the sums fit the slots of 1 KB");
     __shared__ __attribute__((aligned(16))) float sums[kWaves][kSlots * 256];
     __shared__ uint4_t operand[RS * TERMS * 64];
-    __shared__ float growth[16];
+    __shared__ __attribute__((aligned(16))) float growth[16];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c = lane & 15, q = lane >> 4;
     uint4_t* const scratch = reinterpret_cast<uint4_t*>(sums[wave]);

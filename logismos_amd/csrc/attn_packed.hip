@@ -438,7 +438,8 @@ static logismos_status_t attn_packed(bool bf16, const void* q, const void* k, co
     if (logismos_check_attn_packed_shape(num_seqs, total, hq, hkv, d, q_stride, k_stride, v_stride, out_stride,
                                          nullptr, 0) != 0)
         return bad;
-    if (!q || !k || !v || !cu || !out || !(scale > 0.0f) || !isfinite(scale)) return bad;
+    const float scale_log2e = scale * 1.4426950408889634f;
+    if (!q || !k || !v || !cu || !out || !(scale > 0.0f) || !isfinite(scale_log2e)) return bad;
     if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) |
          reinterpret_cast<uintptr_t>(out)) % 16 != 0 ||
         reinterpret_cast<uintptr_t>(cu) % 4 != 0)
@@ -457,7 +458,7 @@ static logismos_status_t attn_packed(bool bf16, const void* q, const void* k, co
     p.k_stride = k_stride;
     p.v_stride = v_stride;
     p.out_stride = out_stride;
-    p.scale_log2e = scale * 1.4426950408889634f;
+    p.scale_log2e = scale_log2e;
     p.causal = causal != 0;
     // (putting them in order takes every workgroup about 1 us: 8 prompts of 100 to 4096 tokens 93 -> 85 us, 8 of 1000 43 -> 40,
     // but 16 of 512 76 -> 79)

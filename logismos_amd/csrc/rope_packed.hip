@@ -194,6 +194,7 @@ logismos_status_t logismos_check_rope_packed_shape(int tokens, int num_q_heads, 
     if (tokens <= 0 || num_q_heads <= 0 || head_dim <= 0)
         return reject(msg, cap, "tokens, num_q_heads and head_dim must be positive (%d, %d, %d)", tokens, num_q_heads,
                       head_dim);
+    if (tokens > lg::kPackedMaxRows) return reject(msg, cap, "tokens exceeds %d (%d)", lg::kPackedMaxRows, tokens);
     if (num_kv_heads < 0) return reject(msg, cap, "num_kv_heads must not be negative (%d)", num_kv_heads);
     if (rotary_dim <= 0 || rotary_dim % 2 != 0 || rotary_dim > head_dim)
         return reject(msg, cap, "rotary_dim must be even, positive and at most head_dim (%d of %d)", rotary_dim,

@@ -55,7 +55,7 @@ def test_attn_packed_arguments(bf16):
         refused(**{name: C.c_void_p(4104)})
     refused(cu=None)
     refused(cu=C.c_void_p(4098))
-    for scale in (0.0, -1.0, math.inf, math.nan):
+    for scale in (0.0, -1.0, math.inf, math.nan, 3e38):
         refused(scale=scale)
 
 
@@ -65,7 +65,7 @@ ROPE = dict(tokens=5, hq=4, hkv=2, d=64, rotary=64, qi=256, ki=128, qo=256, ko=1
 
 @pytest.mark.parametrize("change,frag", [
     (dict(tokens=0), "must be positive"), (dict(hq=0), "must be positive"),
-    (dict(d=0), "must be positive"), (dict(hkv=-1), "must not be negative"),
+    (dict(tokens=(1 << 23) + 1), "exceeds"), (dict(d=0), "must be positive"), (dict(hkv=-1), "must not be negative"),
     (dict(rotary=0), "rotary_dim"), (dict(rotary=33), "rotary_dim"), (dict(rotary=66), "rotary_dim"),
     (dict(d=1026, rotary=64, qi=1 << 14, qo=1 << 14, ki=1 << 14, ko=1 << 14), "at most 1024"),
     (dict(hq=1024, hkv=1, qi=65536, qo=65536), "exceeds 65536"),
