@@ -12,9 +12,9 @@
 // 16 bits, for outputs of 8, three, 24 bits, for fp32 outputs.
 //
 // Bound by memory: x, base and out once, A and B of the adapters in use.  16 prompts of 512 x 4096, rank 64, 24576 outputs in 16
-// bits: 900 MB in 237 us, 3.8 TB/s (a large copy 5.2; the first launch 26 us, the second 211: its beginnings, and
-// vector work that the memory time does not all cover); 13 single rows and 5 chunks of 31 to 600, 8960 columns to 1536 in
-// fp32: 54 MB in 23 us; 32 single rows on 8 adapters, 4096 to 6144: 10.9 us, a chain of dependent loads.
+// bits: 900 MB in 229 us, 3.9 TB/s (a large copy 5.2; the first launch 26 us, the second 203: its beginnings, and
+// products and vector work that the memory time does not all cover; rank 32 192 us); 13 single rows and 5 chunks of 31 to 600, 8960 columns to 1536 in
+// fp32: 54 MB in 23 us; 32 single rows on 8 adapters, 4096 to 6144: 10.5 us, a chain of dependent loads.
 #include "device_utils.hpp"
 #include "launch_common.hpp"
 #include "packed_rows.hpp"
@@ -270,29 +270,45 @@ __global__ __launch_bounds__(256, 2) void adapter_up_kernel(const AdapterParams 
     // (rows behind the tile's last, outputs behind the last and ranks behind the rank: others in their place, which count
     // for nothing -- a load under a condition of its own is a branch around it.  Offsets from the tile's first row and the
     // adapter's B have 32 bits.)
-    // (B 32 ranks at a time, asked for as soon as the products of those before are done: more does not fit)
+    // (B is asked for a step ahead, as soon as the products of the step before with these ranks are done; more than 64 ranks do not
+    // fit and come 32 at a time)
+    constexpr int kHeld = RS <= 2 ? RS : 1;
     four even[MT][4], odd[MT][4];
-    uint4_t bv[kTiles];
+    uint4_t bv[kHeld][kTiles];
     const char* const base = static_cast<const char*>(p.base) + row0 * p.base_stride * kSize;
     char* const out = static_cast<char*>(p.out) + row0 * p.out_stride * kSize;
     const char* const b = reinterpret_cast<const char*>(p.b + (int64_t)(named ? t.of : 0) * p.n * p.max_rank);
-    auto load_base = [&](four(&w)[MT][4], int at_n) LG_INLINE {
-        const unsigned n = (unsigned)min(at_n + kTiles * c, p.n - kTiles);
+    // (WHOLE: everything is there, and one offset per lane serves all rows)
+    const unsigned base_lane = ((unsigned)my_row * (unsigned)p.base_stride + 4u * (unsigned)c) * (unsigned)kSize;
+    auto load_base = [&](auto whole_c, four(&w)[MT][4], int at_n) LG_INLINE {
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                w[m][e] = *reinterpret_cast<const four*>(
-                    base + ((unsigned)min(my_row + 16 * m + e, left - 1) * (unsigned)p.base_stride + n) * (unsigned)kSize);
+            for (int e = 0; e < 4; ++e) {
+                if constexpr (decltype(whole_c)::value != 0) {
+                    w[m][e] = *reinterpret_cast<const four*>(
+                        base + ((int64_t)(16 * m + e) * p.base_stride + at_n) * kSize + base_lane);
+                } else {
+                    const unsigned row = (unsigned)min(my_row + 16 * m + e, left - 1);
+                    const unsigned n = (unsigned)min(at_n + kTiles * c, p.n - kTiles);
+                    w[m][e] = *reinterpret_cast<const four*>(base + (row * (unsigned)p.base_stride + n) * (unsigned)kSize);
+                }
+            }
     };
     int rank = 0;
-    auto load_b = [&](int at_n, int s) LG_INLINE {
+    const unsigned b_lane = (unsigned)(kTiles * operand_row()) * (unsigned)p.max_rank * 2u;
+    auto load_b = [&](auto whole_c, int at_n, int s) LG_INLINE {
         const int r = 32 * s + 8 * operand_chunk();
+        const unsigned chunk = (unsigned)(r < rank ? r : 0) * 2u;
 #pragma unroll
-        for (int j = 0; j < kTiles; ++j)
-            bv[j] = *reinterpret_cast<const uint4_t*>(
-                b + ((unsigned)min(at_n + kTiles * operand_row() + j, p.n - 1) * (unsigned)p.max_rank +
-                     (unsigned)(r < rank ? r : 0)) * 2u);
+        for (int j = 0; j < kTiles; ++j) {
+            if constexpr (decltype(whole_c)::value != 0) {
+                bv[s % kHeld][j] = *reinterpret_cast<const uint4_t*>(b + (int64_t)(at_n + j) * p.max_rank * 2 + (b_lane + chunk));
+            } else {
+                const unsigned n = (unsigned)min(at_n + kTiles * operand_row() + j, p.n - 1);
+                bv[s % kHeld][j] = *reinterpret_cast<const uint4_t*>(b + (n * (unsigned)p.max_rank * 2u + chunk));
+            }
+        }
     };
     // Thread (row, chunk of eight ranks), the chunks of a row side by side; four parts of v at a time.
     struct Parts {
@@ -311,11 +327,12 @@ __global__ __launch_bounds__(256, 2) void adapter_up_kernel(const AdapterParams 
     };
     Parts v;
     load_v(v, v_at(threadIdx.x));
-    load_base(even, n0);
+    load_base(ic<0>{}, even, n0);
     if (named) rank = max(0, min(__builtin_amdgcn_readfirstlane(raw_rank), p.max_rank));
     if (rank == 0 && p.base == p.out) return;
     if (rank > 0) {
-        load_b(n0, 0);
+#pragma unroll
+        for (int s = 0; s < kHeld; ++s) load_b(ic<0>{}, n0, s);
         for (int i = threadIdx.x; i < kRows * kChunks; i += 256) {
             const int row = i / kChunks, chunk = i % kChunks, r = 8 * chunk;
             if (i >= 256) load_v(v, v_at(i));
@@ -344,19 +361,20 @@ __global__ __launch_bounds__(256, 2) void adapter_up_kernel(const AdapterParams 
         __syncthreads();
     }
     uint4_t keep[RS];
-    float4_t grow[MT];
+    const unsigned out_lane = ((unsigned)my_row * (unsigned)p.out_stride + 4u * (unsigned)c) * (unsigned)kSize;
     // One step over the base `w`; WHOLE: of whole tiles, and the next one's B is asked for.
     auto compute = [&](auto adds_c, auto whole_c, four(&w)[MT][4], int at_n, int next_n) LG_INLINE {
         constexpr bool ADDS = decltype(adds_c)::value != 0, WHOLE = decltype(whole_c)::value != 0;
         float4_t acc[MT][kTiles];
         if (ADDS) {
-            asm volatile("" ::: "memory");  // (the terms are read again: kept over the steps they cost a wave its place)
+            asm volatile("" ::: "memory");  // (terms and growth are read again: kept over the steps they cost a wave its place)
 #pragma unroll
             for (int j = 0; j < kTiles; ++j)
 #pragma unroll
                 for (int m = 0; m < MT; ++m) acc[m][j] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int s = 0; s < RS; ++s) {
+                uint4_t(&w_b)[kTiles] = bv[s % kHeld];
                 uint4_t term[MT][TERMS];
 #pragma unroll
                 for (int m = 0; m < MT; ++m)
@@ -364,36 +382,33 @@ __global__ __launch_bounds__(256, 2) void adapter_up_kernel(const AdapterParams 
                     for (int k = 0; k < TERMS; ++k)
                         term[m][k] = operand[(((group * MT + m) * RS + s) * TERMS + k) * 64 + lane];
 #pragma unroll
-                for (int j = 0; j < kTiles; ++j) {
-                    const uint4_t f = operand_of(bv[j] & keep[s], scratch[j]);
+                for (int j = 0; j < kTiles; ++j) w_b[j] = operand_of(w_b[j] & keep[s], scratch[j]);
 #pragma unroll
-                    for (int k = 0; k < TERMS; ++k)
+                for (int k = 0; k < TERMS; ++k)  // (the sums of a tile and row group as far apart as they can be)
 #pragma unroll
-                        for (int m = 0; m < MT; ++m) acc[m][j] = T::mfma16(term[m][k], f, acc[m][j]);
-                }
-                if (s + 1 < RS) load_b(at_n, s + 1);
-                else if (WHOLE) load_b(next_n, 0);
+                    for (int j = 0; j < kTiles; ++j)
+#pragma unroll
+                        for (int m = 0; m < MT; ++m) acc[m][j] = T::mfma16(term[m][k], w_b[j], acc[m][j]);
+                if (s + kHeld < RS) load_b(whole_c, at_n, s + kHeld);
+                else if (WHOLE) load_b(whole_c, next_n, (s + kHeld) % RS);
                 __builtin_amdgcn_sched_barrier(0);  // (into the registers that the products just read)
             }
         }
-        const int n = at_n + kTiles * c;
-        if (!WHOLE && n >= p.n) return;
+        if (!WHOLE && at_n + kTiles * c >= p.n) return;
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
+        for (int m = 0; m < MT; ++m) {
+            float4_t grow;
+            if (ADDS) grow = *reinterpret_cast<const float4_t*>(&growth[my_row + 16 * m]);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 if (!WHOLE && my_row + 16 * m + e >= left) continue;
                 four o = w[m][e];
-                if constexpr (ADDS) o = adapter_sum<T, F32>(o, acc[m], e, grow[m][e]);
-                *reinterpret_cast<four*>(
-                    out + ((unsigned)(my_row + 16 * m + e) * (unsigned)p.out_stride + (unsigned)n) * (unsigned)kSize) = o;
+                if constexpr (ADDS) o = adapter_sum<T, F32>(o, acc[m], e, grow[e]);
+                *reinterpret_cast<four*>(out + ((int64_t)(16 * m + e) * p.out_stride + at_n) * kSize + out_lane) = o;
             }
+        }
     };
     if (rank > 0) {
-#pragma unroll
-        for (int m = 0; m < MT; ++m) {
-            grow[m] = *reinterpret_cast<const float4_t*>(&growth[my_row + 16 * m]);
-        }
 #pragma unroll
         for (int s = 0; s < RS; ++s) keep[s] = adapter_keep(32 * s + 8 * operand_chunk(), rank);
         if (left >= 16 * MT * (group + 1) && n_last % (16 * kTiles) == 0) {
@@ -402,12 +417,12 @@ __global__ __launch_bounds__(256, 2) void adapter_up_kernel(const AdapterParams 
             const int end = n0 < n_last ? n0 + (n_last - 1 - n0) / kAcross * kAcross : 0;
             while (n0 < n_last) {
                 int next = min(n0 + kAcross, end);
-                load_base(odd, next);
+                load_base(ic<1>{}, odd, next);
                 compute(ic<1>{}, ic<1>{}, even, n0, next);
                 n0 += kAcross;
                 if (n0 >= n_last) break;
                 next = min(n0 + kAcross, end);
-                load_base(even, next);
+                load_base(ic<1>{}, even, next);
                 compute(ic<1>{}, ic<1>{}, odd, n0, next);
                 n0 += kAcross;
             }
@@ -416,15 +431,16 @@ __global__ __launch_bounds__(256, 2) void adapter_up_kernel(const AdapterParams 
                 compute(ic<1>{}, ic<0>{}, even, n0, 0);
                 n0 += kAcross;
                 if (n0 >= n_last) break;
-                load_base(even, n0);
-                load_b(n0, 0);
+                load_base(ic<0>{}, even, n0);
+#pragma unroll
+                for (int s = 0; s < kHeld; ++s) load_b(ic<0>{}, n0, s);
             }
         }
     } else {
         while (n0 < n_last) {
             compute(ic<0>{}, ic<0>{}, even, n0, 0);
             n0 += kAcross;
-            if (n0 < n_last) load_base(even, n0);
+            if (n0 < n_last) load_base(ic<0>{}, even, n0);
         }
     }
 }
