@@ -44,7 +44,7 @@ struct AdapterParams {
     int num_seqs, total, adapters, max_rank, n, k;
     int64_t x_stride, base_stride, out_stride;
     int parts, part_steps;  // K parts, steps of 32 columns of a part
-    int n_slice, slices;    // outputs of a workgroup, a multiple of 256; how many of them
+    int n_slice, slices;    // outputs of a workgroup, whole steps of its waves; how many of them
 };
 
 __device__ __forceinline__ int adapter_rank(const AdapterParams& p, int adapter) {
@@ -89,13 +89,11 @@ __global__ __launch_bounds__(256, 2) void adapter_down_kernel(const AdapterParam
     const unsigned short* x[MT];
     const unsigned short* a[RT];
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
+    for (int m = 0; m < MT; ++m)
         x[m] = p.x + (int64_t)(t.row0 + min(r0 + 16 * m + operand_row(), t.rows - 1)) * p.x_stride;
-    }
 #pragma unroll
-    for (int i = 0; i < RT; ++i) {
+    for (int i = 0; i < RT; ++i)
         a[i] = p.a + ((int64_t)t.of * p.max_rank + min(rank0 + 16 * i + operand_row(), p.max_rank - 1)) * p.k;
-    }
     const int all = (p.k + 31) / 32;
     const int first = part * p.part_steps + wave * kDeep;
     const int last = min((part + 1) * p.part_steps, all);
