@@ -171,14 +171,30 @@ __global__ __launch_bounds__(64 * WAVES) void attn_packed_kernel(const AttnPacke
     };
     auto key_of = [&](int u) LG_INLINE { return (tid % kMovers + kMovers * u) / (D / 8); };
     auto piece_of = [&](int u) LG_INLINE { return (tid % kMovers + kMovers * u) % (D / 8); };
+    // Byte offsets in a whole tile; the rest of the address is the same for the whole wave. Where a mover's pieces are
+    // whole keys apart (heads of 32, 64, 128, 256) one offset serves all of them.
+    constexpr bool kEven = kMovers % (D / 8) == 0;
+    constexpr int kOffsets = kEven ? 1 : kPer;
+    unsigned whole_at[kOffsets];
+#pragma unroll
+    for (int u = 0; u < kOffsets; ++u)
+        whole_at[u] = ((unsigned)key_of(u) * (unsigned)stride + 8u * (unsigned)piece_of(u)) * 2u;
     auto gload = [&](int tile, Regs& r) LG_INLINE {
         // (past the last visible key that key again: its probability is 0 for everybody who sees less)
         const int key0 = min(tile * kApKeys, visible - 1);
-        const unsigned short* at = src + (int64_t)key0 * stride;
+        const char* at = reinterpret_cast<const char*>(src + (int64_t)key0 * stride);
+        if (key0 + kApKeys <= visible) {
 #pragma unroll
-        for (int u = 0; u < kPer; ++u) {
-            const unsigned k = (unsigned)min(key_of(u), visible - 1 - key0);
-            r.x[u] = *reinterpret_cast<const uint4_t*>(at + (k * (unsigned)stride + 8u * (unsigned)piece_of(u)));
+            for (int u = 0; u < kPer; ++u) {
+                const char* piece = kEven ? at + (int64_t)stride * (u * (kMovers / (D / 8)) * 2) : at;
+                r.x[u] = *reinterpret_cast<const uint4_t*>(piece + whole_at[kEven ? 0 : u]);
+            }
+        } else {
+#pragma unroll
+            for (int u = 0; u < kPer; ++u) {
+                const unsigned k = (unsigned)min(key_of(u), visible - 1 - key0);
+                r.x[u] = *reinterpret_cast<const uint4_t*>(at + (k * (unsigned)stride + 8u * (unsigned)piece_of(u)) * 2u);
+            }
         }
     };
     auto lstore = [&](int buf, const Regs& r) LG_INLINE {
@@ -240,7 +256,7 @@ __global__ __launch_bounds__(64 * WAVES) void attn_packed_kernel(const AttnPacke
         }
         tm = fmaxf(tm, lane_xor_f32<32>(tm)) * p.scale_log2e;
         const bool raise = tm > m + kApLazy;
-        const float alpha = raise ? fast_exp2(m - tm) : 1.0f;
+        const float m_before = m;
         m = raise ? tm : m;
         const float ref = m == -INFINITY ? 0.0f : -m;
         float16_t s_nxt;
@@ -261,7 +277,6 @@ __global__ __launch_bounds__(64 * WAVES) void attn_packed_kernel(const AttnPacke
             sum += p1;
             pb[e >> 3][(e & 7) >> 1] = T::pack2(p0, p1);
         }
-        l = fmaf(l, alpha, sum);
         if constexpr (!MASKED) {
             // half of the operand reads, then the products, each followed by a read (into registers freed before) and
             // its share of the vector work
@@ -275,13 +290,16 @@ __global__ __launch_bounds__(64 * WAVES) void attn_packed_kernel(const AttnPacke
             }
         }
         // (F belongs to this step: its results are used by the next one only, and would sink there)
-        asm volatile("" : "+v"(pb[0]), "+v"(pb[1]), "+v"(l));
+        asm volatile("" : "+v"(pb[0]), "+v"(pb[1]), "+v"(sum));
         if (__builtin_expect(__builtin_amdgcn_ballot_w64(raise) != 0, 0)) {  // O(tile - 1) was relative to the old one
+            const float alpha = raise ? fast_exp2(m_before - m) : 1.0f;
+            l *= alpha;
 #pragma unroll
             for (int dt = 0; dt < kTiles; ++dt)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) o[dt][e] *= alpha;
         }
+        l += sum;
         s_cur = s_nxt;
         p_prev[0] = pb[0];
         p_prev[1] = pb[1];
