@@ -50,8 +50,9 @@ struct AttnPackedParams {
 
 constexpr int kApKeys = 32;
 
-// Probabilities of the 16 keys that a lane holds of its column (keys first + 8 (e / 4) + e % 4), the running maximum and sum;
-// returns what the sums so far are to be multiplied by.
+// Probabilities of the 16 keys that a lane holds of its column (keys first + 8 (e / 4) + e % 4), the running maximum (of the
+// scores as they are: their differences are taken before the scale) and sum; returns what the sums so far are to be
+// multiplied by.
 template <typename T>
 __device__ __forceinline__ float attn_packed_softmax(float16_t sc, int first, int vis, float scale_log2e, float& m,
                                                      float& l, uint4_t (&pb)[2]) {
@@ -61,16 +62,16 @@ __device__ __forceinline__ float attn_packed_softmax(float16_t sc, int first, in
         sc[e] = first + 8 * (e >> 2) + (e & 3) < vis ? sc[e] : -INFINITY;
         tm = fmaxf(tm, sc[e]);
     }
-    tm = fmaxf(tm, lane_xor_f32<32>(tm)) * scale_log2e;
+    tm = fmaxf(tm, lane_xor_f32<32>(tm));
     const float m_new = fmaxf(m, tm);
     const float ref = m_new == -INFINITY ? 0.0f : m_new;
-    const float alpha = fast_exp2(m - ref);
+    const float alpha = fast_exp2((m - ref) * scale_log2e);
     m = m_new;
     l *= alpha;
 #pragma unroll
     for (int e = 0; e < 16; e += 2) {
-        const float p0 = fast_exp2(fmaf(sc[e], scale_log2e, -ref));
-        const float p1 = fast_exp2(fmaf(sc[e + 1], scale_log2e, -ref));
+        const float p0 = fast_exp2((sc[e] - ref) * scale_log2e);
+        const float p1 = fast_exp2((sc[e + 1] - ref) * scale_log2e);
         l += p0 + p1;
         pb[e >> 3][(e & 7) >> 1] = T::pack2(p0, p1);
     }
@@ -122,6 +123,9 @@ __device__ __forceinline__ void attn_packed_write(unsigned short* out, unsigned 
 }
 
 constexpr float kApLazy = 8.0f;
+// A scaled score less the rounded product of the maximum and the scale, in one rounding: off by up to half a step of the
+// maximum, the same for all keys of a column.  Up to here that is at most 1 in the exponent and falls out of the result.
+constexpr float kApExact = 16777216.0f;
 
 template <typename T, int D, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void attn_packed_kernel(const AttnPackedParams p) {
@@ -351,8 +355,9 @@ __global__ __launch_bounds__(64 * WAVES) void attn_packed_kernel(const AttnPacke
             o[j % kTiles] = T::mfma32(v_operand(buf, j / kTiles, j % kTiles), p_prev[j / kTiles], o[j % kTiles]);
     }
     // A key that a column does not see has the probability 0 there, and 0 times an infinity or NaN of its V row is a NaN.
-    // If the results are not all finite, the keys are gone through again, plainly, and in the tiles in which columns of the wave end
-    // with a pass of its own for every number of keys that one of them sees.
+    // If the results are not all finite, or a maximum is too large for the fused difference, the keys are gone through again,
+    // plainly, and in the tiles in which columns of the wave end with a pass of its own for every number of keys that one of them
+    // sees.
     {
         float odds[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // NaN if a result is not finite
 #pragma unroll
@@ -360,7 +365,7 @@ __global__ __launch_bounds__(64 * WAVES) void attn_packed_kernel(const AttnPacke
 #pragma unroll
             for (int e = 0; e < 16; ++e) odds[e & 3] = fmaf(o[dt][e], 0.0f, odds[e & 3]);
         const float odd = (odds[0] + odds[1]) + (odds[2] + odds[3]);
-        const bool any = __builtin_amdgcn_ballot_w64(odd != odd) != 0;
+        const bool any = __builtin_amdgcn_ballot_w64(odd != odd || fabsf(m) > kApExact) != 0;
         if (lane == 0) odd_waves[wave] = any;
         __syncthreads();
         unsigned all = 0;

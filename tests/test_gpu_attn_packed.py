@@ -244,3 +244,39 @@ def test_two_streams_at_once():
             r.launch()
     for r in runs:
         R.assert_within(r.result(), *_want(r.c, True))
+
+
+@pytest.mark.parametrize("negative", [False, True])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("d", [32, 64, 128, 256])
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_scores_of_which_fp32_holds_no_fraction(dtype, d, causal, negative):
+    """Scores of 2^31 and more: half a step of such a number is hundreds of powers of two, so what a
+    product and its rounded value differ by must not get into an exponent."""
+    rng = np.random.default_rng(d + negative)
+    lens, hq, hkv, scale = [1, 33, 150], 4, 2, 4.0
+    T = sum(lens) + GUARD
+    # small integers times powers of two: every sum is exact in fp32, equal scores are equal, and different ones at
+    # least 2^27 apart, so a row is the mean of v over its best keys
+    q = 2.0 ** 13 * (np.ones((T, hq, d)) if negative else rng.choice([-1.0, 1.0], (T, hq, d)))
+    k = 2.0 ** 12 * (-rng.integers(1, 9, (T, hkv, d)) if negative else rng.integers(-8, 9, (T, hkv, d)))
+    v = rng.integers(-8, 9, (T, hkv, d)).astype(np.float64)
+    rows = np.concatenate([x.reshape(T, -1) for x in (q, k, v)], 1)
+    c = dict(rows=R.to_bits(rows, dtype), lens=lens, hq=hq, hkv=hkv, d=d, dtype=dtype, fused=False, T=T)
+    assert (R.from_bits(c["rows"], dtype) == rows).all()
+    run = Run(c, causal, scale)
+    run.launch()
+    got = run.result().reshape(-1, hq, d)
+    at = 0
+    for n in lens:
+        r = slice(at, at + n)
+        for h in range(hq):
+            s = (q[r, h] @ k[r, h // 2].T) * scale
+            if causal:
+                s[np.triu(np.ones((n, n), bool), 1)] = -np.inf
+            best = (s == s.max(1, keepdims=True)).astype(np.float64)
+            want = best @ v[r, h // 2] / best.sum(1, keepdims=True)
+            # the result's rounding, the reciprocal's and the product's in fp32; sums of ones and integers are exact
+            bound = R.HALF_STEP[dtype] * np.abs(want) * (1 + 2.0 ** -20) + 3 * R.FP32 * np.abs(want)
+            R.assert_within(got[r, h], want, bound, f"sequence of {n}, head {h}")
+        at += n
