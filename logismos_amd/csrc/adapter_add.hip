@@ -624,7 +624,7 @@ static hipError_t adapter_launch(AdapterParams p, bool f32, hipStream_t stream) 
     const int rt = !long_seqs || p.max_rank <= 16 ? 1 : p.max_rank <= 32 ? 2 : 4;
     // K parts: two workgroups per compute unit, and steps for four waves
     const int64_t groups = packed_tiles(p.total, p.num_seqs, 1, 16 * mt) * ((p.max_rank + 16 * rt - 1) / (16 * rt));
-    int parts = 1;  // (at most four for the loads of one round)
+    int parts = 1;
     while (parts < kAdapterMaxParts && groups * parts < 2 * device_cu_count() && steps >= 16 * parts) parts *= 2;
     p.parts = parts;
     p.part_steps = (steps + parts - 1) / parts;

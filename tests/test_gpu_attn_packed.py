@@ -280,3 +280,49 @@ def test_scores_of_which_fp32_holds_no_fraction(dtype, d, causal, negative):
             bound = R.HALF_STEP[dtype] * np.abs(want) * (1 + 2.0 ** -20) + 3 * R.FP32 * np.abs(want)
             R.assert_within(got[r, h], want, bound, f"sequence of {n}, head {h}")
         at += n
+
+
+@pytest.mark.parametrize("dtype,causal", [("bf16", True), ("fp16", False)])
+def test_long_sequences_with_heads_of_128(dtype, causal):
+    """Sequences and heads enough for the form with 256 columns to a workgroup: its results, and with a
+    token whose K and V rows are NaN those of the tokens in front of it and of the other sequence."""
+    hq, hkv, d, lens, kvh, bad = 24, 8, 128, [4097, 4200], 5, 2000
+    c = _case(17, lens, hq, hkv, d, dtype)
+    r = Run(c, causal)
+    r.launch()
+    clean = r.bits().copy()
+    n, heads = sum(lens), slice(3 * kvh, 3 * kvh + 3)
+    q, k, v = (R.from_bits(np.ascontiguousarray(x[:n]), dtype).reshape(n, -1, d) for x in _parts(c))
+    want, bound = R.attention(q[:, heads], k[:, kvh:kvh + 1], v[:, kvh:kvh + 1], lens, r.scale, causal, dtype)
+    R.assert_within(r.result().reshape(n, hq, d)[:, heads], want, bound)
+
+    _, k, v = _parts(c)
+    k[bad], v[bad] = _nan(dtype), _nan(dtype)
+    r = Run(c, causal)
+    r.launch()
+    got = r.result()
+    first = bad if causal else 0
+    assert np.isnan(got[first:lens[0]]).all()
+    assert np.array_equal(r.bits()[lens[0]:], clean[lens[0]:])
+    R.assert_within(got.reshape(n, hq, d)[:first, heads], want[:first], bound[:first])
+
+
+def test_long_sequences_with_scores_beyond_the_fraction():
+    """The same form with one key of each sequence far above all others: its row of v is the result."""
+    hq, hkv, d, lens, dtype = 24, 8, 128, [4097, 4200], "bf16"
+    c = _case(18, lens, hq, hkv, d, dtype)
+    q, k, v = _parts(c)
+    q[:] = R.to_bits(np.full((1,), 2.0 ** 14), dtype)
+    k[:] = R.to_bits(np.full((1,), -2.0 ** 12), dtype)
+    best, at = [70, 4097 + 4000], 0  # (the weight of all others is 2^-(2^29) and less)
+    k[best] = R.to_bits(np.full((1,), -2.0 ** 11), dtype)
+    r = Run(c, True)
+    r.launch()
+    got = r.result().reshape(-1, hq, d)
+    vals = R.from_bits(np.ascontiguousarray(v), dtype).reshape(-1, hkv, d)
+    for n, b in zip(lens, best):
+        for h in range(hq):
+            want = np.broadcast_to(vals[b, h // 3], (at + n - b, d))
+            assert np.array_equal(got[b:at + n, h], want)
+        assert np.isfinite(got[at:b]).all()
+        at += n
