@@ -150,6 +150,21 @@ def test_few_rows(lens, max_rank, dtype, out):
     _check(_case(15, lens, np.arange(len(lens)) % 3 - 1, [max_rank, 1], max_rank, 1024, 4096, dtype, out))
 
 
+@pytest.mark.parametrize("dtype,out", OUTS)
+@pytest.mark.parametrize("max_rank", [72, 128, 200, 256])
+def test_large_ranks_of_long_sequences(max_rank, dtype, out):
+    _check(_case(16, [150, 33, 0, 70], [0, 1, 2, 2], [max_rank, 65, 7], max_rank, 392, 520, dtype, out))
+
+
+@pytest.mark.parametrize("dtype,out", [("fp16", "fp16"), ("bf16", "f32")])
+@pytest.mark.parametrize("max_rank", [32, 64, 128, 256])
+@pytest.mark.parametrize("lens", [[33] * 64, [1] * 200], ids=["33", "1"])
+def test_workgroups_of_several_steps(lens, max_rank, dtype, out):
+    """Enough tiles and outputs that a workgroup walks over its slice; the last slice ends inside a step."""
+    pick = np.arange(len(lens)) % 4 - 1
+    _check(_case(17, lens, pick, [max_rank, max_rank // 2 + 3, 5], max_rank, 11000, 264, dtype, out))
+
+
 def test_a_rank_above_the_slot_is_the_slots():
     c = _case(8, [20], [0], [16], 16, 136, 128, "fp16")
     want = Run(c)
