@@ -23,9 +23,13 @@
 // exceeds it by more than 2^8 (a probability is then at most 2^8 and the sums at most 2^8 times as large, far
 // inside the range of all types), so that rescaling the sums is rare.
 //
-// Bound by the matrix cores at heads of 128 and long sequences (one prompt of 16384 tokens, 32 / 8 heads: 2007 us, 1096 TFLOP/s,
-// a large matrix product of the library 1130); by the vector units at heads of 64 (per step 84 vector
-// instructions, 17 of them exponentials of four times the time, to 8 products: 4 prompts of 8192, 14 / 2 heads, 826 TFLOP/s).
+// Few long sequences: HALVES == 2, twice the waves, of which the second part takes every other key tile; its sums join the
+// first part's, each relative to its own maximum, through LDS.
+//
+// Bound by the matrix cores at heads of 128 and long sequences (one prompt of 16384 tokens, 32 / 8 heads: 2016 us, 1091 TFLOP/s,
+// a large matrix product of the library 1130); by the vector units at heads of 64 (per step 76 vector
+// instructions, 16 of them exponentials, to 8 products; nothing but those takes 520 clocks a step, this 770: 4 prompts of 8192, 14 / 2
+// heads, 580 us, 830 TFLOP/s).
 #include "device_utils.hpp"
 #include "launch_common.hpp"
 #include "packed_rows.hpp"
@@ -127,18 +131,21 @@ constexpr float kApLazy = 8.0f;
 // maximum, the same for all keys of a column.  Up to here that is at most 1 in the exponent and falls out of the result.
 constexpr float kApExact = 16777216.0f;
 
-template <typename T, int D, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void attn_packed_kernel(const AttnPackedParams p) {
+template <typename T, int D, int WAVES, int HALVES>
+__global__ __launch_bounds__(64 * WAVES * HALVES) void attn_packed_kernel(const AttnPackedParams p) {
     constexpr int kCols = 32 * WAVES, kMovers = 32 * WAVES;  // threads that move K, and V
     constexpr int kSteps = D / 16, kTiles = D / 32;  // operands of K (and of V) per key tile; output tiles
     constexpr int kKRow = D + 8, kVRow = D / 32 % 2 ? D : D + 32;  // elements
     constexpr int kKTile = kApKeys * kKRow, kVTile = kApKeys * kVRow;
     constexpr int kPer = kApKeys * D / 8 / kMovers;      // 16-byte pieces that a thread moves per tile
-    __shared__ __attribute__((aligned(16))) unsigned short lds[2 * kKTile + 2 * kVTile];
-    __shared__ unsigned odd_waves[WAVES];
-    unsigned short* const ks = lds;
-    unsigned short* const vs = lds + 2 * kKTile;
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    constexpr int kRings = 2 * kKTile + 2 * kVTile;
+    __shared__ __attribute__((aligned(16))) unsigned short lds[HALVES * kRings];
+    __shared__ unsigned odd_waves[WAVES * HALVES];
+    const int wave_of_all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int part = HALVES == 1 ? 0 : wave_of_all / WAVES;  // (takes the key tiles HALVES t + part)
+    const int wave = wave_of_all - part * WAVES, tid = threadIdx.x - part * 64 * WAVES, lane = tid & 63;
+    unsigned short* const ks = lds + part * kRings;
+    unsigned short* const vs = ks + 2 * kKTile;
     const int h = lane >> 5, col = lane & 31;
     const int kvh = (int)(blockIdx.x % (unsigned)p.hkv);
     const int at = (int)(blockIdx.x / (unsigned)p.hkv);
@@ -166,7 +173,7 @@ __global__ __launch_bounds__(64 * WAVES) void attn_packed_kernel(const AttnPacke
         for (int j = 0; j < kSteps; ++j) qb[j] = *reinterpret_cast<const uint4_t*>(q + 16 * j);
     }
 
-    // ---- movement: waves 0-3 carry K, waves 4-7 V, a thread kPer pieces of 16 bytes of a tile
+    // ---- movement: the first half of a part's waves carries K, the second V, a thread kPer pieces of 16 bytes of a tile
     const bool moves_v = wave >= WAVES / 2;
     const int64_t stride = moves_v ? p.v_stride : p.k_stride;
     const unsigned short* const src = (moves_v ? p.v : p.k) + (int64_t)t.row0 * stride + (int64_t)kvh * D;
@@ -185,7 +192,7 @@ __global__ __launch_bounds__(64 * WAVES) void attn_packed_kernel(const AttnPacke
         whole_at[u] = ((unsigned)key_of(u) * (unsigned)stride + 8u * (unsigned)piece_of(u)) * 2u;
     auto gload = [&](int tile, Regs& r) LG_INLINE {
         // (past the last visible key that key again: its probability is 0 for everybody who sees less)
-        const int key0 = min(tile * kApKeys, visible - 1);
+        const int key0 = min((HALVES * tile + part) * kApKeys, visible - 1);
         const char* at = reinterpret_cast<const char*>(src + (int64_t)key0 * stride);
         if (key0 + kApKeys <= visible) {
 #pragma unroll
@@ -242,7 +249,7 @@ __global__ __launch_bounds__(64 * WAVES) void attn_packed_kernel(const AttnPacke
             ka[j] = k_operand(1 - H, j);
             va[j] = v_operand(1 - H, j / kTiles, j % kTiles);
         }
-        const int key0 = tile * kApKeys;
+        const int key0 = (HALVES * tile + part) * kApKeys;
         float sc[16];
         float tm = -INFINITY;
         if (!MASKED || key0 + kApKeys <= first_vis) {
@@ -309,7 +316,7 @@ __global__ __launch_bounds__(64 * WAVES) void attn_packed_kernel(const AttnPacke
         p_prev[1] = pb[1];
     };
 
-    const int tiles = (visible + kApKeys - 1) / kApKeys;
+    const int tiles = (visible + HALVES * kApKeys - 1) / (HALVES * kApKeys);  // of a part (past the last key: nobody sees it)
     Regs ra, rb;
     {
         // V buffer 1 plays V(-1) in the first step, whose P is 0: finite values
@@ -337,7 +344,7 @@ __global__ __launch_bounds__(64 * WAVES) void attn_packed_kernel(const AttnPacke
             lstore(decltype(h_c)::value, now);  // K(tile + 2), V(tile)
             __syncthreads();
         };
-        const int plain = min(tiles, all_see / kApKeys) & ~1;
+        const int plain = min(tiles, all_see / (HALVES * kApKeys)) & ~1;
         int tile = 0;
         for (; tile < plain; tile += 2) {
             one(ic<0>{}, ic<0>{}, tile, ra, rb);
@@ -358,6 +365,7 @@ __global__ __launch_bounds__(64 * WAVES) void attn_packed_kernel(const AttnPacke
     // If the results are not all finite, or a maximum is too large for the fused difference, the keys are gone through again,
     // plainly, and in the tiles in which columns of the wave end with a pass of its own for every number of keys that one of them
     // sees.
+    float unit = 1.0f;  // of m, in powers of two
     {
         float odds[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // NaN if a result is not finite
 #pragma unroll
@@ -365,13 +373,14 @@ __global__ __launch_bounds__(64 * WAVES) void attn_packed_kernel(const AttnPacke
 #pragma unroll
             for (int e = 0; e < 16; ++e) odds[e & 3] = fmaf(o[dt][e], 0.0f, odds[e & 3]);
         const float odd = (odds[0] + odds[1]) + (odds[2] + odds[3]);
-        const bool any = __builtin_amdgcn_ballot_w64(odd != odd || fabsf(m) > kApExact) != 0;
-        if (lane == 0) odd_waves[wave] = any;
+        const bool any = __builtin_amdgcn_ballot_w64(odd != odd || (fabsf(m) > kApExact && m != -INFINITY)) != 0;
+        if (lane == 0) odd_waves[wave_of_all] = any;
         __syncthreads();
         unsigned all = 0;
 #pragma unroll
-        for (int w = 0; w < WAVES; ++w) all |= odd_waves[w];
+        for (int w = 0; w < WAVES * HALVES; ++w) all |= odd_waves[w];
         if (__builtin_expect(__builtin_amdgcn_readfirstlane(all) != 0, 0)) {
+            unit = p.scale_log2e;
             m = -INFINITY;
             l = 0.0f;
 #pragma unroll
@@ -379,7 +388,7 @@ __global__ __launch_bounds__(64 * WAVES) void attn_packed_kernel(const AttnPacke
 #pragma unroll
                 for (int e = 0; e < 16; ++e) o[dt][e] = 0.0f;
             for (int tile = 0; tile < tiles; ++tile) {
-                const int key0 = tile * kApKeys;
+                const int key0 = (HALVES * tile + part) * kApKeys;
                 __syncthreads();
                 gload(tile, ra);
                 lstore(0, ra);
@@ -418,18 +427,51 @@ __global__ __launch_bounds__(64 * WAVES) void attn_packed_kernel(const AttnPacke
         }
     }
     l += lane_xor_f32<32>(l);
+    unsigned short* stage = lds + wave * 16 * kKRow;
+    if constexpr (HALVES == 2) {
+        // the second part's results through LDS, each wave's own 128 D bytes, then its maxima and sums
+        static_assert(WAVES * (128 * D + 512) <= 2 * HALVES * kRings, "the second part's results fit");
+        float4_t* const theirs = reinterpret_cast<float4_t*>(lds) + wave * 8 * D;
+        float* const ml = reinterpret_cast<float*>(reinterpret_cast<float4_t*>(lds) + WAVES * 8 * D) + wave * 128;
+        if (part == 1) {
+#pragma unroll
+            for (int dt = 0; dt < kTiles; ++dt)
+#pragma unroll
+                for (int b = 0; b < 4; ++b)
+                    theirs[(4 * dt + b) * 64 + lane] =
+                        float4_t{o[dt][4 * b], o[dt][4 * b + 1], o[dt][4 * b + 2], o[dt][4 * b + 3]};
+            ml[lane] = m;
+            ml[64 + lane] = l;
+        }
+        __syncthreads();
+        if (part == 1) return;
+        const float other = ml[lane];
+        const float top = fmaxf(m, other), ref = top == -INFINITY ? 0.0f : top;
+        const float mine = fast_exp2((m - ref) * unit), its = fast_exp2((other - ref) * unit);
+        l = l * mine + ml[64 + lane] * its;
+#pragma unroll
+        for (int dt = 0; dt < kTiles; ++dt)
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                const float4_t w = theirs[(4 * dt + b) * 64 + lane];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[dt][4 * b + e] = o[dt][4 * b + e] * mine + w[e] * its;
+            }
+        stage = reinterpret_cast<unsigned short*>(theirs);
+        __builtin_amdgcn_wave_barrier();
+    }
     if (c0 >= cols) return;
-    static_assert(WAVES * 16 * kKRow <= 2 * kKTile + 2 * kVTile, "the columns on their way out fit");
+    static_assert(WAVES * 16 * kKRow <= kRings && 32 * kKRow <= 128 * D, "the columns on their way out fit");
     const int tok0 = c0 / p.g;  // of the wave's first column
     attn_packed_write<T, D>(p.out + (int64_t)(t.row0 + tok0) * p.out_stride,
                             (unsigned)(tok - tok0) * (unsigned)p.out_stride + (unsigned)(head * D), cols - c0,
-                            lds + wave * 16 * kKRow, o, l);
+                            stage, o, l);
 }
 
-template <typename T, int D, int WAVES>
+template <typename T, int D, int WAVES, int HALVES = 1>
 static hipError_t attn_packed_launch(const AttnPackedParams& p, hipStream_t stream) {
     const int64_t tiles = packed_tiles(p.total, p.num_seqs, p.g, 32 * WAVES);
-    attn_packed_kernel<T, D, WAVES><<<(unsigned)(tiles * p.hkv), 64 * WAVES, 0, stream>>>(p);
+    attn_packed_kernel<T, D, WAVES, HALVES><<<(unsigned)(tiles * p.hkv), 64 * WAVES * HALVES, 0, stream>>>(p);
     return hipGetLastError();
 }
 
@@ -441,11 +483,23 @@ static hipError_t attn_packed_by_width(const AttnPackedParams& p, int d, hipStre
     // 32 / 8, 156 / 154; 16 of 512, 32 / 8, 76 / 71.  64 wide: 4 x 8192, 14 / 2, 586 / 582; one of 2048 41 / 31.
     const bool wide = d == 128 && p.total >= 4096 * (int64_t)p.num_seqs &&
                       packed_tiles(p.total, p.num_seqs, p.g, 256) * p.hkv >= 3 * device_cu_count();
+    // Key tiles dealt out to two parts of a workgroup, joined at its end, where workgroups are few and keys many: the steps of a
+    // workgroup alone on its compute unit are latency (1000 clocks of the 770 that a step takes of three side by side), twice the
+    // waves hide it, but have a join, and no room for a second workgroup beside them.  us, one part / two, 64 wide, 14 / 2 heads:
+    // one of 512 11.8 / 11.3, of 2048 32.1 / 25.6, of 4096 61.9 / 51.7, two of 2048 41.5 / 31.4, but one of 256 8.4 / 8.8, four
+    // of 1024 22.5 / 25.4 and one of 6000 97 / 102; 128 wide, 12 / 2: one of 4096 91 / 76, but 32 / 8, one of 512 16.2 / 16.7.
+    const int64_t groups = (int64_t)p.total * p.g / 128 * p.hkv;
+    const bool split =
+        (groups <= device_cu_count() && p.total >= (d > 64 ? 8 * d : 512) * (int64_t)p.num_seqs) ||
+        (groups <= 2 * device_cu_count() && p.total >= 2048 * (int64_t)p.num_seqs);
     switch (d) {
-        case 32: return attn_packed_launch<T, 32, 4>(p, stream);
-        case 64: return attn_packed_launch<T, 64, 4>(p, stream);
-        case 96: return attn_packed_launch<T, 96, 4>(p, stream);
-        case 128: return wide ? attn_packed_launch<T, 128, 8>(p, stream) : attn_packed_launch<T, 128, 4>(p, stream);
+        case 32: return split ? attn_packed_launch<T, 32, 4, 2>(p, stream) : attn_packed_launch<T, 32, 4>(p, stream);
+        case 64: return split ? attn_packed_launch<T, 64, 4, 2>(p, stream) : attn_packed_launch<T, 64, 4>(p, stream);
+        case 96: return split ? attn_packed_launch<T, 96, 4, 2>(p, stream) : attn_packed_launch<T, 96, 4>(p, stream);
+        case 128:
+            return wide    ? attn_packed_launch<T, 128, 8>(p, stream)
+                   : split ? attn_packed_launch<T, 128, 4, 2>(p, stream)
+                           : attn_packed_launch<T, 128, 4>(p, stream);
         case 160: return attn_packed_launch<T, 160, 4>(p, stream);
         case 192: return attn_packed_launch<T, 192, 4>(p, stream);
         case 224: return attn_packed_launch<T, 224, 4>(p, stream);

@@ -326,3 +326,68 @@ def test_long_sequences_with_scores_beyond_the_fraction():
             assert np.array_equal(got[b:at + n, h], want)
         assert np.isfinite(got[at:b]).all()
         at += n
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("lens", [[1056], [3100, 1, 33], [0, 2113, 31]], ids=str)
+@pytest.mark.parametrize("d", [32, 64, 96, 128])
+def test_few_long_sequences(d, lens, causal, dtype):
+    """Key tiles dealt out to two parts of a workgroup: odd numbers of tiles, sequences and columns of which the
+    second part sees no key."""
+    _check(_case(19, lens, 4, 2, d, dtype, fused=True), causal)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("d", [32, 64, 96, 128])
+@pytest.mark.parametrize("bad", [1, 33, 640, 1089])
+def test_later_keys_of_few_long_sequences(d, bad, dtype):
+    c = _case(20, [1090], 4, 2, d, dtype)
+    want, bound = _want(c, True)
+    q, k, v = _parts(c)
+    k[bad], v[bad] = _nan(dtype), _nan(dtype)
+    r = Run(c, True)
+    r.launch()
+    got = r.result()
+    R.assert_within(got[:bad], want[:bad], bound[:bad])
+    assert np.isnan(got[bad:]).all()
+
+
+@pytest.mark.parametrize("negative", [False, True])
+@pytest.mark.parametrize("d", [32, 64, 96, 128])
+def test_scores_beyond_the_fraction_of_few_long_sequences(d, negative):
+    """One key far above the others (all scores below zero, or above it): its row of v, wherever it lies."""
+    n, hq, hkv, dtype = 1090, 4, 2, "bf16"
+    for best in (0, 31, 32, 700, 1089):
+        c = _case(21, [n], hq, hkv, d, dtype)
+        q, k, v = _parts(c)
+        q[:] = R.to_bits(np.full((1,), 2.0 ** 14), dtype)
+        low, high = (-2.0 ** 12, -2.0 ** 11) if negative else (2.0 ** 11, 2.0 ** 12)
+        k[:] = R.to_bits(np.full((1,), low), dtype)
+        k[best] = R.to_bits(np.full((1,), high), dtype)
+        r = Run(c, True, scale=16.0)
+        r.launch()
+        got = r.result().reshape(n, hq, d)
+        vals = R.from_bits(np.ascontiguousarray(v), dtype).reshape(n + GUARD, hkv, d)
+        for h in range(hq):
+            assert np.array_equal(got[best:, h], np.broadcast_to(vals[best, h // 2], (n - best, d)))
+        assert np.isfinite(got).all()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_keys_of_few_long_sequences_that_score_minus_infinity(d):
+    """The first token sees only such keys, then one part of the workgroup does: zeros, and the mean over the rest."""
+    c = _case(22, [1090], 2, 2, d, "bf16")
+    q, k, v = _parts(c)
+    q[:], k[:] = np.uint16(0x3F80), np.uint16(0)  # 1; 0: all that count score the same
+    hidden = np.arange(1090 + GUARD) // 32 % 2 == 0
+    k[hidden] = np.uint16(0xFF80)  # -inf
+    r = Run(c, True)
+    r.launch()
+    got = r.result()
+    assert (got[:32] == 0).all()
+    seen = np.where(hidden[:1090, None], 0.0, R.from_bits(np.ascontiguousarray(v[:1090]), "bf16"))
+    count = np.maximum(np.cumsum(~hidden[:1090]), 1)[:, None]
+    want, size = np.cumsum(seen, 0) / count, np.cumsum(np.abs(seen), 0) / count
+    # probabilities are exact ones; sums of up to 1090 terms, the reciprocal, the product, the result's rounding
+    R.assert_within(got, want, R.HALF_STEP["bf16"] * np.abs(want) * (1 + 2.0 ** -7) + 1100 * R.FP32 * size)
