@@ -290,14 +290,15 @@ __global__ __launch_bounds__(64 * WAVES * HALVES) void attn_packed_kernel(const 
         }
         if constexpr (!MASKED) {
             // half of the operand reads, then the products, each followed by a read (into registers freed before) and
-            // its share of the vector work
-            constexpr int kReads = 3 * kSteps, kFirst = 12 * kSteps / 8;
+            // its share of the vector work (128 wide, four instructions and not five: one prompt of 16384 2054 -> 2003 us, one of
+            // 8192 at 12 / 2 heads 235 -> 220; 64 wide, ten and not nine: one of 2048 at 14 / 2 heads 27.5 -> 26.4)
+            constexpr int kReads = 3 * kSteps, kFirst = 12 * kSteps / 8, kShare = (D < 128 ? 80 : 72) / (2 * kSteps);
             __builtin_amdgcn_sched_group_barrier(0x100, kFirst, 0);
 #pragma unroll
             for (int g = 0; g < 2 * kSteps; ++g) {
                 __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
                 if (g < kReads - kFirst) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(0x002, 80 / (2 * kSteps), 0);
+                __builtin_amdgcn_sched_group_barrier(0x002, kShare, 0);
             }
         }
         // (F belongs to this step: its results are used by the next one only, and would sink there)
