@@ -289,10 +289,10 @@ __global__ __launch_bounds__(64 * WAVES * HALVES) void attn_packed_kernel(const 
             pb[e >> 3][(e & 7) >> 1] = T::pack2(p0, p1);
         }
         if constexpr (!MASKED) {
-            // half of the operand reads, then the products, each followed by a read (into registers freed before) and
+            // half of the operand reads (64 wide five sixths: 1 to 2.5 % less, 128 wide 2 % more), then the products, each followed by a read (into registers freed before) and
             // its share of the vector work (128 wide, four instructions and not five: one prompt of 16384 2054 -> 2003 us, one of
             // 8192 at 12 / 2 heads 235 -> 220; 64 wide, ten and not nine: one of 2048 at 14 / 2 heads 27.5 -> 26.4)
-            constexpr int kReads = 3 * kSteps, kFirst = 12 * kSteps / 8, kShare = (D < 128 ? 80 : 72) / (2 * kSteps);
+            constexpr int kReads = 3 * kSteps, kFirst = (D > 64 ? 12 : 20) * kSteps / 8, kShare = (D < 128 ? 80 : 72) / (2 * kSteps);
             __builtin_amdgcn_sched_group_barrier(0x100, kFirst, 0);
 #pragma unroll
             for (int g = 0; g < 2 * kSteps; ++g) {
@@ -340,7 +340,11 @@ __global__ __launch_bounds__(64 * WAVES * HALVES) void attn_packed_kernel(const 
         auto one = [&](auto masked_c, auto h_c, int tile, Regs& now, Regs& next) LG_INLINE {
             gload(tile + ahead, next);
             __builtin_amdgcn_sched_barrier(0);
+            // (a wave in the middle of a step goes before one that moves tiles.  us with / without, 32 / 8 heads of 128: one of 4096 155 /
+            // 161, six of 1500 140 / 143; 96 wide 19.2 / 20.0; but 64 wide, three waves to a SIMD, 16 heads, 8 of 1000 42.9 / 37.9)
+            if constexpr (D >= 96) __builtin_amdgcn_s_setprio(1);
             step(masked_c, h_c, tile);
+            if constexpr (D >= 96) __builtin_amdgcn_s_setprio(0);
             __builtin_amdgcn_sched_barrier(0);
             lstore(decltype(h_c)::value, now);  // K(tile + 2), V(tile)
             __syncthreads();
