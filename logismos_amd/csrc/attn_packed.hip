@@ -484,10 +484,10 @@ template <typename T>
 static hipError_t attn_packed_by_width(const AttnPackedParams& p, int d, hipStream_t stream) {
     // 256 columns to a workgroup (eight waves, K and V moved half as often) where the sequences are long and there are
     // many of them; otherwise 128, of which a compute unit holds two or three that fill each other's waits.  us, 8 / 4 waves, 128
-    // wide: one of 16384, 32 / 8 heads, 2007 / 2107; 4 x 4096, 12 / 2, 397 / 416; one of 8192, 12 / 2, 236 / 229; one of 4096,
-    // 32 / 8, 156 / 154; 16 of 512, 32 / 8, 76 / 71.  64 wide: 4 x 8192, 14 / 2, 586 / 582; one of 2048 41 / 31.
-    const bool wide = d == 128 && p.total >= 4096 * (int64_t)p.num_seqs &&
-                      packed_tiles(p.total, p.num_seqs, p.g, 256) * p.hkv >= 3 * device_cu_count();
+    // wide, 32 / 8 heads: one of 16384 2006 / 2132, one of 4096 140 / 149, 8 of 2048 313 / 322, but 16 of 1500 384 / 365, 16 of
+    // 512 74 / 71; 12 / 2: one of 16384 804 / 841, one of 8192 230 / 226.  64 wide: 4 x 8192, 14 / 2, 586 / 582; one of 2048 41 / 31.
+    const bool wide = d == 128 && p.total >= 2048 * (int64_t)p.num_seqs &&
+                      packed_tiles(p.total, p.num_seqs, p.g, 256) * p.hkv >= 2 * device_cu_count();
     // Key tiles dealt out to two parts of a workgroup, joined at its end, where workgroups are few and keys many: the steps of a
     // workgroup alone on its compute unit are latency (1000 clocks of the 770 that a step takes of three side by side), twice the
     // waves hide it, but have a join, and no room for a second workgroup beside them.  us, one part / two, 64 wide, 14 / 2 heads:
