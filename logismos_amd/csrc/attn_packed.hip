@@ -26,7 +26,7 @@
 // Few long sequences: HALVES == 2, twice the waves, of which the second part takes every other key tile; its sums join the
 // first part's, each relative to its own maximum, through LDS.
 //
-// Bound by the matrix cores at heads of 128 and long sequences (one prompt of 16384 tokens, 32 / 8 heads: 2016 us, 1091 TFLOP/s,
+// Bound by the matrix cores at heads of 128 and long sequences (one prompt of 16384 tokens, 32 / 8 heads: 2007 us, 1095 TFLOP/s,
 // a large matrix product of the library 1130); by the vector units at heads of 64 (per step 76 vector
 // instructions, 16 of them exponentials, to 8 products; nothing but those takes 520 clocks a step, this 770: 4 prompts of 8192, 14 / 2
 // heads, 580 us, 830 TFLOP/s).
