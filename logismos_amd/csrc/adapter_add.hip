@@ -28,7 +28,7 @@
 namespace lg {
 
 constexpr int kAdapterMaxRank = 256;
-constexpr int kAdapterMaxParts = 8;   // K parts of v
+constexpr int kAdapterMaxParts = 8;   // K parts of v, read four at a time
 
 struct AdapterParams {
     const unsigned short* x;
@@ -316,15 +316,15 @@ __global__ __launch_bounds__(256, 2) void adapter_up_kernel(const AdapterParams 
     auto v_at = [&](int i) LG_INLINE {
         return p.v + (row0 + min(i / kChunks, left - 1)) * p.max_rank + min(8 * (i % kChunks), p.max_rank - 8);
     };
-    auto load_v = [&](Parts& v, const float* at) LG_INLINE {
+    auto load_v = [&](Parts& v, const float* at, int s0) LG_INLINE {
 #pragma unroll
         for (int s = 0; s < 4; ++s)
 #pragma unroll
             for (int e = 0; e < 2; ++e)
-                v.w[s][e] = *reinterpret_cast<const float4_t*>(at + min(s, p.parts - 1) * part + 4 * e);
+                v.w[s][e] = *reinterpret_cast<const float4_t*>(at + min(s0 + s, p.parts - 1) * part + 4 * e);
     };
     Parts v;
-    load_v(v, v_at(threadIdx.x));
+    load_v(v, v_at(threadIdx.x), 0);
     load_base(ic<0>{}, even, n0);
     if (named) rank = max(0, min(__builtin_amdgcn_readfirstlane(raw_rank), p.max_rank));
     if (rank == 0 && p.base == p.out) return;
@@ -333,24 +333,22 @@ __global__ __launch_bounds__(256, 2) void adapter_up_kernel(const AdapterParams 
         for (int s = 0; s < kHeld; ++s) load_b(ic<0>{}, n0, s);
         for (int i = threadIdx.x; i < kRows * kChunks; i += 256) {
             const int row = i / kChunks, chunk = i % kChunks, r = 8 * chunk;
-            if (i >= 256) load_v(v, v_at(i));
+            if (i >= 256) load_v(v, v_at(i), 0);
             float u[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) u[e] = 0.0f;
+            auto add_v = [&](int s0) LG_INLINE {
 #pragma unroll
-            for (int s = 0; s < 4; ++s)
-                if (s < p.parts) {
+                for (int s = 0; s < 4; ++s)
+                    if (s0 + s < p.parts) {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) u[e] += v.w[s][e >> 2][e & 3];
-                }
-            for (int s = 4; s < p.parts; ++s) {
-                const float4_t* src = reinterpret_cast<const float4_t*>(v_at(i) + s * part);
-                const float4_t u0 = src[0], u1 = src[1];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    u[e] += u0[e];
-                    u[4 + e] += u1[e];
-                }
+                        for (int e = 0; e < 8; ++e) u[e] += v.w[s][e >> 2][e & 3];
+                    }
+            };
+            add_v(0);
+            if (p.parts > 4) {
+                load_v(v, v_at(i), 4);
+                add_v(4);
             }
             adapter_terms<T, TERMS, kChunks>(
                 u, row < left, r, rank, scale, &growth[row],
