@@ -14,7 +14,7 @@
 // Bound by memory: x, base and out once, A and B of the adapters in use.  16 prompts of 512 x 4096, rank 64, 24576 outputs in 16
 // bits: 900 MB in 229 us, 3.9 TB/s (a large copy 5.2; the first launch 26 us, the second 203: its beginnings, and
 // products and vector work that the memory time does not all cover; rank 32 192 us); 13 single rows and 5 chunks of 31 to 600, 8960 columns to 1536 in
-// fp32: 54 MB in 23 us; 32 single rows on 8 adapters, 4096 to 6144: 10.5 us, a chain of dependent loads.
+// fp32: 54 MB in 22 us; 32 single rows on 8 adapters, 4096 to 6144: 10.5 us, a chain of dependent loads.
 #include "device_utils.hpp"
 #include "launch_common.hpp"
 #include "packed_rows.hpp"
