@@ -378,7 +378,9 @@ __global__ __launch_bounds__(64 * WAVES * HALVES) void attn_packed_kernel(const 
 #pragma unroll
             for (int e = 0; e < 16; ++e) odds[e & 3] = fmaf(o[dt][e], 0.0f, odds[e & 3]);
         const float odd = (odds[0] + odds[1]) + (odds[2] + odds[3]);
-        const bool any = __builtin_amdgcn_ballot_w64(odd != odd || (fabsf(m) > kApExact && m != -INFINITY)) != 0;
+        // (a column that sees keys, none of them above -inf times the scale, may hold scores that are finite before it)
+        const bool far = fabsf(m) > kApExact && vis > kApKeys * part;
+        const bool any = __builtin_amdgcn_ballot_w64(odd != odd || far) != 0;
         if (lane == 0) odd_waves[wave_of_all] = any;
         __syncthreads();
         unsigned all = 0;
