@@ -11,17 +11,13 @@
 // The result layout of S^T is the operand layout of P when the keys of a step of 16 are taken in the order
 // 4h + i, 8 + 4h + i (h: half of the wave, i < 4); V comes out of its row-major tile in that order through the
 // transposing LDS read.  P goes in rounded to the rows' type: every term is off by at most half a step of that type
-// relative to itself, as every output is by its own rounding.
+// relative to itself, as every output is by its own rounding (fp16: terms below 2^-25 of the largest by more, see ApRange).
 //
 // Schedule: the stages of a tile -- S(t) and O(t) on the matrix cores, F(t), the softmax, on the vector units -- run
 // one behind the other in a wave: step t issues S(t + 1) and O(t - 1) around F(t), so that the products of a step
 // do not depend on its vector work and the two can be interleaved instruction by instruction.  K is stored into LDS two
 // tiles ahead of its use and V one step, each by half of the waves; the rings are two deep.  Rows of K lie 2 D + 16 bytes
 // apart and those of V an odd multiple of 64: the operand reads of 16 (32) lanes then touch every bank once.
-//
-// The reference that the exponentials are taken relative to follows the maximum lazily: it is raised when a tile
-// exceeds it by more than 2^8 (a probability is then at most 2^8 and the sums at most 2^8 times as large, far
-// inside the range of all types), so that rescaling the sums is rare.
 //
 // Few long sequences: HALVES == 2, twice the waves, of which the second part takes every other key tile; its sums join the
 // first part's, each relative to its own maximum, through LDS.
@@ -54,6 +50,32 @@ struct AttnPackedParams {
 
 constexpr int kApKeys = 32;
 
+// What the exponentials are taken relative to is a reference that follows the maximum lazily: it is raised when a tile
+// exceeds it by more than 2^kLazy, so that rescaling the sums is rare.  The largest probability of a column then lies between
+// 2^kHead and 2^(kHead + kLazy); numerator and denominator carry the same factor.
+//
+// fp16 ends at 2^16 and loses bits below 2^-14, so its probabilities start as high as they can: those down to 2^-25 of a column's largest
+// keep all bits, smaller ones are off by up to 2^-36 of it.  (With the largest at 1, 16384 keys at 2^-21.5 of one whose row of V is
+// zero were off by 6 %, and below 2^-25 they vanished.)
+template <typename T>
+struct ApRange;
+template <>
+struct ApRange<PackedF16> {
+    static constexpr float kHead = 11.0f, kLazy = 4.0f;
+};
+template <>
+struct ApRange<PackedBf16> {
+    static constexpr float kHead = 0.0f, kLazy = 8.0f;
+};
+
+// The reference for a maximum.  (Not fused: the constant is then part of the instruction, and needs no register.)
+template <typename T>
+__device__ __forceinline__ float attn_packed_reference(float top, float scale_log2e) {
+    float scaled = top * scale_log2e;
+    asm("" : "+v"(scaled));
+    return scaled - ApRange<T>::kHead;
+}
+
 // Probabilities of the 16 keys that a lane holds of its column (keys first + 8 (e / 4) + e % 4), the running maximum (of the
 // scores as they are: their differences are taken before the scale) and sum; returns what the sums so far are to be
 // multiplied by.
@@ -74,8 +96,8 @@ __device__ __forceinline__ float attn_packed_softmax(float16_t sc, int first, in
     l *= alpha;
 #pragma unroll
     for (int e = 0; e < 16; e += 2) {
-        const float p0 = fast_exp2((sc[e] - ref) * scale_log2e);
-        const float p1 = fast_exp2((sc[e + 1] - ref) * scale_log2e);
+        const float p0 = fast_exp2(fmaf(sc[e] - ref, scale_log2e, ApRange<T>::kHead));
+        const float p1 = fast_exp2(fmaf(sc[e + 1] - ref, scale_log2e, ApRange<T>::kHead));
         l += p0 + p1;
         pb[e >> 3][(e & 7) >> 1] = T::pack2(p0, p1);
     }
@@ -126,10 +148,12 @@ __device__ __forceinline__ void attn_packed_write(unsigned short* out, unsigned 
     }
 }
 
-constexpr float kApLazy = 8.0f;
 // A scaled score less the rounded product of the maximum and the scale, in one rounding: off by up to half a step of the
 // maximum, the same for all keys of a column.  Up to here that is at most 1 in the exponent and falls out of the result.
 constexpr float kApExact = 16777216.0f;
+// The reference of a column that has seen nothing above -inf yet: finite, so that such a key weighs 0 without a test, and so far
+// down that whoever still has it in the end goes the plain way.
+constexpr float kApNone = -3e38f;
 
 template <typename T, int D, int WAVES, int HALVES>
 __global__ __launch_bounds__(64 * WAVES * HALVES) void attn_packed_kernel(const AttnPackedParams p) {
@@ -229,7 +253,7 @@ __global__ __launch_bounds__(64 * WAVES * HALVES) void attn_packed_kernel(const 
         return *reinterpret_cast<const uint4_t*>(ks + buf * kKTile + col * kKRow + 16 * j + 8 * h);
     };
 
-    float m = -INFINITY, l = 0.0f;
+    float m = kApNone, l = 0.0f;
     float16_t o[kTiles];
 #pragma unroll
     for (int dt = 0; dt < kTiles; ++dt)
@@ -265,11 +289,10 @@ __global__ __launch_bounds__(64 * WAVES * HALVES) void attn_packed_kernel(const 
                 tm = fmaxf(tm, sc[e]);
             }
         }
-        tm = fmaxf(tm, lane_xor_f32<32>(tm)) * p.scale_log2e;
-        const bool raise = tm > m + kApLazy;
+        tm = attn_packed_reference<T>(fmaxf(tm, lane_xor_f32<32>(tm)), p.scale_log2e);
+        const bool raise = tm > m + ApRange<T>::kLazy;
         const float m_before = m;
         m = raise ? tm : m;
-        const float ref = m == -INFINITY ? 0.0f : -m;
         float16_t s_nxt;
 #pragma unroll
         for (int e = 0; e < 16; ++e) s_nxt[e] = 0.0f;
@@ -282,8 +305,8 @@ __global__ __launch_bounds__(64 * WAVES * HALVES) void attn_packed_kernel(const 
         uint4_t pb[2];
 #pragma unroll
         for (int e = 0; e < 16; e += 2) {
-            const float p0 = fast_exp2(fmaf(sc[e], p.scale_log2e, ref));
-            const float p1 = fast_exp2(fmaf(sc[e + 1], p.scale_log2e, ref));
+            const float p0 = fast_exp2(fmaf(sc[e], p.scale_log2e, -m));
+            const float p1 = fast_exp2(fmaf(sc[e + 1], p.scale_log2e, -m));
             sum += p0;
             sum += p1;
             pb[e >> 3][(e & 7) >> 1] = T::pack2(p0, p1);

@@ -53,3 +53,115 @@ def test_scores_that_are_finite_before_the_scale_only(lens, hq, hkv, d, dtype, c
             R.assert_within(got[at:at + n, h], want, (u * (1 + 2.0 ** -20) + 3 * R.FP32) * np.abs(want)
                             + (2.0 ** -25 if dtype == "fp16" else 0.0), f"sequence of {n}, head {h}")
         at += n
+
+
+HALF = {"fp16": 2.0 ** -11, "bf16": 2.0 ** -8}
+SCALE = float(np.float32(np.log(2)))  # scores are powers of two then
+
+
+def _attn_case(lens, hq, hkv, d, dtype, scores, v, odd_head):
+    """Queries (1, 0, ..): the score of a key is its first element.  odd_head: the last query head of
+    every group is NaN, so that every workgroup goes through its keys a second time."""
+    T = sum(lens) + A.GUARD
+    q, k = np.zeros((T, hq, d)), np.zeros((T, hkv, d))
+    q[..., 0] = 1.0
+    k[:len(scores), :, 0] = scores[:, None]
+    rows = R.to_bits(np.concatenate([x.reshape(T, -1) for x in (q, k, v)], 1), dtype)
+    assert np.array_equal(R.from_bits(rows[:, hq * d:(hq + hkv) * d:d], dtype), k[..., 0])
+    if odd_head:
+        g = hq // hkv
+        rows[:, :hq * d].reshape(T, hkv, g, d)[:, :, g - 1] = A._nan(dtype)
+    return dict(rows=rows, lens=lens, hq=hq, hkv=hkv, d=d, dtype=dtype, fused=False, T=T)
+
+
+FORMS = [  # lengths, query and KV heads, head width
+    ([300], 2, 1, 64), ([4096], 2, 1, 192), ([4096], 2, 1, 64), ([4096], 2, 1, 128),
+    ([4097, 4200], 24, 8, 128), ([16384], 2, 2, 64)]
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("odd_head", [False, True], ids=["", "second walk"])
+@pytest.mark.parametrize("below", [16.0, 18.625, 21.5, 23.5, 25.25])
+@pytest.mark.parametrize("lens,hq,hkv,d", FORMS)
+def test_many_small_weights_beside_one_of_nothing(lens, hq, hkv, d, below, odd_head, dtype):
+    """One key of each sequence outweighs every other one by 2^below and has a V row of zeros: the result
+    is what the others add up to."""
+    if odd_head and hq == hkv:
+        pytest.skip("needs two query heads to a KV head")
+    rng = np.random.default_rng(1)
+    T, n_all = sum(lens) + A.GUARD, sum(lens)
+    v = np.broadcast_to(1.0 + rng.integers(0, 8, (hkv, d)) / 8, (T, hkv, d)).copy()
+    scores = np.full(n_all, -below)
+    at = 0
+    sinks = []
+    for i, n in enumerate(lens):
+        sinks.append(at + (0 if i % 2 == 0 else n // 2))
+        at += n
+    scores[sinks] = 0.0
+    v[sinks] = 0.0
+    c = _attn_case(lens, hq, hkv, d, dtype, scores, v, odd_head)
+    g, u = hq // hkv, HALF[dtype]
+    heads = [h for h in range(hq) if not (odd_head and h % g == g - 1)]
+    w = np.exp(-below * SCALE)
+    # A weight is rounded to the rows' type (fp16: those below 2^-25 of the largest to multiples of 2^-35 of
+    # it); its exponent is a rounded difference, the exponential good to 2^-22.
+    one = max(u * w, 2.0 ** -36 if dtype == "fp16" else 0.0)
+    delta = 4 * R.FP32 * (below + 16) + 2.0 ** -22
+    for causal in (False, True):
+        r = A.Run(c, causal, SCALE)
+        r.launch()
+        got = r.result().reshape(n_all, hq, d)
+        at = 0
+        for n, sink in zip(lens, sinks):
+            t = np.arange(n)
+            seen = t + 1.0 if causal else np.full(n, float(n))
+            there = (t >= sink - at) if causal else np.ones(n, bool)  # sees the heavy key
+            others = seen - there
+            weight = np.where(there, w, 1.0)
+            total = others * weight + there
+            mean = (others * weight / total)[:, None]
+            lost = (others * np.where(there, one, u) / total)[:, None]
+            for h in heads:
+                value = v[at + (1 if sink == at else 0), h // g][None]
+                o = mean * value
+                e = lost * value + (2 * delta + 2 * n * R.FP32) * o
+                bound = u * o * (1 + u) + e * (1 + 4 * u) + (2.0 ** -25 if dtype == "fp16" else 0.0)
+                R.assert_within(got[at:at + n, h], o, bound, f"causal={causal}, sequence of {n}, head {h}")
+            at += n
+        if odd_head:
+            assert np.isnan(got[:, g - 1]).all()
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_weights_that_only_count_together(dtype):
+    """131072 keys, each 2^-25.25 of the first, whose V row is zero."""
+    n, d, below = 131072, 64, 25.25
+    v = np.full((n + A.GUARD, 1, d), 1.5)
+    v[0] = 0.0
+    scores = np.full(n, -below)
+    scores[0] = 0.0
+    c = _attn_case([n], 1, 1, d, dtype, scores, v, False)
+    r = A.Run(c, False, SCALE)
+    r.launch()
+    got, w, u = r.result(), np.exp(-below * SCALE), HALF[dtype]
+    total = 1 + (n - 1) * w
+    o = (n - 1) * w / total * 1.5
+    one = max(u * w, 2.0 ** -36 if dtype == "fp16" else 0.0)
+    e = (n - 1) * one / total * 1.5 + (2 * (4 * R.FP32 * (below + 16) + 2.0 ** -22) + 2 * n * R.FP32) * o
+    R.assert_within(got, np.full_like(got, o), u * o * (1 + u) + e * (1 + 4 * u) + 2.0 ** -25)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("d", [32, 64, 128, 256])
+@pytest.mark.parametrize("step", [1, 4, 8])
+def test_scores_that_rise_little_by_little(step, d, dtype):
+    """From key to key by step eighths of a power of two: what the weights are relative to lies as far below
+    the largest as it may, and the largest as high in the type."""
+    n = 256 // step
+    rng = np.random.default_rng(2)
+    v = rng.integers(1, 9, (n + 2 * n + A.GUARD, 2, d)) / 4.0
+    scores = np.concatenate([np.arange(n) * step, np.repeat(np.arange(n), 2) * step // 2]) / 8.0
+    lens = [n, 2 * n]
+    c = _attn_case(lens, 4, 2, d, dtype, np.floor(scores * 8) / 8, v, False)
+    for causal in (False, True):
+        A._check(c, causal, SCALE)
