@@ -682,7 +682,7 @@ logismos_status_t logismos_rope_frequencies(double* inv_freq, float* amplitude, 
  *           16-byte aligned, strides multiples of 8
  *
  * fp32 scores, softmax and sums; the probabilities are rounded to the rows' type for the second product (fp16: those below
- * 2^-25 of a row's largest are off by up to 2^-36 of it).  Elements of keys that a token does not see do not reach its result, whatever they hold; a token whose keys all score
+ * 2^-25 of a row's largest are off by up to 2^-36 of it; bf16: those below 2^-94 of it count as 0).  Elements of keys that a token does not see do not reach its result, whatever they hold; a token whose keys all score
  * -inf gives zeros.  scale > 0 and scale * log2(e) finite (else hipErrorInvalidValue); head_dim a multiple of 32 up to 256; num_q_heads a
  * multiple of num_kv_heads; k, v and out strides up to 2^22; total_tokens * num_q_heads / 128 +
  * num_seqs * num_kv_heads up to 2^22.  out does not overlap q, k or v. */

@@ -57,6 +57,9 @@ constexpr int kApKeys = 32;
 // fp16 ends at 2^16 and loses bits below 2^-14, so its probabilities start as high as they can: those down to 2^-25 of a column's largest
 // keep all bits, smaller ones are off by up to 2^-36 of it.  (With the largest at 1, 16384 keys at 2^-21.5 of one whose row of V is
 // zero were off by 6 %, and below 2^-25 they vanished.)
+//
+// bf16 has the exponents of fp32, and V may hold anything up to 2^128: probabilities of at most 2^-24 add up to less than that over
+// the 2^23 keys that there can be, so that finite values have a finite mean.  Those below 2^-94 of a column's largest vanish.
 template <typename T>
 struct ApRange;
 template <>
@@ -65,7 +68,7 @@ struct ApRange<PackedF16> {
 };
 template <>
 struct ApRange<PackedBf16> {
-    static constexpr float kHead = 0.0f, kLazy = 8.0f;
+    static constexpr float kHead = -32.0f, kLazy = 8.0f;
 };
 
 // The reference for a maximum.  (Not fused: the constant is then part of the instruction, and needs no register.)

@@ -165,3 +165,26 @@ def test_scores_that_rise_little_by_little(step, d, dtype):
     c = _attn_case(lens, 4, 2, d, dtype, np.floor(scores * 8) / 8, v, False)
     for causal in (False, True):
         A._check(c, causal, SCALE)
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("odd_head", [False, True], ids=["", "second walk"])
+@pytest.mark.parametrize("lens,hq,hkv,d", [([2, 33, 150], 4, 2, 64), ([70, 200], 4, 2, 256), ([1090], 4, 2, 64),
+                                           ([1090], 4, 2, 128), ([4097, 4200], 24, 8, 128)])
+def test_the_mean_of_the_largest_values(lens, hq, hkv, d, odd_head, causal):
+    """bf16 values up to 2^127, of which two add up to more than fp32 holds: their weighted mean is finite."""
+    rng = np.random.default_rng(4)
+    c = A._case(23, lens, hq, hkv, d, "bf16")
+    q, _, v = A._parts(c)
+    v[:] = R.to_bits(rng.uniform(0.5, 1, v.shape) * 2.0 ** 127, "bf16")
+    n, g, kvh = sum(lens), hq // hkv, hkv - 1
+    heads = np.arange(kvh * g, kvh * g + g - odd_head)  # (those of the last KV head, the odd ones left out)
+    bits = [np.ascontiguousarray(x[:n]) for x in A._parts(c)]
+    if odd_head:
+        q.reshape(len(q), hkv, g, d)[:, :, g - 1] = A._nan("bf16")
+    r = A.Run(c, causal)
+    r.launch()
+    got = r.result().reshape(n, hq, d)
+    fq, fk, fv = (R.from_bits(x, "bf16").reshape(n, -1, d) for x in bits)
+    want, bound = R.attention(fq[:, heads], fk[:, kvh:kvh + 1], fv[:, kvh:kvh + 1], lens, r.scale, causal, "bf16")
+    R.assert_within(got[:, heads], want, bound)
