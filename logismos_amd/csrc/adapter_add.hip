@@ -7,8 +7,8 @@
 // takes the same rows through B and adds the base.  Products on the matrix cores.
 //
 // s v has to be an operand of the second product, so it is split into 16-bit terms: per row scaled by a power
-// of two that brings its largest value into [1, 2) (exact, and undone in the fp32 result; fp16 could not hold the values
-// as they are), then the rounded value and what the rounding left.  fp16: two terms, 22 bits; bf16: two terms,
+// of two that brings its largest value to where the type has most room (exact, and undone in the fp32 result; fp16 could not hold
+// the values as they are), then the rounded value and what the rounding left.  fp16: two terms, 22 bits; bf16: two terms,
 // 16 bits, for outputs of 8, three, 24 bits, for fp32 outputs.
 //
 // Bound by memory: x, base and out once, A and B of the adapters in use.  16 prompts of 512 x 4096, rank 64, 24576 outputs in 16
@@ -158,9 +158,17 @@ __global__ __launch_bounds__(256, 2) void adapter_down_kernel(const AdapterParam
     }
 }
 
+// Where the terms' type has the row's largest value, as a power of two.  fp16 ends at 2^16 and loses bits below 2^-14: up there two terms
+// are off by 2^-22 of every rank down to 2^-17 of the largest, and by 2^-39 of the largest below.  (With the largest at 1, by 2^-25 of
+// it: a rank 2^-18 below it by 5.6 half steps of fp16, which show in every output whose B is small at the largest.)
+template <typename T>
+constexpr int kAdapterTop = 0;
+template <>
+constexpr int kAdapterTop<PackedF16> = 14;
+
 // Eight ranks u of a row (from rank r on), the chunks of a row in neighbouring lanes: times the adapter's scale, zero behind the
-// rank and the rows, brought by a power of two to where the row's largest value lies in [1, 2), split into terms of the
-// operand's type, 64 words of four apart.  growth: what undoes the power of two.
+// rank and the rows, brought by a power of two to where the row's largest value lies in [2^kAdapterTop, twice that), split into terms of
+// the operand's type, 64 words of four apart.  growth: what undoes the power of two.
 template <typename T, int TERMS, int CHUNKS>
 __device__ __forceinline__ void adapter_terms(float (&u)[8], bool live, int r, int rank, float scale, float* growth,
                                               uint4_t* operand) {
@@ -174,9 +182,10 @@ __device__ __forceinline__ void adapter_terms(float (&u)[8], bool live, int r, i
 #pragma unroll
     for (int m = 1; m < CHUNKS; m *= 2) top = fmaxf(top, shfl_xor_f32(top, m));
     const int ex = (int)(__float_as_uint(top) >> 23);  // (as far as fp32 has the power of two)
-    const int down = ex < 1 ? 1 : ex > 253 ? 253 : ex;
-    const float shrink = __uint_as_float((unsigned)(254 - down) << 23);
-    if (r == 0) *growth = __uint_as_float((unsigned)down << 23);
+    constexpr int kTop = kAdapterTop<T>, kLow = kTop > 0 ? kTop + 1 : 1, kHigh = kTop > 0 ? 254 : 253 + kTop;
+    const int down = ex < kLow ? kLow : ex > kHigh ? kHigh : ex;
+    const float shrink = __uint_as_float((unsigned)(254 + kTop - down) << 23);
+    if (r == 0) *growth = __uint_as_float((unsigned)(down - kTop) << 23);
 #pragma unroll
     for (int e = 0; e < 8; ++e) u[e] *= shrink;
 #pragma unroll

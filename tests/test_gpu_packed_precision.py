@@ -5,6 +5,7 @@ import numpy as np
 import pytest
 
 from tests import packed_reference as R
+from tests import test_gpu_adapter_add as D
 from tests import test_gpu_attn_packed as A
 
 pytestmark = pytest.mark.gpu
@@ -188,3 +189,57 @@ def test_the_mean_of_the_largest_values(lens, hq, hkv, d, odd_head, causal):
     fq, fk, fv = (R.from_bits(x, "bf16").reshape(n, -1, d) for x in bits)
     want, bound = R.attention(fq[:, heads], fk[:, kvh:kvh + 1], fv[:, kvh:kvh + 1], lens, r.scale, causal, "bf16")
     R.assert_within(got[:, heads], want, bound)
+
+
+# What the terms of x . A^T are off by: relative to the value itself, and to the largest of its row.
+TERMS = {("fp16", "fp16"): (2.0 ** -22, 2.0 ** -39), ("bf16", "bf16"): (2.0 ** -16, 0.0)}
+TILES = [[1, 16, 3], [40, 1, 90], [1, 2] * 150, [33] * 40]
+
+
+def _uneven_case(lens, max_rank, n, below, dtype, out):
+    """The first rank's value is 2^below times the others' and its column of B zero: x holds a large and a small
+    element, A one of them per rank."""
+    k = 128
+    c = D._case(24, lens, np.arange(len(lens)) % 2, [max_rank, max_rank - 3], max_rank, n, k, dtype, out)
+    rng = np.random.default_rng(5)
+
+    def between(*shape):
+        return rng.uniform(1, 2, shape) * rng.choice([-1, 1], shape)
+
+    x, a = np.zeros(c["x"].shape), np.zeros(c["a"].shape)
+    x[:, 40], x[:, 7] = 2.0 ** 10 * between(len(x)), between(len(x))
+    a[:, 0, 40], a[:, 1:, 7] = 2.0 ** 10 * between(2), 2.0 ** (20 - below) * between(2, max_rank - 1)
+    b = R.from_bits(c["b"], dtype)
+    b[:, :, 0] = 0.0
+    c["x"], c["a"], c["b"] = (R.to_bits(y, dtype) for y in (x, a, b))
+    c["base"] = np.zeros_like(c["base"])
+    return c
+
+
+def _uneven_want(c, terms):
+    f = lambda y: R.from_bits(y, c["dtype"])  # noqa: E731
+    n, u = sum(c["lens"]), R.HALF_STEP[c["out_dtype"]]
+    want, bound, at = np.zeros((n, c["n"])), np.zeros((n, c["n"])), 0
+    for i, p in zip(c["lens"], c["pick"]):
+        r, s = c["ranks"][p], float(c["scales"][p])
+        v = f(c["x"][at:at + i]) @ f(c["a"][p, :r]).T * s
+        b = f(c["b"][p, :, :r]).T
+        # v: one product that counts, its sum and the scale in fp32; then its terms and the sum over the ranks
+        e = np.abs(v) * (4 * R.FP32 + terms[0]) + np.abs(v).max(1, keepdims=True) * terms[1]
+        y = v @ b
+        ey = e @ np.abs(b) + 3 * (r + 4) * R.FP32 * (np.abs(v) @ np.abs(b))
+        want[at:at + i], bound[at:at + i] = y, ey + u * (np.abs(y) + ey) + (
+            2.0 ** -25 if c["out_dtype"] == "fp16" else 0.0)
+        at += i
+    return want, bound
+
+
+@pytest.mark.parametrize("dtype,out", list(TERMS))
+@pytest.mark.parametrize("below", [12, 18, 22, 26])
+@pytest.mark.parametrize("max_rank", [8, 16, 32, 64, 128, 256])
+@pytest.mark.parametrize("lens", TILES, ids=lambda v: f"{len(v)} of {max(v)}")
+def test_small_ranks_beside_a_large_one(lens, max_rank, below, dtype, out):
+    c = _uneven_case(lens, max_rank, 264, below, dtype, out)
+    r = D.Run(c)
+    r.launch()
+    R.assert_within(R.from_bits(r.bits()[:sum(lens)], out), *_uneven_want(c, TERMS[dtype, out]))
