@@ -717,8 +717,9 @@ logismos_status_t logismos_launch_attn_packed_bf16(const void* q, const void* k,
  *   workspace       `logismos_adapter_add_workspace_bytes(total_tokens, max_rank)` bytes, contents don't matter;
  *                   not shared by calls that can overlap in time
  *
- * fp32 sums; x . A^T is not rounded below what the result's type holds; one rounding at the end.  max_rank a multiple of 8
- * up to 256, n, k and strides multiples of 8, n, k and the strides of base and out at most 2^22; x, a, b, base, out, workspace 16-byte aligned. */
+ * fp32 sums; x . A^T goes into the second product with more bits than the result's type holds: 16 for bf16 outputs, 22
+ * for fp16 (of values down to 2^-17 of their row's largest; below, up to 2^-39 of the largest is lost), all 24 for fp32 (of fp16 rows down to
+ * 2^-15 of the largest, below as for fp16).  One rounding at the end.  max_rank a multiple of 8 up to 256, n, k and strides multiples of 8, n, k and the strides of base and out at most 2^22; x, a, b, base, out, workspace 16-byte aligned. */
 logismos_status_t logismos_check_adapter_add_shape(int num_seqs, int total_tokens, int num_adapters,
                                                    int max_rank, int n, int k, int x_stride, int base_stride,
                                                    int out_stride, char* msg, size_t msg_cap);

@@ -8,8 +8,8 @@
 //
 // s v has to be an operand of the second product, so it is split into 16-bit terms: per row scaled by a power
 // of two that brings its largest value to where the type has most room (exact, and undone in the fp32 result; fp16 could not hold
-// the values as they are), then the rounded value and what the rounding left.  fp16: two terms, 22 bits; bf16: two terms,
-// 16 bits, for outputs of 8, three, 24 bits, for fp32 outputs.
+// the values as they are), then the rounded value and what the rounding left.  Outputs of 16 bits: two terms,
+// 22 bits for fp16's 11, 16 for bf16's 8; fp32 outputs: three, all 24 bits.
 //
 // Bound by memory: x, base and out once, A and B of the adapters in use.  16 prompts of 512 x 4096, rank 64, 24576 outputs in 16
 // bits: 900 MB in 229 us, 3.9 TB/s (a large copy 5.2; the first launch 26 us, the second 203: its beginnings, and
@@ -23,7 +23,6 @@
 #include <math.h>
 
 #include <algorithm>
-#include <type_traits>
 
 namespace lg {
 
@@ -159,7 +158,8 @@ __global__ __launch_bounds__(256, 2) void adapter_down_kernel(const AdapterParam
 }
 
 // Where the terms' type has the row's largest value, as a power of two.  fp16 ends at 2^16 and loses bits below 2^-14: up there two terms
-// are off by 2^-22 of every rank down to 2^-17 of the largest, and by 2^-39 of the largest below.  (With the largest at 1, by 2^-25 of
+// are off by 2^-22 of every rank down to 2^-17 of the largest, three hold all of every rank down to 2^-15 of it, and what
+// lies below is off by 2^-39 of the largest.  (With the largest at 1, by 2^-25 of
 // it: a rank 2^-18 below it by 5.6 half steps of fp16, which show in every output whose B is small at the largest.)
 template <typename T>
 constexpr int kAdapterTop = 0;
@@ -587,7 +587,7 @@ static hipError_t adapter_down(AdapterParams p, hipStream_t stream) {
 
 template <typename T, bool F32, int MT, int RS, int GROUPS>
 static hipError_t adapter_up(AdapterParams p, hipStream_t stream) {
-    constexpr int kTerms = F32 && std::is_same<T, PackedBf16>::value ? 3 : 2;
+    constexpr int kTerms = F32 ? 3 : 2;
     constexpr int kAcross = 64 * (4 / GROUPS);
     const int64_t tiles = packed_tiles(p.total, p.num_seqs, 1, 16 * MT * GROUPS);
     // A workgroup takes one step of outputs, and more as long as there are sixteen workgroups per compute unit: more of them spend
@@ -610,7 +610,7 @@ static hipError_t adapter_up_by_rank(const AdapterParams& p, bool long_seqs, hip
 
 template <typename T, bool F32>
 static hipError_t adapter_small(AdapterParams p, hipStream_t stream) {
-    constexpr int kTerms = F32 && std::is_same<T, PackedBf16>::value ? 3 : 2;
+    constexpr int kTerms = F32 ? 3 : 2;
     p.slices = (p.n + 1023) / 1024;
     const unsigned grid = (unsigned)(packed_tiles(p.total, p.num_seqs, 1, 16) * p.slices);
     if (p.max_rank <= 16) adapter_small_kernel<T, F32, kTerms, 1><<<grid, 1024, 0, stream>>>(p);

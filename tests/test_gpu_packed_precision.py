@@ -192,7 +192,8 @@ def test_the_mean_of_the_largest_values(lens, hq, hkv, d, odd_head, causal):
 
 
 # What the terms of x . A^T are off by: relative to the value itself, and to the largest of its row.
-TERMS = {("fp16", "fp16"): (2.0 ** -22, 2.0 ** -39), ("bf16", "bf16"): (2.0 ** -16, 0.0)}
+TERMS = {("fp16", "fp16"): (2.0 ** -22, 2.0 ** -39), ("bf16", "bf16"): (2.0 ** -16, 0.0),
+         ("fp16", "f32"): (2.0 ** -33, 2.0 ** -39), ("bf16", "f32"): (2.0 ** -24, 0.0)}
 TILES = [[1, 16, 3], [40, 1, 90], [1, 2] * 150, [33] * 40]
 
 
@@ -243,3 +244,34 @@ def test_small_ranks_beside_a_large_one(lens, max_rank, below, dtype, out):
     r = D.Run(c)
     r.launch()
     R.assert_within(R.from_bits(r.bits()[:sum(lens)], out), *_uneven_want(c, TERMS[dtype, out]))
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("max_rank", [8, 16, 32, 64, 128, 256])
+@pytest.mark.parametrize("lens", TILES, ids=lambda v: f"{len(v)} of {max(v)}")
+def test_fp32_results_have_all_bits_of_the_first_product(lens, max_rank, dtype):
+    """x . A^T has 24 bits, every row of B one power of two: the results are exact."""
+    c = D._case(25, lens, np.arange(len(lens)) % 2, [max_rank, max_rank - 3], max_rank, 264, 128, dtype, "f32")
+    rng = np.random.default_rng(6)
+    bits, step = (11, 2.0 ** -2) if dtype == "fp16" else (8, 2.0 ** -8)
+
+    def odd(lo, hi, *shape):
+        return 2.0 * rng.integers(lo // 2, hi // 2, shape) + 1
+
+    x, a, b = np.zeros(c["x"].shape), np.zeros(c["a"].shape), np.zeros(c["b"].shape)
+    x[:, 40], a[:, :, 40] = odd(1 << bits - 1, 1 << bits, len(x)), odd(1 << bits - 1, 1 << bits, 2, max_rank)
+    # (added a step of 32 columns earlier: 22 or 16 bits in front of the point, 2 or 8 behind it)
+    x[:, 7], a[:, :, 7] = 1.0, odd(0, round(1 / step), 2, max_rank) * step
+    b[:, np.arange(264), np.arange(264) % (max_rank - 3)] = 2.0 ** rng.integers(-4, 5, (2, 264))
+    c["x"], c["a"], c["b"] = (R.to_bits(y, dtype) for y in (x, a, b))
+    for bits_of, y in zip((c["x"], c["a"], c["b"]), (x, a, b)):
+        assert (R.from_bits(bits_of, dtype) == y).all()
+    c["base"], c["scales"] = np.zeros_like(c["base"]), np.array([1.0, 2.0], np.float32)
+    r = D.Run(c)
+    r.launch()
+    got, at = r.bits(), 0
+    for n, p in zip(c["lens"], c["pick"]):
+        want = (x[at:at + n] @ a[p].T) @ b[p].T * (1 + p)
+        assert (want == want.astype(np.float32)).all()
+        assert np.array_equal(got[at:at + n], want.astype(np.float32))
+        at += n
