@@ -161,8 +161,11 @@ __global__ __launch_bounds__(256, 2) void adapter_down_kernel(const AdapterParam
 // are off by 2^-22 of every rank down to 2^-17 of the largest, three hold all of every rank down to 2^-15 of it, and what
 // lies below is off by 2^-39 of the largest.  (With the largest at 1, by 2^-25 of
 // it: a rank 2^-18 below it by 5.6 half steps of fp16, which show in every output whose B is small at the largest.)
+//
+// bf16 has the exponents of fp32, and so may B: with the largest below 2^-11, sums over 256 ranks of values up to 2^128 stay below that, so
+// that what is finite in the result is finite on the way.
 template <typename T>
-constexpr int kAdapterTop = 0;
+constexpr int kAdapterTop = -12;
 template <>
 constexpr int kAdapterTop<PackedF16> = 14;
 
@@ -182,7 +185,7 @@ __device__ __forceinline__ void adapter_terms(float (&u)[8], bool live, int r, i
 #pragma unroll
     for (int m = 1; m < CHUNKS; m *= 2) top = fmaxf(top, shfl_xor_f32(top, m));
     const int ex = (int)(__float_as_uint(top) >> 23);  // (as far as fp32 has the power of two)
-    constexpr int kTop = kAdapterTop<T>, kLow = kTop > 0 ? kTop + 1 : 1, kHigh = kTop > 0 ? 254 : 253 + kTop;
+    constexpr int kTop = kAdapterTop<T>, kLow = std::max(1, 1 + kTop), kHigh = std::min(254, 253 + kTop);
     const int down = ex < kLow ? kLow : ex > kHigh ? kHigh : ex;
     const float shrink = __uint_as_float((unsigned)(254 + kTop - down) << 23);
     if (r == 0) *growth = __uint_as_float((unsigned)(down - kTop) << 23);

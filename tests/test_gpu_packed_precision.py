@@ -275,3 +275,18 @@ def test_fp32_results_have_all_bits_of_the_first_product(lens, max_rank, dtype):
         assert (want == want.astype(np.float32)).all()
         assert np.array_equal(got[at:at + n], want.astype(np.float32))
         at += n
+
+
+@pytest.mark.parametrize("out", ["bf16", "f32"])
+@pytest.mark.parametrize("max_rank", [8, 16, 32, 64, 128, 256])
+@pytest.mark.parametrize("lens", TILES, ids=lambda v: f"{len(v)} of {max(v)}")
+def test_sums_that_pass_the_range_only_before_they_are_scaled(lens, max_rank, out):
+    """bf16 rows near 2^-60 and B near 2^127: a sum over the ranks of B alone is more than fp32 holds."""
+    c = D._case(26, lens, np.arange(len(lens)) % 2, [max_rank, max_rank - 3], max_rank, 264, 128, "bf16", out)
+    rng = np.random.default_rng(7)
+    c["x"] = R.to_bits(rng.uniform(0.5, 1, c["x"].shape) * 2.0 ** -60, "bf16")
+    c["a"] = R.to_bits(rng.uniform(0.5, 1, c["a"].shape), "bf16")
+    c["b"] = R.to_bits(rng.uniform(0.5, 1, c["b"].shape) * 2.0 ** 127, "bf16")
+    r = D.Run(c)
+    r.launch()
+    R.assert_within(R.from_bits(r.bits()[:sum(lens)], out), *D._want(c))
