@@ -714,8 +714,8 @@ logismos_status_t logismos_launch_attn_packed_bf16(const void* q, const void* k,
  *   base, out       rows of n of x's type, or fp32 with out_is_f32 != 0 (the products of the shared projection); the
  *                   same address and stride: in place (rows without an adapter are not touched then), otherwise they
  *                   may not overlap.  out does not overlap x
- *   workspace       `logismos_adapter_add_workspace_bytes(total_tokens, max_rank)` bytes, contents don't matter;
- *                   not shared by calls that can overlap in time
+ *   workspace       `logismos_adapter_add_workspace_bytes(total_tokens, max_rank)` bytes, contents don't matter, enough
+ *                   for fewer tokens and smaller ranks too; not shared by calls that can overlap in time
  *
  * fp32 sums; x . A^T goes into the second product with more bits than the result's type holds: 16 for bf16 outputs, 22
  * for fp16 (of values down to 2^-17 of their row's largest; below, up to 2^-39 of the largest is lost), all 24 for fp32 (of fp16 rows down to

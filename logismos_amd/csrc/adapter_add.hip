@@ -28,6 +28,17 @@ namespace lg {
 
 constexpr int kAdapterMaxRank = 256;
 constexpr int kAdapterMaxParts = 8;   // K parts of v, read four at a time
+constexpr int kAdapterUnits = 256;    // compute units that K is dealt out to, at most
+
+// K parts that `groups` workgroups of the first product are wanted in, two per compute unit.
+inline int adapter_parts(int64_t groups, int units) {
+    int parts = 1;
+    while (parts < kAdapterMaxParts && groups * parts < 2 * units) parts *= 2;
+    return parts;
+}
+// What more than one part of v holds: parts / 2 of the groups are less than 2 kAdapterUnits then, and a group is at most 64 rows by 64
+// ranks, so that rows * ranks * parts stay below this.
+constexpr int64_t kAdapterPartElements = 4 * kAdapterUnits * 64 * 64;
 
 struct AdapterParams {
     const unsigned short* x;
@@ -634,8 +645,8 @@ static hipError_t adapter_launch(AdapterParams p, bool f32, hipStream_t stream) 
     const int rt = !long_seqs || p.max_rank <= 16 ? 1 : p.max_rank <= 32 ? 2 : 4;
     // K parts: two workgroups per compute unit, and steps for four waves
     const int64_t groups = packed_tiles(p.total, p.num_seqs, 1, 16 * mt) * ((p.max_rank + 16 * rt - 1) / (16 * rt));
-    int parts = 1;
-    while (parts < kAdapterMaxParts && groups * parts < 2 * device_cu_count() && steps >= 16 * parts) parts *= 2;
+    int parts = adapter_parts(groups, std::min(device_cu_count(), kAdapterUnits));
+    while (parts > 1 && steps < 8 * parts) parts /= 2;
     p.parts = parts;
     p.part_steps = (steps + parts - 1) / parts;
     // Whole rounds of the four waves where fewer parts are then enough (us before / then: 35 steps in rounds of 16, parts 8 to 6, 22.9 /
@@ -727,7 +738,9 @@ logismos_status_t logismos_check_adapter_add_shape(int num_seqs, int total_token
 
 size_t logismos_adapter_add_workspace_bytes(int total_tokens, int max_rank) {
     if (total_tokens <= 0 || max_rank <= 0) return 0;
-    return (size_t)lg::kAdapterMaxParts * (size_t)total_tokens * (size_t)max_rank * sizeof(float);
+    // (never less for more tokens or a larger rank: a caller sizes it once, for the largest batch)
+    const uint64_t rows = (uint64_t)total_tokens * (uint64_t)max_rank, most = lg::kAdapterMaxParts * rows;
+    return (size_t)std::max(rows, std::min<uint64_t>(most, lg::kAdapterPartElements)) * sizeof(float);
 }
 
 #define LOGISMOS_ADAPTER_ADD(name, bf16)                                                                              \
