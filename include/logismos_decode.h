@@ -630,7 +630,7 @@ logismos_status_t logismos_launch_embed_lookup_bf16(const void* table_bf16, cons
  *   inv_freq      double `[rotary_dim / 2]` in device memory, radians per position, e.g. from
  *                 `logismos_rope_frequencies`
  *
- * In place: the same address and stride as output and input.  Otherwise no output may overlap an input.  Addresses are
+ * In place: the same address and stride as output and input (one address with two strides is refused).  Otherwise no output may overlap an input.  Addresses are
  * aligned to an element; where addresses, strides and widths are multiples of 16 bytes it is fastest.
  * rotary_dim even, at most head_dim; head_dim at most 1024; (num_q_heads + num_kv_heads) * head_dim at most 65536. */
 logismos_status_t logismos_check_rope_packed_shape(int tokens, int num_q_heads, int num_kv_heads, int head_dim,

@@ -160,6 +160,10 @@ static logismos_status_t rope_packed(int elem_bytes, int type, const void* q_in,
         at % (uintptr_t)elem_bytes != 0 || reinterpret_cast<uintptr_t>(inv_freq) % 8 != 0 ||
         reinterpret_cast<uintptr_t>(positions) % 4 != 0)
         return static_cast<logismos_status_t>(hipErrorInvalidValue);
+    // (one address with two strides: rows would be read after others were written over them)
+    if (tokens > 1 && ((q_in == q_out && q_in_stride != q_out_stride) ||
+                       (hkv > 0 && k_in == k_out && k_in_stride != k_out_stride)))
+        return static_cast<logismos_status_t>(hipErrorInvalidValue);
     RopeParams p = {};
     p.q_in = q_in;
     p.k_in = k_in;
