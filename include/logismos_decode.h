@@ -665,7 +665,8 @@ logismos_status_t logismos_launch_rope_packed_f32(const void* q_in, const void* 
  *   PARTS   a pair that turns more than turns_fast times over original_positions stays, one that turns less
  *           than turns_slow times is divided by factor, between the two a mixture, linear in the turns; amplitude
  *           0.1 ln(factor) + 1 (YaRN, Peng et al. 2023; turns_fast 32, turns_slow 1 there)
- * amplitude: what the launch multiplies cos and sin by (1 but for PARTS).  No device access. */
+ * amplitude: what the launch multiplies cos and sin by (1 but for PARTS).  A base, changed or not, of which a frequency is not
+ * finite is refused.  No device access. */
 #define LOGISMOS_ROPE_SCALE_NONE 0
 #define LOGISMOS_ROPE_SCALE_LINEAR 1
 #define LOGISMOS_ROPE_SCALE_BASE 2

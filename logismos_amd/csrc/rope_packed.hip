@@ -228,6 +228,8 @@ logismos_status_t logismos_rope_frequencies(double* inv_freq, float* amplitude, 
         return bad;
     const double r = rotary_dim;
     if (scaling == LOGISMOS_ROPE_SCALE_BASE) base *= pow(factor, r / (r - 2.0));
+    // (the largest frequency is base^0 or, for a base below 1, that of the last pair)
+    if (!isfinite(base) || !isfinite(pow(base, -2.0 * (rotary_dim / 2 - 1) / r))) return bad;
     *amplitude = 1.0f;
     for (int i = 0; i < rotary_dim / 2; ++i) {
         double f = pow(base, -2.0 * i / r);
