@@ -12,6 +12,8 @@
 // 4h + i, 8 + 4h + i (h: half of the wave, i < 4); V comes out of its row-major tile in that order through the
 // transposing LDS read.  P goes in rounded to the rows' type: every term is off by at most half a step of that type
 // relative to itself, as every output is by its own rounding (fp16: terms below 2^-25 of the largest by more, see ApRange).
+// The errors against 64 bits are a quarter to a third above those of unrounded probabilities; a second term, as the decode rows of the paged
+// form have it, would be half as many products again.
 //
 // Schedule: the stages of a tile -- S(t) and O(t) on the matrix cores, F(t), the softmax, on the vector units -- run
 // one behind the other in a wave: step t issues S(t + 1) and O(t - 1) around F(t), so that the products of a step
@@ -22,10 +24,12 @@
 // Few long sequences: HALVES == 2, twice the waves, of which the second part takes every other key tile; its sums join the
 // first part's, each relative to its own maximum, through LDS.
 //
-// Bound by the matrix cores at heads of 128 and long sequences (one prompt of 16384 tokens, 32 / 8 heads: 2007 us, 1095 TFLOP/s,
-// a large matrix product of the library 1130); by the vector units at heads of 64 (per step 76 vector
-// instructions, 16 of them exponentials, to 8 products; nothing but those takes 520 clocks a step, this 770: 4 prompts of 8192, 14 / 2
-// heads, 580 us, 830 TFLOP/s).
+// Bound by the matrix cores at heads of 128 and long sequences (one prompt of 16384 tokens, 32 / 8 heads: 1960 to 2080 us by card, 1060 to
+// 1120 TFLOP/s, a large matrix product of the library 1130; the first few calls on a card that has rested take 2270); by the vector units at
+// heads of 64 (per step 76 vector instructions, 16 of them exponentials, to 8 products; nothing but those takes 520 clocks a step, this
+// 770, of which a barrier and a store into LDS for every 32 keys are a part: 4 prompts of 8192, 14 / 2 heads, 580 us, 830 TFLOP/s).
+//
+// The step is that of the paged prefill kernel (paged_attn.hip) with width and type as parameters: a change to one concerns the other.
 #include "device_utils.hpp"
 #include "launch_common.hpp"
 #include "packed_rows.hpp"
@@ -395,7 +399,8 @@ __global__ __launch_bounds__(64 * WAVES * HALVES) void attn_packed_kernel(const 
     // A key that a column does not see has the probability 0 there, and 0 times an infinity or NaN of its V row is a NaN.
     // If the results are not all finite, or a maximum is too large for the fused difference, the keys are gone through again,
     // plainly, and in the tiles in which columns of the wave end with a pass of its own for every number of keys that one of them
-    // sees.
+    // sees.  (Workgroup by workgroup; a call all of whose workgroups do takes 1.8 times as long for short documents, 2.5 at heads of 64
+    // and for one of 16384 at heads of 128, 3.9 where key tiles are dealt out to two parts at heads of 128, whose second walk spills.)
     float unit = 1.0f;  // of m, in powers of two
     {
         float odds[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // NaN if a result is not finite
@@ -512,15 +517,17 @@ template <typename T>
 static hipError_t attn_packed_by_width(const AttnPackedParams& p, int d, hipStream_t stream) {
     // 256 columns to a workgroup (eight waves, K and V moved half as often) where the sequences are long and there are
     // many of them; otherwise 128, of which a compute unit holds two or three that fill each other's waits.  us, 8 / 4 waves, 128
-    // wide, 32 / 8 heads: one of 16384 2006 / 2132, one of 4096 140 / 149, 8 of 2048 313 / 322, but 16 of 1500 384 / 365, 16 of
-    // 512 74 / 71; 12 / 2: one of 16384 804 / 841, one of 8192 230 / 226.  64 wide: 4 x 8192, 14 / 2, 586 / 582; one of 2048 41 / 31.
+    // wide, 32 / 8 heads: one of 16384 1968 / 2079, one of 4096 138 / 145, 8 of 2048 317 / 317, but 16 of 1500 383 / 362, 16 of
+    // 512 72 / 70; 12 / 2: one of 16384 794 / 819, one of 8192 227 / 226.  64 wide: 4 x 8192, 14 / 2, 586 / 582; one of 2048 41 / 31.
     const bool wide = d == 128 && p.total >= 2048 * (int64_t)p.num_seqs &&
                       packed_tiles(p.total, p.num_seqs, p.g, 256) * p.hkv >= 2 * device_cu_count();
     // Key tiles dealt out to two parts of a workgroup, joined at its end, where workgroups are few and keys many: the steps of a
     // workgroup alone on its compute unit are latency (1000 clocks of the 770 that a step takes of three side by side), twice the
     // waves hide it, but have a join, and no room for a second workgroup beside them.  us, one part / two, 64 wide, 14 / 2 heads:
-    // one of 512 11.8 / 11.3, of 2048 32.1 / 25.6, of 4096 61.9 / 51.7, two of 2048 41.5 / 31.4, but one of 256 8.4 / 8.8, four
-    // of 1024 22.5 / 25.4 and one of 6000 97 / 102; 128 wide, 12 / 2: one of 4096 91 / 76, but 32 / 8, one of 512 16.2 / 16.7.
+    // one of 512 11.8 / 11.2, of 2048 33.1 / 27.2, of 4096 64.0 / 54.5, two of 2048 40.2 / 33.6, but one of 256 8.4 / 8.8, four
+    // of 1024 22.6 / 26.7 and one of 6000 97 / 104; 128 wide, 12 / 2: one of 4096 90 / 70, but 32 / 8, one of 512 15.7 / 16.2; 32 wide,
+    // 24 / 4: one of 512 10.0 / 9.4, of 2048 28.0 / 23.7, but one of 256 7.1 / 7.3, four of 600 13.5 / 14.3; 96 wide, 16 / 16: one of 768
+    // 18.0 / 16.6, of 4096 83 / 73, but one of 256 10.0 / 10.5, four of 800 23.8 / 30.3; at worst, 8 / 2, four of 2048 53.0 / 54.1.
     const int64_t groups = (int64_t)p.total * p.g / 128 * p.hkv;
     const bool split =
         (groups <= device_cu_count() && p.total >= (d > 64 ? 8 * d : 512) * (int64_t)p.num_seqs) ||
