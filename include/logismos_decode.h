@@ -612,7 +612,7 @@ logismos_status_t logismos_launch_embed_lookup_bf16(const void* table_bf16, cons
  * ------------------------------------------------------------------------
  * A batch is `total_tokens` rows, the tokens of sequence s in rows [cu_seqlens[s], cu_seqlens[s+1])
  * (int32 `[num_seqs + 1]`, non-decreasing, starting at or behind 0; empty sequences are allowed).  Rows
- * behind the last sequence are neither read nor written.  A stride is the distance of two rows in elements, so that q, k
+ * in front of the first sequence and behind the last are neither read nor written.  A stride is the distance of two rows in elements, so that q, k
  * and v may be columns of one fused projection.  At most 2^23 rows and sequences together.  A call needs
  * nothing but its arguments, allocates nothing and can be captured into a graph; it runs on the device that is current. */
 

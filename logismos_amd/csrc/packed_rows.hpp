@@ -93,7 +93,7 @@ __device__ __forceinline__ PackedTile packed_tile(const int32_t* __restrict__ cu
     t.row0 = r0;
     t.rows = r0 >= 0 && r0 < total ? (r1 < total ? r1 : total) - r0 : 0;
     t.tile = b - start(r0, t.seq);
-    if (t.tile < 0) t.rows = 0;
+    if (t.tile < 0) t.rows = t.tile = 0;  // (rows in front of the first sequence)
     t.of = OF ? __builtin_amdgcn_readlane(of, last) : 0;
     return t;
 }
