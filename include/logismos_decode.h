@@ -630,8 +630,8 @@ logismos_status_t logismos_launch_embed_lookup_bf16(const void* table_bf16, cons
  *   inv_freq      double `[rotary_dim / 2]` in device memory, radians per position, e.g. from
  *                 `logismos_rope_frequencies`
  *
- * In place: the same address and stride as output and input (one address with two strides is refused).  Otherwise no output may overlap an input.  Addresses are
- * aligned to an element; where addresses, strides and widths are multiples of 16 bytes it is fastest.
+ * In place: the same address and stride as output and input (one address with two strides is refused).  Otherwise no
+ * output may overlap an input.  Addresses are aligned to an element; where addresses, strides and widths are multiples of 16 bytes it is fastest.
  * rotary_dim even, at most head_dim; head_dim at most 1024; (num_q_heads + num_kv_heads) * head_dim at most 65536. */
 logismos_status_t logismos_check_rope_packed_shape(int tokens, int num_q_heads, int num_kv_heads, int head_dim,
                                                    int rotary_dim, int q_in_stride, int k_in_stride,
@@ -683,8 +683,8 @@ logismos_status_t logismos_rope_frequencies(double* inv_freq, float* amplitude, 
  *           16-byte aligned, strides multiples of 8
  *
  * fp32 scores, softmax and sums; the probabilities are rounded to the rows' type for the second product (fp16: those below
- * 2^-25 of a row's largest are off by up to 2^-36 of it; bf16: those below 2^-94 of it count as 0).  Elements of keys that a token does not see do not reach its result, whatever they hold; a token whose keys all score
- * -inf gives zeros.  scale > 0 and scale * log2(e) finite (else hipErrorInvalidValue); head_dim a multiple of 32 up to 256; num_q_heads a
+ * 2^-25 of a row's largest are off by up to 2^-36 of it; bf16: those below 2^-94 of it count as 0).  Elements of keys that a
+ * token does not see do not reach its result, whatever they hold; a token whose keys all score -inf gives zeros.  scale > 0 and scale * log2(e) finite (else hipErrorInvalidValue); head_dim a multiple of 32 up to 256; num_q_heads a
  * multiple of num_kv_heads; k, v and out strides up to 2^22; total_tokens * num_q_heads / 128 +
  * num_seqs * num_kv_heads up to 2^22.  out does not overlap q, k or v. */
 logismos_status_t logismos_check_attn_packed_shape(int num_seqs, int total_tokens, int num_q_heads,
@@ -720,7 +720,8 @@ logismos_status_t logismos_launch_attn_packed_bf16(const void* q, const void* k,
  *
  * fp32 sums; x . A^T goes into the second product with more bits than the result's type holds: 16 for bf16 outputs, 22
  * for fp16 (of values down to 2^-17 of their row's largest; below, up to 2^-39 of the largest is lost), all 24 for fp32 (of fp16 rows down to
- * 2^-15 of the largest, below as for fp16).  One rounding at the end.  max_rank a multiple of 8 up to 256, n, k and strides multiples of 8, n, k and the strides of base and out at most 2^22; x, a, b, base, out, workspace 16-byte aligned. */
+ * 2^-15 of the largest, below as for fp16).  One rounding at the end.  max_rank a multiple of 8 up to 256, n, k and strides
+ * multiples of 8, n, k and the strides of base and out at most 2^22; x, a, b, base, out, workspace 16-byte aligned. */
 logismos_status_t logismos_check_adapter_add_shape(int num_seqs, int total_tokens, int num_adapters,
                                                    int max_rank, int n, int k, int x_stride, int base_stride,
                                                    int out_stride, char* msg, size_t msg_cap);

@@ -36,8 +36,8 @@ inline int adapter_parts(int64_t groups, int units) {
     while (parts < kAdapterMaxParts && groups * parts < 2 * units) parts *= 2;
     return parts;
 }
-// What more than one part of v holds: parts / 2 of the groups are less than 2 kAdapterUnits then, and a group is at most 64 rows by 64
-// ranks, so that rows * ranks * parts stay below this.
+// More than one part is made only while groups * parts / 2 < 2 * units, and a group is at most 64 rows by 64 ranks: rows * ranks * parts
+// stay below this.
 constexpr int64_t kAdapterPartElements = 4 * kAdapterUnits * 64 * 64;
 
 struct AdapterParams {

@@ -24,8 +24,8 @@
 // Few long sequences: HALVES == 2, twice the waves, of which the second part takes every other key tile; its sums join the
 // first part's, each relative to its own maximum, through LDS.
 //
-// Bound by the matrix cores at heads of 128 and long sequences (one prompt of 16384 tokens, 32 / 8 heads: 1960 to 2080 us by card, 1060 to
-// 1120 TFLOP/s, a large matrix product of the library 1130; the first few calls on a card that has rested take 2270); by the vector units at
+// Bound by the matrix cores at heads of 128 and long sequences (one prompt of 16384 tokens, 32 / 8 heads: 1950 to 2150 us by card, 1020 to
+// 1130 TFLOP/s, a large matrix product of the library 1130; the first few calls on a card that has rested take 2270); by the vector units at
 // heads of 64 (per step 76 vector instructions, 16 of them exponentials, to 8 products; nothing but those takes 520 clocks a step, this
 // 770, of which a barrier and a store into LDS for every 32 keys are a part: 4 prompts of 8192, 14 / 2 heads, 580 us, 830 TFLOP/s).
 //
