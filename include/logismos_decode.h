@@ -675,6 +675,41 @@ logismos_status_t logismos_rope_frequencies(double* inv_freq, float* amplitude, 
                                             int scaling, double factor, int original_positions,
                                             double turns_fast, double turns_slow);
 
+/* RMS norm of every q and k head and rotary positions in the same pass (`rms_norm`, crates/kernels/src/cpu_f32/mod.rs:137-159,
+ * over the head_dim elements of a head; `rope_halves_in_place` behind it):
+ *   z_i = x_i * gain_i / sqrt(mean(x^2) + eps),  then the pairs of z turn as in `logismos_launch_rope_packed_*`, with
+ *   t = positions[axis_of_pair[pair]][row] * inv_freq[pair].
+ * fp16, bf16 or fp32 in and out; the norm and the products fp32, the angle reduced in 64 bits, one rounding.
+ *
+ *   q_gain, k_gain  fp32 `[head_dim]`, one for all q heads and one for all k heads; NULL: those heads are not normed.  eps > 0
+ *                   where one is given
+ *   positions       int32 `[num_axes]` rows of `[tokens]`, position_stride apart (one axis: the stride is not looked at); several
+ *                   axes: the time, height and width of image and video patches, say
+ *   axis_of_pair    uint8 `[rotary_dim / 2]`, the axis of every pair; a value of num_axes or more: the pair stays at position 0.
+ *                   NULL with one axis: all of them
+ *   rotary_dim      may be 0: the norm alone (positions, axes and frequencies are not looked at)
+ *
+ * Everything else -- strides, in place, alignment, limits -- as for `logismos_launch_rope_packed_*`. */
+logismos_status_t logismos_check_norm_rope_packed_shape(int tokens, int num_q_heads, int num_kv_heads, int head_dim,
+                                                        int rotary_dim, int num_axes, int position_stride,
+                                                        int q_in_stride, int k_in_stride, int q_out_stride,
+                                                        int k_out_stride, char* msg, size_t msg_cap);
+logismos_status_t logismos_launch_norm_rope_packed_fp16(
+    const void* q_in, const void* k_in, void* q_out, void* k_out, const int32_t* positions, const uint8_t* axis_of_pair,
+    const double* inv_freq, const float* q_gain, const float* k_gain, int tokens, int num_q_heads, int num_kv_heads,
+    int head_dim, int rotary_dim, int num_axes, int position_stride, int q_in_stride, int k_in_stride, int q_out_stride,
+    int k_out_stride, float eps, float amplitude, int interleaved, logismos_stream_t stream);
+logismos_status_t logismos_launch_norm_rope_packed_bf16(
+    const void* q_in, const void* k_in, void* q_out, void* k_out, const int32_t* positions, const uint8_t* axis_of_pair,
+    const double* inv_freq, const float* q_gain, const float* k_gain, int tokens, int num_q_heads, int num_kv_heads,
+    int head_dim, int rotary_dim, int num_axes, int position_stride, int q_in_stride, int k_in_stride, int q_out_stride,
+    int k_out_stride, float eps, float amplitude, int interleaved, logismos_stream_t stream);
+logismos_status_t logismos_launch_norm_rope_packed_f32(
+    const void* q_in, const void* k_in, void* q_out, void* k_out, const int32_t* positions, const uint8_t* axis_of_pair,
+    const double* inv_freq, const float* q_gain, const float* k_gain, int tokens, int num_q_heads, int num_kv_heads,
+    int head_dim, int rotary_dim, int num_axes, int position_stride, int q_in_stride, int k_in_stride, int q_out_stride,
+    int k_out_stride, float eps, float amplitude, int interleaved, logismos_stream_t stream);
+
 /* out[t][h][:] = softmax_j( (q[t][h] . k[j][h/g]) * scale ) . v[j][h/g] over the tokens j of t's own sequence, up
  * to t itself where causal != 0 (`QwenAttention::forward` without a cache, crates/transformers/src/attention.rs:225-296,
  * over rows without padding; bidirectional in the encoders).
@@ -1062,6 +1097,110 @@ logismos_status_t logismos_launch_paged_attn_varlen_turbo3(
     int num_seqs, int total_tokens, int max_seqlen_q, int num_q_heads, int num_kv_heads,
     int block_size, int max_blocks_per_seq, int num_splits, float scale,
     logismos_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * KV cache in 8 bits (e4m3), and attention of drafted tokens over a paged cache
+ * ------------------------------------------------------------------------
+ * e4m3 pools hold a head row x of head_dim elements as head_dim e4m3 values (4 exponent and 3 mantissa bits, no infinities,
+ * largest 448; the 8-bit counterpart of the turbo3 pools, any multiple of 32 up to 256) and one power of two:
+ *   e = the smallest integer with max |x_i| <= 448 * 2^e, kept within [-64, 32];  c_i = e4m3(x_i * 2^-e);  x_i ~ c_i * 2^e.
+ * An element is off by at most 2^-4 of itself, or 2^-10 * 2^e where that is more; one beyond 448 * 2^32 counts as that.  Infinities and NaN
+ * become NaN (the maximum is that of the finite elements).
+ *
+ *   k_pool, v_pool  `[num_blocks][block_size][num_kv_heads][head_dim]` bytes, with the slots and block tables of the fp16 pools
+ *   k_exp, v_exp    `[num_blocks][num_kv_heads][block_size]` bytes, e + 127
+ *
+ * 16-byte aligned; block_size a multiple of 16.  A cache of 8 heads of 128 takes 2064 bytes a token and layer, fp16 pools 4096. */
+
+/* The rows of `logismos_launch_kv_write_fp16` (`KvCache::put`, crates/cache/src/lib.rs:57-64), fp16 or bf16 with strides (elements,
+ * multiples of 8, so that k and v may be columns of a fused projection; 16-byte aligned), quantised as they are written to slot
+ * slot_mapping[t].  A slot that is negative or not in the pools is skipped; no two rows have the same slot.  total_tokens may be 0. */
+logismos_status_t logismos_check_kv_e4m3_shape(int total_tokens, int num_kv_heads, int head_dim, int block_size,
+                                               int num_blocks, int k_stride, int v_stride, char* msg, size_t msg_cap);
+logismos_status_t logismos_launch_kv_write_e4m3_fp16(const void* k_new, const void* v_new, void* k_pool, void* k_exp,
+                                                    void* v_pool, void* v_exp, const int64_t* slot_mapping,
+                                                    int total_tokens, int num_kv_heads, int head_dim, int block_size,
+                                                    int num_blocks, int k_stride, int v_stride,
+                                                    logismos_stream_t stream);
+logismos_status_t logismos_launch_kv_write_e4m3_bf16(const void* k_new, const void* v_new, void* k_pool, void* k_exp,
+                                                    void* v_pool, void* v_exp, const int64_t* slot_mapping,
+                                                    int total_tokens, int num_kv_heads, int head_dim, int block_size,
+                                                    int num_blocks, int k_stride, int v_stride,
+                                                    logismos_stream_t stream);
+
+/* Rows of e4m3 pools read back (`KvCache::get`, crates/cache/src/lib.rs:57-68): row t of k_out and v_out is the row at slot
+ * slot_mapping[t], of any sequences in any order (`logismos_launch_pack_ragged` writes such a mapping); a slot that is negative or not in the pools
+ * gives zeros, a slot may be named more than once.  fp16, bf16 or fp32 out, exact but for fp16, whose range ends at 65504 (larger values count as that) and
+ * whose steps end at 2^-24. */
+logismos_status_t logismos_launch_kv_gather_e4m3_fp16(const void* k_pool, const void* k_exp, const void* v_pool,
+                                                     const void* v_exp, const int64_t* slot_mapping, void* k_out,
+                                                     void* v_out, int total_tokens, int num_kv_heads, int head_dim,
+                                                     int block_size, int num_blocks, int k_stride, int v_stride,
+                                                     logismos_stream_t stream);
+logismos_status_t logismos_launch_kv_gather_e4m3_bf16(const void* k_pool, const void* k_exp, const void* v_pool,
+                                                     const void* v_exp, const int64_t* slot_mapping, void* k_out,
+                                                     void* v_out, int total_tokens, int num_kv_heads, int head_dim,
+                                                     int block_size, int num_blocks, int k_stride, int v_stride,
+                                                     logismos_stream_t stream);
+logismos_status_t logismos_launch_kv_gather_e4m3_f32(const void* k_pool, const void* k_exp, const void* v_pool,
+                                                     const void* v_exp, const int64_t* slot_mapping, void* k_out,
+                                                     void* v_out, int total_tokens, int num_kv_heads, int head_dim,
+                                                     int block_size, int num_blocks, int k_stride, int v_stride,
+                                                     logismos_stream_t stream);
+
+/* Attention of drafted tokens over a paged cache: the step that verifies a draft.  The new rows of a sequence (its
+ * n = cu_seqlens_q[s + 1] - cu_seqlens_q[s] query rows) are the nodes of one or several token trees, in any order; their K and V rows
+ * are already in the pools, at positions prior .. prior + n - 1 with prior = context_lens[s] - n.  A row sees the whole
+ * context in front of them and the new rows that its mask names:
+ *
+ *   out[t][h][:] = softmax_j( (q[t][h] . k[j][h/g]) * scale ) . v[j][h/g]  over j < prior, and j = prior + i with bit i of row t
+ *
+ *   q, out         rows of `[num_q_heads][head_dim]`, strides in elements (multiples of 8)
+ *   tree_mask      uint64 `[total_tokens][mask_words]`: bit i % 64 of word i / 64 of a row stands for new row i of its own sequence.
+ *                  A token tree names every row's ancestors and itself (`logismos_tree_mask`), a chain of tokens bits 0 .. i; any bits
+ *                  are allowed, bits of n and above are not looked at
+ *   context_lens, block_tables, cu_seqlens_q, max_seqlen_q, scale  as for `logismos_launch_paged_attn_varlen_fp16`; head_dim a
+ *                  multiple of 32 up to 256, any group size; total_tokens and num_seqs up to 65535, sequences may be empty
+ *   num_blocks     blocks of the pools.  A table entry that names none of them hides its keys from everybody (nothing outside the pools is
+ *                  read)
+ *   mask_words     1 to 4: up to 256 new rows a sequence
+ *   workspace      `logismos_paged_attn_tree_workspace_bytes(...)` bytes, 16-byte aligned, contents don't matter; not shared by
+ *                  calls that can overlap in time
+ *
+ * One new row per sequence with bit 0 set is a plain decode step.  fp32 scores, softmax and sums; the probabilities are rounded to fp16 for the second
+ * product (those below 2^-25 of a row's largest are off by up to 2^-36 of it).  Rows that see no key are zeros.  Elements
+ * of keys that a row does not see do not reach its result, whatever they hold.
+ * fp16 pools: fp16 rows.  e4m3 pools: fp16 or bf16 rows; K and V as `logismos_launch_kv_gather_e4m3_f32` returns them, but that V (and for
+ * fp16 rows K) of 32 neighbouring keys is taken relative to the largest exponent among them, in fp16: elements below 2^-15 of 2^e of that row lose
+ * bits, to 2^-25 of it. */
+logismos_status_t logismos_check_paged_attn_tree_shape(int num_seqs, int total_tokens, int max_seqlen_q,
+                                                       int num_q_heads, int num_kv_heads, int head_dim,
+                                                       int block_size, int max_blocks_per_seq, int num_blocks,
+                                                       int mask_words, int q_stride, int out_stride, char* msg,
+                                                       size_t msg_cap);
+size_t logismos_paged_attn_tree_workspace_bytes(int total_tokens, int max_seqlen_q, int num_q_heads, int num_kv_heads,
+                                                int head_dim);
+logismos_status_t logismos_launch_paged_attn_tree_fp16(
+    const void* q, const void* k_pool, const void* v_pool, const int32_t* block_tables, const int32_t* cu_seqlens_q,
+    const int32_t* context_lens, const uint64_t* tree_mask, void* out, void* workspace, int num_seqs, int total_tokens,
+    int max_seqlen_q, int num_q_heads, int num_kv_heads, int head_dim, int block_size, int max_blocks_per_seq,
+    int num_blocks, int mask_words, int q_stride, int out_stride, float scale, logismos_stream_t stream);
+logismos_status_t logismos_launch_paged_attn_tree_e4m3_fp16(
+    const void* q, const void* k_pool, const void* k_exp, const void* v_pool, const void* v_exp,
+    const int32_t* block_tables, const int32_t* cu_seqlens_q, const int32_t* context_lens, const uint64_t* tree_mask,
+    void* out, void* workspace, int num_seqs, int total_tokens, int max_seqlen_q, int num_q_heads, int num_kv_heads,
+    int head_dim, int block_size, int max_blocks_per_seq, int num_blocks, int mask_words, int q_stride, int out_stride,
+    float scale, logismos_stream_t stream);
+logismos_status_t logismos_launch_paged_attn_tree_e4m3_bf16(
+    const void* q, const void* k_pool, const void* k_exp, const void* v_pool, const void* v_exp,
+    const int32_t* block_tables, const int32_t* cu_seqlens_q, const int32_t* context_lens, const uint64_t* tree_mask,
+    void* out, void* workspace, int num_seqs, int total_tokens, int max_seqlen_q, int num_q_heads, int num_kv_heads,
+    int head_dim, int block_size, int max_blocks_per_seq, int num_blocks, int mask_words, int q_stride, int out_stride,
+    float scale, logismos_stream_t stream);
+/* The masks of a tree of drafted tokens, on the host: parents[i] is the token that token i hangs on, an earlier one, or -1
+ * for one that follows the context itself; mask `[tokens][mask_words]` gets every token's ancestors and the token itself.  Refused
+ * (hipErrorInvalidValue): a parent that is not earlier, more tokens than bits.  No device access. */
+logismos_status_t logismos_tree_mask(const int32_t* parents, int tokens, int mask_words, uint64_t* mask);
 
 /* ------------------------------------------------------------------------
  * Memory-system probes (measurement aids; the reference has no counterpart,

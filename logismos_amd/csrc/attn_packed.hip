@@ -122,39 +122,6 @@ __device__ __forceinline__ uint4_t attn_packed_first_keys(uint4_t v, int kb, int
     return v;
 }
 
-// Normalises a wave's 32 columns and writes them, 16 at a time through its part of LDS (`stage`, 16 rows of D + 8): straight
-// from the registers a store would put 16 bytes into each of 32 rows, from there it writes whole head rows.  `to` is where this
-// lane's column goes, in elements from `out`, less than 2^31; cols the number of columns that are there.
-template <typename T, int D>
-__device__ __forceinline__ void attn_packed_write(unsigned short* out, unsigned to, int cols, unsigned short* stage,
-                                                  const float16_t (&o)[D / 32], float l) {
-    constexpr int kRow = D + 8, kLanes = D / 8;
-    const int lane = threadIdx.x & 63, h = lane >> 5, col = lane & 31;
-    const float inv = l > 0.0f ? 1.0f / l : l == l ? 0.0f : l;  // (only keys that score -inf: zeros)
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-        if (16 * half >= cols) break;
-        if ((col >> 4) == half) {
-#pragma unroll
-            for (int dt = 0; dt < D / 32; ++dt)
-#pragma unroll
-                for (int b = 0; b < 4; ++b)
-                    *reinterpret_cast<uint2_t*>(stage + (col & 15) * kRow + 32 * dt + 8 * b + 4 * h) =
-                        uint2_t{T::pack2(o[dt][4 * b] * inv, o[dt][4 * b + 1] * inv),
-                                T::pack2(o[dt][4 * b + 2] * inv, o[dt][4 * b + 3] * inv)};
-        }
-        __builtin_amdgcn_wave_barrier();
-#pragma unroll
-        for (int i = lane; i < 16 * kLanes; i += 64) {
-            const int c = i / kLanes, piece = i % kLanes;
-            const unsigned at = __shfl(to, 16 * half + c);
-            const uint4_t v = *reinterpret_cast<const uint4_t*>(stage + c * kRow + 8 * piece);
-            if (16 * half + c < cols) *reinterpret_cast<uint4_t*>(out + (at + 8u * piece)) = v;
-        }
-        __builtin_amdgcn_wave_barrier();
-    }
-}
-
 // A scaled score less the rounded product of the maximum and the scale, in one rounding: off by up to half a step of the
 // maximum, the same for all keys of a column.  Up to here that is at most 1 in the exponent and falls out of the result.
 constexpr float kApExact = 16777216.0f;

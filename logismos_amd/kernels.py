@@ -103,6 +103,22 @@ _SIGNATURES = {
     "logismos_launch_rope_packed_f32": (C.c_uint32, [_vp] * 6 + [_i] * 9 + [_f, _i, _vp]),
     "logismos_rope_frequencies":
         (C.c_uint32, [_vp, C.POINTER(_f), _i, _d, _i, _d, _i, _d, _d]),
+    "logismos_check_norm_rope_packed_shape": (C.c_uint32, [_i] * 11 + [C.c_char_p, _sz]),
+    "logismos_launch_norm_rope_packed_fp16": (C.c_uint32, [_vp] * 9 + [_i] * 11 + [_f, _f, _i, _vp]),
+    "logismos_launch_norm_rope_packed_bf16": (C.c_uint32, [_vp] * 9 + [_i] * 11 + [_f, _f, _i, _vp]),
+    "logismos_launch_norm_rope_packed_f32": (C.c_uint32, [_vp] * 9 + [_i] * 11 + [_f, _f, _i, _vp]),
+    "logismos_check_kv_e4m3_shape": (C.c_uint32, [_i] * 7 + [C.c_char_p, _sz]),
+    "logismos_launch_kv_write_e4m3_fp16": (C.c_uint32, [_vp] * 7 + [_i] * 7 + [_vp]),
+    "logismos_launch_kv_write_e4m3_bf16": (C.c_uint32, [_vp] * 7 + [_i] * 7 + [_vp]),
+    "logismos_launch_kv_gather_e4m3_fp16": (C.c_uint32, [_vp] * 7 + [_i] * 7 + [_vp]),
+    "logismos_launch_kv_gather_e4m3_bf16": (C.c_uint32, [_vp] * 7 + [_i] * 7 + [_vp]),
+    "logismos_launch_kv_gather_e4m3_f32": (C.c_uint32, [_vp] * 7 + [_i] * 7 + [_vp]),
+    "logismos_check_paged_attn_tree_shape": (C.c_uint32, [_i] * 12 + [C.c_char_p, _sz]),
+    "logismos_paged_attn_tree_workspace_bytes": (_sz, [_i] * 5),
+    "logismos_launch_paged_attn_tree_fp16": (C.c_uint32, [_vp] * 9 + [_i] * 12 + [_f, _vp]),
+    "logismos_launch_paged_attn_tree_e4m3_fp16": (C.c_uint32, [_vp] * 11 + [_i] * 12 + [_f, _vp]),
+    "logismos_launch_paged_attn_tree_e4m3_bf16": (C.c_uint32, [_vp] * 11 + [_i] * 12 + [_f, _vp]),
+    "logismos_tree_mask": (C.c_uint32, [_vp, _i, _i, _vp]),
     "logismos_check_attn_packed_shape": (C.c_uint32, [_i] * 9 + [C.c_char_p, _sz]),
     "logismos_launch_attn_packed_fp16": (C.c_uint32, [_vp] * 5 + [_i] * 9 + [_f, _i, _vp]),
     "logismos_launch_attn_packed_bf16": (C.c_uint32, [_vp] * 5 + [_i] * 9 + [_f, _i, _vp]),
@@ -527,6 +543,77 @@ def launch_kv_gather_turbo3_f32(k_pool, v_pool, block_table_row, k_out, v_out, s
         n_tokens, num_kv_heads, block_size, _raw(stream)))
 
 
+def launch_kv_write_e4m3(k_new, v_new, k_pool, k_exp, v_pool, v_exp, slot_mapping, total_tokens: int,
+                         num_kv_heads: int, head_dim: int, block_size: int, num_blocks: int,
+                         k_stride=None, v_stride=None, bf16: bool = False, stream=None) -> None:
+    """K and V rows quantised into e4m3 pools; strides in elements, None: rows one behind the other."""
+    name = "kv_write_e4m3_bf16" if bf16 else "kv_write_e4m3_fp16"
+    width = num_kv_heads * head_dim
+    dims = (total_tokens, num_kv_heads, head_dim, block_size, num_blocks,
+            width if k_stride is None else k_stride, width if v_stride is None else v_stride)
+    code = _launcher(name)(k_new, v_new, k_pool, k_exp, v_pool, v_exp, slot_mapping, *dims, _raw(stream))
+    if code != 0:
+        _refused(name, code, library().logismos_check_kv_e4m3_shape, *dims)
+
+
+def launch_kv_gather_e4m3(k_pool, k_exp, v_pool, v_exp, slot_mapping, k_out, v_out, total_tokens: int,
+                          num_kv_heads: int, head_dim: int, block_size: int, num_blocks: int,
+                          k_stride=None, v_stride=None, dtype: str = "fp16", stream=None) -> None:
+    """Rows of e4m3 pools read back as fp16, bf16 or f32."""
+    if dtype not in ("fp16", "bf16", "f32"):
+        raise ValueError(f"dtype must be fp16, bf16 or f32, not {dtype!r}")
+    name = "kv_gather_e4m3_" + dtype
+    width = num_kv_heads * head_dim
+    dims = (total_tokens, num_kv_heads, head_dim, block_size, num_blocks,
+            width if k_stride is None else k_stride, width if v_stride is None else v_stride)
+    code = _launcher(name)(k_pool, k_exp, v_pool, v_exp, slot_mapping, k_out, v_out, *dims, _raw(stream))
+    if code != 0:
+        _refused(name, code, library().logismos_check_kv_e4m3_shape, *dims)
+
+
+def tree_mask(parents, mask_words: int = 0) -> np.ndarray:
+    """uint64 [tokens][mask_words] for `launch_paged_attn_tree`: of every drafted token its ancestors and
+    itself; parents[i] is an earlier token or -1; 0 words: as many as the tokens need."""
+    parents = np.ascontiguousarray(parents, np.int32)
+    words = mask_words or max(1, (parents.size + 63) // 64)
+    out = np.empty((parents.size, max(words, 1)), np.uint64)
+    if parents.ndim != 1 or library().logismos_tree_mask(
+            parents.ctypes.data_as(_vp), parents.size, words, out.ctypes.data_as(_vp)) != 0:
+        raise UnsupportedShape("tree_mask", "a parent is not an earlier token or -1, or the tokens do not "
+                               "fit the words (at most 4)")
+    return out
+
+
+def paged_attn_tree_workspace_bytes(total_tokens: int, max_seqlen_q: int, num_q_heads: int,
+                                    num_kv_heads: int, head_dim: int) -> int:
+    return library().logismos_paged_attn_tree_workspace_bytes(total_tokens, max_seqlen_q, num_q_heads,
+                                                              num_kv_heads, head_dim)
+
+
+def launch_paged_attn_tree(q, k_pool, v_pool, block_tables, cu_seqlens_q, context_lens, tree_mask, out,
+                           workspace, num_seqs: int, total_tokens: int, max_seqlen_q: int,
+                           num_q_heads: int, num_kv_heads: int, head_dim: int, block_size: int,
+                           max_blocks_per_seq: int, num_blocks: int, scale: float,
+                           mask_words: int = 1, k_exp=None, v_exp=None, q_stride=None,
+                           out_stride=None, bf16: bool = False, stream=None) -> None:
+    """Attention of drafted tokens over fp16 pools, or over e4m3 pools with k_exp and v_exp (fp16 or bf16 rows)."""
+    width = num_q_heads * head_dim
+    dims = (num_seqs, total_tokens, max_seqlen_q, num_q_heads, num_kv_heads, head_dim, block_size,
+            max_blocks_per_seq, num_blocks, mask_words, width if q_stride is None else q_stride,
+            width if out_stride is None else out_stride)
+    rest = (block_tables, cu_seqlens_q, context_lens, tree_mask, out, workspace, *dims, scale, _raw(stream))
+    if k_exp is None and v_exp is None:
+        if bf16:
+            raise ValueError("fp16 pools take fp16 rows")
+        name = "paged_attn_tree_fp16"
+        code = _launcher(name)(q, k_pool, v_pool, *rest)
+    else:
+        name = "paged_attn_tree_e4m3_bf16" if bf16 else "paged_attn_tree_e4m3_fp16"
+        code = _launcher(name)(q, k_pool, k_exp, v_pool, v_exp, *rest)
+    if code != 0:
+        _refused(name, code, library().logismos_check_paged_attn_tree_shape, *dims)
+
+
 def launch_kv_write_fp16(k_new, v_new, k_pool, v_pool, slot_mapping, total_tokens: int,
                          num_kv_heads: int, head_dim: int, stream=None) -> None:
     _status("kv_write_fp16", library().logismos_launch_kv_write_fp16(
@@ -622,6 +709,29 @@ def launch_rope_packed(q_in, k_in, q_out, k_out, positions, inv_freq, tokens: in
                            1 if interleaved else 0, _raw(stream))
     if code != 0:
         _refused(name, code, library().logismos_check_rope_packed_shape, *dims)
+
+
+def launch_norm_rope_packed(q_in, k_in, q_out, k_out, positions, axis_of_pair, inv_freq, q_gain,
+                            k_gain, tokens: int, num_q_heads: int, num_kv_heads: int, head_dim: int,
+                            rotary_dim: int, num_axes: int = 1, eps: float = 1e-6,
+                            interleaved: bool = False, amplitude: float = 1.0, position_stride=None,
+                            q_in_stride=None, k_in_stride=None, q_out_stride=None, k_out_stride=None,
+                            dtype: str = "fp16", stream=None) -> None:
+    """RMS norm of every q and k head and rotary positions of one axis or several; a gain may be None (no
+    norm of those heads), axis_of_pair too with one axis, rotary_dim 0 (no rotation)."""
+    if dtype not in ("fp16", "bf16", "f32"):
+        raise ValueError(f"dtype must be fp16, bf16 or f32, not {dtype!r}")
+    name = "norm_rope_packed_" + dtype
+    qw, kw = num_q_heads * head_dim, num_kv_heads * head_dim
+    dims = (tokens, num_q_heads, num_kv_heads, head_dim, rotary_dim, num_axes,
+            tokens if position_stride is None else position_stride,
+            qw if q_in_stride is None else q_in_stride, kw if k_in_stride is None else k_in_stride,
+            qw if q_out_stride is None else q_out_stride,
+            kw if k_out_stride is None else k_out_stride)
+    code = _launcher(name)(q_in, k_in, q_out, k_out, positions, axis_of_pair, inv_freq, q_gain, k_gain,
+                           *dims, eps, amplitude, 1 if interleaved else 0, _raw(stream))
+    if code != 0:
+        _refused(name, code, library().logismos_check_norm_rope_packed_shape, *dims)
 
 
 def launch_attn_packed(q, k, v, cu_seqlens, out, num_seqs: int, total_tokens: int,
