@@ -46,6 +46,7 @@ struct TreeParams {
     int64_t q_stride, out_stride;
     float scale_log2e;
     int workers;
+    int step_blocks, step_rows;  // what lies between two tiles of a part: whole blocks and rows
     int slot_waves;  // waves that a slot of the workspace has room for
 };
 
@@ -57,8 +58,19 @@ struct TreeChunk {
     unsigned end;                              // ... with the last lane's
 };
 
+// The launch's parameters read anew where they are needed: kept in scalar registers, those that the loop over the tiles has no use for
+// would push out those that it has.
+typedef const TreeParams __attribute__((address_space(4)))* TreeCold;
+__device__ __forceinline__ TreeCold tree_cold() {
+    auto at = (TreeCold)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(at));
+    return at;
+}
+
 template <int COLS>
-__device__ __forceinline__ TreeChunk tree_chunk(const TreeParams& p, int first, unsigned before) {
+__device__ __forceinline__ TreeChunk tree_chunk(int first, unsigned before) {
+    const TreeCold c0 = tree_cold();
+    const auto& p = *c0;
     const int lane = threadIdx.x & 63, s = first + lane;
     TreeChunk c;
     c.first = first;
@@ -123,300 +135,601 @@ constexpr int tree_wave_floats(int d) { return 32 * d + 128; }
 // 2^kTreeHead and 2^(kTreeHead + kTreeLazy), so that those down to 2^-25 of a column's largest keep all bits of fp16.
 constexpr float kTreeHead = 11.0f, kTreeLazy = 4.0f;
 
-template <typename T, int D, int WAVES, bool E4M3>
-__global__ __launch_bounds__(64 * WAVES) void paged_attn_tree_kernel(const TreeParams p) {
-    constexpr int kCols = 32 * WAVES, kMovers = 32 * WAVES;  // threads that move K, and V
+// Scores beyond this (in units of log 2) are multiplied and subtracted in two roundings, the same for the maximum, and their
+// probabilities start at 1: a fused difference is off by up to half a step of the maximum, which is a factor of all of them as long as it
+// is small.
+constexpr float kTreeFar = 1048576.0f;
+
+// Elements of the rings of a part, and workgroups that a compute unit holds (by LDS, and two waves to a SIMD by registers).
+constexpr int tree_rings(int d) { return 2 * kTreeKeys * (d + 8 + (d / 32 % 2 ? d : d + 32)); }
+constexpr int tree_blocks(int d, int colw, int parts) {
+    return colw * parts > 4 || d > 128 || (d > 64 && parts > 1) || 2 * parts * tree_rings(d) > 80 * 1024 ? 1 : 2;
+}
+
+// COLW waves side by side hold a unit's columns, PARTS groups of them take its tiles in turn.  One wave alone moves K and V of its
+// tiles itself and waits for nobody; otherwise half of a part's waves move K and half V.
+template <typename T, int D, int COLW, int PARTS, bool E4M3>
+__global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) void paged_attn_tree_kernel(const TreeParams p) {
+    constexpr bool kAlone = COLW == 1;
+    constexpr int kCols = 32 * COLW, kMovers = kAlone ? 64 : 32 * COLW;  // threads that move K, and V
     constexpr int kSteps = D / 16, kTiles = D / 32;
     constexpr int kKRow = D + 8, kVRow = D / 32 % 2 ? D : D + 32;  // elements
-    constexpr int kPer = kTreeKeys * D / 8 / kMovers;              // pieces of 8 elements that a thread moves per tile
-    constexpr int kPiece = E4M3 ? 8 : 16;                          // their bytes
-    constexpr int kRow = E4M3 ? D : 2 * D;                         // bytes of a head row
-    constexpr int kTile = kTreeKeys * (kKRow + kVRow), kWayOut = WAVES * 16 * (D + 8);
-    __shared__ __attribute__((aligned(16))) unsigned short lds[kTile > kWayOut ? kTile : kWayOut];
-    __shared__ int tops[2];  // of the tile: exponents of K and V
-    unsigned short* const ks = lds;
-    unsigned short* const vs = lds + kTreeKeys * kKRow;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, col = lane & 31;
-    const bool moves_v = wave >= WAVES / 2;
+    constexpr int kKTile = kTreeKeys * kKRow, kVTile = kTreeKeys * kVRow;
+    constexpr int kStride = kTreeKeys * PARTS;         // keys between two tiles of a part
+    constexpr int kPer = kTreeKeys * D / 8 / kMovers;  // pieces of 8 elements that a thread moves per tile
+    constexpr int kPiece = E4M3 ? 8 : 16;              // their bytes
+    constexpr int kRow = E4M3 ? D : 2 * D;             // bytes of a head row
+    constexpr int kRings = tree_rings(D);
+    static_assert(kRings == 2 * kKTile + 2 * kVTile, "two tiles each");
+    constexpr bool kWide = D > 128;  // four operands of K and V at a time: there are no registers for more
+    // Steps between asking for a tile and storing it: two, one where a wave alone has no registers for more.
+    constexpr int kDeep = (kAlone && !E4M3 && D > 64) || kWide ? 1 : 2;
+    constexpr bool kAsIs = E4M3 && __is_same(T, PackedBf16);  // K in bf16, whose range is that of the cache
+    static_assert(kPer * kMovers * 8 == kTreeKeys * D, "whole pieces");
+    __shared__ __attribute__((aligned(16))) unsigned short lds[PARTS * kRings];
+    __shared__ int odd_parts[PARTS], far_parts[PARTS];
+    const int wave_of_all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int part = wave_of_all / COLW, wave = wave_of_all - part * COLW;
+    const int tid = threadIdx.x - part * 64 * COLW, lane = tid & 63, h = lane >> 5, col = lane & 31;
+    unsigned short* const ks = lds + part * kRings;
+    unsigned short* const vs = ks + 2 * kKTile;
+    const bool moves_k = kAlone || wave < COLW / 2, moves_v = kAlone || wave >= COLW / 2;
+    const int mover = tid % kMovers;
     const int s16 = lane & 15;
     const int v_lane = (4 * h + (s16 >> 2)) * kVRow + 16 * ((lane >> 4) & 1) + 4 * (s16 & 3);
+    auto together = [&] LG_INLINE {
+        if constexpr (kAlone) __builtin_amdgcn_wave_barrier();
+        else __syncthreads();
+    };
 
     unsigned total = 0;
-    for (int first = 0; first < p.num_seqs; first += 64) total = tree_chunk<kCols>(p, first, total).end;
-    const unsigned per = tree_share(total, p.workers);
+    for (int first = 0; first < tree_cold()->num_seqs; first += 64) total = tree_chunk<kCols>(first, total).end;
+    const unsigned per = tree_share(total, tree_cold()->workers);
     unsigned pos = blockIdx.x * per;
-    const unsigned end = total - pos < per ? total : pos + per;
     if (pos >= total) return;
-    TreeChunk chunk = tree_chunk<kCols>(p, 0, 0);
+    const unsigned end = total - pos < per ? total : pos + per;
+    int first = 0;  // of the 64 sequences that the next unit is in, and the tiles in front of them
+    unsigned before = 0;
     while (pos < end) {
-        while (pos >= chunk.end) chunk = tree_chunk<kCols>(p, chunk.first + 64, chunk.end);
+        TreeChunk chunk = tree_chunk<kCols>(first, before);
+        while (pos >= chunk.end) {
+            first += 64;
+            before = chunk.end;
+            chunk = tree_chunk<kCols>(first, before);
+        }
         const TreeUnit u = tree_unit(chunk, p.hkv, pos);
         const int tile0 = u.tile;
         const int tile1 = (unsigned)(u.tiles - tile0) < end - pos ? u.tiles : tile0 + (int)(end - pos);
         pos += (unsigned)(tile1 - tile0);
+        const int steps = u.ctx > 0 ? (tile1 - tile0 + PARTS - 1) / PARTS : 0;  // of every part
 
-        const int cols = u.rows * p.g;
+        const int cols = u.rows * tree_cold()->g;
         const int c0 = u.group * kCols + wave * 32;
-        const int gc = c0 + col < cols ? c0 + col : cols - 1;
-        const int tok = gc / p.g, head = u.head * p.g + gc - tok * p.g;
         const bool active = c0 < cols;
-        const uint32_t* const mask = p.mask + (int64_t)(u.row0 + tok) * p.words;
+        // This lane's token and head (worked out anew where they are needed: registers are what the loop is short of).
+        struct Column {
+            int tok, head;
+        };
+        auto column = [&] LG_INLINE {
+            int c = c0 + col;
+            asm volatile("" : "+v"(c));
+            c = c < cols ? c : cols - 1;
+            const int g = tree_cold()->g, tok = c / g;
+            return Column{tok, u.head * g + c - tok * g};
+        };
 
         uint4_t qb[kSteps];
         {
-            const unsigned short* q = p.q + (int64_t)(u.row0 + tok) * p.q_stride + (int64_t)head * D + 8 * h;
+            const Column c = column();
+            const TreeCold t = tree_cold();
+            const unsigned short* q = t->q + (int64_t)(u.row0 + c.tok) * t->q_stride + (int64_t)c.head * D + 8 * h;
 #pragma unroll
             for (int j = 0; j < kSteps; ++j) qb[j] = *reinterpret_cast<const uint4_t*>(q + 16 * j);
         }
 
-        // ---- movement: the first half of the waves carries K, the second V
+        // ---- where the tiles of this part lie: the table 64 entries at a time, one to a lane, and the next ones on their way
         const int32_t* const table = p.tables + (int64_t)u.seq * p.max_blocks;
-        const uint8_t* const pool = moves_v ? p.v_pool : p.k_pool;
-        const uint8_t* const exps = moves_v ? p.v_exp : p.k_exp;
-        struct Regs {
-            uint4_t x[kPer];
-            int e;  // exponent of key lane % 32
+        const int in_table = (u.ctx + p.block_size - 1) / p.block_size;
+        auto entries = [&](int first) LG_INLINE { return first + lane < in_table ? table[first + lane] : -1; };
+        int at_tile, at_block, at_row, base, ids, ids_next;
+        auto start = [&](int which) LG_INLINE {
+            at_tile = tile0 + which;
+            at_block = at_tile * kTreeKeys / p.block_size;
+            at_row = at_tile * kTreeKeys - at_block * p.block_size;
+            base = at_block;
+            ids = entries(base);
+            ids_next = entries(base + 32);
         };
-        auto key_of = [&](int i) LG_INLINE { return (tid % kMovers + kMovers * i) / (D / 8); };
-        auto piece_of = [&](int i) LG_INLINE { return (tid % kMovers + kMovers * i) % (D / 8); };
-        // The blocks of the two halves of a tile; bit 0 / 1 of `there`: the half has one.
-        struct Blocks {
-            int id[2], off[2], there;
+        // A tile: the rows of the pools where its halves begin, -1: not there.
+        struct Place {
+            int row[2];
         };
-        auto blocks_of = [&](int tile) LG_INLINE {
-            Blocks b;
-            b.there = 0;
+        // ... and, of e4m3 pools, where the exponents of the halves begin, in a pool.
+        int64_t exps_at[2];
+        auto walk = [&] LG_INLINE {
+            Place w;
+            const bool exists = at_tile < tile1;
+            if (at_block - base >= 48) {
+                base += 32;
+                ids = ids_next;
+                ids_next = entries(base + 32);
+            }
+            int block = at_block, row = at_row;
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const int key = tile * kTreeKeys + 16 * i;
-                const int at = key < u.ctx ? key / p.block_size : 0;
-                const int id = key < u.ctx ? table[at] : -1;
+                const int id = exists ? __builtin_amdgcn_readlane(ids, (block - base) & 63) : -1;
                 const bool ok = id >= 0 && id < p.num_blocks;
-                b.id[i] = ok ? id : 0;
-                b.off[i] = key < u.ctx ? key - at * p.block_size : 0;
-                b.there |= ok ? 1 << i : 0;
+                w.row[i] = ok ? id * p.block_size + row : -1;
+                if constexpr (E4M3) exps_at[i] = ok ? ((int64_t)id * p.hkv + u.head) * p.block_size + row : 0;
+                row += 16;
+                if (row >= p.block_size) {
+                    row = 0;
+                    ++block;
+                }
             }
-            return b;
+            at_tile += PARTS;
+            at_block += p.step_blocks;
+            at_row += p.step_rows;
+            if (at_row >= p.block_size) {
+                at_row -= p.block_size;
+                ++at_block;
+            }
+            return w;
         };
-        auto gload = [&](const Blocks& b, int tile, Regs& r) LG_INLINE {
-            const int left = u.ctx - tile * kTreeKeys;  // keys behind the last one: that one again
-            int64_t row[2];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) row[i] = (int64_t)b.id[i] * p.block_size + b.off[i];
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) {
-                const int key = key_of(i) < left ? key_of(i) : left - 1;
-                const int64_t at = (key < 16 ? row[0] : row[1]) + (key & 15);
-                const uint8_t* src = pool + (at * p.hkv + u.head) * kRow + kPiece * piece_of(i);
+        auto is_there = [](const Place& w) LG_INLINE { return (w.row[0] & w.row[1]) >= 0; };   // one half at least
+        auto is_whole = [](const Place& w) LG_INLINE { return (w.row[0] | w.row[1]) >= 0; };
+
+        struct Regs {
+            uint4_t k[kAlone ? kPer : 1], v[kPer];  // (SPLIT: v holds whichever the wave moves)
+            int e;  // exponent of K (lower half of the wave) or V of key lane % 32
+        };
+        // Piece i of a mover: of key key_of(i).  Where a round of the movers' pieces is whole keys, it lies kRound keys behind piece
+        // i - 1 and one offset serves all; within a wave they are then of the same half of the tile.
+        constexpr bool kEven = kMovers % (D / 8) == 0;
+        constexpr int kRound = kMovers / (D / 8);
+        auto key_of = [&](int i) LG_INLINE {
+            return kEven ? mover / (D / 8) + kRound * i : (mover + kMovers * i) / (D / 8);
+        };
+        auto piece_of = [&](int i) LG_INLINE { return (mover + (kEven ? 0 : kMovers * i)) % (D / 8); };
+        const unsigned row_bytes = (unsigned)p.hkv * kRow;
+        const int wave_key = __builtin_amdgcn_readfirstlane(mover / (D / 8)) & ~15;  // (kEven: of which 16 keys piece 0 is)
+        const unsigned even_at = ((unsigned)key_of(0) & 15u) * row_bytes + (unsigned)(kPiece * piece_of(0));
+        auto load = [&](const uint8_t* pool, const Place& w, int key0, uint4_t* x) LG_INLINE {
+            const int left = u.ctx - key0;  // keys behind the last one, and in a half that is not there: others that are
+            const uint8_t* const half0 = pool + (int64_t)max(w.row[0], 0) * row_bytes + u.head * kRow;
+            const uint8_t* const half1 = pool + (int64_t)max(w.row[1], 0) * row_bytes + u.head * kRow;
+            auto take = [&](int i, const uint8_t* src) LG_INLINE {
                 if constexpr (E4M3) {
-                    const uint2_t v = *reinterpret_cast<const uint2_t*>(src);
-                    r.x[i][0] = v[0];
-                    r.x[i][1] = v[1];
+                    const uint2_t b = *reinterpret_cast<const uint2_t*>(src);
+                    x[i][0] = b[0];
+                    x[i][1] = b[1];
                 } else {
-                    r.x[i] = *reinterpret_cast<const uint4_t*>(src);
+                    x[i] = *reinterpret_cast<const uint4_t*>(src);
                 }
-            }
-            if constexpr (E4M3) {
-                const int key = col < left ? col : left - 1;
-                const int half = key >> 4;
-                const int64_t at = ((int64_t)(half ? b.id[1] : b.id[0]) * p.hkv + u.head) * p.block_size +
-                                   (half ? b.off[1] : b.off[0]) + (key & 15);
-                r.e = exps[at];
+            };
+            if (kEven && left >= kTreeKeys) {
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) {
+                    const uint8_t* from = wave_key + kRound * i < 16 ? half0 : half1;
+                    take(i, from + (unsigned)(kRound * i % 16) * row_bytes + even_at);
+                }
+            } else {
+                int m = mover;
+                asm volatile("" : "+v"(m));
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) {
+                    const int at = (m + kMovers * i) / (D / 8), key = at < left ? at : left - 1;
+                    take(i, (key < 16 ? half0 : half1) + ((unsigned)(key & 15) * row_bytes + kPiece * ((m + kMovers * i) % (D / 8))));
+                }
             }
         };
-        auto lstore = [&](const Regs& r) LG_INLINE {
-            unsigned short* at = moves_v ? vs : ks;
-            const int row = moves_v ? kVRow : kKRow;
-            int top = 127;
-            constexpr bool kAsIs = __is_same(T, PackedBf16);  // K in bf16
-            if constexpr (E4M3) {
-                if (!kAsIs || moves_v) {
-                    top = r.e;
-                    top = max(top, lane_xor_i32<1>(top));
-                    top = max(top, lane_xor_i32<2>(top));
-                    top = max(top, lane_xor_i32<4>(top));
-                    top = max(top, lane_xor_i32<8>(top));
-                    top = max(top, lane_xor_i32<16>(top));
-                }
-                if (tid % kMovers == 0) tops[moves_v] = top - 127;
+        const uint8_t* const exps = E4M3 ? (h ? p.v_exp : p.k_exp) : nullptr;
+        auto load_exps = [&](int key0) LG_INLINE {  // of the tile that walk() came to last
+            const int left = u.ctx - key0, key = col < left ? col : left - 1;
+            return (int)exps[(key < 16 ? exps_at[0] : exps_at[1]) + (key & 15)];
+        };
+        // The largest exponents of a tile's rows of K and V.
+        struct Tops {
+            int k, v;
+        };
+        auto tops_of = [&](int e) LG_INLINE {
+            e = max(e, dpp_i32<kDppRowRor + 8>(e));
+            e = max(e, dpp_i32<kDppRowRor + 4>(e));
+            e = max(e, dpp_i32<kDppRowRor + 2>(e));
+            e = max(e, dpp_i32<kDppRowRor + 1>(e));
+            Tops t;
+            t.k = max(__builtin_amdgcn_readlane(e, 0), __builtin_amdgcn_readlane(e, 16)) - 127;
+            t.v = max(__builtin_amdgcn_readlane(e, 32), __builtin_amdgcn_readlane(e, 48)) - 127;
+            if (kAsIs) t.k = 0;
+            return t;
+        };
+        // A piece of 8 as the kernel wants it: e4m3 rows times 2^(e - top) in 16 bits.
+        auto decoded = [&](const uint4_t& x, int e, int top, bool as_bf16) LG_INLINE {
+            if constexpr (!E4M3) return x;
+            const float scale = __int_as_float(max(e - top, 0) << 23);
+            uint4_t y;
+            if (as_bf16) {
+                y[0] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x[0], scale, false));
+                y[1] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x[0], scale, true));
+                y[2] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x[1], scale, false));
+                y[3] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x[1], scale, true));
+            } else {
+                y[0] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x[0], scale, false));
+                y[1] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x[0], scale, true));
+                y[2] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x[1], scale, false));
+                y[3] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x[1], scale, true));
             }
+            return y;
+        };
+        auto store_k = [&](int buf, const uint4_t* x, int e, const Tops& top) LG_INLINE {
+            unsigned short* const to = ks + buf * kKTile;
 #pragma unroll
             for (int i = 0; i < kPer; ++i) {
-                unsigned short* to = at + key_of(i) * row + 8 * piece_of(i);
-                if constexpr (E4M3) {
-                    const float scale = __int_as_float(max(__shfl(r.e, key_of(i)) - top + 127, 0) << 23);
-                    uint4_t y;
-                    if (kAsIs && !moves_v) {
-                        y[0] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(r.x[i][0], scale, false));
-                        y[1] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(r.x[i][0], scale, true));
-                        y[2] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(r.x[i][1], scale, false));
-                        y[3] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(r.x[i][1], scale, true));
-                    } else {
-                        y[0] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(r.x[i][0], scale, false));
-                        y[1] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(r.x[i][0], scale, true));
-                        y[2] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(r.x[i][1], scale, false));
-                        y[3] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(r.x[i][1], scale, true));
+                const int row = E4M3 ? __shfl(e, key_of(i)) : 0;
+                *reinterpret_cast<uint4_t*>(to + key_of(i) * kKRow + 8 * piece_of(i)) = decoded(x[i], row, top.k, kAsIs);
+            }
+        };
+        // A key that a column does not see has the probability 0 there, and 0 times an infinity or NaN of its V row is NaN: in
+        // tiles that are not seen whole such elements go in as 0, and are added at the end for the columns that see them.
+        auto store_v = [&](int buf, const uint4_t* x, int e, const Tops& top, const Place& w, int key0) LG_INLINE {
+            unsigned short* const to = vs + buf * kVTile;
+            const bool whole = is_whole(w) && key0 + kTreeKeys <= u.prior;
+            bool odd = false;
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                const int row = E4M3 ? __shfl(e, 32 + key_of(i)) : 0;
+                uint4_t y = decoded(x[i], row, top.v, false);
+                if (!whole) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const unsigned bad = ((y[j] & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
+                        odd |= bad != 0;
+                        y[j] = !is_there(w) ? 0u : y[j] & ~((bad >> 15) * 0xffffu);
                     }
-                    *reinterpret_cast<uint4_t*>(to) = y;
-                } else {
-                    *reinterpret_cast<uint4_t*>(to) = r.x[i];
                 }
+                *reinterpret_cast<uint4_t*>(to + key_of(i) * kVRow + 8 * piece_of(i)) = y;
             }
+            if (!whole && __builtin_amdgcn_ballot_w64(odd) != 0 && lane == 0) odd_parts[part] = 1;
         };
-        auto v_operand = [&](int kb, int dt) LG_INLINE {
+        auto v_operand = [&](int buf, int kb, int dt) LG_INLINE {
             typedef short short4_t __attribute__((ext_vector_type(4)));
             typedef __attribute__((address_space(3))) short4_t lds_short4_t;
-            const unsigned short* a = vs + v_lane + 16 * kb * kVRow + 32 * dt;
+            const unsigned short* a = vs + buf * kVTile + v_lane + 16 * kb * kVRow + 32 * dt;
             const uint2_t lo = __builtin_bit_cast(uint2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4_t*)a));
             const uint2_t hi =
                 __builtin_bit_cast(uint2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4_t*)(a + 8 * kVRow)));
             return uint4_t{lo[0], lo[1], hi[0], hi[1]};
         };
-        auto k_operand = [&](int j) LG_INLINE {
-            return *reinterpret_cast<const uint4_t*>(ks + col * kKRow + 16 * j + 8 * h);
+        auto k_operand = [&](int buf, int j) LG_INLINE {
+            return *reinterpret_cast<const uint4_t*>(ks + buf * kKTile + col * kKRow + 16 * j + 8 * h);
+        };
+        // Which keys of a tile this column sees.
+        auto window = [&](const Place& w, int key0) LG_INLINE {
+            unsigned win = ~0u;
+            const int j0 = key0 - u.prior;
+            if (j0 > -32) {
+                const TreeCold t = tree_cold();
+                const int words = t->words;
+                const uint32_t* const mask = t->mask + (int64_t)(u.row0 + column().tok) * words;
+                auto word = [&](int i) LG_INLINE { return i < words ? mask[i] : 0u; };
+                if (j0 < 0) {
+                    win = word(0) << -j0 | ((1u << -j0) - 1u);
+                } else {
+                    const int i = j0 >> 5;
+                    win = (unsigned)(((uint64_t)word(i + 1) << 32 | word(i)) >> (j0 & 31));
+                }
+            }
+            const int left = u.ctx - key0;
+            if (left < 32) win &= left > 0 ? (1u << left) - 1u : 0u;
+            if (w.row[0] < 0) win &= 0xffff0000u;
+            if (w.row[1] < 0) win &= 0x0000ffffu;
+            return win;
         };
 
-        float m = -INFINITY, l = 0.0f;
+        float m, l;
         float16_t o[kTiles];
-#pragma unroll
-        for (int dt = 0; dt < kTiles; ++dt)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) o[dt][e] = 0.0f;
+        uint4_t p_prev[2];
+        float16_t s_cur;
 
-        Regs r;
-        Blocks b = blocks_of(tile0);
-        if (u.ctx > 0) gload(b, tile0, r);
-        for (int tile = tile0; tile < tile1 && u.ctx > 0; ++tile) {
-            const int key0 = tile * kTreeKeys, there = b.there;
-            __syncthreads();
-            lstore(r);
-            __syncthreads();
-            if (tile + 1 < tile1) {
-                b = blocks_of(tile + 1);
-                gload(b, tile + 1, r);
-            }
-            if (!active) continue;
-            float scale = p.scale_log2e, v_top = 0.0f;
-            if constexpr (E4M3) {
-                scale = ldexpf(scale, tops[0]);
-                v_top = (float)tops[1];
-            }
-            float16_t s;
+        // Tile i with S(i) in s_cur, K(i + 1) in K buffer 1 - H and V(i - 1) in V buffer 1 - H; leaves S(i + 1) and P(i).
+        auto step = [&](auto h_c, const Place& w, int key0, const Tops& top, bool careful) LG_INLINE {
+            constexpr int H = decltype(h_c)::value;
+            float scale = E4M3 ? ldexpf(p.scale_log2e, top.k) : p.scale_log2e;
+            float v_top = E4M3 ? (float)top.v : 0.0f;
+            if (!is_whole(w) || key0 + kTreeKeys > u.prior) {
+                const unsigned win = window(w, key0) >> (4 * h);
 #pragma unroll
-            for (int e = 0; e < 16; ++e) s[e] = 0.0f;
+                for (int e = 0; e < 16; ++e) s_cur[e] = (win >> (8 * (e >> 2) + (e & 3))) & 1u ? s_cur[e] : -INFINITY;
+            }
+            if (__builtin_expect(careful, 0)) {
 #pragma unroll
-            for (int j = 0; j < kSteps; ++j) s = T::mfma32(k_operand(j), qb[j], s);
-            // which of the tile's keys this column sees
-            const bool masked = key0 + kTreeKeys > u.prior || there != 3;
-            unsigned win = ~0u;
-            if (masked) {
-                const int j0 = key0 - u.prior;
-                if (j0 > -32) {
-                    auto word = [&](int i) LG_INLINE { return i < p.words ? mask[i] : 0u; };
-                    if (j0 < 0) {
-                        win = word(0) << -j0 | ((1u << -j0) - 1u);
-                    } else {
-                        const int i = j0 >> 5;
-                        win = (unsigned)(((uint64_t)word(i + 1) << 32 | word(i)) >> (j0 & 31));
-                    }
+                for (int e = 0; e < 16; ++e) s_cur[e] = __fadd_rn(__fmul_rn(s_cur[e], scale), v_top);
+                scale = 1.0f;
+                v_top = 0.0f;
+            }
+            uint4_t ka[kSteps], va[kSteps];
+            if constexpr (!kWide)
+#pragma unroll
+                for (int j = 0; j < kSteps; ++j) {
+                    ka[j] = k_operand(1 - H, j);
+                    va[j] = v_operand(1 - H, j / kTiles, j % kTiles);
                 }
-                const int left = u.ctx - key0;
-                if (left < 32) win &= (1u << left) - 1u;
-                if ((there & 1) == 0) win &= 0xffff0000u;
-                if ((there & 2) == 0) win &= 0x0000ffffu;
-            }
-            float x[16], tm = -INFINITY;
+            float tm = -INFINITY;
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                x[e] = s[e] * scale;
-                if (masked) x[e] = (win >> (8 * (e >> 2) + 4 * h + (e & 3))) & 1u ? x[e] : -INFINITY;
-                tm = fmaxf(tm, x[e]);
-            }
+            for (int e = 0; e < 16; ++e) tm = fmaxf(tm, s_cur[e]);
             // (exponents of the tile's probabilities and of its rows of V together)
-            tm = fmaxf(tm, lane_xor_f32<32>(tm)) + v_top - kTreeHead;
+            tm = __fadd_rn(__fmul_rn(fmaxf(tm, lane_xor_f32<32>(tm)), scale), v_top);
+            tm = fabsf(tm) < kTreeFar ? tm - kTreeHead : tm;
             const bool raise = tm > m + kTreeLazy;
-            if (__builtin_amdgcn_ballot_w64(raise) != 0) {
-                const float alpha = raise ? fast_exp2(m - tm) : 1.0f;
-                m = raise ? tm : m;
+            const float m_before = m;
+            m = raise ? tm : m;
+            float16_t s_nxt;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s_nxt[e] = 0.0f;
+#pragma unroll
+            for (int j = 0; j < kSteps; ++j) {
+                if constexpr (kWide) {
+                    if (j % 4 == 0) __builtin_amdgcn_sched_barrier(0);
+                    ka[j] = k_operand(1 - H, j);
+                    va[j] = v_operand(1 - H, j / kTiles, j % kTiles);
+                }
+                s_nxt = T::mfma32(ka[j], qb[j], s_nxt);
+                o[j % kTiles] = PackedF16::mfma32(va[j], p_prev[j / kTiles], o[j % kTiles]);
+            }
+            float sum = 0.0f;
+            uint4_t pb[2];
+            const float off = v_top - (m == -INFINITY ? 0.0f : m);
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) {
+                const float p0 = fast_exp2(fmaf(s_cur[e], scale, off));
+                const float p1 = fast_exp2(fmaf(s_cur[e + 1], scale, off));
+                sum += p0;
+                sum += p1;
+                pb[e >> 3][(e & 7) >> 1] = PackedF16::pack2(p0, p1);
+            }
+            if constexpr (COLW >= 4 && !kWide) {
+                // half of the operand reads, then the products, each followed by a read and its share of the vector work
+                constexpr int kReads = 3 * kSteps, kFirst = (D > 64 ? 12 : 20) * kSteps / 8, kShare = (D < 128 ? 80 : 72) / (2 * kSteps);
+                __builtin_amdgcn_sched_group_barrier(0x100, kFirst, 0);
+#pragma unroll
+                for (int g = 0; g < 2 * kSteps; ++g) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                    if (g < kReads - kFirst) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x002, kShare, 0);
+                }
+            }
+            // (F belongs to this step: its results are used by the next one only, and would sink there)
+            asm volatile("" : "+v"(pb[0]), "+v"(pb[1]), "+v"(sum));
+            if (__builtin_expect(__builtin_amdgcn_ballot_w64(raise) != 0, 0)) {  // O(i - 1) was relative to the old one
+                const float alpha = raise ? fast_exp2(m_before - m) : 1.0f;
                 l *= alpha;
 #pragma unroll
                 for (int dt = 0; dt < kTiles; ++dt)
 #pragma unroll
                     for (int e = 0; e < 16; ++e) o[dt][e] *= alpha;
+                if (__builtin_amdgcn_ballot_w64(raise && fabsf(m) >= kTreeFar) != 0 && lane == 0) far_parts[part] = 1;
             }
-            const float ref = (m == -INFINITY ? 0.0f : m) - v_top;
-            float sum = 0.0f;
-            uint4_t pb[2];
+            l += E4M3 ? ldexpf(sum, -top.v) : sum;
+            s_cur = s_nxt;
+            p_prev[0] = pb[0];
+            p_prev[1] = pb[1];
+        };
+
+        // The tiles of the part; `careful`: as if none was seen whole.
+        auto walk_tiles = [&](bool careful) LG_INLINE {
+            m = -INFINITY;
+            l = 0.0f;
+            p_prev[0] = p_prev[1] = uint4_t{0, 0, 0, 0};
 #pragma unroll
-            for (int e = 0; e < 16; e += 2) {
-                x[e] = fast_exp2(x[e] - ref);
-                x[e + 1] = fast_exp2(x[e + 1] - ref);
-                sum += x[e];
-                sum += x[e + 1];
-                pb[e >> 3][(e & 7) >> 1] = PackedF16::pack2(x[e], x[e + 1]);
+            for (int dt = 0; dt < kTiles; ++dt)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[dt][e] = 0.0f;
+            start(part);
+            int key0 = at_tile * kTreeKeys;  // of tile i
+            Place w0 = walk(), w1, w2, w3;
+            Regs ra, rb;
+            Tops t0 = {0, 0}, t1 = {0, 0}, t2 = {0, 0};
+            int e0 = 127, e1 = 127;  // exponents of the rows of tiles i and i + 1
+            ra.e = 127;
+            auto kregs = [](Regs& r) LG_INLINE { return kAlone ? r.k : r.v; };
+            {
+                uint4_t x0[kPer];
+                if (is_there(w0)) {
+                    if constexpr (E4M3) e0 = load_exps(key0);
+                    if (moves_k) load(p.k_pool, w0, key0, x0);
+                }
+                w1 = walk();
+                if (is_there(w1)) {
+                    if constexpr (E4M3) e1 = load_exps(key0 + kStride);
+                    if (moves_k) load(p.k_pool, w1, key0 + kStride, kregs(rb));
+                }
+                if constexpr (kDeep == 2) {
+                    w2 = walk();
+                    if (is_there(w2)) {
+                        if constexpr (E4M3) ra.e = load_exps(key0 + 2 * kStride);
+                        if (moves_k) load(p.k_pool, w2, key0 + 2 * kStride, kregs(ra));
+                    }
+                    if (moves_v && is_there(w0)) load(p.v_pool, w0, key0, ra.v);
+                }
+                if constexpr (E4M3) {
+                    t0 = tops_of(e0);
+                    t1 = tops_of(e1);
+                }
+                if (moves_k) {
+                    store_k(0, x0, e0, t0);
+                    store_k(1, kregs(rb), e1, t1);
+                }
             }
-            l += E4M3 ? ldexpf(sum, -(int)v_top) : sum;
-            uint4_t va[kSteps];
+            // V buffer 1 plays V(-1) in the first step, whose P is 0: finite values
+            for (int i = tid; i < kVTile / 2; i += 64 * COLW) reinterpret_cast<unsigned*>(vs + kVTile)[i] = 0u;
+            together();
 #pragma unroll
-            for (int j = 0; j < kSteps; ++j) va[j] = v_operand(j / kTiles, j % kTiles);
-            // A key that a column does not see has the probability 0 there, and 0 times an infinity or NaN of its V row is NaN: in
-            // the new tokens' tiles such elements stay out of the product, and are added for the columns that see them.
-            bool odd = false;
-            if (masked) {
+            for (int e = 0; e < 16; ++e) s_cur[e] = 0.0f;
+#pragma unroll
+            for (int j = 0; j < kSteps; ++j) s_cur = T::mfma32(k_operand(0, j), qb[j], s_cur);
+            together();  // (the first step ends with a store into the buffer just read)
+            // step i, H its parity: what a later step needs is asked for in front of it and goes to LDS behind it
+            auto one = [&](auto h_c, Regs& now, Regs& next) LG_INLINE {
+                constexpr int H = decltype(h_c)::value;
+                Place& lead = kDeep == 2 ? w3 : w2;
+                lead = walk();
+                next.e = 127;
+                if (is_there(lead)) {
+                    if constexpr (E4M3) next.e = load_exps(key0 + (kDeep + 1) * kStride);
+                    if (moves_k) load(p.k_pool, lead, key0 + (kDeep + 1) * kStride, kregs(next));
+                }
+                const Place& behind = kDeep == 2 ? w1 : w0;
+                if (moves_v && is_there(behind)) load(p.v_pool, behind, key0 + (kDeep - 1) * kStride, next.v);
+                __builtin_amdgcn_sched_barrier(0);
+                if (active) step(h_c, w0, key0, t0, careful);
+                __builtin_amdgcn_sched_barrier(0);
+                Regs& then = kDeep == 2 ? now : next;
+                if constexpr (E4M3) t2 = tops_of(then.e);
+                if (moves_k) store_k(H, kregs(then), then.e, t2);  // K(i + 2)
+                if (moves_v) store_v(H, then.v, e0, t0, w0, key0);  // V(i)
+                e0 = e1;
+                e1 = then.e;
+                t0 = t1;
+                t1 = t2;
+                w0 = w1;
+                w1 = w2;
+                w2 = w3;
+                key0 += kStride;
+                together();
+            };
+            int i = 0;
+            for (; i + 1 < steps; i += 2) {
+                one(ic<0>{}, ra, rb);
+                one(ic<1>{}, rb, ra);
+            }
+            if (i < steps) one(ic<0>{}, ra, rb);
+            const int buf = (steps - 1) & 1;
+            if (active) {
 #pragma unroll
                 for (int j = 0; j < kSteps; ++j)
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        const unsigned bad = ((va[j][w] & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
-                        odd |= bad != 0;
-                        va[j][w] &= ~((bad >> 15) * 0xffffu);
-                    }
+                    o[j % kTiles] = PackedF16::mfma32(v_operand(buf, j / kTiles, j % kTiles), p_prev[j / kTiles], o[j % kTiles]);
             }
+        };
+
+        if (wave_of_all == 0 && lane < PARTS) odd_parts[lane] = far_parts[lane] = 0;
+        __syncthreads();
+        m = -INFINITY;
+        l = 0.0f;
 #pragma unroll
-            for (int j = 0; j < kSteps; ++j)
-                o[j % kTiles] = PackedF16::mfma32(va[j], pb[j / kTiles], o[j % kTiles]);
-            if (__builtin_expect(__builtin_amdgcn_ballot_w64(odd) != 0, 0)) {
+        for (int dt = 0; dt < kTiles; ++dt)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[dt][e] = 0.0f;
+        for (int careful = 0; careful < 2 && steps > 0; ++careful) {
+            walk_tiles(careful != 0);
+            __syncthreads();
+            int far = 0;
+#pragma unroll
+            for (int q = 0; q < PARTS; ++q) far |= far_parts[q];
+            if (__builtin_expect(__builtin_amdgcn_readfirstlane(far) == 0, 1)) break;
+            __syncthreads();  // (the first tiles go where the last ones were)
+        }
+        if (__builtin_expect(__builtin_amdgcn_readfirstlane(odd_parts[part]) != 0, 0)) {
+            start(part);
+            int key0 = at_tile * kTreeKeys;
+            for (int t = 0; t < steps && active; ++t, key0 += kStride) {
+                const Place w = walk();
+                if (!is_there(w) || (is_whole(w) && key0 + kTreeKeys <= u.prior)) continue;
+                const unsigned win = window(w, key0);
                 for (int key = 0; key < kTreeKeys; ++key) {
-                    const int at = 4 * (key >> 3) + (key & 3);
-                    float mine = x[0];
-#pragma unroll
-                    for (int e = 1; e < 16; ++e) mine = at == e ? x[e] : mine;
-                    const float prob = __shfl(mine, col + 32 * ((key >> 2) & 1));
-                    const bool seen = (win >> key) & 1u;
+                    const bool sees = (win >> key) & 1u;
+                    if (__builtin_amdgcn_ballot_w64(sees) == 0) continue;  // (nobody: perhaps it is not there)
+                    const uint8_t* row =
+                        p.v_pool + ((int64_t)(key < 16 ? w.row[0] : w.row[1]) + (key & 15)) * row_bytes + u.head * kRow;
 #pragma unroll
                     for (int dt = 0; dt < kTiles; ++dt)
 #pragma unroll
-                        for (int q4 = 0; q4 < 4; ++q4) {
-                            const half4_t v =
-                                *reinterpret_cast<const half4_t*>(vs + key * kVRow + 32 * dt + 8 * q4 + 4 * h);
-#pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                o[dt][4 * q4 + i] += seen && !(fabsf((float)v[i]) < INFINITY) ? prob * (float)v[i] : 0.0f;
+                        for (int e = 0; e < 16; ++e) {
+                            const int at = 32 * dt + 8 * (e >> 2) + 4 * h + (e & 3);
+                            float v;
+                            if constexpr (E4M3) v = (row[at] & 0x7f) == 0x7f ? NAN : 0.0f;
+                            else v = (float)reinterpret_cast<const _Float16*>(row)[at];
+                            o[dt][e] += sees && !(fabsf(v) < INFINITY) ? v : 0.0f;
                         }
                 }
             }
         }
         l += lane_xor_f32<32>(l);
-        __syncthreads();  // (the next unit's tiles, and the columns on their way out, go where the last tile was)
-        if (!active) continue;
-        if (tile0 == 0 && tile1 == u.tiles) {
-            const int tok0 = c0 / p.g;
-            attn_packed_write<T, D>(p.out + (int64_t)(u.row0 + tok0) * p.out_stride,
-                                    (unsigned)(tok - tok0) * (unsigned)p.out_stride + (unsigned)(head * D), cols - c0,
-                                    lds + wave * 16 * (D + 8), o, l);
+        __syncthreads();  // (the next unit's tiles, and the columns on their way out, go where the last tiles were)
+        const bool all = tile0 == 0 && tile1 == u.tiles;
+        // a part of a unit: slot 1 of the workgroup holds the end of one, slot 0 everything else
+        const TreeCold t = tree_cold();
+        float* const slot = t->ws + ((int64_t)(2 * blockIdx.x + (tile1 == u.tiles ? 1 : 0)) * t->slot_waves + wave) *
+                                        tree_wave_floats(D);
+        if constexpr (PARTS == 1) {
+            if (!active) continue;
+            if (all) {
+                const int tok0 = c0 / t->g;
+                const Column c = column();
+                static_assert(COLW * 16 * (D + 8) <= kRings, "the columns on their way out fit");
+                attn_packed_write<T, D>(t->out + (int64_t)(u.row0 + tok0) * t->out_stride,
+                                        (unsigned)(c.tok - tok0) * (unsigned)t->out_stride + (unsigned)(c.head * D), cols - c0,
+                                        lds + wave * 16 * (D + 8), o, l);
+            } else {
+#pragma unroll
+                for (int dt = 0; dt < kTiles; ++dt)
+#pragma unroll
+                    for (int q4 = 0; q4 < 4; ++q4)
+                        reinterpret_cast<float4_t*>(slot)[(4 * dt + q4) * 64 + lane] =
+                            float4_t{o[dt][4 * q4], o[dt][4 * q4 + 1], o[dt][4 * q4 + 2], o[dt][4 * q4 + 3]};
+                slot[32 * D + lane] = m;
+                slot[32 * D + 64 + lane] = l;
+            }
         } else {
-            // a part: slot 1 of the workgroup holds the end of a unit, slot 0 everything else
-            float* const slot = p.ws + ((int64_t)(2 * blockIdx.x + (tile1 == u.tiles ? 1 : 0)) * p.slot_waves + wave) *
-                                           tree_wave_floats(D);
+            // the parts through LDS; of a wave's 32 columns each part then joins every PARTS-th 32 elements
+            static_assert(COLW * PARTS * tree_wave_floats(D) * 4 <= 2 * PARTS * kRings, "the parts' results fit");
+            float* const mine = reinterpret_cast<float*>(lds) + (wave * PARTS + part) * tree_wave_floats(D);
 #pragma unroll
             for (int dt = 0; dt < kTiles; ++dt)
 #pragma unroll
                 for (int q4 = 0; q4 < 4; ++q4)
-                    reinterpret_cast<float4_t*>(slot)[(4 * dt + q4) * 64 + lane] =
+                    reinterpret_cast<float4_t*>(mine)[(4 * dt + q4) * 64 + lane] =
                         float4_t{o[dt][4 * q4], o[dt][4 * q4 + 1], o[dt][4 * q4 + 2], o[dt][4 * q4 + 3]};
-            slot[32 * D + lane] = m;
-            slot[32 * D + 64 + lane] = l;
+            mine[32 * D + lane] = m;
+            mine[32 * D + 64 + lane] = l;
+            __syncthreads();
+            if (active) {
+                const float* const parts = reinterpret_cast<const float*>(lds) + wave * PARTS * tree_wave_floats(D);
+                float weight[PARTS], top = -INFINITY, sum = 0.0f;
+#pragma unroll
+                for (int q = 0; q < PARTS; ++q) {
+                    weight[q] = parts[q * tree_wave_floats(D) + 32 * D + lane];
+                    top = fmaxf(top, weight[q]);
+                }
+#pragma unroll
+                for (int q = 0; q < PARTS; ++q) {
+                    weight[q] = fast_exp2(weight[q] - (top == -INFINITY ? 0.0f : top));
+                    sum += parts[q * tree_wave_floats(D) + 32 * D + 64 + lane] * weight[q];
+                }
+                const float inv = sum > 0.0f ? 1.0f / sum : sum == sum ? 0.0f : sum;
+                const Column c = column();
+                unsigned short* const out =
+                    t->out + (int64_t)(u.row0 + c.tok) * t->out_stride + (int64_t)c.head * D + 4 * h;
+                for (int dt = part; dt < kTiles; dt += PARTS)
+#pragma unroll
+                    for (int q4 = 0; q4 < 4; ++q4) {
+                        float4_t v = {0, 0, 0, 0};
+#pragma unroll
+                        for (int q = 0; q < PARTS; ++q) {
+                            const float4_t w = reinterpret_cast<const float4_t*>(parts + q * tree_wave_floats(D))[(4 * dt + q4) * 64 + lane];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) v[e] += w[e] * weight[q];
+                        }
+                        if (!all) reinterpret_cast<float4_t*>(slot)[(4 * dt + q4) * 64 + lane] = v;
+                        else if (c0 + col < cols)
+                            *reinterpret_cast<uint2_t*>(out + 32 * dt + 8 * q4) =
+                                uint2_t{T::pack2(v[0] * inv, v[1] * inv), T::pack2(v[2] * inv, v[3] * inv)};
+                    }
+                if (!all && part == 0) {
+                    slot[32 * D + lane] = top;
+                    slot[32 * D + 64 + lane] = sum;
+                }
+            }
+            __syncthreads();
         }
     }
 }
@@ -432,10 +745,10 @@ __global__ __launch_bounds__(256) void paged_attn_tree_merge_kernel(const TreePa
     const int of_unit = blockIdx.x / kTiles % p.slot_waves;  // which 32 columns of a unit
     int unit = blockIdx.x / kTiles / p.slot_waves;           // of all units
     unsigned total = 0;
-    for (int first = 0; first < p.num_seqs; first += 64) total = tree_chunk<kCols>(p, first, total).end;
+    for (int first = 0; first < p.num_seqs; first += 64) total = tree_chunk<kCols>(first, total).end;
     const unsigned per = tree_share(total, p.workers);
     // the sequence of the unit: units are counted as tiles are
-    TreeChunk c = tree_chunk<kCols>(p, 0, 0);
+    TreeChunk c = tree_chunk<kCols>(0, 0);
     int seq_lane = 0;
     for (;;) {
         unsigned units = (unsigned)c.units;
@@ -452,7 +765,7 @@ __global__ __launch_bounds__(256) void paged_attn_tree_merge_kernel(const TreePa
         }
         unit -= (int)all;
         if (c.first + 64 >= p.num_seqs) return;
-        c = tree_chunk<kCols>(p, c.first + 64, c.end);
+        c = tree_chunk<kCols>(c.first + 64, c.end);
     }
     const unsigned tiles = (unsigned)__builtin_amdgcn_readlane(c.tiles, seq_lane);
     const unsigned pos = (unsigned)__builtin_amdgcn_readlane((int)c.before, seq_lane) + (unsigned)unit * tiles;
@@ -509,30 +822,40 @@ __global__ __launch_bounds__(256) void paged_attn_tree_merge_kernel(const TreePa
             uint2_t{T::pack2(o[q4][0] * inv, o[q4][1] * inv), T::pack2(o[q4][2] * inv, o[q4][3] * inv)};
 }
 
-// Waves of a workgroup.
-static int tree_waves(int) { return 4; }
-
 static int tree_slot_waves(int max_q, int g, int waves) {
     const int64_t need = ((int64_t)max_q * g + 31) / 32;
     return need < waves ? (int)need : waves;
 }
 
-template <typename T, int D, bool E4M3>
-static hipError_t tree_launch(TreeParams p, hipStream_t stream) {
-    constexpr int WAVES = 4;
-    p.slot_waves = tree_slot_waves(p.max_q, p.g, WAVES);
-    const int64_t most = packed_tiles(p.total, p.num_seqs, p.g, 32 * WAVES) * p.hkv;  // units
+template <typename T, int D, int COLW, int PARTS, bool E4M3>
+static hipError_t tree_launch_as(TreeParams p, hipStream_t stream) {
+    p.slot_waves = tree_slot_waves(p.max_q, p.g, COLW);
+    p.step_blocks = kTreeKeys * PARTS / p.block_size;
+    p.step_rows = kTreeKeys * PARTS % p.block_size;
+    const int64_t most = packed_tiles(p.total, p.num_seqs, p.g, 32 * COLW) * p.hkv;  // units
     const int64_t room = (int64_t)p.block_size * p.max_blocks;
     const int64_t tiles = most * ((room + kTreeKeys - 1) / kTreeKeys);
-    int64_t workers = 2 * device_cu_count();
-    if (workers > kTreeWorkers) workers = kTreeWorkers;
+    int64_t workers = tree_blocks(D, COLW, PARTS) * device_cu_count();
+    if (workers > kTreeWorkers * 4 / (COLW > 4 ? COLW : 4)) workers = kTreeWorkers * 4 / (COLW > 4 ? COLW : 4);
     if (workers > (tiles + kTreeLeast - 1) / kTreeLeast) workers = (tiles + kTreeLeast - 1) / kTreeLeast;
     p.workers = (int)workers;
-    paged_attn_tree_kernel<T, D, WAVES, E4M3><<<(unsigned)workers, 64 * WAVES, 0, stream>>>(p);
+    paged_attn_tree_kernel<T, D, COLW, PARTS, E4M3><<<(unsigned)workers, 64 * COLW * PARTS, 0, stream>>>(p);
     hipError_t rc = hipGetLastError();
     if (rc != hipSuccess || workers == 1) return rc;
-    paged_attn_tree_merge_kernel<T, D, WAVES><<<(unsigned)(most * p.slot_waves * (D / 32)), 256, 0, stream>>>(p);
+    paged_attn_tree_merge_kernel<T, D, COLW><<<(unsigned)(most * p.slot_waves * (D / 32)), 256, 0, stream>>>(p);
     return hipGetLastError();
+}
+
+template <typename T, int D, bool E4M3>
+static hipError_t tree_launch(const TreeParams& p, hipStream_t stream) {
+    const int64_t cols = (int64_t)p.max_q * p.g;  // of the longest tree
+    if constexpr (D <= 128) {
+        if (cols <= 32) return tree_launch_as<T, D, 1, 4, E4M3>(p, stream);
+        if (cols <= 64) return tree_launch_as<T, D, 2, 2, E4M3>(p, stream);
+    }
+    if constexpr (D == 64 || D == 128)
+        if (cols > 128) return tree_launch_as<T, D, 8, 1, E4M3>(p, stream);
+    return tree_launch_as<T, D, 4, 1, E4M3>(p, stream);
 }
 
 template <typename T, bool E4M3>
@@ -631,7 +954,7 @@ size_t logismos_paged_attn_tree_workspace_bytes(int total_tokens, int max_seqlen
     if (total_tokens <= 0 || max_seqlen_q <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0) return 0;
     if (max_seqlen_q > total_tokens || num_q_heads % num_kv_heads != 0 || head_dim > 256) return 0;
     const int g = num_q_heads / num_kv_heads;
-    const int waves = lg::tree_slot_waves(max_seqlen_q, g, 4);
+    const int waves = lg::tree_slot_waves(max_seqlen_q, g, 4);  // (eight: half as many workgroups)
     return (size_t)2 * lg::kTreeWorkers * (size_t)waves * (size_t)lg::tree_wave_floats(head_dim) * sizeof(float);
 }
 
