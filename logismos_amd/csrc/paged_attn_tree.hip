@@ -132,12 +132,21 @@ __device__ __forceinline__ unsigned tree_share(unsigned total, int workers) {
 constexpr int tree_wave_floats(int d) { return 32 * d + 128; }
 
 // Probabilities are relative to a reference that follows the maximum lazily, as in attn_packed.hip: the largest lies between
-// 2^kTreeHead and 2^(kTreeHead + kTreeLazy), so that those down to 2^-25 of a column's largest keep all bits of fp16.
+// 2^kTreeHead and 2^(kTreeHead + kTreeLazy), so that those down to 2^-25 of a column's largest keep all bits of fp16.  It is the
+// exponent of a probability, a score in units of log 2, and of a tile's rows of V together, and kept as the two: in one number the second
+// would be rounded to steps of the first.
 constexpr float kTreeHead = 11.0f, kTreeLazy = 4.0f;
+struct TreeRef {
+    float x, v;
+};
+__device__ __forceinline__ float tree_above(TreeRef a, TreeRef b) { return (a.x - b.x) + (a.v - b.v); }
+// exp2 of how far one of two references is below `top`, nothing where it is none.
+__device__ __forceinline__ float tree_weight(TreeRef a, TreeRef top) {
+    return fast_exp2(top.x == -INFINITY ? -INFINITY : tree_above(a, top));
+}
 
-// Scores beyond this (in units of log 2) are multiplied and subtracted in two roundings, the same for the maximum, and their
-// probabilities start at 1: a fused difference is off by up to half a step of the maximum, which is a factor of all of them as long as it
-// is small.
+// Scores beyond this (in units of log 2) go through once more, multiplied and subtracted in two roundings, the same for the maximum: a
+// fused difference is off by up to half a step of the maximum, which is a factor of all probabilities as long as it is small.
 constexpr float kTreeFar = 1048576.0f;
 
 // Elements of the rings of a part, and workgroups that a compute unit holds (by LDS, and two waves to a SIMD by registers).
@@ -227,18 +236,23 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
             for (int j = 0; j < kSteps; ++j) qb[j] = *reinterpret_cast<const uint4_t*>(q + 16 * j);
         }
 
-        // ---- where the tiles of this part lie: the table 64 entries at a time, one to a lane, and the next ones on their way
-        const int32_t* const table = p.tables + (int64_t)u.seq * p.max_blocks;
-        const int in_table = (u.ctx + p.block_size - 1) / p.block_size;
-        auto entries = [&](int first) LG_INLINE { return first + lane < in_table ? table[first + lane] : -1; };
-        int at_tile, at_block, at_row, base, ids, ids_next;
+        // ---- where the tiles of this part lie
+        // (table entries through scalar loads, a tile ahead of their use: everything else that is asked for in the loop is asked for in every
+        // step, whether there is such a tile or not -- behind a load that may have been skipped, a wait is one for all loads in flight)
+        typedef const int32_t __attribute__((address_space(4)))* ScalarTable;
+        const ScalarTable table = (ScalarTable)(uintptr_t)(p.tables + (int64_t)u.seq * p.max_blocks);
+        const int last_entry = (u.ctx + p.block_size - 1) / p.block_size - 1;
+        int at_tile, at_block, at_row, ids[2];
+        auto entries = [&] LG_INLINE {  // of the tile that comes next
+            const int second = at_row + 16 < p.block_size ? at_block : at_block + 1;
+            ids[0] = table[min(at_block, last_entry)];
+            ids[1] = table[min(second, last_entry)];
+        };
         auto start = [&](int which) LG_INLINE {
             at_tile = tile0 + which;
             at_block = at_tile * kTreeKeys / p.block_size;
             at_row = at_tile * kTreeKeys - at_block * p.block_size;
-            base = at_block;
-            ids = entries(base);
-            ids_next = entries(base + 32);
+            entries();
         };
         // A tile: the rows of the pools where its halves begin, -1: not there.
         struct Place {
@@ -248,24 +262,13 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
         int64_t exps_at[2];
         auto walk = [&] LG_INLINE {
             Place w;
-            const bool exists = at_tile < tile1;
-            if (at_block - base >= 48) {
-                base += 32;
-                ids = ids_next;
-                ids_next = entries(base + 32);
-            }
-            int block = at_block, row = at_row;
+            const int key0 = at_tile * kTreeKeys;
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const int id = exists ? __builtin_amdgcn_readlane(ids, (block - base) & 63) : -1;
-                const bool ok = id >= 0 && id < p.num_blocks;
-                w.row[i] = ok ? id * p.block_size + row : -1;
-                if constexpr (E4M3) exps_at[i] = ok ? ((int64_t)id * p.hkv + u.head) * p.block_size + row : 0;
-                row += 16;
-                if (row >= p.block_size) {
-                    row = 0;
-                    ++block;
-                }
+                const bool ok = at_tile < tile1 && key0 + 16 * i < u.ctx && ids[i] >= 0 && ids[i] < p.num_blocks;
+                const int row = i == 0 ? at_row : at_row + 16 < p.block_size ? at_row + 16 : 0;
+                w.row[i] = ok ? ids[i] * p.block_size + row : -1;
+                if constexpr (E4M3) exps_at[i] = ok ? ((int64_t)ids[i] * p.hkv + u.head) * p.block_size + row : 0;
             }
             at_tile += PARTS;
             at_block += p.step_blocks;
@@ -274,6 +277,7 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
                 at_row -= p.block_size;
                 ++at_block;
             }
+            entries();
             return w;
         };
         auto is_there = [](const Place& w) LG_INLINE { return (w.row[0] & w.row[1]) >= 0; };   // one half at least
@@ -295,7 +299,8 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
         const int wave_key = __builtin_amdgcn_readfirstlane(mover / (D / 8)) & ~15;  // (kEven: of which 16 keys piece 0 is)
         const unsigned even_at = ((unsigned)key_of(0) & 15u) * row_bytes + (unsigned)(kPiece * piece_of(0));
         auto load = [&](const uint8_t* pool, const Place& w, int key0, uint4_t* x) LG_INLINE {
-            const int left = u.ctx - key0;  // keys behind the last one, and in a half that is not there: others that are
+            // keys behind the last one, and in a half that is not there: others that are
+            const int left = is_there(w) ? u.ctx - key0 : kTreeKeys;
             const uint8_t* const half0 = pool + (int64_t)max(w.row[0], 0) * row_bytes + u.head * kRow;
             const uint8_t* const half1 = pool + (int64_t)max(w.row[1], 0) * row_bytes + u.head * kRow;
             auto take = [&](int i, const uint8_t* src) LG_INLINE {
@@ -324,8 +329,8 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
             }
         };
         const uint8_t* const exps = E4M3 ? (h ? p.v_exp : p.k_exp) : nullptr;
-        auto load_exps = [&](int key0) LG_INLINE {  // of the tile that walk() came to last
-            const int left = u.ctx - key0, key = col < left ? col : left - 1;
+        auto load_exps = [&](const Place& w, int key0) LG_INLINE {  // of the tile that walk() came to last
+            const int left = is_there(w) ? u.ctx - key0 : kTreeKeys, key = col < left ? col : left - 1;
             return (int)exps[(key < 16 ? exps_at[0] : exps_at[1]) + (key & 15)];
         };
         // The largest exponents of a tile's rows of K and V.
@@ -426,26 +431,48 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
             return win;
         };
 
-        float m, l;
+        // What the probabilities and sums of a column are relative to, as two numbers, of a score and of a tile of V (see TreeRef).
+        TreeRef m;
+        float l;
         float16_t o[kTiles];
         uint4_t p_prev[2];
         float16_t s_cur;
 
         // Tile i with S(i) in s_cur, K(i + 1) in K buffer 1 - H and V(i - 1) in V buffer 1 - H; leaves S(i + 1) and P(i).
-        auto step = [&](auto h_c, const Place& w, int key0, const Tops& top, bool careful) LG_INLINE {
+        auto step = [&](auto h_c, const Place& w, int key0, const Tops& top, auto careful_c) LG_INLINE {
             constexpr int H = decltype(h_c)::value;
+            constexpr bool careful = decltype(careful_c)::value != 0;
             float scale = E4M3 ? ldexpf(p.scale_log2e, top.k) : p.scale_log2e;
-            float v_top = E4M3 ? (float)top.v : 0.0f;
+            const float v_top = E4M3 ? (float)top.v : 0.0f;
             if (!is_whole(w) || key0 + kTreeKeys > u.prior) {
                 const unsigned win = window(w, key0) >> (4 * h);
 #pragma unroll
                 for (int e = 0; e < 16; ++e) s_cur[e] = (win >> (8 * (e >> 2) + (e & 3))) & 1u ? s_cur[e] : -INFINITY;
             }
-            if (__builtin_expect(careful, 0)) {
+            bool raise = false;
+            float drop = 0.0f;  // what raising the reference takes off the exponents so far
+            float ref = m.x;
+            auto follow = [&](float tm) LG_INLINE {
+                raise = tree_above({tm, v_top}, m) > kTreeLazy;
+                drop = tree_above(m, {tm, v_top});
+                m.x = raise ? tm : m.x;
+                if (E4M3) m.v = raise ? v_top : m.v;
+                ref = m.x == -INFINITY ? 0.0f : m.x;
+            };
+            if constexpr (careful) {
+                float tm = -INFINITY;
 #pragma unroll
-                for (int e = 0; e < 16; ++e) s_cur[e] = __fadd_rn(__fmul_rn(s_cur[e], scale), v_top);
+                for (int e = 0; e < 16; ++e) {
+                    float x = s_cur[e] * scale;
+                    asm volatile("" : "+v"(x));  // (a product of its own, not half of a fused one)
+                    s_cur[e] = x;
+                    tm = fmaxf(tm, x);
+                }
+                follow(fmaxf(tm, lane_xor_f32<32>(tm)));
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s_cur[e] -= ref;
                 scale = 1.0f;
-                v_top = 0.0f;
+                ref = 0.0f;
             }
             uint4_t ka[kSteps], va[kSteps];
             if constexpr (!kWide)
@@ -454,15 +481,12 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
                     ka[j] = k_operand(1 - H, j);
                     va[j] = v_operand(1 - H, j / kTiles, j % kTiles);
                 }
-            float tm = -INFINITY;
+            if constexpr (!careful) {
+                float tm = -INFINITY;
 #pragma unroll
-            for (int e = 0; e < 16; ++e) tm = fmaxf(tm, s_cur[e]);
-            // (exponents of the tile's probabilities and of its rows of V together)
-            tm = __fadd_rn(__fmul_rn(fmaxf(tm, lane_xor_f32<32>(tm)), scale), v_top);
-            tm = fabsf(tm) < kTreeFar ? tm - kTreeHead : tm;
-            const bool raise = tm > m + kTreeLazy;
-            const float m_before = m;
-            m = raise ? tm : m;
+                for (int e = 0; e < 16; ++e) tm = fmaxf(tm, s_cur[e]);
+                follow(fmaxf(tm, lane_xor_f32<32>(tm)) * scale);
+            }
             float16_t s_nxt;
 #pragma unroll
             for (int e = 0; e < 16; ++e) s_nxt[e] = 0.0f;
@@ -478,7 +502,7 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
             }
             float sum = 0.0f;
             uint4_t pb[2];
-            const float off = v_top - (m == -INFINITY ? 0.0f : m);
+            const float off = kTreeHead + (v_top - m.v) - ref;
 #pragma unroll
             for (int e = 0; e < 16; e += 2) {
                 const float p0 = fast_exp2(fmaf(s_cur[e], scale, off));
@@ -501,13 +525,13 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
             // (F belongs to this step: its results are used by the next one only, and would sink there)
             asm volatile("" : "+v"(pb[0]), "+v"(pb[1]), "+v"(sum));
             if (__builtin_expect(__builtin_amdgcn_ballot_w64(raise) != 0, 0)) {  // O(i - 1) was relative to the old one
-                const float alpha = raise ? fast_exp2(m_before - m) : 1.0f;
+                const float alpha = raise ? fast_exp2(drop) : 1.0f;
                 l *= alpha;
 #pragma unroll
                 for (int dt = 0; dt < kTiles; ++dt)
 #pragma unroll
                     for (int e = 0; e < 16; ++e) o[dt][e] *= alpha;
-                if (__builtin_amdgcn_ballot_w64(raise && fabsf(m) >= kTreeFar) != 0 && lane == 0) far_parts[part] = 1;
+                if (__builtin_amdgcn_ballot_w64(raise && fabsf(m.x) >= kTreeFar) != 0 && lane == 0) far_parts[part] = 1;
             }
             l += E4M3 ? ldexpf(sum, -top.v) : sum;
             s_cur = s_nxt;
@@ -515,9 +539,9 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
             p_prev[1] = pb[1];
         };
 
-        // The tiles of the part; `careful`: as if none was seen whole.
-        auto walk_tiles = [&](bool careful) LG_INLINE {
-            m = -INFINITY;
+        // The tiles of the part, for scores of any size with careful_c.
+        auto walk_tiles = [&](auto careful_c) LG_INLINE {
+            m = TreeRef{-INFINITY, 0.0f};
             l = 0.0f;
             p_prev[0] = p_prev[1] = uint4_t{0, 0, 0, 0};
 #pragma unroll
@@ -532,24 +556,27 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
             int e0 = 127, e1 = 127;  // exponents of the rows of tiles i and i + 1
             ra.e = 127;
             auto kregs = [](Regs& r) LG_INLINE { return kAlone ? r.k : r.v; };
+            // SPLIT: a wave's own kind of tile, out of `lead` (K) or `behind` (V)
+            auto ask = [&](const Place& lead, const Place& behind, int lead0, int behind0, Regs& r) LG_INLINE {
+                if constexpr (kAlone) {
+                    load(p.k_pool, lead, lead0, r.k);
+                    load(p.v_pool, behind, behind0, r.v);
+                } else {
+                    const Place w = {{moves_v ? behind.row[0] : lead.row[0], moves_v ? behind.row[1] : lead.row[1]}};
+                    load(moves_v ? p.v_pool : p.k_pool, w, moves_v ? behind0 : lead0, r.v);
+                }
+            };
             {
                 uint4_t x0[kPer];
-                if (is_there(w0)) {
-                    if constexpr (E4M3) e0 = load_exps(key0);
-                    if (moves_k) load(p.k_pool, w0, key0, x0);
-                }
+                if constexpr (E4M3) e0 = load_exps(w0, key0);
+                load(p.k_pool, w0, key0, x0);
                 w1 = walk();
-                if (is_there(w1)) {
-                    if constexpr (E4M3) e1 = load_exps(key0 + kStride);
-                    if (moves_k) load(p.k_pool, w1, key0 + kStride, kregs(rb));
-                }
+                if constexpr (E4M3) e1 = load_exps(w1, key0 + kStride);
+                load(p.k_pool, w1, key0 + kStride, kregs(rb));
                 if constexpr (kDeep == 2) {
                     w2 = walk();
-                    if (is_there(w2)) {
-                        if constexpr (E4M3) ra.e = load_exps(key0 + 2 * kStride);
-                        if (moves_k) load(p.k_pool, w2, key0 + 2 * kStride, kregs(ra));
-                    }
-                    if (moves_v && is_there(w0)) load(p.v_pool, w0, key0, ra.v);
+                    if constexpr (E4M3) ra.e = load_exps(w2, key0 + 2 * kStride);
+                    ask(w2, w0, key0 + 2 * kStride, key0, ra);
                 }
                 if constexpr (E4M3) {
                     t0 = tops_of(e0);
@@ -573,15 +600,10 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
                 constexpr int H = decltype(h_c)::value;
                 Place& lead = kDeep == 2 ? w3 : w2;
                 lead = walk();
-                next.e = 127;
-                if (is_there(lead)) {
-                    if constexpr (E4M3) next.e = load_exps(key0 + (kDeep + 1) * kStride);
-                    if (moves_k) load(p.k_pool, lead, key0 + (kDeep + 1) * kStride, kregs(next));
-                }
-                const Place& behind = kDeep == 2 ? w1 : w0;
-                if (moves_v && is_there(behind)) load(p.v_pool, behind, key0 + (kDeep - 1) * kStride, next.v);
+                if constexpr (E4M3) next.e = load_exps(lead, key0 + (kDeep + 1) * kStride);
+                ask(lead, kDeep == 2 ? w1 : w0, key0 + (kDeep + 1) * kStride, key0 + (kDeep - 1) * kStride, next);
                 __builtin_amdgcn_sched_barrier(0);
-                if (active) step(h_c, w0, key0, t0, careful);
+                if (active) step(h_c, w0, key0, t0, careful_c);
                 __builtin_amdgcn_sched_barrier(0);
                 Regs& then = kDeep == 2 ? now : next;
                 if constexpr (E4M3) t2 = tops_of(then.e);
@@ -613,20 +635,22 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
 
         if (wave_of_all == 0 && lane < PARTS) odd_parts[lane] = far_parts[lane] = 0;
         __syncthreads();
-        m = -INFINITY;
+        m = TreeRef{-INFINITY, 0.0f};
         l = 0.0f;
 #pragma unroll
         for (int dt = 0; dt < kTiles; ++dt)
 #pragma unroll
             for (int e = 0; e < 16; ++e) o[dt][e] = 0.0f;
-        for (int careful = 0; careful < 2 && steps > 0; ++careful) {
-            walk_tiles(careful != 0);
+        if (steps > 0) {
+            walk_tiles(ic<0>{});
             __syncthreads();
             int far = 0;
 #pragma unroll
             for (int q = 0; q < PARTS; ++q) far |= far_parts[q];
-            if (__builtin_expect(__builtin_amdgcn_readfirstlane(far) == 0, 1)) break;
-            __syncthreads();  // (the first tiles go where the last ones were)
+            if (__builtin_expect(__builtin_amdgcn_readfirstlane(far) != 0, 0)) {
+                __syncthreads();  // (the first tiles go where the last ones were)
+                walk_tiles(ic<1>{});
+            }
         }
         if (__builtin_expect(__builtin_amdgcn_readfirstlane(odd_parts[part]) != 0, 0)) {
             start(part);
@@ -676,7 +700,7 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
                     for (int q4 = 0; q4 < 4; ++q4)
                         reinterpret_cast<float4_t*>(slot)[(4 * dt + q4) * 64 + lane] =
                             float4_t{o[dt][4 * q4], o[dt][4 * q4 + 1], o[dt][4 * q4 + 2], o[dt][4 * q4 + 3]};
-                slot[32 * D + lane] = m;
+                slot[32 * D + lane] = h ? m.v : m.x;
                 slot[32 * D + 64 + lane] = l;
             }
         } else {
@@ -689,20 +713,21 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
                 for (int q4 = 0; q4 < 4; ++q4)
                     reinterpret_cast<float4_t*>(mine)[(4 * dt + q4) * 64 + lane] =
                         float4_t{o[dt][4 * q4], o[dt][4 * q4 + 1], o[dt][4 * q4 + 2], o[dt][4 * q4 + 3]};
-            mine[32 * D + lane] = m;
+            mine[32 * D + lane] = h ? m.v : m.x;
             mine[32 * D + 64 + lane] = l;
             __syncthreads();
             if (active) {
                 const float* const parts = reinterpret_cast<const float*>(lds) + wave * PARTS * tree_wave_floats(D);
-                float weight[PARTS], top = -INFINITY, sum = 0.0f;
+                TreeRef refs[PARTS], top = {-INFINITY, 0.0f};
+                float weight[PARTS], sum = 0.0f;
 #pragma unroll
                 for (int q = 0; q < PARTS; ++q) {
-                    weight[q] = parts[q * tree_wave_floats(D) + 32 * D + lane];
-                    top = fmaxf(top, weight[q]);
+                    refs[q] = {parts[q * tree_wave_floats(D) + 32 * D + col], parts[q * tree_wave_floats(D) + 32 * D + 32 + col]};
+                    if (tree_above(refs[q], top) > 0.0f) top = refs[q];
                 }
 #pragma unroll
                 for (int q = 0; q < PARTS; ++q) {
-                    weight[q] = fast_exp2(weight[q] - (top == -INFINITY ? 0.0f : top));
+                    weight[q] = tree_weight(refs[q], top);
                     sum += parts[q * tree_wave_floats(D) + 32 * D + 64 + lane] * weight[q];
                 }
                 const float inv = sum > 0.0f ? 1.0f / sum : sum == sum ? 0.0f : sum;
@@ -725,7 +750,7 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
                                 uint2_t{T::pack2(v[0] * inv, v[1] * inv), T::pack2(v[2] * inv, v[3] * inv)};
                     }
                 if (!all && part == 0) {
-                    slot[32 * D + lane] = top;
+                    slot[32 * D + lane] = h ? top.v : top.x;
                     slot[32 * D + 64 + lane] = sum;
                 }
             }
@@ -734,54 +759,38 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
     }
 }
 
-// The parts of the units that were cut: a workgroup takes 32 columns and 32 elements of the heads, its waves every fourth part.
-template <typename T, int D, int WAVES>
+// The units that were cut: a workgroup takes the first cut of one, 32 of its columns and 32 elements of the heads, its waves every fourth
+// part of the unit, a few of them in flight.
+template <typename T, int D, int COLW>
 __global__ __launch_bounds__(256) void paged_attn_tree_merge_kernel(const TreeParams p) {
-    constexpr int kCols = 32 * WAVES, kTiles = D / 32;
+    constexpr int kCols = 32 * COLW, kTiles = D / 32, kAhead = 4;
     __shared__ float4_t theirs[3][4][64];
-    __shared__ float ml[3][2][64];
+    __shared__ float ml[3][3][64];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int dt = blockIdx.x % kTiles;
-    const int of_unit = blockIdx.x / kTiles % p.slot_waves;  // which 32 columns of a unit
-    int unit = blockIdx.x / kTiles / p.slot_waves;           // of all units
-    unsigned total = 0;
-    for (int first = 0; first < p.num_seqs; first += 64) total = tree_chunk<kCols>(first, total).end;
-    const unsigned per = tree_share(total, p.workers);
-    // the sequence of the unit: units are counted as tiles are
+    const int of_unit = blockIdx.x / kTiles % p.slot_waves;       // which 32 columns of a unit
+    const int cut = (int)(blockIdx.x / kTiles) / p.slot_waves;    // behind the tiles of this workgroup
     TreeChunk c = tree_chunk<kCols>(0, 0);
-    int seq_lane = 0;
-    for (;;) {
-        unsigned units = (unsigned)c.units;
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-            const unsigned other = __shfl_up(units, d);
-            units += lane >= d ? other : 0u;
-        }
-        const unsigned all = (unsigned)__builtin_amdgcn_readlane((int)units, 63);
-        if ((unsigned)unit < all) {
-            seq_lane = __builtin_ctzll(__builtin_amdgcn_ballot_w64(units > (unsigned)unit));
-            unit -= __builtin_amdgcn_readlane((int)units, seq_lane) - __builtin_amdgcn_readlane(c.units, seq_lane);
-            break;
-        }
-        unit -= (int)all;
-        if (c.first + 64 >= p.num_seqs) return;
-        c = tree_chunk<kCols>(c.first + 64, c.end);
-    }
-    const unsigned tiles = (unsigned)__builtin_amdgcn_readlane(c.tiles, seq_lane);
-    const unsigned pos = (unsigned)__builtin_amdgcn_readlane((int)c.before, seq_lane) + (unsigned)unit * tiles;
-    const int first = (int)(pos / per), last = (int)((pos + tiles - 1) / per);
-    if (first == last) return;
+    unsigned total = c.end;
+    for (int first = 64; first < p.num_seqs; first += 64) total = tree_chunk<kCols>(first, total).end;
+    const unsigned per = tree_share(total, p.workers);
+    const unsigned pos = (unsigned)(cut + 1) * per;
+    if (pos >= total) return;
+    while (pos >= c.end) c = tree_chunk<kCols>(c.first + 64, c.end);
     const TreeUnit u = tree_unit(c, p.hkv, pos);
+    const unsigned begin = pos - (unsigned)u.tile;
+    const int first = (int)(begin / per), last = (int)((begin + (unsigned)u.tiles - 1) / per);
     const int cols = u.rows * p.g, c0 = u.group * kCols + of_unit * 32;
-    if (c0 >= cols) return;
+    if (u.tile == 0 || first != cut || c0 >= cols) return;
 
-    float m = -INFINITY, l = 0.0f;
+    TreeRef m = {-INFINITY, 0.0f};
+    float l = 0.0f;
     float4_t o[4];
 #pragma unroll
     for (int q4 = 0; q4 < 4; ++q4) o[q4] = float4_t{0, 0, 0, 0};
-    auto join = [&](float m2, float l2, const float4_t* o2) LG_INLINE {
-        const float top = fmaxf(m, m2), ref = top == -INFINITY ? 0.0f : top;
-        const float mine = fast_exp2(m - ref), its = fast_exp2(m2 - ref);
+    auto join = [&](TreeRef m2, float l2, const float4_t* o2) LG_INLINE {
+        const TreeRef top = tree_above(m2, m) > 0.0f ? m2 : m;
+        const float mine = tree_weight(m, top), its = tree_weight(m2, top);
         m = top;
         l = l * mine + l2 * its;
 #pragma unroll
@@ -789,19 +798,30 @@ __global__ __launch_bounds__(256) void paged_attn_tree_merge_kernel(const TreePa
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[q4][e] = o[q4][e] * mine + o2[q4][e] * its;
     };
-    for (int w = first + wave; w <= last; w += 4) {
-        const float* slot =
-            p.ws + ((int64_t)(2 * w + (w == last ? 1 : 0)) * p.slot_waves + of_unit) * tree_wave_floats(D);
-        float4_t o2[4];
+    for (int w0 = first + wave; w0 <= last; w0 += 4 * kAhead) {
+        float4_t o2[kAhead][4];
+        TreeRef m2[kAhead];
+        float l2[kAhead];
 #pragma unroll
-        for (int q4 = 0; q4 < 4; ++q4) o2[q4] = reinterpret_cast<const float4_t*>(slot)[(4 * dt + q4) * 64 + lane];
-        join(slot[32 * D + lane], slot[32 * D + 64 + lane], o2);
+        for (int a = 0; a < kAhead; ++a) {
+            const int w = w0 + 4 * a <= last ? w0 + 4 * a : w0;
+            const float* slot =
+                p.ws + ((int64_t)(2 * w + (w == last ? 1 : 0)) * p.slot_waves + of_unit) * tree_wave_floats(D);
+            m2[a] = {slot[32 * D + (lane & 31)], slot[32 * D + 32 + (lane & 31)]};
+            l2[a] = slot[32 * D + 64 + lane];
+#pragma unroll
+            for (int q4 = 0; q4 < 4; ++q4) o2[a][q4] = reinterpret_cast<const float4_t*>(slot)[(4 * dt + q4) * 64 + lane];
+        }
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a)
+            if (w0 + 4 * a <= last) join(m2[a], l2[a], o2[a]);
     }
     if (wave > 0) {
 #pragma unroll
         for (int q4 = 0; q4 < 4; ++q4) theirs[wave - 1][q4][lane] = o[q4];
-        ml[wave - 1][0][lane] = m;
-        ml[wave - 1][1][lane] = l;
+        ml[wave - 1][0][lane] = m.x;
+        ml[wave - 1][1][lane] = m.v;
+        ml[wave - 1][2][lane] = l;
     }
     __syncthreads();
     if (wave > 0) return;
@@ -809,7 +829,7 @@ __global__ __launch_bounds__(256) void paged_attn_tree_merge_kernel(const TreePa
         float4_t o2[4];
 #pragma unroll
         for (int q4 = 0; q4 < 4; ++q4) o2[q4] = theirs[w][q4][lane];
-        join(ml[w][0][lane], ml[w][1][lane], o2);
+        join({ml[w][0][lane], ml[w][1][lane]}, ml[w][2][lane], o2);
     }
     const int h = lane >> 5, gc = c0 + (lane & 31);
     if (gc >= cols) return;
@@ -842,7 +862,7 @@ static hipError_t tree_launch_as(TreeParams p, hipStream_t stream) {
     paged_attn_tree_kernel<T, D, COLW, PARTS, E4M3><<<(unsigned)workers, 64 * COLW * PARTS, 0, stream>>>(p);
     hipError_t rc = hipGetLastError();
     if (rc != hipSuccess || workers == 1) return rc;
-    paged_attn_tree_merge_kernel<T, D, COLW><<<(unsigned)(most * p.slot_waves * (D / 32)), 256, 0, stream>>>(p);
+    paged_attn_tree_merge_kernel<T, D, COLW><<<(unsigned)((workers - 1) * p.slot_waves * (D / 32)), 256, 0, stream>>>(p);
     return hipGetLastError();
 }
 

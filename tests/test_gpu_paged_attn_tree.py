@@ -272,6 +272,30 @@ def test_scales(scale, pool, dtype):
     Case(15, [10, 3], [400, 40], 6, 2, 64, pool, dtype, scale=scale).check()
 
 
+@pytest.mark.parametrize("pool,dtype", KINDS)
+@pytest.mark.parametrize("shift", [10, 19, 20, 21, 23, 24, 26, 27, 28, 29, 40, 100])
+def test_scores_far_apart(shift, pool, dtype):
+    """Whole numbers as scores, times 2^shift: the keys with the largest share all the weight."""
+    c = Case(30 + shift, [9, 40], [300, 70], 6, 2, 64, pool, dtype, scale=2.0 ** shift)
+    rng = np.random.default_rng(31)
+    c.q = P.to_bits(rng.integers(-1, 2, c.q.shape), dtype)
+    c.set_rows(rng.integers(-1, 2, c.k16.shape).astype(np.float16), c.v16)
+    out = c.run()
+    for s in range(2):
+        (k, _), (v, ve) = c.values(s)
+        q = P.from_bits(c.q[c.cu[s]:c.cu[s + 1]], dtype).reshape(-1, c.hq, c.d)
+        got = P.from_bits(out[c.cu[s]:c.cu[s + 1]], dtype).reshape(q.shape)
+        seen = c.visible(s)
+        for h in range(c.hq):
+            score = np.where(seen, q[:, h] @ k[:, h // 3].T, -np.inf)
+            w = (score == score.max(1, keepdims=True)).astype(float)
+            w /= w.sum(1, keepdims=True)
+            want, size = w @ v[:, h // 3], w @ np.abs(v[:, h // 3])
+            # equal weights, off by half a step of fp16 and by fp32 sums; of neighbours' rows of V 2^-25 of the largest step
+            bound = (2.0 ** -11 + 2.0 ** -16) * size + 2.0 ** -24 * np.abs(v).max() + P.HALF_STEP[dtype] * np.abs(want) + 2.0 ** -25
+            P.assert_within(got[:, h], want, bound)
+
+
 @pytest.mark.parametrize("dtype", ["fp16", "bf16"])
 def test_small_exponents(dtype):
     """Rows near the lowest numbers of fp16 beside ordinary ones, one of them with all the weight."""
