@@ -46,7 +46,7 @@ struct TreeParams {
     int64_t q_stride, out_stride;
     float scale_log2e;
     int workers;
-    int step_blocks, step_rows;  // what lies between two tiles of a part: whole blocks and rows
+    int by_unit;     // the second launch has a workgroup for every unit, not for every cut
     int slot_waves;  // waves that a slot of the workspace has room for
 };
 
@@ -102,6 +102,7 @@ __device__ __forceinline__ TreeChunk tree_chunk(int first, unsigned before) {
 // A unit and which of its tiles: everything the same in the whole wave.
 struct TreeUnit {
     int seq, row0, rows, ctx, prior, head, group, tile, tiles;
+    unsigned at;  // the tile, counted over all units
 };
 __device__ __forceinline__ TreeUnit tree_unit(const TreeChunk& c, int hkv, unsigned pos) {
     const uint64_t behind = __builtin_amdgcn_ballot_w64(c.behind > pos);
@@ -109,6 +110,7 @@ __device__ __forceinline__ TreeUnit tree_unit(const TreeChunk& c, int hkv, unsig
     auto of = [&](int v) LG_INLINE { return __builtin_amdgcn_readlane(v, l); };
     TreeUnit u;
     u.seq = c.first + l;
+    u.at = pos;
     u.row0 = of(c.row0);
     u.rows = of(c.rows);
     u.ctx = of(c.ctx);
@@ -170,12 +172,17 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
     constexpr int kRow = E4M3 ? D : 2 * D;             // bytes of a head row
     constexpr int kRings = tree_rings(D);
     static_assert(kRings == 2 * kKTile + 2 * kVTile, "two tiles each");
+    constexpr int kTab = E4M3 && PARTS * D > 256 ? 128 : 256;  // tiles whose places are in LDS at a time
+    constexpr int kPlaces = kTab + 4 * PARTS;                  // ... with those that a step may ask for behind the last
     constexpr bool kWide = D > 128;  // four operands of K and V at a time: there are no registers for more
     // Steps between asking for a tile and storing it: two, one where a wave alone has no registers for more.
     constexpr int kDeep = (kAlone && !E4M3 && D > 64) || kWide ? 1 : 2;
     constexpr bool kAsIs = E4M3 && __is_same(T, PackedBf16);  // K in bf16, whose range is that of the cache
     static_assert(kPer * kMovers * 8 == kTreeKeys * D, "whole pieces");
     __shared__ __attribute__((aligned(16))) unsigned short lds[PARTS * kRings];
+    __shared__ __attribute__((aligned(16))) int rows_lds[2 * kPlaces];
+    __shared__ __attribute__((aligned(16))) uint8_t exps_lds[E4M3 ? 64 * kPlaces : 16];
+    __shared__ __attribute__((aligned(16))) unsigned short tops_lds[E4M3 ? 2 * kPlaces : 8];
     __shared__ int odd_parts[PARTS], far_parts[PARTS];
     const int wave_of_all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int part = wave_of_all / COLW, wave = wave_of_all - part * COLW;
@@ -210,7 +217,6 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
         const int tile0 = u.tile;
         const int tile1 = (unsigned)(u.tiles - tile0) < end - pos ? u.tiles : tile0 + (int)(end - pos);
         pos += (unsigned)(tile1 - tile0);
-        const int steps = u.ctx > 0 ? (tile1 - tile0 + PARTS - 1) / PARTS : 0;  // of every part
 
         const int cols = u.rows * tree_cold()->g;
         const int c0 = u.group * kCols + wave * 32;
@@ -236,56 +242,71 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
             for (int j = 0; j < kSteps; ++j) qb[j] = *reinterpret_cast<const uint4_t*>(q + 16 * j);
         }
 
-        // ---- where the tiles of this part lie
-        // (table entries through scalar loads, a tile ahead of their use: everything else that is asked for in the loop is asked for in every
-        // step, whether there is such a tile or not -- behind a load that may have been skipped, a wait is one for all loads in flight)
-        typedef const int32_t __attribute__((address_space(4)))* ScalarTable;
-        const ScalarTable table = (ScalarTable)(uintptr_t)(p.tables + (int64_t)u.seq * p.max_blocks);
-        const int last_entry = (u.ctx + p.block_size - 1) / p.block_size - 1;
-        int at_tile, at_block, at_row, ids[2];
-        auto entries = [&] LG_INLINE {  // of the tile that comes next
-            const int second = at_row + 16 < p.block_size ? at_block : at_block + 1;
-            ids[0] = table[min(at_block, last_entry)];
-            ids[1] = table[min(second, last_entry)];
-        };
-        auto start = [&](int which) LG_INLINE {
-            at_tile = tile0 + which;
-            at_block = at_tile * kTreeKeys / p.block_size;
-            at_row = at_tile * kTreeKeys - at_block * p.block_size;
-            entries();
-        };
-        // A tile: the rows of the pools where its halves begin, -1: not there.
+        // ---- where the tiles lie: for kTab of them at a time in LDS, worked out by all threads together
         struct Place {
-            int row[2];
+            int row[2];  // of the pools, at which the halves begin; -1: there is none, or the table's entry names no block
         };
-        // ... and, of e4m3 pools, where the exponents of the halves begin, in a pool.
-        int64_t exps_at[2];
-        auto walk = [&] LG_INLINE {
-            Place w;
-            const int key0 = at_tile * kTreeKeys;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const bool ok = at_tile < tile1 && key0 + 16 * i < u.ctx && ids[i] >= 0 && ids[i] < p.num_blocks;
-                const int row = i == 0 ? at_row : at_row + 16 < p.block_size ? at_row + 16 : 0;
-                w.row[i] = ok ? ids[i] * p.block_size + row : -1;
-                if constexpr (E4M3) exps_at[i] = ok ? ((int64_t)ids[i] * p.hkv + u.head) * p.block_size + row : 0;
-            }
-            at_tile += PARTS;
-            at_block += p.step_blocks;
-            at_row += p.step_rows;
-            if (at_row >= p.block_size) {
-                at_row -= p.block_size;
-                ++at_block;
-            }
-            entries();
-            return w;
-        };
-        auto is_there = [](const Place& w) LG_INLINE { return (w.row[0] & w.row[1]) >= 0; };   // one half at least
+        auto is_there = [](const Place& w) LG_INLINE { return (w.row[0] & w.row[1]) >= 0; };  // one half at least
         auto is_whole = [](const Place& w) LG_INLINE { return (w.row[0] | w.row[1]) >= 0; };
+        auto row_of = [&](int key, int& block, int& off) LG_INLINE {
+            const TreeCold t = tree_cold();
+            const int entry = key / t->block_size;
+            off = key - entry * t->block_size;
+            block = -1;
+            if (key < u.ctx) block = t->tables[(int64_t)u.seq * t->max_blocks + entry];
+            return block >= 0 && block < t->num_blocks ? block * t->block_size + off : -1;
+        };
+        auto fill = [&](int from, int count, int steps) LG_INLINE {
+            for (int i = threadIdx.x; i < 2 * (steps + 4) * PARTS; i += 64 * COLW * PARTS) {
+                const int key = i < 2 * count ? from * kTreeKeys + 16 * i : u.ctx;
+                int block, off;
+                const int row = row_of(key, block, off);
+                rows_lds[i] = row;
+                if constexpr (E4M3) {
+                    // the exponents of the 16 rows of K and of V (of those that there are), and the largest of each
+                    const TreeCold t = tree_cold();
+                    const int64_t at = row < 0 ? 0 : ((int64_t)block * t->hkv + u.head) * t->block_size + off;
+                    const int left = row < 0 ? 0 : u.ctx - key;
+                    unsigned top[2];
+#pragma unroll
+                    for (int kind = 0; kind < 2; ++kind) {
+                        uint4_t e = *reinterpret_cast<const uint4_t*>((kind ? t->v_exp : t->k_exp) + at);
+                        unsigned most = 0;
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) {
+                            const int bytes = left - 4 * w;
+                            e[w] = bytes >= 4 ? e[w] : bytes > 0 ? e[w] & ((1u << (8 * bytes)) - 1u) : 0u;
+                            most = max(max(most, e[w] >> 24), max(e[w] & 0xffu, max((e[w] >> 8) & 0xffu, (e[w] >> 16) & 0xffu)));
+                        }
+                        top[kind] = most;
+                        *reinterpret_cast<uint4_t*>(exps_lds + (i >> 1) * 64 + 32 * kind + 16 * (i & 1)) = e;
+                    }
+                    tops_lds[i] = (unsigned short)(top[0] | top[1] << 8);
+                }
+            }
+        };
+        // Tile i of this part in the table: as it comes, in vector registers, and for the whole wave.
+        auto place = [&](int i) LG_INLINE {
+            return *reinterpret_cast<const uint2_t*>(rows_lds + 2 * (i * PARTS + part));
+        };
+        auto uniform = [](uint2_t v) LG_INLINE {
+            return Place{{__builtin_amdgcn_readfirstlane((int)v[0]), __builtin_amdgcn_readfirstlane((int)v[1])}};
+        };
+        // The largest exponents of a tile's rows of K and V.
+        struct Tops {
+            int k, v;
+        };
+        auto tops_of = [&](int i) LG_INLINE {
+            const unsigned both = __builtin_amdgcn_readfirstlane(*reinterpret_cast<const unsigned*>(tops_lds + 2 * (i * PARTS + part)));
+            Tops t;
+            t.k = max((int)(both & 0xffu), (int)((both >> 16) & 0xffu)) - 127;
+            t.v = max((int)((both >> 8) & 0xffu), (int)(both >> 24)) - 127;
+            if (kAsIs) t.k = 0;
+            return t;
+        };
 
         struct Regs {
-            uint4_t k[kAlone ? kPer : 1], v[kPer];  // (SPLIT: v holds whichever the wave moves)
-            int e;  // exponent of K (lower half of the wave) or V of key lane % 32
+            uint4_t k[kAlone ? kPer : 1], v[kPer];  // (of several waves: v holds whichever a wave moves)
         };
         // Piece i of a mover: of key key_of(i).  Where a round of the movers' pieces is whole keys, it lies kRound keys behind piece
         // i - 1 and one offset serves all; within a wave they are then of the same half of the tile.
@@ -328,26 +349,6 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
                 }
             }
         };
-        const uint8_t* const exps = E4M3 ? (h ? p.v_exp : p.k_exp) : nullptr;
-        auto load_exps = [&](const Place& w, int key0) LG_INLINE {  // of the tile that walk() came to last
-            const int left = is_there(w) ? u.ctx - key0 : kTreeKeys, key = col < left ? col : left - 1;
-            return (int)exps[(key < 16 ? exps_at[0] : exps_at[1]) + (key & 15)];
-        };
-        // The largest exponents of a tile's rows of K and V.
-        struct Tops {
-            int k, v;
-        };
-        auto tops_of = [&](int e) LG_INLINE {
-            e = max(e, dpp_i32<kDppRowRor + 8>(e));
-            e = max(e, dpp_i32<kDppRowRor + 4>(e));
-            e = max(e, dpp_i32<kDppRowRor + 2>(e));
-            e = max(e, dpp_i32<kDppRowRor + 1>(e));
-            Tops t;
-            t.k = max(__builtin_amdgcn_readlane(e, 0), __builtin_amdgcn_readlane(e, 16)) - 127;
-            t.v = max(__builtin_amdgcn_readlane(e, 32), __builtin_amdgcn_readlane(e, 48)) - 127;
-            if (kAsIs) t.k = 0;
-            return t;
-        };
         // A piece of 8 as the kernel wants it: e4m3 rows times 2^(e - top) in 16 bits.
         auto decoded = [&](const uint4_t& x, int e, int top, bool as_bf16) LG_INLINE {
             if constexpr (!E4M3) return x;
@@ -366,23 +367,24 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
             }
             return y;
         };
-        auto store_k = [&](int buf, const uint4_t* x, int e, const Tops& top) LG_INLINE {
+        auto exps_at = [&](int i, int kind) LG_INLINE { return exps_lds + (i * PARTS + part) * 64 + 32 * kind; };
+        auto store_k = [&](int buf, const uint4_t* x, const uint8_t* e, const Tops& top) LG_INLINE {
             unsigned short* const to = ks + buf * kKTile;
 #pragma unroll
             for (int i = 0; i < kPer; ++i) {
-                const int row = E4M3 ? __shfl(e, key_of(i)) : 0;
+                const int row = E4M3 ? e[key_of(i)] : 0;
                 *reinterpret_cast<uint4_t*>(to + key_of(i) * kKRow + 8 * piece_of(i)) = decoded(x[i], row, top.k, kAsIs);
             }
         };
         // A key that a column does not see has the probability 0 there, and 0 times an infinity or NaN of its V row is NaN: in
         // tiles that are not seen whole such elements go in as 0, and are added at the end for the columns that see them.
-        auto store_v = [&](int buf, const uint4_t* x, int e, const Tops& top, const Place& w, int key0) LG_INLINE {
+        auto store_v = [&](int buf, const uint4_t* x, const uint8_t* e, const Tops& top, const Place& w, int key0) LG_INLINE {
             unsigned short* const to = vs + buf * kVTile;
             const bool whole = is_whole(w) && key0 + kTreeKeys <= u.prior;
             bool odd = false;
 #pragma unroll
             for (int i = 0; i < kPer; ++i) {
-                const int row = E4M3 ? __shfl(e, 32 + key_of(i)) : 0;
+                const int row = E4M3 ? e[key_of(i)] : 0;
                 uint4_t y = decoded(x[i], row, top.v, false);
                 if (!whole) {
 #pragma unroll
@@ -543,93 +545,88 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
         auto walk_tiles = [&](auto careful_c) LG_INLINE {
             m = TreeRef{-INFINITY, 0.0f};
             l = 0.0f;
-            p_prev[0] = p_prev[1] = uint4_t{0, 0, 0, 0};
 #pragma unroll
             for (int dt = 0; dt < kTiles; ++dt)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) o[dt][e] = 0.0f;
-            start(part);
-            int key0 = at_tile * kTreeKeys;  // of tile i
-            Place w0 = walk(), w1, w2, w3;
-            Regs ra, rb;
-            Tops t0 = {0, 0}, t1 = {0, 0}, t2 = {0, 0};
-            int e0 = 127, e1 = 127;  // exponents of the rows of tiles i and i + 1
-            ra.e = 127;
-            auto kregs = [](Regs& r) LG_INLINE { return kAlone ? r.k : r.v; };
-            // SPLIT: a wave's own kind of tile, out of `lead` (K) or `behind` (V)
-            auto ask = [&](const Place& lead, const Place& behind, int lead0, int behind0, Regs& r) LG_INLINE {
-                if constexpr (kAlone) {
-                    load(p.k_pool, lead, lead0, r.k);
-                    load(p.v_pool, behind, behind0, r.v);
-                } else {
-                    const Place w = {{moves_v ? behind.row[0] : lead.row[0], moves_v ? behind.row[1] : lead.row[1]}};
-                    load(moves_v ? p.v_pool : p.k_pool, w, moves_v ? behind0 : lead0, r.v);
+            for (int from = tile0; from < tile1; from += kTab) {
+                const int count = min(tile1 - from, kTab), steps = (count + PARTS - 1) / PARTS;
+                if (from != tile0) __syncthreads();  // (the last waves are done with the table)
+                fill(from, count, steps);
+                __syncthreads();
+                int key0 = (from + part) * kTreeKeys;  // of tile i
+                p_prev[0] = p_prev[1] = uint4_t{0, 0, 0, 0};
+                Place w0 = uniform(place(0)), w1 = uniform(place(1)), w2 = uniform(place(2)), w3 = w2;
+                uint2_t ahead = place(1 + kDeep);
+                Regs ra, rb;
+                Tops t0 = {0, 0}, t1 = {0, 0}, t2 = {0, 0};
+                auto kregs = [](Regs& r) LG_INLINE { return kAlone ? r.k : r.v; };
+                // K out of `lead` and V out of `behind`; of several waves each its own kind
+                auto ask = [&](const Place& lead, const Place& behind, int lead0, int behind0, Regs& r) LG_INLINE {
+                    if constexpr (kAlone) {
+                        load(p.k_pool, lead, lead0, r.k);
+                        load(p.v_pool, behind, behind0, r.v);
+                    } else {
+                        const Place w = {{moves_v ? behind.row[0] : lead.row[0], moves_v ? behind.row[1] : lead.row[1]}};
+                        load(moves_v ? p.v_pool : p.k_pool, w, moves_v ? behind0 : lead0, r.v);
+                    }
+                };
+                {
+                    uint4_t x0[kPer];
+                    load(p.k_pool, w0, key0, x0);
+                    load(p.k_pool, w1, key0 + kStride, kregs(rb));
+                    if constexpr (kDeep == 2) ask(w2, w0, key0 + 2 * kStride, key0, ra);
+                    if constexpr (E4M3) {
+                        t0 = tops_of(0);
+                        t1 = tops_of(1);
+                    }
+                    if (moves_k) {
+                        store_k(0, x0, exps_at(0, 0), t0);
+                        store_k(1, kregs(rb), exps_at(1, 0), t1);
+                    }
                 }
-            };
-            {
-                uint4_t x0[kPer];
-                if constexpr (E4M3) e0 = load_exps(w0, key0);
-                load(p.k_pool, w0, key0, x0);
-                w1 = walk();
-                if constexpr (E4M3) e1 = load_exps(w1, key0 + kStride);
-                load(p.k_pool, w1, key0 + kStride, kregs(rb));
-                if constexpr (kDeep == 2) {
-                    w2 = walk();
-                    if constexpr (E4M3) ra.e = load_exps(w2, key0 + 2 * kStride);
-                    ask(w2, w0, key0 + 2 * kStride, key0, ra);
-                }
-                if constexpr (E4M3) {
-                    t0 = tops_of(e0);
-                    t1 = tops_of(e1);
-                }
-                if (moves_k) {
-                    store_k(0, x0, e0, t0);
-                    store_k(1, kregs(rb), e1, t1);
-                }
-            }
-            // V buffer 1 plays V(-1) in the first step, whose P is 0: finite values
-            for (int i = tid; i < kVTile / 2; i += 64 * COLW) reinterpret_cast<unsigned*>(vs + kVTile)[i] = 0u;
-            together();
-#pragma unroll
-            for (int e = 0; e < 16; ++e) s_cur[e] = 0.0f;
-#pragma unroll
-            for (int j = 0; j < kSteps; ++j) s_cur = T::mfma32(k_operand(0, j), qb[j], s_cur);
-            together();  // (the first step ends with a store into the buffer just read)
-            // step i, H its parity: what a later step needs is asked for in front of it and goes to LDS behind it
-            auto one = [&](auto h_c, Regs& now, Regs& next) LG_INLINE {
-                constexpr int H = decltype(h_c)::value;
-                Place& lead = kDeep == 2 ? w3 : w2;
-                lead = walk();
-                if constexpr (E4M3) next.e = load_exps(lead, key0 + (kDeep + 1) * kStride);
-                ask(lead, kDeep == 2 ? w1 : w0, key0 + (kDeep + 1) * kStride, key0 + (kDeep - 1) * kStride, next);
-                __builtin_amdgcn_sched_barrier(0);
-                if (active) step(h_c, w0, key0, t0, careful_c);
-                __builtin_amdgcn_sched_barrier(0);
-                Regs& then = kDeep == 2 ? now : next;
-                if constexpr (E4M3) t2 = tops_of(then.e);
-                if (moves_k) store_k(H, kregs(then), then.e, t2);  // K(i + 2)
-                if (moves_v) store_v(H, then.v, e0, t0, w0, key0);  // V(i)
-                e0 = e1;
-                e1 = then.e;
-                t0 = t1;
-                t1 = t2;
-                w0 = w1;
-                w1 = w2;
-                w2 = w3;
-                key0 += kStride;
+                // V buffer 1 plays V(-1) in the first step, whose P is 0: finite values
+                for (int i = tid; i < kVTile / 2; i += 64 * COLW) reinterpret_cast<unsigned*>(vs + kVTile)[i] = 0u;
                 together();
-            };
-            int i = 0;
-            for (; i + 1 < steps; i += 2) {
-                one(ic<0>{}, ra, rb);
-                one(ic<1>{}, rb, ra);
-            }
-            if (i < steps) one(ic<0>{}, ra, rb);
-            const int buf = (steps - 1) & 1;
-            if (active) {
 #pragma unroll
-                for (int j = 0; j < kSteps; ++j)
-                    o[j % kTiles] = PackedF16::mfma32(v_operand(buf, j / kTiles, j % kTiles), p_prev[j / kTiles], o[j % kTiles]);
+                for (int e = 0; e < 16; ++e) s_cur[e] = 0.0f;
+#pragma unroll
+                for (int j = 0; j < kSteps; ++j) s_cur = T::mfma32(k_operand(0, j), qb[j], s_cur);
+                together();  // (the first step ends with a store into the buffer just read)
+                // step i, H its parity: what a later step needs is asked for in front of it and goes to LDS behind it
+                auto one = [&](auto h_c, int i, Regs& now, Regs& next) LG_INLINE {
+                    constexpr int H = decltype(h_c)::value;
+                    Place& lead = kDeep == 2 ? w3 : w2;
+                    lead = uniform(ahead);
+                    ahead = place(i + 2 + kDeep);
+                    ask(lead, kDeep == 2 ? w1 : w0, key0 + (kDeep + 1) * kStride, key0 + (kDeep - 1) * kStride, next);
+                    if constexpr (E4M3) t2 = tops_of(i + 2);
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (active) step(h_c, w0, key0, t0, careful_c);
+                    __builtin_amdgcn_sched_barrier(0);
+                    Regs& then = kDeep == 2 ? now : next;
+                    if (moves_k) store_k(H, kregs(then), exps_at(i + 2, 0), t2);       // K(i + 2)
+                    if (moves_v) store_v(H, then.v, exps_at(i, 1), t0, w0, key0);  // V(i)
+                    t0 = t1;
+                    t1 = t2;
+                    w0 = w1;
+                    w1 = w2;
+                    w2 = w3;
+                    key0 += kStride;
+                    together();
+                };
+                int i = 0;
+                for (; i + 1 < steps; i += 2) {
+                    one(ic<0>{}, i, ra, rb);
+                    one(ic<1>{}, i + 1, rb, ra);
+                }
+                if (i < steps) one(ic<0>{}, i, ra, rb);
+                const int buf = (steps - 1) & 1;
+                if (active) {
+#pragma unroll
+                    for (int j = 0; j < kSteps; ++j)
+                        o[j % kTiles] = PackedF16::mfma32(v_operand(buf, j / kTiles, j % kTiles), p_prev[j / kTiles], o[j % kTiles]);
+                }
             }
         };
 
@@ -641,7 +638,7 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
         for (int dt = 0; dt < kTiles; ++dt)
 #pragma unroll
             for (int e = 0; e < 16; ++e) o[dt][e] = 0.0f;
-        if (steps > 0) {
+        if (u.ctx > 0) {
             walk_tiles(ic<0>{});
             __syncthreads();
             int far = 0;
@@ -653,11 +650,13 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
             }
         }
         if (__builtin_expect(__builtin_amdgcn_readfirstlane(odd_parts[part]) != 0, 0)) {
-            start(part);
-            int key0 = at_tile * kTreeKeys;
-            for (int t = 0; t < steps && active; ++t, key0 += kStride) {
-                const Place w = walk();
-                if (!is_there(w) || (is_whole(w) && key0 + kTreeKeys <= u.prior)) continue;
+            for (int tile = tile0; tile < tile1 && active; ++tile) {
+                const int key0 = tile * kTreeKeys;
+                int block, off;
+                const Place w = {{__builtin_amdgcn_readfirstlane(row_of(key0, block, off)),
+                                  __builtin_amdgcn_readfirstlane(row_of(key0 + 16, block, off))}};
+                // (each part for its own tiles: the parts are added up)
+                if ((tile - tile0) % kTab % PARTS != part || !is_there(w) || (is_whole(w) && key0 + kTreeKeys <= u.prior)) continue;
                 const unsigned win = window(w, key0);
                 for (int key = 0; key < kTreeKeys; ++key) {
                     const bool sees = (win >> key) & 1u;
@@ -769,19 +768,44 @@ __global__ __launch_bounds__(256) void paged_attn_tree_merge_kernel(const TreePa
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int dt = blockIdx.x % kTiles;
     const int of_unit = blockIdx.x / kTiles % p.slot_waves;       // which 32 columns of a unit
-    const int cut = (int)(blockIdx.x / kTiles) / p.slot_waves;    // behind the tiles of this workgroup
+    const int cut = (int)(blockIdx.x / kTiles) / p.slot_waves;    // behind the tiles of this workgroup, or the unit
     TreeChunk c = tree_chunk<kCols>(0, 0);
     unsigned total = c.end;
     for (int first = 64; first < p.num_seqs; first += 64) total = tree_chunk<kCols>(first, total).end;
     const unsigned per = tree_share(total, p.workers);
-    const unsigned pos = (unsigned)(cut + 1) * per;
-    if (pos >= total) return;
-    while (pos >= c.end) c = tree_chunk<kCols>(c.first + 64, c.end);
-    const TreeUnit u = tree_unit(c, p.hkv, pos);
-    const unsigned begin = pos - (unsigned)u.tile;
+    TreeUnit u;
+    if (p.by_unit) {
+        // unit `cut` of all: units are counted as tiles are
+        int unit = cut;
+        for (;;) {
+            unsigned units = (unsigned)c.units;
+#pragma unroll
+            for (int d = 1; d < 64; d *= 2) {
+                const unsigned other = __shfl_up(units, d);
+                units += lane >= d ? other : 0u;
+            }
+            if (unit < __builtin_amdgcn_readlane((int)units, 63)) {
+                const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(units > (unsigned)unit));
+                unit -= __builtin_amdgcn_readlane((int)units, l) - __builtin_amdgcn_readlane(c.units, l);
+                u = tree_unit(c, p.hkv, (unsigned)__builtin_amdgcn_readlane((int)c.before, l) +
+                                            (unsigned)unit * (unsigned)__builtin_amdgcn_readlane(c.tiles, l));
+                break;
+            }
+            unit -= __builtin_amdgcn_readlane((int)units, 63);
+            if (c.first + 64 >= p.num_seqs) return;
+            c = tree_chunk<kCols>(c.first + 64, c.end);
+        }
+    } else {
+        const unsigned pos = (unsigned)(cut + 1) * per;
+        if (pos >= total) return;
+        while (pos >= c.end) c = tree_chunk<kCols>(c.first + 64, c.end);
+        u = tree_unit(c, p.hkv, pos);
+        if (u.tile == 0) return;
+    }
+    const unsigned begin = u.at - (unsigned)u.tile;
     const int first = (int)(begin / per), last = (int)((begin + (unsigned)u.tiles - 1) / per);
     const int cols = u.rows * p.g, c0 = u.group * kCols + of_unit * 32;
-    if (u.tile == 0 || first != cut || c0 >= cols) return;
+    if (first == last || (!p.by_unit && first != cut) || c0 >= cols) return;
 
     TreeRef m = {-INFINITY, 0.0f};
     float l = 0.0f;
@@ -850,8 +874,6 @@ static int tree_slot_waves(int max_q, int g, int waves) {
 template <typename T, int D, int COLW, int PARTS, bool E4M3>
 static hipError_t tree_launch_as(TreeParams p, hipStream_t stream) {
     p.slot_waves = tree_slot_waves(p.max_q, p.g, COLW);
-    p.step_blocks = kTreeKeys * PARTS / p.block_size;
-    p.step_rows = kTreeKeys * PARTS % p.block_size;
     const int64_t most = packed_tiles(p.total, p.num_seqs, p.g, 32 * COLW) * p.hkv;  // units
     const int64_t room = (int64_t)p.block_size * p.max_blocks;
     const int64_t tiles = most * ((room + kTreeKeys - 1) / kTreeKeys);
@@ -859,10 +881,12 @@ static hipError_t tree_launch_as(TreeParams p, hipStream_t stream) {
     if (workers > kTreeWorkers * 4 / (COLW > 4 ? COLW : 4)) workers = kTreeWorkers * 4 / (COLW > 4 ? COLW : 4);
     if (workers > (tiles + kTreeLeast - 1) / kTreeLeast) workers = (tiles + kTreeLeast - 1) / kTreeLeast;
     p.workers = (int)workers;
+    p.by_unit = most < workers;
     paged_attn_tree_kernel<T, D, COLW, PARTS, E4M3><<<(unsigned)workers, 64 * COLW * PARTS, 0, stream>>>(p);
     hipError_t rc = hipGetLastError();
     if (rc != hipSuccess || workers == 1) return rc;
-    paged_attn_tree_merge_kernel<T, D, COLW><<<(unsigned)((workers - 1) * p.slot_waves * (D / 32)), 256, 0, stream>>>(p);
+    paged_attn_tree_merge_kernel<T, D, COLW>
+        <<<(unsigned)((p.by_unit ? most : workers - 1) * p.slot_waves * (D / 32)), 256, 0, stream>>>(p);
     return hipGetLastError();
 }
 
