@@ -27,7 +27,7 @@ namespace lg {
 
 constexpr int kTreeKeys = 32;       // keys of a tile
 constexpr int kTreeWorkers = 512;   // workgroups that share the tiles, at most
-constexpr int kTreeLeast = 8;       // tiles of a workgroup, at least
+constexpr int kTreeLeast = 2;       // tiles of a workgroup, at least
 constexpr int kTreeMaskWords = 4;
 
 struct TreeParams {
@@ -142,10 +142,19 @@ struct TreeRef {
     float x, v;
 };
 __device__ __forceinline__ float tree_above(TreeRef a, TreeRef b) { return (a.x - b.x) + (a.v - b.v); }
-// exp2 of how far one of two references is below `top`, nothing where it is none.
-__device__ __forceinline__ float tree_weight(TreeRef a, TreeRef top) {
-    return fast_exp2(top.x == -INFINITY ? -INFINITY : tree_above(a, top));
-}
+__device__ __forceinline__ float tree_weight(TreeRef a, TreeRef top) { return fast_exp2(tree_above(a, top)); }
+// The reference of a column that has seen nothing above -inf yet: finite, so that such a key weighs 0 without a test.
+constexpr float kTreeNone = -3e38f;
+
+// 8 elements as they lie in the pools.
+template <bool E4M3>
+struct TreePiece {
+    typedef uint4_t type;
+};
+template <>
+struct TreePiece<true> {
+    typedef uint2_t type;
+};
 
 // Scores beyond this (in units of log 2) go through once more, multiplied and subtracted in two roundings, the same for the maximum: a
 // fused difference is off by up to half a step of the maximum, which is a factor of all probabilities as long as it is small.
@@ -279,6 +288,17 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
                             most = max(max(most, e[w] >> 24), max(e[w] & 0xffu, max((e[w] >> 8) & 0xffu, (e[w] >> 16) & 0xffu)));
                         }
                         top[kind] = most;
+                        // (kept as what the rows are to be multiplied by, relative to the tile's largest)
+                        const unsigned other = (unsigned)lane_xor_i32<1>((int)most);
+                        const int top_of_tile = kAsIs && kind == 0 ? 127 : (int)max(most, other);
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) {
+                            unsigned r = 0;
+#pragma unroll
+                            for (int y = 0; y < 4; ++y)
+                                r |= (unsigned)max((int)((e[w] >> (8 * y)) & 0xffu) - top_of_tile + 127, 0) << (8 * y);
+                            e[w] = r;
+                        }
                         *reinterpret_cast<uint4_t*>(exps_lds + (i >> 1) * 64 + 32 * kind + 16 * (i & 1)) = e;
                     }
                     tops_lds[i] = (unsigned short)(top[0] | top[1] << 8);
@@ -296,8 +316,9 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
         struct Tops {
             int k, v;
         };
-        auto tops_of = [&](int i) LG_INLINE {
-            const unsigned both = __builtin_amdgcn_readfirstlane(*reinterpret_cast<const unsigned*>(tops_lds + 2 * (i * PARTS + part)));
+        auto top_bytes = [&](int i) LG_INLINE { return *reinterpret_cast<const unsigned*>(tops_lds + 2 * (i * PARTS + part)); };
+        auto tops_of = [&](unsigned bytes) LG_INLINE {
+            const unsigned both = __builtin_amdgcn_readfirstlane(bytes);
             Tops t;
             t.k = max((int)(both & 0xffu), (int)((both >> 16) & 0xffu)) - 127;
             t.v = max((int)((both >> 8) & 0xffu), (int)(both >> 24)) - 127;
@@ -305,8 +326,9 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
             return t;
         };
 
+        typedef typename TreePiece<E4M3>::type piece_t;
         struct Regs {
-            uint4_t k[kAlone ? kPer : 1], v[kPer];  // (of several waves: v holds whichever a wave moves)
+            piece_t k[kAlone ? kPer : 1], v[kPer];  // (of several waves: v holds whichever a wave moves)
         };
         // Piece i of a mover: of key key_of(i).  Where a round of the movers' pieces is whole keys, it lies kRound keys behind piece
         // i - 1 and one offset serves all; within a wave they are then of the same half of the tile.
@@ -318,41 +340,32 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
         auto piece_of = [&](int i) LG_INLINE { return (mover + (kEven ? 0 : kMovers * i)) % (D / 8); };
         const unsigned row_bytes = (unsigned)p.hkv * kRow;
         const int wave_key = __builtin_amdgcn_readfirstlane(mover / (D / 8)) & ~15;  // (kEven: of which 16 keys piece 0 is)
-        const unsigned even_at = ((unsigned)key_of(0) & 15u) * row_bytes + (unsigned)(kPiece * piece_of(0));
-        auto load = [&](const uint8_t* pool, const Place& w, int key0, uint4_t* x) LG_INLINE {
-            // keys behind the last one, and in a half that is not there: others that are
-            const int left = is_there(w) ? u.ctx - key0 : kTreeKeys;
+        unsigned piece_at[kEven ? 1 : kPer];
+#pragma unroll
+        for (int i = 0; i < (kEven ? 1 : kPer); ++i)
+            piece_at[i] = ((unsigned)key_of(i) & 15u) * row_bytes + (unsigned)(kPiece * piece_of(i));
+        // (a half that is not there: the first rows of the pool; rows behind the last key lie in its block)
+        auto load = [&](const uint8_t* pool, const Place& w, piece_t* x) LG_INLINE {
             const uint8_t* const half0 = pool + (int64_t)max(w.row[0], 0) * row_bytes + u.head * kRow;
             const uint8_t* const half1 = pool + (int64_t)max(w.row[1], 0) * row_bytes + u.head * kRow;
-            auto take = [&](int i, const uint8_t* src) LG_INLINE {
-                if constexpr (E4M3) {
-                    const uint2_t b = *reinterpret_cast<const uint2_t*>(src);
-                    x[i][0] = b[0];
-                    x[i][1] = b[1];
+            // (a scalar base and 32-bit offsets: otherwise the compiler keeps 64-bit sums of everything that does not change)
+            unsigned at0 = piece_at[0];
+            asm volatile("" : "+v"(at0));
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                if constexpr (kEven) {
+                    const uint8_t* from = (wave_key + kRound * i < 16 ? half0 : half1) + (unsigned)(kRound * i % 16) * row_bytes;
+                    x[i] = *reinterpret_cast<const piece_t*>(from + at0);
                 } else {
-                    x[i] = *reinterpret_cast<const uint4_t*>(src);
-                }
-            };
-            if (kEven && left >= kTreeKeys) {
-#pragma unroll
-                for (int i = 0; i < kPer; ++i) {
-                    const uint8_t* from = wave_key + kRound * i < 16 ? half0 : half1;
-                    take(i, from + (unsigned)(kRound * i % 16) * row_bytes + even_at);
-                }
-            } else {
-                int m = mover;
-                asm volatile("" : "+v"(m));
-#pragma unroll
-                for (int i = 0; i < kPer; ++i) {
-                    const int at = (m + kMovers * i) / (D / 8), key = at < left ? at : left - 1;
-                    take(i, (key < 16 ? half0 : half1) + ((unsigned)(key & 15) * row_bytes + kPiece * ((m + kMovers * i) % (D / 8))));
+                    x[i] = *reinterpret_cast<const piece_t*>((key_of(i) < 16 ? half0 : half1) + piece_at[i]);
                 }
             }
         };
         // A piece of 8 as the kernel wants it: e4m3 rows times 2^(e - top) in 16 bits.
-        auto decoded = [&](const uint4_t& x, int e, int top, bool as_bf16) LG_INLINE {
+        auto decoded = [&](const piece_t& x, int e, bool as_bf16) LG_INLINE {
             if constexpr (!E4M3) return x;
-            const float scale = __int_as_float(max(e - top, 0) << 23);
+            else {
+            const float scale = __int_as_float(e << 23);
             uint4_t y;
             if (as_bf16) {
                 y[0] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x[0], scale, false));
@@ -366,26 +379,27 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
                 y[3] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x[1], scale, true));
             }
             return y;
+            }
         };
         auto exps_at = [&](int i, int kind) LG_INLINE { return exps_lds + (i * PARTS + part) * 64 + 32 * kind; };
-        auto store_k = [&](int buf, const uint4_t* x, const uint8_t* e, const Tops& top) LG_INLINE {
+        auto store_k = [&](int buf, const piece_t* x, const uint8_t* e) LG_INLINE {
             unsigned short* const to = ks + buf * kKTile;
 #pragma unroll
             for (int i = 0; i < kPer; ++i) {
                 const int row = E4M3 ? e[key_of(i)] : 0;
-                *reinterpret_cast<uint4_t*>(to + key_of(i) * kKRow + 8 * piece_of(i)) = decoded(x[i], row, top.k, kAsIs);
+                *reinterpret_cast<uint4_t*>(to + key_of(i) * kKRow + 8 * piece_of(i)) = decoded(x[i], row, kAsIs);
             }
         };
         // A key that a column does not see has the probability 0 there, and 0 times an infinity or NaN of its V row is NaN: in
         // tiles that are not seen whole such elements go in as 0, and are added at the end for the columns that see them.
-        auto store_v = [&](int buf, const uint4_t* x, const uint8_t* e, const Tops& top, const Place& w, int key0) LG_INLINE {
+        auto store_v = [&](int buf, const piece_t* x, const uint8_t* e, const Place& w, int key0) LG_INLINE {
             unsigned short* const to = vs + buf * kVTile;
             const bool whole = is_whole(w) && key0 + kTreeKeys <= u.prior;
             bool odd = false;
 #pragma unroll
             for (int i = 0; i < kPer; ++i) {
                 const int row = E4M3 ? e[key_of(i)] : 0;
-                uint4_t y = decoded(x[i], row, top.v, false);
+                uint4_t y = decoded(x[i], row, false);
                 if (!whole) {
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
@@ -455,11 +469,11 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
             float drop = 0.0f;  // what raising the reference takes off the exponents so far
             float ref = m.x;
             auto follow = [&](float tm) LG_INLINE {
-                raise = tree_above({tm, v_top}, m) > kTreeLazy;
                 drop = tree_above(m, {tm, v_top});
+                raise = drop < -kTreeLazy;
                 m.x = raise ? tm : m.x;
                 if (E4M3) m.v = raise ? v_top : m.v;
-                ref = m.x == -INFINITY ? 0.0f : m.x;
+                ref = m.x;
             };
             if constexpr (careful) {
                 float tm = -INFINITY;
@@ -476,54 +490,51 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
                 scale = 1.0f;
                 ref = 0.0f;
             }
+            // The products in pairs of S and O, so that none waits for the one before it, operands kLead pairs ahead, and between any two of
+            // them a share of the softmax: its maximum first, then the probabilities.
+            constexpr int kLead = kWide ? 2 : 3, kSlots = 2 * kSteps, kFirst = kSlots * 3 / 16 > 1 ? kSlots * 3 / 16 : 1;
             uint4_t ka[kSteps], va[kSteps];
-            if constexpr (!kWide)
-#pragma unroll
-                for (int j = 0; j < kSteps; ++j) {
-                    ka[j] = k_operand(1 - H, j);
-                    va[j] = v_operand(1 - H, j / kTiles, j % kTiles);
-                }
-            if constexpr (!careful) {
-                float tm = -INFINITY;
-#pragma unroll
-                for (int e = 0; e < 16; ++e) tm = fmaxf(tm, s_cur[e]);
-                follow(fmaxf(tm, lane_xor_f32<32>(tm)) * scale);
-            }
             float16_t s_nxt;
 #pragma unroll
             for (int e = 0; e < 16; ++e) s_nxt[e] = 0.0f;
-#pragma unroll
-            for (int j = 0; j < kSteps; ++j) {
-                if constexpr (kWide) {
-                    if (j % 4 == 0) __builtin_amdgcn_sched_barrier(0);
-                    ka[j] = k_operand(1 - H, j);
-                    va[j] = v_operand(1 - H, j / kTiles, j % kTiles);
-                }
-                s_nxt = T::mfma32(ka[j], qb[j], s_nxt);
-                o[j % kTiles] = PackedF16::mfma32(va[j], p_prev[j / kTiles], o[j % kTiles]);
-            }
-            float sum = 0.0f;
+            float tm = -INFINITY, off = 0.0f, sum = 0.0f, even = 0.0f;
             uint4_t pb[2];
-            const float off = kTreeHead + (v_top - m.v) - ref;
+            auto read = [&](int j) LG_INLINE {
+                ka[j] = k_operand(1 - H, j);
+                va[j] = v_operand(1 - H, j / kTiles, j % kTiles);
+            };
+            auto share = [&](auto slot_c) LG_INLINE {
+                constexpr int kSlot = decltype(slot_c)::value;
+                if constexpr (kSlot == 0 && !careful) {
 #pragma unroll
-            for (int e = 0; e < 16; e += 2) {
-                const float p0 = fast_exp2(fmaf(s_cur[e], scale, off));
-                const float p1 = fast_exp2(fmaf(s_cur[e + 1], scale, off));
-                sum += p0;
-                sum += p1;
-                pb[e >> 3][(e & 7) >> 1] = PackedF16::pack2(p0, p1);
-            }
-            if constexpr (COLW >= 4 && !kWide) {
-                // half of the operand reads, then the products, each followed by a read and its share of the vector work
-                constexpr int kReads = 3 * kSteps, kFirst = (D > 64 ? 12 : 20) * kSteps / 8, kShare = (D < 128 ? 80 : 72) / (2 * kSteps);
-                __builtin_amdgcn_sched_group_barrier(0x100, kFirst, 0);
-#pragma unroll
-                for (int g = 0; g < 2 * kSteps; ++g) {
-                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                    if (g < kReads - kFirst) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-                    __builtin_amdgcn_sched_group_barrier(0x002, kShare, 0);
+                    for (int e = 0; e < 16; ++e) tm = fmaxf(tm, s_cur[e]);
                 }
-            }
+                if constexpr (kSlot == kFirst - 1) {
+                    if constexpr (!careful) follow(fmaxf(tm, lane_xor_f32<32>(tm)) * scale);
+                    off = kTreeHead + (v_top - m.v) - ref;
+                }
+                static_for<16>([&](auto e_c) LG_INLINE {
+                    constexpr int e = decltype(e_c)::value;
+                    if constexpr (kFirst + e * (kSlots - kFirst) / 16 == kSlot) {
+                        const float prob = fast_exp2(fmaf(s_cur[e], scale, off));
+                        sum += prob;
+                        if constexpr (e % 2 == 0) even = prob;
+                        else pb[e >> 3][(e & 7) >> 1] = PackedF16::pack2(even, prob);
+                    }
+                });
+            };
+#pragma unroll
+            for (int j = 0; j < kLead; ++j) read(j);
+            static_for<kSteps>([&](auto step_c) LG_INLINE {
+                constexpr int j = decltype(step_c)::value;
+                if constexpr (j + kLead < kSteps) read(j + kLead);
+                s_nxt = T::mfma32(ka[j], qb[j], s_nxt);
+                share(ic<2 * j>{});
+                __builtin_amdgcn_sched_barrier(0);
+                o[j % kTiles] = PackedF16::mfma32(va[j], p_prev[j / kTiles], o[j % kTiles]);
+                share(ic<2 * j + 1>{});
+                __builtin_amdgcn_sched_barrier(0);
+            });
             // (F belongs to this step: its results are used by the next one only, and would sink there)
             asm volatile("" : "+v"(pb[0]), "+v"(pb[1]), "+v"(sum));
             if (__builtin_expect(__builtin_amdgcn_ballot_w64(raise) != 0, 0)) {  // O(i - 1) was relative to the old one
@@ -543,7 +554,7 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
 
         // The tiles of the part, for scores of any size with careful_c.
         auto walk_tiles = [&](auto careful_c) LG_INLINE {
-            m = TreeRef{-INFINITY, 0.0f};
+            m = TreeRef{kTreeNone, 0.0f};
             l = 0.0f;
 #pragma unroll
             for (int dt = 0; dt < kTiles; ++dt)
@@ -558,31 +569,33 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
                 p_prev[0] = p_prev[1] = uint4_t{0, 0, 0, 0};
                 Place w0 = uniform(place(0)), w1 = uniform(place(1)), w2 = uniform(place(2)), w3 = w2;
                 uint2_t ahead = place(1 + kDeep);
+                unsigned tops_ahead = 0;
                 Regs ra, rb;
                 Tops t0 = {0, 0}, t1 = {0, 0}, t2 = {0, 0};
                 auto kregs = [](Regs& r) LG_INLINE { return kAlone ? r.k : r.v; };
                 // K out of `lead` and V out of `behind`; of several waves each its own kind
-                auto ask = [&](const Place& lead, const Place& behind, int lead0, int behind0, Regs& r) LG_INLINE {
+                auto ask = [&](const Place& lead, const Place& behind, Regs& r) LG_INLINE {
                     if constexpr (kAlone) {
-                        load(p.k_pool, lead, lead0, r.k);
-                        load(p.v_pool, behind, behind0, r.v);
+                        load(p.k_pool, lead, r.k);
+                        load(p.v_pool, behind, r.v);
                     } else {
                         const Place w = {{moves_v ? behind.row[0] : lead.row[0], moves_v ? behind.row[1] : lead.row[1]}};
-                        load(moves_v ? p.v_pool : p.k_pool, w, moves_v ? behind0 : lead0, r.v);
+                        load(moves_v ? p.v_pool : p.k_pool, w, r.v);
                     }
                 };
                 {
-                    uint4_t x0[kPer];
-                    load(p.k_pool, w0, key0, x0);
-                    load(p.k_pool, w1, key0 + kStride, kregs(rb));
-                    if constexpr (kDeep == 2) ask(w2, w0, key0 + 2 * kStride, key0, ra);
+                    piece_t x0[kPer];
+                    load(p.k_pool, w0, x0);
+                    load(p.k_pool, w1, kregs(rb));
+                    if constexpr (kDeep == 2) ask(w2, w0, ra);
                     if constexpr (E4M3) {
-                        t0 = tops_of(0);
-                        t1 = tops_of(1);
+                        t0 = tops_of(top_bytes(0));
+                        t1 = tops_of(top_bytes(1));
+                        tops_ahead = top_bytes(2);
                     }
                     if (moves_k) {
-                        store_k(0, x0, exps_at(0, 0), t0);
-                        store_k(1, kregs(rb), exps_at(1, 0), t1);
+                        store_k(0, x0, exps_at(0, 0));
+                        store_k(1, kregs(rb), exps_at(1, 0));
                     }
                 }
                 // V buffer 1 plays V(-1) in the first step, whose P is 0: finite values
@@ -599,14 +612,27 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
                     Place& lead = kDeep == 2 ? w3 : w2;
                     lead = uniform(ahead);
                     ahead = place(i + 2 + kDeep);
-                    ask(lead, kDeep == 2 ? w1 : w0, key0 + (kDeep + 1) * kStride, key0 + (kDeep - 1) * kStride, next);
-                    if constexpr (E4M3) t2 = tops_of(i + 2);
+                    ask(lead, kDeep == 2 ? w1 : w0, next);
+                    if constexpr (E4M3) {
+                        t2 = tops_of(tops_ahead);
+                        tops_ahead = top_bytes(i + 3);
+                    }
                     __builtin_amdgcn_sched_barrier(0);
+                    
+                    if constexpr (COLW >= 4 && D >= 96) __builtin_amdgcn_s_setprio(1);
                     if (active) step(h_c, w0, key0, t0, careful_c);
+                    if constexpr (COLW >= 4 && D >= 96) __builtin_amdgcn_s_setprio(0);
+                    
                     __builtin_amdgcn_sched_barrier(0);
                     Regs& then = kDeep == 2 ? now : next;
-                    if (moves_k) store_k(H, kregs(then), exps_at(i + 2, 0), t2);       // K(i + 2)
-                    if (moves_v) store_v(H, then.v, exps_at(i, 1), t0, w0, key0);  // V(i)
+                    // (waited for here, whichever of the two follows: not known to have arrived, they would be waited for with the next ones)
+#pragma unroll
+                    for (int j = 0; j < kPer; ++j) {
+                        if constexpr (kAlone) asm volatile("" : "+v"(then.k[j]));
+                        asm volatile("" : "+v"(then.v[j]));
+                    }
+                    if (moves_k) store_k(H, kregs(then), exps_at(i + 2, 0));   // K(i + 2)
+                    if (moves_v) store_v(H, then.v, exps_at(i, 1), w0, key0);  // V(i)
                     t0 = t1;
                     t1 = t2;
                     w0 = w1;
@@ -632,7 +658,7 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
 
         if (wave_of_all == 0 && lane < PARTS) odd_parts[lane] = far_parts[lane] = 0;
         __syncthreads();
-        m = TreeRef{-INFINITY, 0.0f};
+        m = TreeRef{kTreeNone, 0.0f};
         l = 0.0f;
 #pragma unroll
         for (int dt = 0; dt < kTiles; ++dt)
@@ -717,7 +743,7 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
             __syncthreads();
             if (active) {
                 const float* const parts = reinterpret_cast<const float*>(lds) + wave * PARTS * tree_wave_floats(D);
-                TreeRef refs[PARTS], top = {-INFINITY, 0.0f};
+                TreeRef refs[PARTS], top = {kTreeNone, 0.0f};
                 float weight[PARTS], sum = 0.0f;
 #pragma unroll
                 for (int q = 0; q < PARTS; ++q) {
@@ -807,7 +833,7 @@ __global__ __launch_bounds__(256) void paged_attn_tree_merge_kernel(const TreePa
     const int cols = u.rows * p.g, c0 = u.group * kCols + of_unit * 32;
     if (first == last || (!p.by_unit && first != cut) || c0 >= cols) return;
 
-    TreeRef m = {-INFINITY, 0.0f};
+    TreeRef m = {kTreeNone, 0.0f};
     float l = 0.0f;
     float4_t o[4];
 #pragma unroll
