@@ -67,6 +67,20 @@ __device__ __forceinline__ TreeCold tree_cold() {
     return at;
 }
 
+// Inclusive sum over the lanes of a wave.
+__device__ __forceinline__ unsigned wave_scan(unsigned v) {
+    auto add = [&](auto ctrl, auto rows) LG_INLINE {
+        v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, decltype(ctrl)::value, decltype(rows)::value, 0xf, false);
+    };
+    add(ic<0x111>{}, ic<0xf>{});  // from 1, 2, 4, 8 lanes below in a row of 16
+    add(ic<0x112>{}, ic<0xf>{});
+    add(ic<0x114>{}, ic<0xf>{});
+    add(ic<0x118>{}, ic<0xf>{});
+    add(ic<0x142>{}, ic<0xa>{});  // the first (third) row's total to the second (fourth)
+    add(ic<0x143>{}, ic<0xc>{});  // that of the first two to the others
+    return v;
+}
+
 template <int COLS>
 __device__ __forceinline__ TreeChunk tree_chunk(int first, unsigned before) {
     const TreeCold c0 = tree_cold();
@@ -86,14 +100,8 @@ __device__ __forceinline__ TreeChunk tree_chunk(int first, unsigned before) {
     c.prior = c.ctx - rows;
     c.units = (rows * p.g + COLS - 1) / COLS * p.hkv;
     c.tiles = c.ctx > 0 ? (c.ctx + kTreeKeys - 1) / kTreeKeys : 1;
-    unsigned sum = (unsigned)c.units * (unsigned)c.tiles;
-    const unsigned mine = sum;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const unsigned other = __shfl_up(sum, d);
-        sum += lane >= d ? other : 0u;
-    }
-    c.behind = before + sum;
+    const unsigned mine = (unsigned)c.units * (unsigned)c.tiles;
+    c.behind = before + wave_scan(mine);
     c.before = c.behind - mine;
     c.end = (unsigned)__builtin_amdgcn_readlane((int)c.behind, 63);
     return c;
@@ -207,16 +215,16 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
         else __syncthreads();
     };
 
-    unsigned total = 0;
-    for (int first = 0; first < tree_cold()->num_seqs; first += 64) total = tree_chunk<kCols>(first, total).end;
-    const unsigned per = tree_share(total, tree_cold()->workers);
+    int first = 0;  // of the 64 sequences that the next unit is in, and the tiles in front of them
+    unsigned before = 0;
+    TreeChunk chunk = tree_chunk<kCols>(0, 0);
+    unsigned total = chunk.end;
+    for (int f = 64; f < p.num_seqs; f += 64) total = tree_chunk<kCols>(f, total).end;
+    const unsigned per = tree_share(total, p.workers);
     unsigned pos = blockIdx.x * per;
     if (pos >= total) return;
     const unsigned end = total - pos < per ? total : pos + per;
-    int first = 0;  // of the 64 sequences that the next unit is in, and the tiles in front of them
-    unsigned before = 0;
-    while (pos < end) {
-        TreeChunk chunk = tree_chunk<kCols>(first, before);
+    for (; pos < end; chunk = tree_chunk<kCols>(first, before)) {
         while (pos >= chunk.end) {
             first += 64;
             before = chunk.end;
@@ -227,7 +235,8 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
         const int tile1 = (unsigned)(u.tiles - tile0) < end - pos ? u.tiles : tile0 + (int)(end - pos);
         pos += (unsigned)(tile1 - tile0);
 
-        const int cols = u.rows * tree_cold()->g;
+        const TreeCold unit_cold = tree_cold();
+        const int g = unit_cold->g, cols = u.rows * g;
         const int c0 = u.group * kCols + wave * 32;
         const bool active = c0 < cols;
         // This lane's token and head (worked out anew where they are needed: registers are what the loop is short of).
@@ -238,15 +247,15 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
             int c = c0 + col;
             asm volatile("" : "+v"(c));
             c = c < cols ? c : cols - 1;
-            const int g = tree_cold()->g, tok = c / g;
+            const int tok = c / g;
             return Column{tok, u.head * g + c - tok * g};
         };
 
         uint4_t qb[kSteps];
         {
             const Column c = column();
-            const TreeCold t = tree_cold();
-            const unsigned short* q = t->q + (int64_t)(u.row0 + c.tok) * t->q_stride + (int64_t)c.head * D + 8 * h;
+            const unsigned short* q =
+                unit_cold->q + (int64_t)(u.row0 + c.tok) * unit_cold->q_stride + (int64_t)c.head * D + 8 * h;
 #pragma unroll
             for (int j = 0; j < kSteps; ++j) qb[j] = *reinterpret_cast<const uint4_t*>(q + 16 * j);
         }
@@ -257,29 +266,49 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
         };
         auto is_there = [](const Place& w) LG_INLINE { return (w.row[0] & w.row[1]) >= 0; };  // one half at least
         auto is_whole = [](const Place& w) LG_INLINE { return (w.row[0] | w.row[1]) >= 0; };
-        auto row_of = [&](int key, int& block, int& off) LG_INLINE {
+        // A key's entry of the table (-1: none) and row in its block; the entry's row of the pools, -1: it names no block.
+        struct Entry {
+            int block, off;
+        };
+        auto entry_of = [&](int key) LG_INLINE {
             const TreeCold t = tree_cold();
             const int entry = key / t->block_size;
-            off = key - entry * t->block_size;
-            block = -1;
-            if (key < u.ctx) block = t->tables[(int64_t)u.seq * t->max_blocks + entry];
-            return block >= 0 && block < t->num_blocks ? block * t->block_size + off : -1;
+            Entry e = {-1, key - entry * t->block_size};
+            if (key < u.ctx) e.block = t->tables[(int64_t)u.seq * t->max_blocks + entry];
+            if (e.block >= t->num_blocks) e.block = -1;
+            return e;
         };
-        auto fill = [&](int from, int count, int steps) LG_INLINE {
-            for (int i = threadIdx.x; i < 2 * (steps + 4) * PARTS; i += 64 * COLW * PARTS) {
-                const int key = i < 2 * count ? from * kTreeKeys + 16 * i : u.ctx;
-                int block, off;
-                const int row = row_of(key, block, off);
-                rows_lds[i] = row;
-                if constexpr (E4M3) {
+        auto row_of = [&](const Entry& e) LG_INLINE { return e.block < 0 ? -1 : e.block * p.block_size + e.off; };
+        // First the rows, then (they are loaded while the first tiles are on their way) the exponents.
+        constexpr int kThreads = 64 * COLW * PARTS, kRounds = (2 * kPlaces + kThreads - 1) / kThreads;
+        auto half_key = [&](int i, int from, int count) LG_INLINE { return i < 2 * count ? from * kTreeKeys + 16 * i : u.ctx; };
+        auto fill = [&](int from, int count, int halves, Entry (&entry)[kRounds]) LG_INLINE {
+#pragma unroll
+            for (int r = 0; r < kRounds; ++r) {
+                const int i = threadIdx.x + r * kThreads;
+                if (i < halves) {
+                    entry[r] = entry_of(half_key(i, from, count));
+                    rows_lds[i] = row_of(entry[r]);
+                }
+            }
+        };
+        auto fill_exps = [&](int from, int count, int halves, const Entry (&entry)[kRounds]) LG_INLINE {
+#pragma unroll
+            for (int r = 0; r < kRounds; ++r) {
+                const int i = threadIdx.x + r * kThreads;
+                if (i < halves) {
                     // the exponents of the 16 rows of K and of V (of those that there are), and the largest of each
                     const TreeCold t = tree_cold();
-                    const int64_t at = row < 0 ? 0 : ((int64_t)block * t->hkv + u.head) * t->block_size + off;
-                    const int left = row < 0 ? 0 : u.ctx - key;
+                    const Entry& at = entry[r];
+                    const int64_t first = at.block < 0 ? 0 : ((int64_t)at.block * t->hkv + u.head) * t->block_size + at.off;
+                    const int left = at.block < 0 ? 0 : u.ctx - half_key(i, from, count);
                     unsigned top[2];
+                    uint4_t both[2];
+                    both[0] = *reinterpret_cast<const uint4_t*>(t->k_exp + first);
+                    both[1] = *reinterpret_cast<const uint4_t*>(t->v_exp + first);
 #pragma unroll
                     for (int kind = 0; kind < 2; ++kind) {
-                        uint4_t e = *reinterpret_cast<const uint4_t*>((kind ? t->v_exp : t->k_exp) + at);
+                        uint4_t e = both[kind];
                         unsigned most = 0;
 #pragma unroll
                         for (int w = 0; w < 4; ++w) {
@@ -293,11 +322,11 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
                         const int top_of_tile = kAsIs && kind == 0 ? 127 : (int)max(most, other);
 #pragma unroll
                         for (int w = 0; w < 4; ++w) {
-                            unsigned r = 0;
+                            unsigned r4 = 0;
 #pragma unroll
                             for (int y = 0; y < 4; ++y)
-                                r |= (unsigned)max((int)((e[w] >> (8 * y)) & 0xffu) - top_of_tile + 127, 0) << (8 * y);
-                            e[w] = r;
+                                r4 |= (unsigned)max((int)((e[w] >> (8 * y)) & 0xffu) - top_of_tile + 127, 0) << (8 * y);
+                            e[w] = r4;
                         }
                         *reinterpret_cast<uint4_t*>(exps_lds + (i >> 1) * 64 + 32 * kind + 16 * (i & 1)) = e;
                     }
@@ -563,7 +592,9 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
             for (int from = tile0; from < tile1; from += kTab) {
                 const int count = min(tile1 - from, kTab), steps = (count + PARTS - 1) / PARTS;
                 if (from != tile0) __syncthreads();  // (the last waves are done with the table)
-                fill(from, count, steps);
+                const int halves = 2 * (steps + 4) * PARTS;
+                Entry entry[kRounds];
+                fill(from, count, halves, entry);
                 __syncthreads();
                 int key0 = (from + part) * kTreeKeys;  // of tile i
                 p_prev[0] = p_prev[1] = uint4_t{0, 0, 0, 0};
@@ -589,6 +620,8 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
                     load(p.k_pool, w1, kregs(rb));
                     if constexpr (kDeep == 2) ask(w2, w0, ra);
                     if constexpr (E4M3) {
+                        fill_exps(from, count, halves, entry);
+                        __syncthreads();
                         t0 = tops_of(top_bytes(0));
                         t1 = tops_of(top_bytes(1));
                         tops_ahead = top_bytes(2);
@@ -678,9 +711,8 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
         if (__builtin_expect(__builtin_amdgcn_readfirstlane(odd_parts[part]) != 0, 0)) {
             for (int tile = tile0; tile < tile1 && active; ++tile) {
                 const int key0 = tile * kTreeKeys;
-                int block, off;
-                const Place w = {{__builtin_amdgcn_readfirstlane(row_of(key0, block, off)),
-                                  __builtin_amdgcn_readfirstlane(row_of(key0 + 16, block, off))}};
+                const Place w = {{__builtin_amdgcn_readfirstlane(row_of(entry_of(key0))),
+                                  __builtin_amdgcn_readfirstlane(row_of(entry_of(key0 + 16)))}};
                 // (each part for its own tiles: the parts are added up)
                 if ((tile - tile0) % kTab % PARTS != part || !is_there(w) || (is_whole(w) && key0 + kTreeKeys <= u.prior)) continue;
                 const unsigned win = window(w, key0);
@@ -712,7 +744,7 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
         if constexpr (PARTS == 1) {
             if (!active) continue;
             if (all) {
-                const int tok0 = c0 / t->g;
+                const int tok0 = c0 / g;
                 const Column c = column();
                 static_assert(COLW * 16 * (D + 8) <= kRings, "the columns on their way out fit");
                 attn_packed_write<T, D>(t->out + (int64_t)(u.row0 + tok0) * t->out_stride,
@@ -784,17 +816,17 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
     }
 }
 
-// The units that were cut: a workgroup takes the first cut of one, 32 of its columns and 32 elements of the heads, its waves every fourth
-// part of the unit, a few of them in flight.
-template <typename T, int D, int COLW>
+// The units that were cut: a workgroup takes the first cut of one (or the unit), 32 of its columns and 8 Q elements of the heads, its
+// waves every fourth part of the unit, a few of them in flight.
+template <typename T, int D, int COLW, int Q>
 __global__ __launch_bounds__(256) void paged_attn_tree_merge_kernel(const TreeParams p) {
-    constexpr int kCols = 32 * COLW, kTiles = D / 32, kAhead = 4;
-    __shared__ float4_t theirs[3][4][64];
+    constexpr int kCols = 32 * COLW, kPieces = D / 8 / Q, kAhead = 16 / Q;
+    __shared__ float4_t theirs[3][Q][64];
     __shared__ float ml[3][3][64];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int dt = blockIdx.x % kTiles;
-    const int of_unit = blockIdx.x / kTiles % p.slot_waves;       // which 32 columns of a unit
-    const int cut = (int)(blockIdx.x / kTiles) / p.slot_waves;    // behind the tiles of this workgroup, or the unit
+    const int piece = blockIdx.x % kPieces;
+    const int of_unit = blockIdx.x / kPieces % p.slot_waves;     // which 32 columns of a unit
+    const int cut = (int)(blockIdx.x / kPieces) / p.slot_waves;  // behind the tiles of this workgroup, or the unit
     TreeChunk c = tree_chunk<kCols>(0, 0);
     unsigned total = c.end;
     for (int first = 64; first < p.num_seqs; first += 64) total = tree_chunk<kCols>(first, total).end;
@@ -804,12 +836,7 @@ __global__ __launch_bounds__(256) void paged_attn_tree_merge_kernel(const TreePa
         // unit `cut` of all: units are counted as tiles are
         int unit = cut;
         for (;;) {
-            unsigned units = (unsigned)c.units;
-#pragma unroll
-            for (int d = 1; d < 64; d *= 2) {
-                const unsigned other = __shfl_up(units, d);
-                units += lane >= d ? other : 0u;
-            }
+            const unsigned units = wave_scan((unsigned)c.units);
             if (unit < __builtin_amdgcn_readlane((int)units, 63)) {
                 const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(units > (unsigned)unit));
                 unit -= __builtin_amdgcn_readlane((int)units, l) - __builtin_amdgcn_readlane(c.units, l);
@@ -835,21 +862,21 @@ __global__ __launch_bounds__(256) void paged_attn_tree_merge_kernel(const TreePa
 
     TreeRef m = {kTreeNone, 0.0f};
     float l = 0.0f;
-    float4_t o[4];
+    float4_t o[Q];
 #pragma unroll
-    for (int q4 = 0; q4 < 4; ++q4) o[q4] = float4_t{0, 0, 0, 0};
+    for (int q4 = 0; q4 < Q; ++q4) o[q4] = float4_t{0, 0, 0, 0};
     auto join = [&](TreeRef m2, float l2, const float4_t* o2) LG_INLINE {
         const TreeRef top = tree_above(m2, m) > 0.0f ? m2 : m;
         const float mine = tree_weight(m, top), its = tree_weight(m2, top);
         m = top;
         l = l * mine + l2 * its;
 #pragma unroll
-        for (int q4 = 0; q4 < 4; ++q4)
+        for (int q4 = 0; q4 < Q; ++q4)
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[q4][e] = o[q4][e] * mine + o2[q4][e] * its;
     };
     for (int w0 = first + wave; w0 <= last; w0 += 4 * kAhead) {
-        float4_t o2[kAhead][4];
+        float4_t o2[kAhead][Q];
         TreeRef m2[kAhead];
         float l2[kAhead];
 #pragma unroll
@@ -860,7 +887,7 @@ __global__ __launch_bounds__(256) void paged_attn_tree_merge_kernel(const TreePa
             m2[a] = {slot[32 * D + (lane & 31)], slot[32 * D + 32 + (lane & 31)]};
             l2[a] = slot[32 * D + 64 + lane];
 #pragma unroll
-            for (int q4 = 0; q4 < 4; ++q4) o2[a][q4] = reinterpret_cast<const float4_t*>(slot)[(4 * dt + q4) * 64 + lane];
+            for (int q4 = 0; q4 < Q; ++q4) o2[a][q4] = reinterpret_cast<const float4_t*>(slot)[(Q * piece + q4) * 64 + lane];
         }
 #pragma unroll
         for (int a = 0; a < kAhead; ++a)
@@ -868,7 +895,7 @@ __global__ __launch_bounds__(256) void paged_attn_tree_merge_kernel(const TreePa
     }
     if (wave > 0) {
 #pragma unroll
-        for (int q4 = 0; q4 < 4; ++q4) theirs[wave - 1][q4][lane] = o[q4];
+        for (int q4 = 0; q4 < Q; ++q4) theirs[wave - 1][q4][lane] = o[q4];
         ml[wave - 1][0][lane] = m.x;
         ml[wave - 1][1][lane] = m.v;
         ml[wave - 1][2][lane] = l;
@@ -876,18 +903,18 @@ __global__ __launch_bounds__(256) void paged_attn_tree_merge_kernel(const TreePa
     __syncthreads();
     if (wave > 0) return;
     for (int w = 0; w < 3; ++w) {
-        float4_t o2[4];
+        float4_t o2[Q];
 #pragma unroll
-        for (int q4 = 0; q4 < 4; ++q4) o2[q4] = theirs[w][q4][lane];
+        for (int q4 = 0; q4 < Q; ++q4) o2[q4] = theirs[w][q4][lane];
         join({ml[w][0][lane], ml[w][1][lane]}, ml[w][2][lane], o2);
     }
     const int h = lane >> 5, gc = c0 + (lane & 31);
     if (gc >= cols) return;
     const float inv = l > 0.0f ? 1.0f / l : l == l ? 0.0f : l;
     const int tok = gc / p.g, head = u.head * p.g + gc - tok * p.g;
-    unsigned short* out = p.out + (int64_t)(u.row0 + tok) * p.out_stride + (int64_t)head * D + 32 * dt + 4 * h;
+    unsigned short* out = p.out + (int64_t)(u.row0 + tok) * p.out_stride + (int64_t)head * D + 8 * Q * piece + 4 * h;
 #pragma unroll
-    for (int q4 = 0; q4 < 4; ++q4)
+    for (int q4 = 0; q4 < Q; ++q4)
         *reinterpret_cast<uint2_t*>(out + 8 * q4) =
             uint2_t{T::pack2(o[q4][0] * inv, o[q4][1] * inv), T::pack2(o[q4][2] * inv, o[q4][3] * inv)};
 }
@@ -911,8 +938,12 @@ static hipError_t tree_launch_as(TreeParams p, hipStream_t stream) {
     paged_attn_tree_kernel<T, D, COLW, PARTS, E4M3><<<(unsigned)workers, 64 * COLW * PARTS, 0, stream>>>(p);
     hipError_t rc = hipGetLastError();
     if (rc != hipSuccess || workers == 1) return rc;
-    paged_attn_tree_merge_kernel<T, D, COLW>
-        <<<(unsigned)((p.by_unit ? most : workers - 1) * p.slot_waves * (D / 32)), 256, 0, stream>>>(p);
+    // (32 elements of the heads to a workgroup where there are enough of them, 8 otherwise)
+    const int64_t groups = (p.by_unit ? most : workers - 1) * p.slot_waves;
+    if (groups * (D / 32) >= 2 * device_cu_count())
+        paged_attn_tree_merge_kernel<T, D, COLW, 4><<<(unsigned)(groups * (D / 32)), 256, 0, stream>>>(p);
+    else
+        paged_attn_tree_merge_kernel<T, D, COLW, 1><<<(unsigned)(groups * (D / 8)), 256, 0, stream>>>(p);
     return hipGetLastError();
 }
 
