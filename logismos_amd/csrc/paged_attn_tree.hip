@@ -196,7 +196,8 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
     constexpr int kDeep = (kAlone && !E4M3 && D > 64) || kWide ? 1 : 2;
     constexpr bool kAsIs = E4M3 && __is_same(T, PackedBf16);  // K in bf16, whose range is that of the cache
     static_assert(kPer * kMovers * 8 == kTreeKeys * D, "whole pieces");
-    __shared__ __attribute__((aligned(16))) unsigned short lds[PARTS * kRings];
+    constexpr int kJoin = PARTS > 1 ? COLW * PARTS * tree_wave_floats(D) * 2 : 0;  // where the parts' results meet
+    __shared__ __attribute__((aligned(16))) unsigned short lds[PARTS * kRings > kJoin ? PARTS * kRings : kJoin];
     __shared__ __attribute__((aligned(16))) int rows_lds[2 * kPlaces];
     __shared__ __attribute__((aligned(16))) uint8_t exps_lds[E4M3 ? 64 * kPlaces : 16];
     __shared__ __attribute__((aligned(16))) unsigned short tops_lds[E4M3 ? 2 * kPlaces : 8];
@@ -762,7 +763,6 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
             }
         } else {
             // the parts through LDS; of a wave's 32 columns each part then joins every PARTS-th 32 elements
-            static_assert(COLW * PARTS * tree_wave_floats(D) * 4 <= 2 * PARTS * kRings, "the parts' results fit");
             float* const mine = reinterpret_cast<float*>(lds) + (wave * PARTS + part) * tree_wave_floats(D);
 #pragma unroll
             for (int dt = 0; dt < kTiles; ++dt)
@@ -953,6 +953,13 @@ static hipError_t tree_launch(const TreeParams& p, hipStream_t stream) {
     if constexpr (D <= 128) {
         if (cols <= 32) return tree_launch_as<T, D, 1, 4, E4M3>(p, stream);
         if (cols <= 64) return tree_launch_as<T, D, 2, 2, E4M3>(p, stream);
+        // Few units of many tiles: eight waves of two parts, one workgroup to a compute unit, leave half as many parts of units to be put together
+        // as two workgroups of four waves do.  us, four / eight waves, 32 / 8 heads of 128, 24 rows: one context of 131072 126 / 117, of
+        // 65536 57 / 54, but e4m3 15 rows of 12 / 2 heads, 16 contexts of 500 19.1 / 21.4.
+        const int64_t units = packed_tiles(p.total, p.num_seqs, p.g, 128) * p.hkv;
+        const int64_t tiles = ((int64_t)p.block_size * p.max_blocks + kTreeKeys - 1) / kTreeKeys;
+        if (cols <= 128 && units <= 64 && units * tiles >= 16 * kTreeWorkers)
+            return tree_launch_as<T, D, 4, 2, E4M3>(p, stream);
     }
     if constexpr (D == 64 || D == 128)
         if (cols > 128) return tree_launch_as<T, D, 8, 1, E4M3>(p, stream);
