@@ -10,8 +10,9 @@
 // more of the range of a type whose steps grow with the values, for two more roundings).  The exponents of neighbouring rows of a head lie
 // side by side, so that the attention reads those of 16 keys at once.
 //
-// Bound by memory: an element is read and written once.  d / 8 lanes take a head row, 16 bytes each.  A workgroup takes the
-// rows of up to 16 neighbouring tokens, so that the exponent bytes of a block are written within one compute unit.
+// Bound by memory: an element is read and written once.  d / 8 lanes take a head row, 16 bytes each; its maximum is taken of the
+// values' bits, and the conversions scale (two elements an instruction; written out in fp32, conversion, product, clamp and NaN, they
+// were as long as the memory: 32768 rows of 8 heads of 128, 202 MB, 52 us, now 42, 4.8 TB/s; read back 47, a large copy 5.2).
 #include "device_utils.hpp"
 #include "launch_common.hpp"
 #include "packed_rows.hpp"
@@ -38,14 +39,38 @@ struct E4m3Params {
 
 // Largest of the LANES lanes of a head row (LANES a power of two up to 32).
 template <int LANES>
-__device__ __forceinline__ float row_lanes_max(float v) {
-    if constexpr (LANES > 1) v = fmaxf(v, lane_xor_f32<1>(v));
-    if constexpr (LANES > 2) v = fmaxf(v, lane_xor_f32<2>(v));
-    if constexpr (LANES > 4) v = fmaxf(v, lane_xor_f32<4>(v));
-    if constexpr (LANES > 8) v = fmaxf(v, lane_xor_f32<8>(v));
-    if constexpr (LANES > 16) v = fmaxf(v, lane_xor_f32<16>(v));
+__device__ __forceinline__ int row_lanes_max(int v) {
+    if constexpr (LANES > 1) v = max(v, lane_xor_i32<1>(v));
+    if constexpr (LANES > 2) v = max(v, lane_xor_i32<2>(v));
+    if constexpr (LANES > 4) v = max(v, lane_xor_i32<4>(v));
+    if constexpr (LANES > 8) v = max(v, lane_xor_i32<8>(v));
+    if constexpr (LANES > 16) v = max(v, lane_xor_i32<16>(v));
     return v;
 }
+
+// The 16-bit types: magnitudes compare as their bits do.
+struct E4m3F16 {
+    static constexpr unsigned kInf = 0x7c00u;
+    static __device__ __forceinline__ float value(unsigned bits) {
+        return (float)__builtin_bit_cast(_Float16, (unsigned short)bits);
+    }
+    template <bool HI>
+    static __device__ __forceinline__ unsigned pack(unsigned into, unsigned pair, float scale) {
+        typedef short short2_t __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(
+                                                __builtin_bit_cast(short2_t, into), __builtin_bit_cast(half2_t, pair), scale, HI));
+    }
+};
+struct E4m3Bf16 {
+    static constexpr unsigned kInf = 0x7f80u;
+    static __device__ __forceinline__ float value(unsigned bits) { return __uint_as_float(bits << 16); }
+    template <bool HI>
+    static __device__ __forceinline__ unsigned pack(unsigned into, unsigned pair, float scale) {
+        typedef short short2_t __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(
+                                                __builtin_bit_cast(short2_t, into), __builtin_bit_cast(bf16x2_t, pair), scale, HI));
+    }
+};
 
 // The exponent of a row whose largest finite magnitude is `top` (0: the lowest).
 __device__ __forceinline__ int e4m3_exponent(float top) {
@@ -71,51 +96,64 @@ __device__ __forceinline__ E4m3Item e4m3_item(const E4m3Params& p, int t0, int i
     return {t0 + t, rest >= p.hkv ? rest - p.hkv : rest, rest >= p.hkv};
 }
 
-template <typename E, int LANES>
+template <typename T, int LANES>
 __global__ __launch_bounds__(kE4m3Threads) void kv_write_e4m3_kernel(const E4m3Params p) {
-    typedef E elems __attribute__((ext_vector_type(8)));
     constexpr int kGroups = kE4m3Threads / LANES, kAhead = 4;  // items that a group has in flight
     const int t0 = blockIdx.x * p.tok;
     const int n = (p.tokens - t0 < p.tok ? p.tokens - t0 : p.tok) * 2 * p.hkv;
     const int at = threadIdx.x % LANES;
     const bool mine = 8 * at < p.d;  // (a width that is no power of two leaves lanes over)
     for (int i0 = threadIdx.x / LANES; i0 < n; i0 += kAhead * kGroups) {
-        elems x[kAhead];
+        uint4_t x[kAhead];
         int64_t slot[kAhead];
 #pragma unroll
         for (int a = 0; a < kAhead; ++a) {
             const int i = i0 + a * kGroups;
             slot[a] = -1;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[a][j] = (E)0.0f;
+            x[a] = uint4_t{0, 0, 0, 0};
             if (i >= n) continue;
             const E4m3Item it = e4m3_item(p, t0, i);
             slot[a] = p.slots[it.token];
-            const E* src = static_cast<const E*>(it.is_v ? p.v_in : p.k_in) +
-                           it.token * (it.is_v ? p.v_stride : p.k_stride) + (int64_t)it.head * p.d + 8 * at;
-            if (mine) x[a] = *reinterpret_cast<const elems*>(src);
+            const unsigned short* src = static_cast<const unsigned short*>(it.is_v ? p.v_in : p.k_in) +
+                                        it.token * (it.is_v ? p.v_stride : p.k_stride) + (int64_t)it.head * p.d + 8 * at;
+            if (mine) x[a] = *reinterpret_cast<const uint4_t*>(src);
         }
 #pragma unroll
         for (int a = 0; a < kAhead; ++a) {
-            float f[8], top = 0.0f;
+            unsigned most = 0;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                f[j] = (float)x[a][j];
-                const float m = fabsf(f[j]);
-                top = fmaxf(top, m < INFINITY ? m : 0.0f);  // (of the finite ones)
+            for (int w = 0; w < 4; ++w)
+                most = max(most, max(x[a][w] & 0x7fffu, (x[a][w] >> 16) & 0x7fffu));
+            most = (unsigned)row_lanes_max<LANES>((int)most);
+            int e = e4m3_exponent(T::value(most));
+            uint2_t c;
+            if (__builtin_expect(most < T::kInf && !(T::value(most) > 448.0f * 4294967296.0f), 1)) {
+                const float scale = __int_as_float((127 + e) << 23);
+                c[0] = T::template pack<true>(T::template pack<false>(0u, x[a][0], scale), x[a][1], scale);
+                c[1] = T::template pack<true>(T::template pack<false>(0u, x[a][2], scale), x[a][3], scale);
+            } else {  // infinities, NaN, values beyond the cache's range
+                unsigned finite = 0;
+#pragma unroll
+                for (int w = 0; w < 4; ++w)
+#pragma unroll
+                    for (int y = 0; y < 2; ++y) {
+                        const unsigned m = (x[a][w] >> (16 * y)) & 0x7fffu;
+                        finite = max(finite, m < T::kInf ? m : 0u);
+                    }
+                e = e4m3_exponent(T::value((unsigned)row_lanes_max<LANES>((int)finite)));
+                const float scale = __int_as_float((127 - e) << 23);
+#pragma unroll
+                for (int w = 0; w < 2; ++w) {
+                    float f[4];
+#pragma unroll
+                    for (int y = 0; y < 4; ++y)
+                        f[y] = e4m3_in_range(T::value((x[a][2 * w + (y >> 1)] >> (16 * (y & 1))) & 0xffffu) * scale);
+                    const int word = __builtin_amdgcn_cvt_pk_fp8_f32(f[0], f[1], 0, false);
+                    c[w] = (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(f[2], f[3], word, true);
+                }
             }
-            const int e = e4m3_exponent(row_lanes_max<LANES>(top));
             if (slot[a] < 0 || slot[a] >= p.rows) continue;
             const E4m3Item it = e4m3_item(p, t0, i0 + a * kGroups);
-            const float scale = __int_as_float((127 - e) << 23);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) f[j] = e4m3_in_range(f[j] * scale);
-            uint2_t c;
-#pragma unroll
-            for (int w = 0; w < 2; ++w) {
-                int word = __builtin_amdgcn_cvt_pk_fp8_f32(f[4 * w], f[4 * w + 1], 0, false);
-                c[w] = (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(f[4 * w + 2], f[4 * w + 3], word, true);
-            }
             uint8_t* dst = static_cast<uint8_t*>(it.is_v ? p.v_out : p.k_out) +
                            (slot[a] * p.hkv + it.head) * p.d + 8 * at;
             if (mine) *reinterpret_cast<uint2_t*>(dst) = c;
@@ -132,6 +170,24 @@ template <typename E>
 struct alignas(16) E4m3Out {
     E e[8];
 };
+
+// Eight values times a power of two.
+template <typename E>
+__device__ __forceinline__ void e4m3_decode(uint2_t c, float scale, E (&y)[8]) {
+    typedef E pair_t __attribute__((ext_vector_type(2)));
+    static_for<2>([&](auto word) LG_INLINE {
+        static_for<2>([&](auto half) LG_INLINE {
+            constexpr int w = decltype(word)::value;
+            constexpr bool kHi = decltype(half)::value != 0;
+            pair_t v;
+            if constexpr (__is_same(E, float)) v = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(c[w], scale, kHi);
+            else if constexpr (__is_same(E, _Float16)) v = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c[w], scale, kHi);
+            else v = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c[w], scale, kHi);
+            y[4 * w + 2 * kHi] = v[0];
+            y[4 * w + 2 * kHi + 1] = v[1];
+        });
+    });
+}
 
 template <typename E, int LANES>
 __global__ __launch_bounds__(kE4m3Threads) void kv_gather_e4m3_kernel(const E4m3Params p) {
@@ -165,20 +221,16 @@ __global__ __launch_bounds__(kE4m3Threads) void kv_gather_e4m3_kernel(const E4m3
             const E4m3Item it = e4m3_item(p, t0, i);
             const float scale = __int_as_float((int)(e[a] << 23));
             E4m3Out<E> y;
+            constexpr bool kF16 = __is_same(E, _Float16);
+            if (!kF16 || __builtin_expect(e[a] <= 127 + 7, 1)) {  // (448 * 2^7 is within fp16)
+                e4m3_decode(c[a], scale, y.e);
+            } else {  // fp16 ends earlier than the cache
+                float f[8];
+                e4m3_decode(c[a], scale, f);
 #pragma unroll
-            for (int w = 0; w < 2; ++w) {
-                typedef float float2_t __attribute__((ext_vector_type(2)));
-                const float2_t lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)c[a][w], false);
-                const float2_t hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)c[a][w], true);
-                const float f[4] = {lo[0], lo[1], hi[0], hi[1]};
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    float v = f[j] * scale;
-                    if constexpr (sizeof(E) == 2 && !__is_same(E, __bf16)) {  // fp16 ends earlier than the cache
-                        const float in = __builtin_amdgcn_fmed3f(v, -65504.0f, 65504.0f);
-                        v = v == v ? in : v;
-                    }
-                    y.e[4 * w + j] = (E)v;
+                for (int j = 0; j < 8; ++j) {
+                    const float in = __builtin_amdgcn_fmed3f(f[j], -65504.0f, 65504.0f);
+                    y.e[j] = (E)(f[j] == f[j] ? in : f[j]);
                 }
             }
             E* dst = static_cast<E*>(it.is_v ? p.v_out : p.k_out) + it.token * (it.is_v ? p.v_stride : p.k_stride) +
@@ -188,22 +240,35 @@ __global__ __launch_bounds__(kE4m3Threads) void kv_gather_e4m3_kernel(const E4m3
     }
 }
 
+template <typename E>
+struct E4m3Rows {
+    typedef E4m3F16 type;
+};
+template <>
+struct E4m3Rows<__bf16> {
+    typedef E4m3Bf16 type;
+};
+
 template <typename E, bool WRITE>
 static hipError_t kv_e4m3_by_width(E4m3Params p, hipStream_t stream) {
-    // up to 16 tokens to a workgroup, fewer where workgroups are what is missing
-    int tok = 16;
-    while (tok > 1 && p.tokens < 4 * tok * device_cu_count()) tok /= 2;
+    // as many tokens to a workgroup as keep all its lanes at work, fewer where workgroups are what is missing
+    const int lanes = p.d <= 32 ? 4 : p.d <= 64 ? 8 : p.d <= 128 ? 16 : 32;
+    int tok = 2 * kE4m3Threads / lanes / p.hkv;
+    tok = tok < 1 ? 1 : tok > 64 ? 64 : tok;
+    while (tok > 1 && p.tokens < 2 * (int64_t)tok * device_cu_count()) tok /= 2;
     p.tok = tok;
     const unsigned grid = (unsigned)((p.tokens + tok - 1) / tok);
     auto go = [&](auto lanes) {
         constexpr int L = decltype(lanes)::value;
-        if constexpr (WRITE) kv_write_e4m3_kernel<E, L><<<grid, kE4m3Threads, 0, stream>>>(p);
+        if constexpr (WRITE) kv_write_e4m3_kernel<typename E4m3Rows<E>::type, L><<<grid, kE4m3Threads, 0, stream>>>(p);
         else kv_gather_e4m3_kernel<E, L><<<grid, kE4m3Threads, 0, stream>>>(p);
     };
-    if (p.d <= 32) go(ic<4>{});
-    else if (p.d <= 64) go(ic<8>{});
-    else if (p.d <= 128) go(ic<16>{});
-    else go(ic<32>{});
+    switch (lanes) {
+        case 4: go(ic<4>{}); break;
+        case 8: go(ic<8>{}); break;
+        case 16: go(ic<16>{}); break;
+        default: go(ic<32>{});
+    }
     return hipGetLastError();
 }
 
