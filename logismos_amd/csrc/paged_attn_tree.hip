@@ -46,6 +46,7 @@ struct TreeParams {
     int64_t q_stride, out_stride;
     float scale_log2e;
     int workers;
+    int whole;       // a workgroup has a unit, whole
     int by_unit;     // the second launch has a workgroup for every unit, not for every cut
     int slot_waves;  // waves that a slot of the workspace has room for
 };
@@ -131,6 +132,26 @@ __device__ __forceinline__ TreeUnit tree_unit(const TreeChunk& c, int hkv, unsig
     u.head = unit / groups;
     u.group = unit - u.head * groups;
     return u;
+}
+
+// Where unit `unit` of all begins, counted in tiles (units are counted as tiles are), and its tiles; 0: there is no such unit.  Leaves
+// the chunk that it is in.
+template <int COLS>
+__device__ __forceinline__ unsigned tree_unit_at(TreeChunk& c, int num_seqs, int unit, unsigned& pos) {
+    for (;;) {
+        const unsigned units = wave_scan((unsigned)c.units);
+        const int all = __builtin_amdgcn_readlane((int)units, 63);
+        if (unit < all) {
+            const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(units > (unsigned)unit));
+            unit -= __builtin_amdgcn_readlane((int)units, l) - __builtin_amdgcn_readlane(c.units, l);
+            const unsigned tiles = (unsigned)__builtin_amdgcn_readlane(c.tiles, l);
+            pos = (unsigned)__builtin_amdgcn_readlane((int)c.before, l) + (unsigned)unit * tiles;
+            return tiles;
+        }
+        unit -= all;
+        if (c.first + 64 >= num_seqs) return 0;
+        c = tree_chunk<COLS>(c.first + 64, c.end);
+    }
 }
 
 __device__ __forceinline__ unsigned tree_share(unsigned total, int workers) {
@@ -219,13 +240,21 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
     int first = 0;  // of the 64 sequences that the next unit is in, and the tiles in front of them
     unsigned before = 0;
     TreeChunk chunk = tree_chunk<kCols>(0, 0);
-    unsigned total = chunk.end;
-    for (int f = 64; f < p.num_seqs; f += 64) total = tree_chunk<kCols>(f, total).end;
-    const unsigned per = tree_share(total, p.workers);
-    unsigned pos = blockIdx.x * per;
-    if (pos >= total) return;
-    const unsigned end = total - pos < per ? total : pos + per;
-    for (; pos < end; chunk = tree_chunk<kCols>(first, before)) {
+    unsigned pos, end;
+    if (p.whole) {
+        const unsigned tiles = tree_unit_at<kCols>(chunk, p.num_seqs, blockIdx.x, pos);
+        if (tiles == 0) return;
+        end = pos + tiles;
+    } else {
+        unsigned total = chunk.end;
+        for (int f = 64; f < p.num_seqs; f += 64) total = tree_chunk<kCols>(f, total).end;
+        const unsigned per = tree_share(total, p.workers);
+        pos = blockIdx.x * per;
+        if (pos >= total) return;
+        end = total - pos < per ? total : pos + per;
+    }
+    for (bool again = false; pos < end; again = true) {
+        if (again) chunk = tree_chunk<kCols>(first, before);
         while (pos >= chunk.end) {
             first += 64;
             before = chunk.end;
@@ -833,21 +862,9 @@ __global__ __launch_bounds__(256) void paged_attn_tree_merge_kernel(const TreePa
     const unsigned per = tree_share(total, p.workers);
     TreeUnit u;
     if (p.by_unit) {
-        // unit `cut` of all: units are counted as tiles are
-        int unit = cut;
-        for (;;) {
-            const unsigned units = wave_scan((unsigned)c.units);
-            if (unit < __builtin_amdgcn_readlane((int)units, 63)) {
-                const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(units > (unsigned)unit));
-                unit -= __builtin_amdgcn_readlane((int)units, l) - __builtin_amdgcn_readlane(c.units, l);
-                u = tree_unit(c, p.hkv, (unsigned)__builtin_amdgcn_readlane((int)c.before, l) +
-                                            (unsigned)unit * (unsigned)__builtin_amdgcn_readlane(c.tiles, l));
-                break;
-            }
-            unit -= __builtin_amdgcn_readlane((int)units, 63);
-            if (c.first + 64 >= p.num_seqs) return;
-            c = tree_chunk<kCols>(c.first + 64, c.end);
-        }
+        unsigned pos;
+        if (tree_unit_at<kCols>(c, p.num_seqs, cut, pos) == 0) return;
+        u = tree_unit(c, p.hkv, pos);
     } else {
         const unsigned pos = (unsigned)(cut + 1) * per;
         if (pos >= total) return;
@@ -930,6 +947,13 @@ static hipError_t tree_launch_as(TreeParams p, hipStream_t stream) {
     const int64_t most = packed_tiles(p.total, p.num_seqs, p.g, 32 * COLW) * p.hkv;  // units
     const int64_t room = (int64_t)p.block_size * p.max_blocks;
     const int64_t tiles = most * ((room + kTreeKeys - 1) / kTreeKeys);
+    // Few tiles to a unit: a workgroup for every unit, whole, and no second launch.  us, cut / whole, 12 / 2 heads of 128, 7 rows behind 300:
+    // 15.0 / 12.4; 32 / 8, 16 rows behind 200: 21.6 / 13.0; 40 behind 250: 17.5 / 15.6; but heads of 256, 8 rows behind 250: 16.2 / 18.0.
+    p.whole = (room + kTreeKeys - 1) / kTreeKeys <= (D > 128 ? 4 : 8) * PARTS;
+    if (p.whole) {
+        paged_attn_tree_kernel<T, D, COLW, PARTS, E4M3><<<(unsigned)most, 64 * COLW * PARTS, 0, stream>>>(p);
+        return hipGetLastError();
+    }
     int64_t workers = tree_blocks(D, COLW, PARTS) * device_cu_count();
     if (workers > kTreeWorkers * 4 / (COLW > 4 ? COLW : 4)) workers = kTreeWorkers * 4 / (COLW > 4 ? COLW : 4);
     if (workers > (tiles + kTreeLeast - 1) / kTreeLeast) workers = (tiles + kTreeLeast - 1) / kTreeLeast;
@@ -940,7 +964,7 @@ static hipError_t tree_launch_as(TreeParams p, hipStream_t stream) {
     if (rc != hipSuccess || workers == 1) return rc;
     // (32 elements of the heads to a workgroup where there are enough of them, 8 otherwise)
     const int64_t groups = (p.by_unit ? most : workers - 1) * p.slot_waves;
-    if (groups * (D / 32) >= 2 * device_cu_count())
+    if (groups * (D / 32) >= device_cu_count() / 2)
         paged_attn_tree_merge_kernel<T, D, COLW, 4><<<(unsigned)(groups * (D / 32)), 256, 0, stream>>>(p);
     else
         paged_attn_tree_merge_kernel<T, D, COLW, 1><<<(unsigned)(groups * (D / 8)), 256, 0, stream>>>(p);
