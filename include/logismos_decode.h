@@ -1171,7 +1171,7 @@ logismos_status_t logismos_launch_kv_gather_e4m3_f32(const void* k_pool, const v
  * product (those below 2^-25 of a row's largest are off by up to 2^-36 of it).  Rows that see no key are zeros.  Elements
  * of keys that a row does not see do not reach its result, whatever they hold.
  * fp16 pools: fp16 rows.  e4m3 pools: fp16 or bf16 rows; K and V as `logismos_launch_kv_gather_e4m3_f32` returns them, but that V (and for
- * fp16 rows K) of 32 neighbouring keys is taken relative to the largest exponent among them, in fp16: elements below 2^-15 of 2^e of that row lose
+ * fp16 rows K) of 32 neighbouring keys is taken relative to the largest exponent among them, in fp16: elements below 2^-21 of 2^e of that row lose
  * bits, to 2^-25 of it. */
 logismos_status_t logismos_check_paged_attn_tree_shape(int num_seqs, int total_tokens, int max_seqlen_q,
                                                        int num_q_heads, int num_kv_heads, int head_dim,

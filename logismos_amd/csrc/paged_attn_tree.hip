@@ -3,7 +3,7 @@
 //
 //   out[t][h] = softmax_j(q[t][h] . k[j][h / g] * scale) . v[j][h / g],   j < prior, or bit j - prior of t's mask
 //
-// A column is a (token, head of the group) pair of one KV head; a unit is up to 32 WAVES columns of one sequence and KV head, a
+// A column is a (token, head of the group) pair of one KV head; a unit is up to 32 COLW columns of one sequence and KV head, a
 // wave holds 32 of them, and every tile of 32 keys that a unit reads serves all its columns:
 //
 //   S^T[32 keys x 32 columns] = K . Q^T         v_mfma_f32_32x32x16
@@ -11,11 +11,26 @@
 //   O^T[D x 32 columns] += V^T . P              v_mfma_f32_32x32x16, keys in the order that S^T leaves them in
 //
 // The tiles of all units, one behind the other, are dealt out to the workgroups in equal shares, whatever the contexts are; a
-// unit that was cut is put together by a second, small launch from its parts (sums and the maxima they are relative to).
+// unit that was cut is put together by a second, small launch from its parts (sums and what they are relative to).  Where a unit has
+// few tiles at most, every unit has a workgroup and nothing is cut.
 //
-// e4m3 pools: a tile is decoded once, on its way into LDS: c * 2^(e - top) in 16 bits, top the largest exponent of the tile's
-// rows, which goes into the scores of the tile (K) and into the exponents of its probabilities (V).  Elements below 2^-14 of the
-// tile's largest row's step lose bits, to 2^-25 of it; bf16 queries take K as c * 2^e, which bf16 holds as it is.
+// Workgroups: eight waves side by side for more than 128 columns, four for 65 to 128 (two parts of four where units are few and long), two
+// for 33 to 64 in two parts that take the tiles in turn, single waves in four parts for up to 32, so that narrow trees have several tiles in
+// flight too; heads wider than 128 always four. 
+//
+// Schedule as in attn_packed.hip: step i issues S(i + 1) and O(i - 1) around the softmax of tile i; K goes into LDS two tiles
+// ahead of its use and V one, asked for two steps before that.  Where the tiles lie (rows of the pools, for e4m3 the factors of
+// every row) is worked out for 256 tiles at a time and kept in LDS: looked up step by step it was longer than the products.
+//
+// e4m3 pools: a tile is decoded once, on its way into LDS: c * 2^(e - top) in fp16, top the largest exponent of the tile's rows, which
+// goes into the scores of the tile (K) and into the exponents of its probabilities (V).  Elements below 2^-21 of 2^top lose bits, to 2^-25 of it;
+// bf16 queries take K as c * 2^e, which bf16 holds as it is.
+//
+// Bound by memory for narrow trees (one context of 131072, 32 / 8 heads of 128, fp16, 24 rows: 537 MB in 116 us, 4.6 TB/s, 102 of them
+// the first launch), by the matrix cores and what surrounds their steps for wide ones: 32 contexts of 1000 to 8192, e4m3, 64 rows, 113 GFLOP in
+// 182 us.  A step of eight waves over 32 keys takes 2300 clocks, of which its products are 1024 on each of the four matrix cores; beginning a
+// unit costs 6 us (its sequence, its places, its first tiles), and of a wide unit that is cut the parts are 135 KB each, written and read again: 23
+// us of the 182.
 #include "device_utils.hpp"
 #include "launch_common.hpp"
 #include "packed_rows.hpp"
@@ -212,7 +227,7 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
     static_assert(kRings == 2 * kKTile + 2 * kVTile, "two tiles each");
     constexpr int kTab = E4M3 && PARTS * D > 256 ? 128 : 256;  // tiles whose places are in LDS at a time
     constexpr int kPlaces = kTab + 4 * PARTS;                  // ... with those that a step may ask for behind the last
-    constexpr bool kWide = D > 128;  // four operands of K and V at a time: there are no registers for more
+    constexpr bool kWide = D > 128;  // (short of registers)
     // Steps between asking for a tile and storing it: two, one where a wave alone has no registers for more.
     constexpr int kDeep = (kAlone && !E4M3 && D > 64) || kWide ? 1 : 2;
     constexpr bool kAsIs = E4M3 && __is_same(T, PackedBf16);  // K in bf16, whose range is that of the cache
