@@ -54,6 +54,8 @@ EXTRA_FLAGS = {
     "qgemm_q4g32.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "attn_packed.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "paged_attn_tree.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "paged_attn_tree_e4m3_fp16.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "paged_attn_tree_e4m3_bf16.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 
 # Kernels that ask for operands in one assembly statement and wait for them in a later one, so that

@@ -29,6 +29,16 @@ def test_widths(n, d, pool, dtype):
 
 
 @pytest.mark.parametrize("pool,dtype", KINDS)
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("n", [1, 8, 16])
+def test_narrow_trees_by_the_tiles_of_all_units(n, d, pool, dtype):
+    """Up to 64 columns, cut: parts of a workgroup for fewer than 2048 tiles and from 12288 on, four waves side by side between."""
+    c = Case(n + d + 7, [n, 2, n // 2], [900, 77, 30], 8, 2, d, pool, dtype)
+    for more in (400, 1500, 6000):
+        _in_a_wide_table(c, more).check()
+
+
+@pytest.mark.parametrize("pool,dtype", KINDS)
 @pytest.mark.parametrize("n", ROWS)
 def test_what_is_not_seen_does_not_matter(n, pool, dtype):
     """NaN in K and V of a new token: only those that see it notice, in any shape of workgroup."""
