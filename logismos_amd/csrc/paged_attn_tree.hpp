@@ -698,11 +698,9 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
                         tops_ahead = top_bytes(i + 3);
                     }
                     __builtin_amdgcn_sched_barrier(0);
-                    
                     if constexpr (COLW >= 4 && D >= 96) __builtin_amdgcn_s_setprio(1);
                     if (active) step(h_c, w0, key0, t0, careful_c);
                     if constexpr (COLW >= 4 && D >= 96) __builtin_amdgcn_s_setprio(0);
-                    
                     __builtin_amdgcn_sched_barrier(0);
                     Regs& then = kDeep == 2 ? now : next;
                     // (waited for here, whichever of the two follows: not known to have arrived, they would be waited for with the next ones)
