@@ -206,6 +206,10 @@ struct TreePiece<true> {
 // fused difference is off by up to half a step of the maximum, which is a factor of all probabilities as long as it is small.
 constexpr float kTreeFar = 1048576.0f;
 
+// Matrix operands of a product, and how many of them are read ahead of it (heads wider than 128 are short of registers).
+constexpr int tree_steps(int d) { return d / 16; }
+constexpr int tree_lead(int d) { return d > 128 ? 2 : tree_steps(d) < 3 ? tree_steps(d) : 3; }
+
 // Elements of the rings of a part, and workgroups that a compute unit holds (by LDS, and two waves to a SIMD by registers).
 constexpr int tree_rings(int d) { return 2 * kTreeKeys * (d + 8 + (d / 32 % 2 ? d : d + 32)); }
 constexpr int tree_blocks(int d, int colw, int parts) {
@@ -218,7 +222,7 @@ template <typename T, int D, int COLW, int PARTS, bool E4M3>
 __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) void paged_attn_tree_kernel(const TreeParams p) {
     constexpr bool kAlone = COLW == 1;
     constexpr int kCols = 32 * COLW, kMovers = kAlone ? 64 : 32 * COLW;  // threads that move K, and V
-    constexpr int kSteps = D / 16, kTiles = D / 32;
+    constexpr int kSteps = tree_steps(D), kTiles = D / 32;
     constexpr int kKRow = D + 8, kVRow = D / 32 % 2 ? D : D + 32;  // elements
     constexpr int kKTile = kTreeKeys * kKRow, kVTile = kTreeKeys * kVRow;
     constexpr int kStride = kTreeKeys * PARTS;         // keys between two tiles of a part
@@ -568,7 +572,8 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
             }
             // The products in pairs of S and O, so that none waits for the one before it, operands kLead pairs ahead, and between any two of
             // them a share of the softmax: its maximum first, then the probabilities.
-            constexpr int kLead = kWide ? 2 : 3, kSlots = 2 * kSteps, kFirst = kSlots * 3 / 16 > 1 ? kSlots * 3 / 16 : 1;
+            constexpr int kLead = tree_lead(D), kSlots = 2 * kSteps, kFirst = kSlots * 3 / 16 > 1 ? kSlots * 3 / 16 : 1;
+            static_assert(kLead <= kSteps, "no operand behind the last");
             uint4_t ka[kSteps], va[kSteps];
             float16_t s_nxt;
 #pragma unroll
