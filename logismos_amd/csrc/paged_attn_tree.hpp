@@ -402,7 +402,8 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
             Tops t;
             t.k = max((int)(both & 0xffu), (int)((both >> 16) & 0xffu)) - 127;
             t.v = max((int)((both >> 8) & 0xffu), (int)(both >> 24)) - 127;
-            if (kAsIs) t.k = 0;
+            // (a tile without rows: its factor would leave nothing of a small scale, and -inf times 0 is NaN)
+            if (kAsIs || t.k == -127) t.k = 0;
             return t;
         };
 
