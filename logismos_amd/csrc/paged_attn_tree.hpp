@@ -472,7 +472,8 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
             }
         };
         // A key that a column does not see has the probability 0 there, and 0 times an infinity or NaN of its V row is NaN: in
-        // tiles that are not seen whole such elements go in as 0, and are added at the end for the columns that see them.
+        // tiles that are not seen whole such elements go in as 0, and are added at the end for the columns that see them, from the part's
+        // first tile on in which there is one (of keys that somebody may see: what lies behind the last one costs nothing).
         auto store_v = [&](int buf, const piece_t* x, const uint8_t* e, const Place& w, int key0) LG_INLINE {
             unsigned short* const to = vs + buf * kVTile;
             const bool whole = is_whole(w) && key0 + kTreeKeys <= u.prior;
@@ -482,16 +483,20 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
                 const int row = E4M3 ? e[key_of(i)] : 0;
                 uint4_t y = decoded(x[i], row, false);
                 if (!whole) {
+                    const int key = key_of(i);
+                    const bool there = key0 + key < u.ctx && (key < 16 ? w.row[0] : w.row[1]) >= 0;
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         const unsigned bad = ((y[j] & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
-                        odd |= bad != 0;
+                        odd |= there && bad != 0;
                         y[j] = !is_there(w) ? 0u : y[j] & ~((bad >> 15) * 0xffffu);
                     }
                 }
                 *reinterpret_cast<uint4_t*>(to + key_of(i) * kVRow + 8 * piece_of(i)) = y;
             }
-            if (!whole && __builtin_amdgcn_ballot_w64(odd) != 0 && lane == 0) odd_parts[part] = 1;
+            // (several waves of a part, if more than one finds such an element first: in the same tile)
+            if (!whole && __builtin_amdgcn_ballot_w64(odd) != 0 && lane == 0 && odd_parts[part] < 0)
+                odd_parts[part] = key0 / kTreeKeys;
         };
         auto v_operand = [&](int buf, int kb, int dt) LG_INLINE {
             typedef short short4_t __attribute__((ext_vector_type(4)));
@@ -740,7 +745,7 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
             }
         };
 
-        if (wave_of_all == 0 && lane < PARTS) odd_parts[lane] = far_parts[lane] = 0;
+        if (wave_of_all == 0 && lane < PARTS) odd_parts[lane] = -1, far_parts[lane] = 0;
         __syncthreads();
         m = TreeRef{kTreeNone, 0.0f};
         l = 0.0f;
@@ -759,8 +764,9 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
                 walk_tiles(ic<1>{});
             }
         }
-        if (__builtin_expect(__builtin_amdgcn_readfirstlane(odd_parts[part]) != 0, 0)) {
-            for (int tile = tile0; tile < tile1 && active; ++tile) {
+        const int odd0 = __builtin_amdgcn_readfirstlane(odd_parts[part]);
+        if (__builtin_expect(odd0 >= 0, 0)) {
+            for (int tile = odd0; tile < tile1 && active; ++tile) {
                 const int key0 = tile * kTreeKeys;
                 const Place w = {{__builtin_amdgcn_readfirstlane(row_of(entry_of(key0))),
                                   __builtin_amdgcn_readfirstlane(row_of(entry_of(key0 + 16)))}};
