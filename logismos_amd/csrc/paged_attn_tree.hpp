@@ -24,7 +24,9 @@
 //
 // e4m3 pools: a tile is decoded once, on its way into LDS: c * 2^(e - top) in fp16, top the largest exponent of the tile's rows, which
 // goes into the scores of the tile (K) and into the exponents of its probabilities (V).  Elements below 2^-21 of 2^top lose bits, to 2^-25 of it;
-// bf16 queries take K as c * 2^e, which bf16 holds as it is.
+// bf16 queries take K as c * 2^e, which bf16 holds as it is.  Of a tile that not all columns see all of (drafted tokens, blocks that are not
+// there) the rows go in as c, and their exponents into scores and probabilities key by key: otherwise a row that a column does not
+// see would take bits from those that it does.  Such a tile takes 2 us more, two or three of them in a unit (32 users below 181 -> 190).
 //
 // Bound by memory for narrow trees (one context of 131072, 32 / 8 heads of 128, fp16, 24 rows: 537 MB in 116 us, 4.6 TB/s, 102 of them
 // the first launch), by the matrix cores and what surrounds their steps for wide ones: 32 contexts of 1000 to 8192, e4m3, 64 rows, 113 GFLOP in
@@ -180,17 +182,19 @@ __device__ __forceinline__ unsigned tree_share(unsigned total, int workers) {
 constexpr int tree_wave_floats(int d) { return 32 * d + 128; }
 
 // Probabilities are relative to a reference that follows the maximum lazily, as in attn_packed.hip: the largest lies between
-// 2^kTreeHead and 2^(kTreeHead + kTreeLazy), so that those down to 2^-25 of a column's largest keep all bits of fp16.  It is the
-// exponent of a probability, a score in units of log 2, and of a tile's rows of V together, and kept as the two: in one number the second
-// would be rounded to steps of the first.
+// 2^kTreeHead and 2^(kTreeHead + kTreeLazy), so that those down to 2^-25 of a column's largest keep all bits of fp16.  It stands for the
+// exponent of a probability and of the row of V that it goes with together, s * scale + v, and is kept as the score s and the exponent v:
+// differences of scores are taken before the scale, and in one number the exponent would be rounded to steps of the score.
 constexpr float kTreeHead = 11.0f, kTreeLazy = 4.0f;
 struct TreeRef {
-    float x, v;
+    float s, v;
 };
-__device__ __forceinline__ float tree_above(TreeRef a, TreeRef b) { return (a.x - b.x) + (a.v - b.v); }
-__device__ __forceinline__ float tree_weight(TreeRef a, TreeRef top) { return fast_exp2(tree_above(a, top)); }
-// The reference of a column that has seen nothing above -inf yet: finite, so that such a key weighs 0 without a test.
-constexpr float kTreeNone = -3e38f;
+// (s is NaN while a column has seen nothing above -inf)
+__device__ __forceinline__ bool tree_none(TreeRef a) { return a.s != a.s; }
+__device__ __forceinline__ float tree_above(TreeRef a, TreeRef b, float scale) {
+    return tree_none(a) ? -INFINITY : tree_none(b) ? INFINITY : fmaf(a.s - b.s, scale, a.v - b.v);
+}
+__device__ __forceinline__ float tree_weight(TreeRef a, TreeRef top, float scale) { return fast_exp2(tree_above(a, top, scale)); }
 
 // 8 elements as they lie in the pools.
 template <bool E4M3>
@@ -202,9 +206,9 @@ struct TreePiece<true> {
     typedef uint2_t type;
 };
 
-// Scores beyond this (in units of log 2) go through once more, multiplied and subtracted in two roundings, the same for the maximum: a
-// fused difference is off by up to half a step of the maximum, which is a factor of all probabilities as long as it is small.
-constexpr float kTreeFar = 1048576.0f;
+// A scaled score less the rounded product of the reference and the scale, in one rounding, is off by up to half a step of the reference, a
+// factor of a tile's probabilities: up to here (in units of log 2) 2^-13, beyond it the difference of a column comes before the scale.
+constexpr float kTreeFar = 4096.0f;
 
 // Matrix operands of a product, and how many of them are read ahead of it (heads wider than 128 are short of registers).
 constexpr int tree_steps(int d) { return d / 16; }
@@ -237,13 +241,14 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
     // Steps between asking for a tile and storing it: two, one where a wave alone has no registers for more.
     constexpr int kDeep = (kAlone && !E4M3 && D > 64) || kWide ? 1 : 2;
     constexpr bool kAsIs = E4M3 && __is_same(T, PackedBf16);  // K in bf16, whose range is that of the cache
+    constexpr bool kUnits = E4M3 && !kAsIs;                   // the scores of a tile have a unit of their own
     static_assert(kPer * kMovers * 8 == kTreeKeys * D, "whole pieces");
     constexpr int kJoin = PARTS > 1 ? COLW * PARTS * tree_wave_floats(D) * 2 : 0;  // where the parts' results meet
     __shared__ __attribute__((aligned(16))) unsigned short lds[PARTS * kRings > kJoin ? PARTS * kRings : kJoin];
     __shared__ __attribute__((aligned(16))) int rows_lds[2 * kPlaces];
     __shared__ __attribute__((aligned(16))) uint8_t exps_lds[E4M3 ? 64 * kPlaces : 16];
     __shared__ __attribute__((aligned(16))) unsigned short tops_lds[E4M3 ? 2 * kPlaces : 8];
-    __shared__ int odd_parts[PARTS], far_parts[PARTS];
+    __shared__ int odd_parts[PARTS];
     const int wave_of_all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int part = wave_of_all / COLW, wave = wave_of_all - part * COLW;
     const int tid = threadIdx.x - part * 64 * COLW, lane = tid & 63, h = lane >> 5, col = lane & 31;
@@ -316,7 +321,10 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
             int row[2];  // of the pools, at which the halves begin; -1: there is none, or the table's entry names no block
         };
         auto is_there = [](const Place& w) LG_INLINE { return (w.row[0] & w.row[1]) >= 0; };  // one half at least
-        auto is_whole = [](const Place& w) LG_INLINE { return (w.row[0] | w.row[1]) >= 0; };
+        // A tile that all columns see, all of it.
+        auto is_whole = [&](const Place& w, int key0) LG_INLINE {
+            return (w.row[0] | w.row[1]) >= 0 && key0 + kTreeKeys <= u.prior;
+        };
         // A key's entry of the table (-1: none) and row in its block; the entry's row of the pools, -1: it names no block.
         struct Entry {
             int block, off;
@@ -357,6 +365,8 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
                     uint4_t both[2];
                     both[0] = *reinterpret_cast<const uint4_t*>(t->k_exp + first);
                     both[1] = *reinterpret_cast<const uint4_t*>(t->v_exp + first);
+                    const bool other_there = lane_xor_i32<1>(at.block) >= 0;
+                    const bool whole = at.block >= 0 && other_there && half_key(i & ~1, from, count) + kTreeKeys <= u.prior;
 #pragma unroll
                     for (int kind = 0; kind < 2; ++kind) {
                         uint4_t e = both[kind];
@@ -367,10 +377,11 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
                             e[w] = bytes >= 4 ? e[w] : bytes > 0 ? e[w] & ((1u << (8 * bytes)) - 1u) : 0u;
                             most = max(max(most, e[w] >> 24), max(e[w] & 0xffu, max((e[w] >> 8) & 0xffu, (e[w] >> 16) & 0xffu)));
                         }
-                        top[kind] = most;
-                        // (kept as what the rows are to be multiplied by, relative to the tile's largest)
+                        // (kept as what the rows are to be multiplied by, relative to the tile's largest; where not all columns see the same
+                        // rows, as they come)
                         const unsigned other = (unsigned)lane_xor_i32<1>((int)most);
-                        const int top_of_tile = kAsIs && kind == 0 ? 127 : (int)max(most, other);
+                        top[kind] = whole ? most : 127u;
+                        const int top_of_tile = !whole || (kAsIs && kind == 0) ? 127 : (int)max(most, other);
 #pragma unroll
                         for (int w = 0; w < 4; ++w) {
                             unsigned r4 = 0;
@@ -392,7 +403,7 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
         auto uniform = [](uint2_t v) LG_INLINE {
             return Place{{__builtin_amdgcn_readfirstlane((int)v[0]), __builtin_amdgcn_readfirstlane((int)v[1])}};
         };
-        // The largest exponents of a tile's rows of K and V.
+        // The largest exponents of a tile's rows of K and V (0: every row is taken by its own).
         struct Tops {
             int k, v;
         };
@@ -402,8 +413,7 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
             Tops t;
             t.k = max((int)(both & 0xffu), (int)((both >> 16) & 0xffu)) - 127;
             t.v = max((int)((both >> 8) & 0xffu), (int)(both >> 24)) - 127;
-            // (a tile without rows: its factor would leave nothing of a small scale, and -inf times 0 is NaN)
-            if (kAsIs || t.k == -127) t.k = 0;
+            if (kAsIs) t.k = 0;
             return t;
         };
 
@@ -442,7 +452,7 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
                 }
             }
         };
-        // A piece of 8 as the kernel wants it: e4m3 rows times 2^(e - top) in 16 bits.
+        // A piece of 8 as the kernel wants it: e4m3 rows times 2^(e - top) in 16 bits, those of a tile that is not whole as they are.
         auto decoded = [&](const piece_t& x, int e, bool as_bf16) LG_INLINE {
             if constexpr (!E4M3) return x;
             else {
@@ -463,11 +473,17 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
             }
         };
         auto exps_at = [&](int i, int kind) LG_INLINE { return exps_lds + (i * PARTS + part) * 64 + 32 * kind; };
-        auto store_k = [&](int buf, const piece_t* x, const uint8_t* e) LG_INLINE {
+        // (a row's byte without a branch around its read: 1 where the tile is not whole)
+        struct Byte {
+            int keep, set;
+        };
+        auto byte_if = [](bool by_row) LG_INLINE { return by_row ? Byte{0xff, 0} : Byte{0, 127}; };
+        auto store_k = [&](int buf, const piece_t* x, const uint8_t* e, const Place& w, int key0) LG_INLINE {
             unsigned short* const to = ks + buf * kKTile;
+            const Byte which = byte_if(kAsIs || is_whole(w, key0));
 #pragma unroll
             for (int i = 0; i < kPer; ++i) {
-                const int row = E4M3 ? e[key_of(i)] : 0;
+                const int row = E4M3 ? (e[key_of(i)] & which.keep) | which.set : 0;
                 *reinterpret_cast<uint4_t*>(to + key_of(i) * kKRow + 8 * piece_of(i)) = decoded(x[i], row, kAsIs);
             }
         };
@@ -476,27 +492,30 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
         // first tile on in which there is one (of keys that somebody may see: what lies behind the last one costs nothing).
         auto store_v = [&](int buf, const piece_t* x, const uint8_t* e, const Place& w, int key0) LG_INLINE {
             unsigned short* const to = vs + buf * kVTile;
-            const bool whole = is_whole(w) && key0 + kTreeKeys <= u.prior;
+            if (__builtin_expect(is_whole(w, key0), 1)) {
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) {
+                    const int row = E4M3 ? e[key_of(i)] : 0;
+                    *reinterpret_cast<uint4_t*>(to + key_of(i) * kVRow + 8 * piece_of(i)) = decoded(x[i], row, false);
+                }
+                return;
+            }
             bool odd = false;
 #pragma unroll
             for (int i = 0; i < kPer; ++i) {
-                const int row = E4M3 ? e[key_of(i)] : 0;
-                uint4_t y = decoded(x[i], row, false);
-                if (!whole) {
-                    const int key = key_of(i);
-                    const bool there = key0 + key < u.ctx && (key < 16 ? w.row[0] : w.row[1]) >= 0;
+                uint4_t y = decoded(x[i], 127, false);
+                const int key = key_of(i);
+                const bool there = key0 + key < u.ctx && (key < 16 ? w.row[0] : w.row[1]) >= 0;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const unsigned bad = ((y[j] & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
-                        odd |= there && bad != 0;
-                        y[j] = !is_there(w) ? 0u : y[j] & ~((bad >> 15) * 0xffffu);
-                    }
+                for (int j = 0; j < 4; ++j) {
+                    const unsigned bad = ((y[j] & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
+                    odd |= there && bad != 0;
+                    y[j] = !is_there(w) ? 0u : y[j] & ~((bad >> 15) * 0xffffu);
                 }
-                *reinterpret_cast<uint4_t*>(to + key_of(i) * kVRow + 8 * piece_of(i)) = y;
+                *reinterpret_cast<uint4_t*>(to + key * kVRow + 8 * piece_of(i)) = y;
             }
             // (several waves of a part, if more than one finds such an element first: in the same tile)
-            if (!whole && __builtin_amdgcn_ballot_w64(odd) != 0 && lane == 0 && odd_parts[part] < 0)
-                odd_parts[part] = key0 / kTreeKeys;
+            if (__builtin_amdgcn_ballot_w64(odd) != 0 && lane == 0 && odd_parts[part] < 0) odd_parts[part] = key0 / kTreeKeys;
         };
         auto v_operand = [&](int buf, int kb, int dt) LG_INLINE {
             typedef short short4_t __attribute__((ext_vector_type(4)));
@@ -533,55 +552,81 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
             return win;
         };
 
-        // What the probabilities and sums of a column are relative to, as two numbers, of a score and of a tile of V (see TreeRef).
-        TreeRef m;
+        TreeRef m;  // what the probabilities and sums of a column are relative to
         float l;
         float16_t o[kTiles];
         uint4_t p_prev[2];
-        float16_t s_cur;
+        float16_t s_even, s_odd;  // scores of a tile by its parity
 
-        // Tile i with S(i) in s_cur, K(i + 1) in K buffer 1 - H and V(i - 1) in V buffer 1 - H; leaves S(i + 1) and P(i).
-        auto step = [&](auto h_c, const Place& w, int key0, const Tops& top, auto careful_c) LG_INLINE {
-            constexpr int H = decltype(h_c)::value;
-            constexpr bool careful = decltype(careful_c)::value != 0;
-            float scale = E4M3 ? ldexpf(p.scale_log2e, top.k) : p.scale_log2e;
-            const float v_top = E4M3 ? (float)top.v : 0.0f;
-            if (!is_whole(w) || key0 + kTreeKeys > u.prior) {
-                const unsigned win = window(w, key0) >> (4 * h);
+        // A tile that not all columns see all of, in front of its step: leaves in s_cur what the exponents of the probabilities are above the
+        // reference, and for e4m3 rows the sum without those of V; returns what raising the reference takes off the exponents so far.
+        // The exponents of e4m3 rows (at `exps`) go into the scores and into those of the probabilities key by key, so that a column has
+        // to do with the keys alone that it sees: its reference is the largest sum of the two.
+        auto apart = [&](float16_t& s_cur, const Place& w, int key0, const uint8_t* exps, float& sum) LG_INLINE {
+            const float scale = p.scale_log2e;
+            const unsigned win = window(w, key0) >> (4 * h);
+            unsigned ek[4], ev[4];
+            if constexpr (E4M3) {
 #pragma unroll
-                for (int e = 0; e < 16; ++e) s_cur[e] = (win >> (8 * (e >> 2) + (e & 3))) & 1u ? s_cur[e] : -INFINITY;
-            }
-            bool raise = false;
-            float drop = 0.0f;  // what raising the reference takes off the exponents so far
-            float ref = m.x;
-            auto follow = [&](float tm) LG_INLINE {
-                drop = tree_above(m, {tm, v_top});
-                raise = drop < -kTreeLazy;
-                m.x = raise ? tm : m.x;
-                if (E4M3) m.v = raise ? v_top : m.v;
-                ref = m.x;
-            };
-            if constexpr (careful) {
-                float tm = -INFINITY;
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    float x = s_cur[e] * scale;
-                    asm volatile("" : "+v"(x));  // (a product of its own, not half of a fused one)
-                    s_cur[e] = x;
-                    tm = fmaxf(tm, x);
+                for (int b = 0; b < 4; ++b) {
+                    ek[b] = *reinterpret_cast<const unsigned*>(exps + 8 * b + 4 * h);
+                    ev[b] = *reinterpret_cast<const unsigned*>(exps + 32 + 8 * b + 4 * h);
                 }
-                follow(fmaxf(tm, lane_xor_f32<32>(tm)));
+            }
+            auto byte = [](const unsigned (&x)[4], int e) LG_INLINE { return (x[e >> 2] >> (8 * (e & 3))) & 0xffu; };
+            float tm = -INFINITY;
 #pragma unroll
-                for (int e = 0; e < 16; ++e) s_cur[e] -= ref;
+            for (int e = 0; e < 16; ++e) {
+                const float x = kUnits ? ldexpf(s_cur[e], (int)byte(ek, e) - 127) : s_cur[e];
+                const unsigned sees = (unsigned)((int)(win << (31 - (8 * (e >> 2) + (e & 3)))) >> 31);  // all bits, or none
+                s_cur[e] = __uint_as_float((__float_as_uint(x) & sees) | (0xff800000u & ~sees));
+                tm = fmaxf(tm, s_cur[e]);
+            }
+            tm = fmaxf(tm, lane_xor_f32<32>(tm));
+            const float base = tm == -INFINITY ? 0.0f : tm;
+            float most = -INFINITY;  // (e4m3: the exponents as their bytes)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                s_cur[e] = E4M3 ? fmaf(s_cur[e] - base, scale, (float)byte(ev, e)) : (s_cur[e] - base) * scale;
+                most = fmaxf(most, s_cur[e]);
+            }
+            most = E4M3 ? fmaxf(most, lane_xor_f32<32>(most)) - 127.0f : tm == -INFINITY ? tm : 0.0f;
+            const bool none = tree_none(m);
+            const float rel = fmaf(base - m.s, scale, most - m.v);
+            // (a little before the step would do it)
+            const bool up = none ? tm > -INFINITY : rel > kTreeLazy - 0.0625f;
+            m.s = up ? tm : m.s;
+            if (E4M3) m.v = up ? most : m.v;
+            const float off = (up ? -most : none ? 0.0f : fmaf(base - m.s, scale, -m.v)) - (E4M3 ? 127.0f : 0.0f);
+            sum = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                s_cur[e] += off;
+                if (E4M3) sum += fast_exp2(s_cur[e] - (float)byte(ev, e) + (127.0f + kTreeHead));
+            }
+            return up ? (none ? -INFINITY : -rel) : 0.0f;
+        };
+
+        // Tile i with S(i) in s_cur (of parity H), K(i + 1) in K buffer 1 - H and V(i - 1) in V buffer 1 - H; leaves S(i + 1) and P(i).
+        auto step = [&](auto h_c, const Place& w, int key0, const Tops& top, const uint8_t* exps) LG_INLINE {
+            constexpr int H = decltype(h_c)::value;
+            float16_t &s_cur = H ? s_odd : s_even, &s_nxt = H ? s_even : s_odd;
+            const bool whole = is_whole(w, key0);
+            // The tile's scores in its own unit, the reference in it and the exponents of V above that of the reference; what raising the reference
+            // takes off the exponents so far.
+            float scale = kUnits ? fminf(ldexpf(p.scale_log2e, top.k), 3e38f) : p.scale_log2e;
+            float ref = kUnits ? ldexpf(m.s, -top.k) : m.s, v_above = E4M3 ? (float)top.v - m.v : 0.0f, drop = 0.0f;
+            float sum_apart = 0.0f;
+            if (__builtin_expect(!whole, 0)) {
+                drop = apart(s_cur, w, key0, exps, sum_apart);
                 scale = 1.0f;
-                ref = 0.0f;
+                ref = v_above = 0.0f;
             }
             // The products in pairs of S and O, so that none waits for the one before it, operands kLead pairs ahead, and between any two of
             // them a share of the softmax: its maximum first, then the probabilities.
-            constexpr int kLead = tree_lead(D), kSlots = 2 * kSteps, kFirst = kSlots * 3 / 16 > 1 ? kSlots * 3 / 16 : 1;
+            constexpr int kLead = tree_lead(D), kSlots = 2 * kSteps, kFirst = kSlots * 3 / 16 > 2 ? kSlots * 3 / 16 : 2;
             static_assert(kLead <= kSteps, "no operand behind the last");
             uint4_t ka[kSteps], va[kSteps];
-            float16_t s_nxt;
 #pragma unroll
             for (int e = 0; e < 16; ++e) s_nxt[e] = 0.0f;
             float tm = -INFINITY, off = 0.0f, sum = 0.0f, even = 0.0f;
@@ -592,13 +637,28 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
             };
             auto share = [&](auto slot_c) LG_INLINE {
                 constexpr int kSlot = decltype(slot_c)::value;
-                if constexpr (kSlot == 0 && !careful) {
+                if constexpr (kSlot == 0) {
 #pragma unroll
                     for (int e = 0; e < 16; ++e) tm = fmaxf(tm, s_cur[e]);
                 }
                 if constexpr (kSlot == kFirst - 1) {
-                    if constexpr (!careful) follow(fmaxf(tm, lane_xor_f32<32>(tm)) * scale);
-                    off = kTreeHead + (v_top - m.v) - ref;
+                    tm = fmaxf(tm, lane_xor_f32<32>(tm));
+                    const float rel = fmaf(tm - ref, scale, v_above);
+                    off = fmaf(-ref, scale, kTreeHead + v_above);
+                    const bool rare = !(rel <= kTreeLazy) | !(fabsf(ref * scale) < kTreeFar);  // (nothing seen so far: NaN)
+                    if (__builtin_expect(__builtin_amdgcn_ballot_w64(rare) != 0, 0)) {
+                        const bool none = tree_none(m), up = none ? tm > -INFINITY : rel > kTreeLazy;
+                        drop = up ? (none ? -INFINITY : -rel) : drop;
+                        m.s = up ? (kUnits ? ldexpf(tm, top.k) : tm) : m.s;
+                        if (E4M3) m.v = up ? (float)top.v : m.v;
+                        ref = up ? tm : none ? 0.0f : ref;
+                        v_above = up ? 0.0f : v_above;
+                        const bool far = !(fabsf(ref * scale) < kTreeFar);
+                        const float by = far ? ref : 0.0f;
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) s_cur[e] -= by;
+                        off = fmaf(far ? 0.0f : -ref, scale, kTreeHead + v_above);
+                    }
                 }
                 static_for<16>([&](auto e_c) LG_INLINE {
                     constexpr int e = decltype(e_c)::value;
@@ -624,29 +684,21 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
             });
             // (F belongs to this step: its results are used by the next one only, and would sink there)
             asm volatile("" : "+v"(pb[0]), "+v"(pb[1]), "+v"(sum));
-            if (__builtin_expect(__builtin_amdgcn_ballot_w64(raise) != 0, 0)) {  // O(i - 1) was relative to the old one
-                const float alpha = raise ? fast_exp2(drop) : 1.0f;
+            if (__builtin_expect(__builtin_amdgcn_ballot_w64(drop != 0.0f) != 0, 0)) {  // O(i - 1) was relative to the old one
+                const float alpha = fast_exp2(drop);
                 l *= alpha;
 #pragma unroll
                 for (int dt = 0; dt < kTiles; ++dt)
 #pragma unroll
                     for (int e = 0; e < 16; ++e) o[dt][e] *= alpha;
-                if (__builtin_amdgcn_ballot_w64(raise && fabsf(m.x) >= kTreeFar) != 0 && lane == 0) far_parts[part] = 1;
             }
-            l += E4M3 ? ldexpf(sum, -top.v) : sum;
-            s_cur = s_nxt;
+            l += !E4M3 ? sum : whole ? ldexpf(sum, -top.v) : sum_apart;
             p_prev[0] = pb[0];
             p_prev[1] = pb[1];
         };
 
-        // The tiles of the part, for scores of any size with careful_c.
-        auto walk_tiles = [&](auto careful_c) LG_INLINE {
-            m = TreeRef{kTreeNone, 0.0f};
-            l = 0.0f;
-#pragma unroll
-            for (int dt = 0; dt < kTiles; ++dt)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) o[dt][e] = 0.0f;
+        // The tiles of the part.
+        auto walk_tiles = [&] LG_INLINE {
             for (int from = tile0; from < tile1; from += kTab) {
                 const int count = min(tile1 - from, kTab), steps = (count + PARTS - 1) / PARTS;
                 if (from != tile0) __syncthreads();  // (the last waves are done with the table)
@@ -685,17 +737,17 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
                         tops_ahead = top_bytes(2);
                     }
                     if (moves_k) {
-                        store_k(0, x0, exps_at(0, 0));
-                        store_k(1, kregs(rb), exps_at(1, 0));
+                        store_k(0, x0, exps_at(0, 0), w0, key0);
+                        store_k(1, kregs(rb), exps_at(1, 0), w1, key0 + kStride);
                     }
                 }
                 // V buffer 1 plays V(-1) in the first step, whose P is 0: finite values
                 for (int i = tid; i < kVTile / 2; i += 64 * COLW) reinterpret_cast<unsigned*>(vs + kVTile)[i] = 0u;
                 together();
 #pragma unroll
-                for (int e = 0; e < 16; ++e) s_cur[e] = 0.0f;
+                for (int e = 0; e < 16; ++e) s_even[e] = 0.0f;
 #pragma unroll
-                for (int j = 0; j < kSteps; ++j) s_cur = T::mfma32(k_operand(0, j), qb[j], s_cur);
+                for (int j = 0; j < kSteps; ++j) s_even = T::mfma32(k_operand(0, j), qb[j], s_even);
                 together();  // (the first step ends with a store into the buffer just read)
                 // step i, H its parity: what a later step needs is asked for in front of it and goes to LDS behind it
                 auto one = [&](auto h_c, int i, Regs& now, Regs& next) LG_INLINE {
@@ -710,7 +762,7 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
                     }
                     __builtin_amdgcn_sched_barrier(0);
                     if constexpr (COLW >= 4 && D >= 96) __builtin_amdgcn_s_setprio(1);
-                    if (active) step(h_c, w0, key0, t0, careful_c);
+                    if (active) step(h_c, w0, key0, t0, exps_at(i, 0));
                     if constexpr (COLW >= 4 && D >= 96) __builtin_amdgcn_s_setprio(0);
                     __builtin_amdgcn_sched_barrier(0);
                     Regs& then = kDeep == 2 ? now : next;
@@ -720,7 +772,7 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
                         if constexpr (kAlone) asm volatile("" : "+v"(then.k[j]));
                         asm volatile("" : "+v"(then.v[j]));
                     }
-                    if (moves_k) store_k(H, kregs(then), exps_at(i + 2, 0));   // K(i + 2)
+                    if (moves_k) store_k(H, kregs(then), exps_at(i + 2, 0), w2, key0 + 2 * kStride);  // K(i + 2)
                     if (moves_v) store_v(H, then.v, exps_at(i, 1), w0, key0);  // V(i)
                     t0 = t1;
                     t1 = t2;
@@ -745,25 +797,16 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
             }
         };
 
-        if (wave_of_all == 0 && lane < PARTS) odd_parts[lane] = -1, far_parts[lane] = 0;
+        if (wave_of_all == 0 && lane < PARTS) odd_parts[lane] = -1;
         __syncthreads();
-        m = TreeRef{kTreeNone, 0.0f};
+        m = TreeRef{NAN, 0.0f};
         l = 0.0f;
 #pragma unroll
         for (int dt = 0; dt < kTiles; ++dt)
 #pragma unroll
             for (int e = 0; e < 16; ++e) o[dt][e] = 0.0f;
-        if (u.ctx > 0) {
-            walk_tiles(ic<0>{});
-            __syncthreads();
-            int far = 0;
-#pragma unroll
-            for (int q = 0; q < PARTS; ++q) far |= far_parts[q];
-            if (__builtin_expect(__builtin_amdgcn_readfirstlane(far) != 0, 0)) {
-                __syncthreads();  // (the first tiles go where the last ones were)
-                walk_tiles(ic<1>{});
-            }
-        }
+        if (u.ctx > 0) walk_tiles();
+        __syncthreads();
         const int odd0 = __builtin_amdgcn_readfirstlane(odd_parts[part]);
         if (__builtin_expect(odd0 >= 0, 0)) {
             for (int tile = odd0; tile < tile1 && active; ++tile) {
@@ -771,7 +814,7 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
                 const Place w = {{__builtin_amdgcn_readfirstlane(row_of(entry_of(key0))),
                                   __builtin_amdgcn_readfirstlane(row_of(entry_of(key0 + 16)))}};
                 // (each part for its own tiles: the parts are added up)
-                if ((tile - tile0) % kTab % PARTS != part || !is_there(w) || (is_whole(w) && key0 + kTreeKeys <= u.prior)) continue;
+                if ((tile - tile0) % kTab % PARTS != part || !is_there(w) || is_whole(w, key0)) continue;
                 const unsigned win = window(w, key0);
                 for (int key = 0; key < kTreeKeys; ++key) {
                     const bool sees = (win >> key) & 1u;
@@ -814,7 +857,7 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
                     for (int q4 = 0; q4 < 4; ++q4)
                         reinterpret_cast<float4_t*>(slot)[(4 * dt + q4) * 64 + lane] =
                             float4_t{o[dt][4 * q4], o[dt][4 * q4 + 1], o[dt][4 * q4 + 2], o[dt][4 * q4 + 3]};
-                slot[32 * D + lane] = h ? m.v : m.x;
+                slot[32 * D + lane] = h ? m.v : m.s;
                 slot[32 * D + 64 + lane] = l;
             }
         } else {
@@ -826,21 +869,21 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
                 for (int q4 = 0; q4 < 4; ++q4)
                     reinterpret_cast<float4_t*>(mine)[(4 * dt + q4) * 64 + lane] =
                         float4_t{o[dt][4 * q4], o[dt][4 * q4 + 1], o[dt][4 * q4 + 2], o[dt][4 * q4 + 3]};
-            mine[32 * D + lane] = h ? m.v : m.x;
+            mine[32 * D + lane] = h ? m.v : m.s;
             mine[32 * D + 64 + lane] = l;
             __syncthreads();
             if (active) {
                 const float* const parts = reinterpret_cast<const float*>(lds) + wave * PARTS * tree_wave_floats(D);
-                TreeRef refs[PARTS], top = {kTreeNone, 0.0f};
+                TreeRef refs[PARTS], top = {NAN, 0.0f};
                 float weight[PARTS], sum = 0.0f;
 #pragma unroll
                 for (int q = 0; q < PARTS; ++q) {
                     refs[q] = {parts[q * tree_wave_floats(D) + 32 * D + col], parts[q * tree_wave_floats(D) + 32 * D + 32 + col]};
-                    if (tree_above(refs[q], top) > 0.0f) top = refs[q];
+                    if (tree_above(refs[q], top, t->scale_log2e) > 0.0f) top = refs[q];
                 }
 #pragma unroll
                 for (int q = 0; q < PARTS; ++q) {
-                    weight[q] = tree_weight(refs[q], top);
+                    weight[q] = tree_weight(refs[q], top, t->scale_log2e);
                     sum += parts[q * tree_wave_floats(D) + 32 * D + 64 + lane] * weight[q];
                 }
                 const float inv = sum > 0.0f ? 1.0f / sum : sum == sum ? 0.0f : sum;
@@ -863,7 +906,7 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
                                 uint2_t{T::pack2(v[0] * inv, v[1] * inv), T::pack2(v[2] * inv, v[3] * inv)};
                     }
                 if (!all && part == 0) {
-                    slot[32 * D + lane] = h ? top.v : top.x;
+                    slot[32 * D + lane] = h ? top.v : top.s;
                     slot[32 * D + 64 + lane] = sum;
                 }
             }
@@ -905,14 +948,14 @@ __global__ __launch_bounds__(256) void paged_attn_tree_merge_kernel(const TreePa
     const int cols = u.rows * p.g, c0 = u.group * kCols + of_unit * 32;
     if (first == last || (!p.by_unit && first != cut) || c0 >= cols) return;
 
-    TreeRef m = {kTreeNone, 0.0f};
+    TreeRef m = {NAN, 0.0f};
     float l = 0.0f;
     float4_t o[Q];
 #pragma unroll
     for (int q4 = 0; q4 < Q; ++q4) o[q4] = float4_t{0, 0, 0, 0};
     auto join = [&](TreeRef m2, float l2, const float4_t* o2) LG_INLINE {
-        const TreeRef top = tree_above(m2, m) > 0.0f ? m2 : m;
-        const float mine = tree_weight(m, top), its = tree_weight(m2, top);
+        const TreeRef top = tree_above(m2, m, p.scale_log2e) > 0.0f ? m2 : m;
+        const float mine = tree_weight(m, top, p.scale_log2e), its = tree_weight(m2, top, p.scale_log2e);
         m = top;
         l = l * mine + l2 * its;
 #pragma unroll
@@ -941,7 +984,7 @@ __global__ __launch_bounds__(256) void paged_attn_tree_merge_kernel(const TreePa
     if (wave > 0) {
 #pragma unroll
         for (int q4 = 0; q4 < Q; ++q4) theirs[wave - 1][q4][lane] = o[q4];
-        ml[wave - 1][0][lane] = m.x;
+        ml[wave - 1][0][lane] = m.s;
         ml[wave - 1][1][lane] = m.v;
         ml[wave - 1][2][lane] = l;
     }

@@ -5,6 +5,8 @@ import numpy as np
 import pytest
 
 from logismos_amd import hip
+from tests import packed_reference as P
+from tests import tree_reference as R
 from tests.test_gpu_paged_attn_tree import KINDS, Case
 
 pytestmark = pytest.mark.gpu
@@ -48,3 +50,83 @@ def test_rows_that_nobody_sees_take_no_time():
         outs.append(c.bufs["out"].to_numpy(c.q.dtype, c.q.shape))
     assert np.array_equal(*outs)
     assert times[1] < 1.4 * times[0], times
+
+
+def _wide(c, blocks=2000):
+    """The same sequences in a table with room for many more blocks: their units may be cut."""
+    c.table = np.concatenate([c.table, np.full((len(c.table), blocks), -1, np.int32)], 1)
+    return c
+
+
+def _drafted(c, s, j):
+    """Block and row of drafted token j of sequence s."""
+    at = int(c.ctx[s] - c.new[s]) + j
+    return c.table[s, at // c.block], at % c.block
+
+
+def _bounded_by_what_is_seen(c, s):
+    """The formula row by row, the bound of each by the exponents of those keys alone that it sees."""
+    (k, ke), (v, ve) = c.values(s)
+    seen = c.visible(s)
+    q = P.from_bits(c.q[c.cu[s]:c.cu[s + 1], :c.hq * c.d], c.dtype).reshape(-1, c.hq, c.d)
+    found = []
+    for i in range(len(q)):
+        mine = seen[i:i + 1]
+        only = [np.where(mine[0][:, None], e, R.LOWEST) for e in (ke, ve)]
+        found.append(R.tree_attention(q[i:i + 1], *(np.where(mine[0][:, None, None], x, 0.0) for x in (k, v)), mine, c.scale,
+                                      c.dtype, *only))
+    return [np.concatenate(x) for x in zip(*found)]
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("which", ["k", "v", "both"])
+@pytest.mark.parametrize("n", ROWS[1:])
+def test_large_rows_of_other_branches(n, which, dtype):
+    """Finite rows at the cache's largest exponent (and bytes beyond it) that some tokens do not see: to those they might as well be
+    zeros, bit for bit; those that see the V row get what the formula gives."""
+    for exponent in (32, 14, 128):
+        c = Case(n, [n, 3 + n // 2], [333, 64], 8, 2, 64, "e4m3", dtype)
+        hit = [(s, int(c.new[s]) // 2) for s in range(2)]
+        for s, j in hit:  # (what the others see, with nothing there)
+            b, row = _drafted(c, s, j)
+            c.k[b, row] = c.v[b, row] = 0
+            c.k_exp[b, :, row] = c.v_exp[b, :, row] = 127 + R.LOWEST
+        for wide in (False, True):
+            if wide:
+                _wide(c)
+            clean = c.run()
+            kept = c.k.copy(), c.v.copy(), c.k_exp.copy(), c.v_exp.copy()
+            rng = np.random.default_rng(n)
+            for s, j in hit:
+                b, row = _drafted(c, s, j)
+                for name in "kv" if which == "both" else which:
+                    getattr(c, name)[b, row] = rng.integers(0x60, 0x7F, (2, 64)) | rng.integers(0, 2, (2, 64)) * 0x80
+                    getattr(c, name + "_exp")[b, :, row] = 127 + exponent
+            out = c.run()
+            for s, j in hit:
+                rows, sees = np.arange(c.cu[s], c.cu[s + 1]), np.asarray(c.seen[s])[:, j]
+                assert (~sees).any() and np.array_equal(out[rows[~sees]], clean[rows[~sees]])
+                if which == "v" and exponent < 127 and dtype == "bf16":
+                    want, bound = _bounded_by_what_is_seen(c, s)
+                    P.assert_within(P.from_bits(out[rows], dtype).reshape(want.shape), want, bound, f"sequence {s}")
+            c.k, c.v, c.k_exp, c.v_exp = kept
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("n", ROWS)
+def test_drafted_rows_of_any_exponents(n, dtype):
+    """Drafted K and V rows from 2^-60 to 2^10 of one another; every row to a bound of what it sees itself."""
+    c = Case(n + 50, [n, 2 * n // 3 + 1], [90, 0], 8, 2, 64, "e4m3", dtype)
+    rng = np.random.default_rng(n)
+    for s in range(2):
+        for j in range(int(c.new[s])):
+            b, row = _drafted(c, s, j)
+            c.k_exp[b, :, row] = 127 + rng.integers(-40, -6, 2)
+            c.v_exp[b, :, row] = 127 + rng.integers(-64, 5, 2)
+    for wide in (False, True):
+        if wide:
+            _wide(c)
+        out = c.run()
+        for s in range(2):
+            want, bound = _bounded_by_what_is_seen(c, s)
+            P.assert_within(P.from_bits(out[c.cu[s]:c.cu[s + 1]], dtype).reshape(want.shape), want, bound, f"sequence {s}")
