@@ -597,7 +597,8 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
             const bool up = none ? tm > -INFINITY : rel > kTreeLazy - 0.0625f;
             m.s = up ? tm : m.s;
             if (E4M3) m.v = up ? most : m.v;
-            const float off = (up ? -most : none ? 0.0f : fmaf(base - m.s, scale, -m.v)) - (E4M3 ? 127.0f : 0.0f);
+            // (nothing to see: from anywhere, since the difference times the scale may be beyond fp32)
+            const float off = (up ? -most : tm == -INFINITY ? 0.0f : fmaf(base - m.s, scale, -m.v)) - (E4M3 ? 127.0f : 0.0f);
             sum = 0.0f;
 #pragma unroll
             for (int e = 0; e < 16; ++e) {

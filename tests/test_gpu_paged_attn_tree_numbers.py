@@ -130,3 +130,48 @@ def test_drafted_rows_of_any_exponents(n, dtype):
         for s in range(2):
             want, bound = _bounded_by_what_is_seen(c, s)
             P.assert_within(P.from_bits(out[c.cu[s]:c.cu[s + 1]], dtype).reshape(want.shape), want, bound, f"sequence {s}")
+
+
+@pytest.mark.parametrize("pool,dtype", KINDS)
+@pytest.mark.parametrize("n", [1, 16, 60])
+@pytest.mark.parametrize("shift,low", [(120, 0), (126, 0), (126, 300), (90, 0)])
+def test_scores_that_are_beyond_fp32_with_the_scale(shift, low, n, pool, dtype):
+    """Whole numbers as scores (less `low`, the same for all keys), times a scale with which they are no numbers of 32 bits: the keys
+    with the largest share all the weight.  e4m3: also with K at the cache's largest exponent."""
+    for exponent in (None, 32) if pool == "e4m3" else (None,):
+        c = Case(n + shift, [n, 3], [300, 40], 8, 2, 64, pool, dtype, scale=2.0 ** shift)
+        rng = np.random.default_rng(n)
+        q, k = rng.integers(-1, 2, c.q.shape), rng.integers(-1, 2, c.k16.shape)
+        q.reshape(-1, 8, 64)[..., 0], k[..., 0] = 16, -low / 16
+        c.q = P.to_bits(q, dtype)
+        if pool == "e4m3":
+            k[..., 0] = -low // 16 // 2 * 2  # (a number of e4m3 beside 1)
+        c.set_rows(k.astype(np.float16), c.v16)
+        if exponent is not None:
+            c.k_exp[:] = 127 + exponent
+        for wide in (False, True):
+            if wide:
+                _wide(c)
+            out = c.run()
+            for s in range(2):
+                (k, _), (v, ve) = c.values(s)
+                q = P.from_bits(c.q[c.cu[s]:c.cu[s + 1]], dtype).reshape(-1, 8, 64)
+                got, seen = P.from_bits(out[c.cu[s]:c.cu[s + 1]], dtype).reshape(q.shape), c.visible(s)
+                for h in range(8):
+                    score = np.where(seen, q[:, h] @ k[:, h // 4].T, -np.inf)
+                    w = (score == score.max(1, keepdims=True)).astype(float)
+                    w /= w.sum(1, keepdims=True)
+                    want, size = w @ v[:, h // 4], w @ np.abs(v[:, h // 4])
+                    # equal weights, off by half a step of fp16 and by fp32 sums; of neighbours' rows of V 2^-25 of the largest step
+                    bound = (2.0 ** -11 + 2.0 ** -16) * size + 2.0 ** -24 * np.abs(v).max() + P.HALF_STEP[dtype] * np.abs(want) + 2.0 ** -25
+                    P.assert_within(got[:, h], want, bound)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("scale", [1e-30, 1e-37])
+def test_scales_that_vanish_beside_the_exponents_of_k(scale, dtype):
+    """Rows of K at the cache's lowest exponent: every key weighs the same."""
+    c = Case(3, [20, 5], [200, 31], 8, 2, 64, "e4m3", dtype, scale=scale)
+    c.k_exp[:] = 127 - 64
+    c.check()
+    _wide(c).check()
