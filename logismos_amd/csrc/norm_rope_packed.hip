@@ -59,12 +59,12 @@ __device__ __forceinline__ float head_lanes_sum(float v) {
     return v;
 }
 
-// 1 / sqrt(sum / d + eps), the sum that of the squares times 2^(2 down): rows whose squares leave the range of fp32 (bf16 and fp32 values
-// beyond 2^63) are summed again in units of 2^70.
-constexpr float kNormDown = 0x1p-70f;
+// 1 / sqrt(sum / d + eps).  Rows whose squares leave the range of fp32 (bf16 and fp32 values beyond 2^59) are summed again in units of
+// 2^70, and their elements taken in units of 2^30: the reciprocal of a large root, and a small gain times it, would be below fp32's range.
+constexpr float kNormDown = 0x1p-70f, kNormUnit = 0x1p-30f;
 __device__ __forceinline__ float inv_rms(float sum, float d, float eps) { return 1.0f / sqrtf(sum / d + eps); }
 __device__ __forceinline__ float inv_rms_down(float sum, float d, float eps) {
-    return kNormDown / sqrtf(sum / d + eps * kNormDown * kNormDown);
+    return kNormDown / kNormUnit / sqrtf(sum / d + eps * kNormDown * kNormDown);
 }
 
 template <typename E, int V, bool INTERLEAVED, int LANES>
@@ -121,6 +121,7 @@ __global__ __launch_bounds__(kNormRopeThreads) void norm_rope_packed_kernel(cons
             return sum;
         };
         float inv = 1.0f;
+        bool down = false;
         const bool once = p.units <= LANES;  // (uniform)
         if (once && lane < p.units) load(lane);
         if (gain != nullptr) {
@@ -134,7 +135,8 @@ __global__ __launch_bounds__(kNormRopeThreads) void norm_rope_packed_kernel(cons
             };
             const float sum = total(1.0f);
             inv = inv_rms(sum, (float)p.d, p.eps);
-            if (__builtin_expect(!(sum < INFINITY), 0)) inv = inv_rms_down(total(kNormDown), (float)p.d, p.eps);
+            down = !(sum < INFINITY);
+            if (__builtin_expect(down, 0)) inv = inv_rms_down(total(kNormDown), (float)p.d, p.eps);
         }
         for (int u = lane; u < p.units; u += LANES) {
             if (!once) load(u);
@@ -146,6 +148,13 @@ __global__ __launch_bounds__(kNormRopeThreads) void norm_rope_packed_kernel(cons
                 y[e] = (float)b.e[e];
             }
             if (gain != nullptr) {
+                if (__builtin_expect(down, 0)) {
+#pragma unroll
+                    for (int e = 0; e < V; ++e) {
+                        x[e] *= kNormUnit;
+                        y[e] *= kNormUnit;
+                    }
+                }
 #pragma unroll
                 for (int e = 0; e < V; ++e) {
                     x[e] *= inv * gain[a0 + e];
