@@ -955,9 +955,10 @@ __global__ __launch_bounds__(256) void paged_attn_tree_merge_kernel(const TreePa
 #pragma unroll
     for (int q4 = 0; q4 < Q; ++q4) o[q4] = float4_t{0, 0, 0, 0};
     auto join = [&](TreeRef m2, float l2, const float4_t* o2) LG_INLINE {
-        const TreeRef top = tree_above(m2, m, p.scale_log2e) > 0.0f ? m2 : m;
-        const float mine = tree_weight(m, top, p.scale_log2e), its = tree_weight(m2, top, p.scale_log2e);
-        m = top;
+        const float above = tree_above(m2, m, p.scale_log2e);
+        const bool up = above > 0.0f;
+        const float other = fast_exp2(-fabsf(above)), mine = up ? other : 1.0f, its = up ? 1.0f : other;
+        m = {up ? m2.s : m.s, up ? m2.v : m.v};
         l = l * mine + l2 * its;
 #pragma unroll
         for (int q4 = 0; q4 < Q; ++q4)
