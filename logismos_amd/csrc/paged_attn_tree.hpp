@@ -283,6 +283,7 @@ __global__ __launch_bounds__(64 * COLW * PARTS, tree_blocks(D, COLW, PARTS)) voi
         if (again) chunk = tree_chunk<kCols>(first, before);
         while (pos >= chunk.end) {
             first += 64;
+            if (first >= p.num_seqs) return;  // (lengths that overlap: their tiles may be more than 32 bits count)
             before = chunk.end;
             chunk = tree_chunk<kCols>(first, before);
         }
@@ -940,7 +941,10 @@ __global__ __launch_bounds__(256) void paged_attn_tree_merge_kernel(const TreePa
     } else {
         const unsigned pos = (unsigned)(cut + 1) * per;
         if (pos >= total) return;
-        while (pos >= c.end) c = tree_chunk<kCols>(c.first + 64, c.end);
+        while (pos >= c.end) {
+            if (c.first + 64 >= p.num_seqs) return;
+            c = tree_chunk<kCols>(c.first + 64, c.end);
+        }
         u = tree_unit(c, p.hkv, pos);
         if (u.tile == 0) return;
     }
