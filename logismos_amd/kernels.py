@@ -574,10 +574,11 @@ def launch_kv_gather_e4m3(k_pool, k_exp, v_pool, v_exp, slot_mapping, k_out, v_o
 def tree_mask(parents, mask_words: int = 0) -> np.ndarray:
     """uint64 [tokens][mask_words] for `launch_paged_attn_tree`: of every drafted token its ancestors and
     itself; parents[i] is an earlier token or -1; 0 words: as many as the tokens need."""
-    parents = np.ascontiguousarray(parents, np.int32)
+    given = np.asarray(parents)
+    parents = np.ascontiguousarray(given, np.int32)
     words = mask_words or max(1, (parents.size + 63) // 64)
     out = np.empty((parents.size, max(words, 1)), np.uint64)
-    if parents.ndim != 1 or library().logismos_tree_mask(
+    if given.ndim != 1 or not np.array_equal(given, parents) or library().logismos_tree_mask(
             parents.ctypes.data_as(_vp), parents.size, words, out.ctypes.data_as(_vp)) != 0:
         raise UnsupportedShape("tree_mask", "a parent is not an earlier token or -1, or the tokens do not "
                                "fit the words (at most 4)")
