@@ -1062,11 +1062,13 @@ static hipError_t tree_launch(const TreeParams& p, hipStream_t stream) {
         const bool between = units * tiles >= 4 * kTreeWorkers && units * tiles < 24 * kTreeWorkers;
         if (cols <= 32 && (!between || tiles <= 32)) return tree_launch_as<T, D, 1, 4, E4M3>(p, stream);
         if (cols <= 64 && (!between || tiles <= 16)) return tree_launch_as<T, D, 2, 2, E4M3>(p, stream);
-        // Few units of many tiles: eight waves of two parts, one workgroup to a compute unit, leave half as many parts of units to be put together
-        // as two workgroups of four waves do.  us, four / eight waves, 32 / 8 heads of 128, 24 rows: one context of 131072 126 / 117, of
-        // 65536 57 / 54, but e4m3 15 rows of 12 / 2 heads, 16 contexts of 500 19.1 / 21.4.
-        if (cols > 64 && cols <= 128 && units <= 64 && units * tiles >= 16 * kTreeWorkers)
-            return tree_launch_as<T, D, 4, 2, E4M3>(p, stream);
+        // Few units of many tiles over fp16 pools: eight waves of two parts, one workgroup to a compute unit, leave half as many parts of units to be
+        // put together as two workgroups of four waves do.  us, four / eight waves, 32 / 8 heads of 128, 28 rows: one context of 131072 124.8 / 119.0,
+        // of 65536 66.8 / 62.9, four of 40000, 24 rows, 148.6 / 140.8; heads of 96 98.3 / 99.0, 52.6 / 51.5, 115.9 / 110.3; but of 64 72.5 / 71.2,
+        // 43.5 / 43.4, 82.3 / 85.0, and e4m3, whose step is short of registers in eight waves, 109.6 / 106.6, 61.2 / 61.8, 118.3 / 127.9.
+        if constexpr (!E4M3 && D >= 96)
+            if (cols > 64 && cols <= 128 && units <= 64 && units * tiles >= 16 * kTreeWorkers)
+                return tree_launch_as<T, D, 4, 2, E4M3>(p, stream);
     }
     // More than 128 columns: eight waves, which read a tile once where two workgroups of four read it twice, unless the last has few columns.
     // us, four / eight waves, e4m3: 32 contexts of 1000 to 8192, 256 columns of heads of 128, 208 / 192; of 4096, 448 columns of heads of 64,
