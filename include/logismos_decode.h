@@ -1167,9 +1167,11 @@ logismos_status_t logismos_launch_kv_gather_e4m3_f32(const void* k_pool, const v
  *   workspace      `logismos_paged_attn_tree_workspace_bytes(...)` bytes, 16-byte aligned, contents don't matter; not shared by
  *                  calls that can overlap in time
  *
- * One new row per sequence with bit 0 set is a plain decode step.  fp32 scores, softmax and sums; the probabilities are rounded to fp16 for the second
- * product (those below 2^-25 of a row's largest are off by up to 2^-36 of it; e4m3 pools: of the probabilities times 2^e of their V rows).  Rows
- * that see no key are zeros.  Nothing of a key that a row does not see reaches its result, whatever it holds.
+ * One new row per sequence with bit 0 set is a plain decode step.  fp32 scores, softmax and sums.  The probabilities are rounded to fp16 for the
+ * second product, which adds half as much again to the rounding of fp16 results (`logismos_launch_paged_attn_varlen_fp16` has them in two terms);
+ * those below 2^-25 of a row's largest are off by up to 2^-36 of it (e4m3 pools: of the probabilities times 2^e of their V rows, the largest e of 32
+ * neighbouring keys of the context).  Rows that see no key are zeros.  Nothing of a key that a row does not see reaches its result, whatever it holds.
+ * Scores may be any fp32 numbers, and their products with the scale beyond fp32.
  * fp16 pools: fp16 rows.  e4m3 pools: fp16 or bf16 rows; K and V as `logismos_launch_kv_gather_e4m3_f32` returns them, but that V (and for
  * fp16 rows K) of 32 neighbouring keys of the context is taken relative to the largest exponent among them, in fp16: elements below 2^-21 of
  * 2^e of that row lose bits, to 2^-25 of it.  (Not where new tokens are among the 32, or a table entry that names no block.) */

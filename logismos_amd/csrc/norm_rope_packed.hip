@@ -11,9 +11,10 @@
 // a wave has lanes are walked twice, the second time out of the cache.  A workgroup takes a few tokens, whose cos and sin, evaluated once,
 // serve all heads.
 //
-// 32768 rows of 32 + 8 heads of 128, bf16, 671 MB: 134 us, 5.0 TB/s, of the 5.2 of a copy (the rotation alone, rope_packed.hip, 126); 8190 rows of
-// 12 + 2 heads, three axes, pairs side by side 14.4; 24 rows of 14 + 2 heads of 64, fp32, 3.5.  Gains kept in registers took 162 us of the first, the next
-// head's elements asked for ahead 150, eight tokens to a workgroup 145; two 132.6, but more of the small calls.
+// 32768 rows of 32 + 8 heads of 128, bf16, 671 MB: 132 us, 5.1 TB/s, of the 5.2 of a copy (the rotation alone, rope_packed.hip, 126); 8190 rows of
+// 12 + 2 heads, three axes, pairs side by side 14.4; 24 rows of 14 + 2 heads of 64, fp32, 3.6.  Gains kept in registers took 162 us of the first, the next
+// head's elements asked for ahead 150, eight tokens to a workgroup 145; two 132.6, but more of the small calls.  An access is the greatest power of two that
+// divides pairs, rest, width, strides and addresses: with 120 of 128 elements turning (8 bytes) 250 us, with 126 (2 bytes, heads walked twice) 649.
 #include "device_utils.hpp"
 #include "launch_common.hpp"
 #include "packed_rows.hpp"

@@ -11,12 +11,14 @@
 //   O^T[D x 32 columns] += V^T . P              v_mfma_f32_32x32x16, keys in the order that S^T leaves them in
 //
 // The tiles of all units, one behind the other, are dealt out to the workgroups in equal shares, whatever the contexts are; a
-// unit that was cut is put together by a second, small launch from its parts (sums and what they are relative to).  Where a unit has
-// few tiles at most, every unit has a workgroup and nothing is cut.
+// unit that was cut is put together by a second, small launch from its parts (sums and what they are relative to).  Where a table has room
+// for few tiles, every unit has a workgroup and nothing is cut.
 //
-// Workgroups: eight waves side by side for more than 128 columns, four for 65 to 128 (two parts of four where units are few and long), two
-// for 33 to 64 in two parts that take the tiles in turn, single waves in four parts for up to 32, so that narrow trees have several tiles in
-// flight too (four side by side here as well for a middling number of tiles); heads wider than 128 always four.  The rules and both sides are at tree_launch.
+// Workgroups: eight waves side by side for more than 128 columns of heads of 64 and 128; four for 65 to 128, for any number of columns of other heads and
+// always for heads wider than 128 (two parts of four where units of fp16 pools are few and long); two for 33 to 64 in two parts that take the tiles in turn,
+// single waves in four parts for up to 32, so that narrow trees have several tiles in flight too (four side by side here as well for a middling
+// number of tiles).  The rules and both sides are at tree_launch.  They go by the width of the block table, since only the device knows the contexts: short
+// contexts in a wide table are dealt out and put together as long ones are (7 rows behind 300 15.2 us instead of 13.4, 16 behind 184 21.6 instead of 14.5).
 //
 // Schedule as in attn_packed.hip: step i issues S(i + 1) and O(i - 1) around the softmax of tile i; K goes into LDS two tiles
 // ahead of its use and V one, asked for two steps before that.  Where the tiles lie (rows of the pools, for e4m3 the factors of
@@ -28,11 +30,16 @@
 // there) the rows go in as c, and their exponents into scores and probabilities key by key: otherwise a row that a column does not
 // see would take bits from those that it does.  Such a tile takes 2 us more, two or three of them in a unit (32 users below 181 -> 190).
 //
-// Bound by memory for narrow trees (one context of 131072, 32 / 8 heads of 128, fp16, 24 rows: 537 MB in 116 us, 4.6 TB/s, 102 of them
+// Probabilities enter the second product as one fp16 term: results of fp16 rows are off by 2.6e-4 to 2.8e-4 of their size, of which
+// rounding them is 2.1e-4 (bf16 rows 1.7e-3, all of it their rounding).  With a second term for what the rounding left it is 2.1e-4, but a
+// context of 131072 took 142 instead of 119 us, 8 users over e4m3 76 instead of 63, trees of up to 64 columns up to 20 % more (registers).
+//
+// Bound by memory for narrow trees (one context of 131072, 32 / 8 heads of 128, fp16, 24 rows: 537 MB in 117 us, 4.6 TB/s, 107 of them
 // the first launch), by the matrix cores and what surrounds their steps for wide ones: 32 contexts of 1000 to 8192, e4m3, 64 rows, 113 GFLOP in
-// 182 us.  A step of eight waves over 32 keys takes 2300 clocks, of which its products are 1024 on each of the four matrix cores; beginning a
-// unit costs 6 us (its sequence, its places, its first tiles), and of a wide unit that is cut the parts are 135 KB each, written and read again: 23
-// us of the 182.
+// 191 us.  A step of eight waves over 32 keys takes 2300 clocks, of which its products are 1024 on each of the four matrix cores and the reads of
+// K and V out of LDS (16 KB for each wave) as much; beginning a unit costs 6 us (its sequence, its places, its first tiles), and of a wide unit that is
+// cut the parts are 135 KB each, written and read again: 28 us of the 191 under the profiler.  Heads of 128 and 96 take all 256 registers that two waves
+// to a SIMD leave: 2 spilled in eight waves, 17 to 25 in four over e4m3 pools.
 #pragma once
 
 #include "device_utils.hpp"
@@ -1025,7 +1032,7 @@ static hipError_t tree_launch_as(TreeParams p, hipStream_t stream) {
     const int64_t room = (int64_t)p.block_size * p.max_blocks;
     const int64_t tiles = most * ((room + kTreeKeys - 1) / kTreeKeys);
     // Few tiles to a unit: a workgroup for every unit, whole, and no second launch.  us, cut / whole, 12 / 2 heads of 128, 7 rows behind 300:
-    // 15.0 / 12.4; 32 / 8, 16 rows behind 200: 21.6 / 13.0; 40 behind 250: 17.5 / 15.6; but heads of 256, 8 rows behind 250: 16.2 / 18.0.
+    // 15.2 / 13.4; 32 / 8, 16 rows behind 184: 21.6 / 14.5; four times 40 behind 210: 19.3 / 16.5; but heads of 256, 8 rows behind 242 eight times: 15.0 / 18.6.
     p.whole = (room + kTreeKeys - 1) / kTreeKeys <= (D > 128 ? 4 : 8) * PARTS;
     if (p.whole) {
         paged_attn_tree_kernel<T, D, COLW, PARTS, E4M3><<<(unsigned)most, 64 * COLW * PARTS, 0, stream>>>(p);
@@ -1055,10 +1062,11 @@ static hipError_t tree_launch(const TreeParams& p, hipStream_t stream) {
         const int64_t units = packed_tiles(p.total, p.num_seqs, p.g, 128) * p.hkv;
         const int64_t tiles = ((int64_t)p.block_size * p.max_blocks + kTreeKeys - 1) / kTreeKeys;
         // Up to 64 columns: the waves that have none take tiles of their own, which pays where workgroups have few tiles or many, not
-        // between, where joining the parts costs more.  us, parts / four waves side by side, heads of 128, by 32-key tiles of all units:
-        // up to 32 columns 1000 21.4 / 27.4, 1024 18.1 / 18.7, 4000 31.7 / 27.6 and 32.0 / 26.4, 8064 38.2 / 34.1, 16000 51.7 / 58.1,
-        // 16384 43.1 / 51.9 (but 256 17.8 / 15.4); up to 64 columns 1024 19.7 / 21.3, 4000 34.1 / 31.8, 8064 44.5 / 40.4, 16384 57.0 / 57.0
-        // and, fp16, 62.6 / 65.1.
+        // between, where joining the parts costs more.  us, parts / four waves side by side, heads of 128, by 32-key tiles of all units, e4m3 and
+        // fp16: up to 32 columns 1000 21.7 / 28.2 and 20.4 / 26.0, 1024 18.3 / 20.2 and 17.2 / 18.2, 4000 32.5 / 29.3 and 30.3 / 26.1, 4750 33.1 / 28.2
+        // and 30.5 / 25.9, 9954 40.0 / 35.6 and 37.3 / 34.0, 16384 42.9 / 44.2 and 53.3 / 55.3, 19000 52.0 / 48.8 and 53.6 / 54.2 (but 256 18.5 / 16.1 and
+        // 17.0 / 14.2); up to 64 columns 1000 24.3 / 30.8 and 23.1 / 29.8, 1280 21.4 / 24.1 and 19.8 / 22.7, 5500 35.1 / 32.4 and 31.6 / 28.7, 11466 46.5 / 42.1
+        // and 40.2 / 39.4, 16384 57.3 / 52.1 and 55.5 / 59.4.
         const bool between = units * tiles >= 4 * kTreeWorkers && units * tiles < 24 * kTreeWorkers;
         if (cols <= 32 && (!between || tiles <= 32)) return tree_launch_as<T, D, 1, 4, E4M3>(p, stream);
         if (cols <= 64 && (!between || tiles <= 16)) return tree_launch_as<T, D, 2, 2, E4M3>(p, stream);
@@ -1070,9 +1078,10 @@ static hipError_t tree_launch(const TreeParams& p, hipStream_t stream) {
             if (cols > 64 && cols <= 128 && units <= 64 && units * tiles >= 16 * kTreeWorkers)
                 return tree_launch_as<T, D, 4, 2, E4M3>(p, stream);
     }
-    // More than 128 columns: eight waves, which read a tile once where two workgroups of four read it twice, unless the last has few columns.
-    // us, four / eight waves, e4m3: 32 contexts of 1000 to 8192, 256 columns of heads of 128, 208 / 192; of 4096, 448 columns of heads of 64,
-    // 79 / 75; 64 contexts of 1000, 168 columns of them, 33.3 / 30.0; but 336 columns, of which the last eight waves have 80, 67 / 77.
+    // More than 128 columns of heads of 64 and 128: eight waves, which read a tile once where two workgroups of four read it twice.  us, four / eight
+    // waves, e4m3 and fp16: 32 contexts of 1000 to 8192, 256 columns of heads of 128, 217 / 200 and 225 / 203; of 4096, 448 columns of heads of 64,
+    // 76.3 / 75.8 and 72.6 / 67.7; 64 contexts of 1000, 168 columns of them, 35.3 / 31.8 and 31.7 / 28.7; 210 columns 45.0 / 44.5 and 40.5 / 39.9.  It loses where
+    // the last eight waves have few columns, which the rule does not look at: 280 columns 65.6 / 75.6 and 57.7 / 66.9, 336 65.9 / 75.9 and 59.5 / 67.0.
     if constexpr (D == 64 || D == 128)
         if (cols > 128) return tree_launch_as<T, D, 8, 1, E4M3>(p, stream);
     return tree_launch_as<T, D, 4, 1, E4M3>(p, stream);
